@@ -169,6 +169,35 @@ class HotExpert(C.Structure):
     _fields_ = [("layer", C.c_uint32), ("expert", C.c_uint32), ("uses", C.c_uint64)]
 
 
+KV_KIND = {"int8": 0, "e4m3": 1}
+ROW_DTYPE = {"f32": F32, "f16": F16, "bf16": BF16}  # of activation rows
+
+
+class KvPages(C.Structure):
+    """`ditch_kv_pages`: a pool of pages of 8-bit keys and values."""
+    _fields_ = [("codes", C.c_void_p), ("codes_bytes", C.c_uint64), ("scales", C.c_void_p),
+                ("scales_bytes", C.c_uint64), ("kind", C.c_int32)] + \
+        [(n, C.c_uint32) for n in ("layers", "n_pages", "page_tokens", "kv_heads", "head_dim", "v_head_dim")]
+
+
+class KvBatch(C.Structure):
+    """`ditch_kv_batch`: rows of several sequences and their page tables."""
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("starts", C.c_void_p), ("pos", C.c_void_p), ("n_rows", C.c_uint64), ("max_rows", C.c_uint32),
+                ("max_len", C.c_uint32)]
+
+
+class KvRows(C.Structure):
+    """`ditch_kv_rows`: a row buffer."""
+    _fields_ = [("data", C.c_void_p), ("bytes", C.c_uint64), ("stride", C.c_uint64)]
+
+
+class KvRope(C.Structure):
+    """`ditch_kv_rope`: rotation tables."""
+    _fields_ = [("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("len", C.c_uint64), ("half", C.c_uint32),
+                ("style", C.c_int32)]
+
+
 P = C.c_void_p
 U64 = C.c_uint64
 I32 = C.c_int32
@@ -229,6 +258,15 @@ PROTOTYPES = {
     "ditch_hip_forward_cached": (I32, [P, P, P, P, U64, P, U64, P, U64]),
     "ditch_hip_sampler_init": (I32, [P, U64, FLT, U64, FLT]),
     "ditch_hip_pick_tokens_device": (I32, [P, P, P, U64, U64, P, P]),
+    "ditch_hip_kv_pages_codes_bytes": (U64, [P]),
+    "ditch_hip_kv_pages_scales_bytes": (U64, [P]),
+    "ditch_hip_kv_pages_append_device": (I32, [P, P, U32, P, I32, P, P, P, P, P, U64, P]),
+    "ditch_hip_kv_pages_read_device": (I32, [P, P, U32, P, I32, P, P, P]),
+    "ditch_hip_kv_pages_attention_workspace": (U64, [P, P, U64, I32, U32, U32]),
+    "ditch_hip_kv_pages_attention_device": (I32, [P, P, U32, P, I32, P, P, U64, FLT, U32, U32, P, U64, P]),
+    "ditch_hip_kv_pages_fork_device": (I32, [P, P, P, P, P, U64, P, P, P, U64, U64, P]),
+    "ditch_hip_beam_select_workspace": (U64, [U64, U64, U64, U64]),
+    "ditch_hip_beam_select_device": (I32, [P, P, P, P, P, P, U64, U64, U64, U64, P, U64, P]),
     "ditch_hip_generate": (I32, [P, P, P, P, U64, U64, P, U64, P, P, P, P]),
     "ditch_hip_edit_delta": (I32, [P, P, P, P, P, U64, FLT]),
     "ditch_hip_model_edit": (I32, [P, I32, I32, I32, P, U64, FLT]),

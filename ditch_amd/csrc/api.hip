@@ -10,6 +10,7 @@
 
 #include "internal.h"
 #include "model.h"
+#include "pages.h"
 
 namespace ditch {
 void dequant_to_host(ditch_hip *h, void *out, const ditch_weight *w, uint64_t row0, uint64_t nrows);
@@ -769,6 +770,170 @@ int32_t ditch_hip_model_path_stats(const ditch_hip_model *m, ditch_model_path_st
     out->moe_device_planned = m->moe_device_planned;
     out->moe_host_planned = m->moe_host_planned;
     return DITCH_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Paged 8-bit keys and values, the beam step
+
+// The context's device as the current one for the length of a call.
+struct OnDevice {
+    int was = -1;
+    explicit OnDevice(int device) {
+        int now = -1;
+        DITCH_TRY_HIP(hipGetDevice(&now));
+        if (now == device) return;
+        DITCH_TRY_HIP(hipSetDevice(device));
+        was = now;
+    }
+    ~OnDevice() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+};
+
+uint64_t ditch_hip_kv_pages_codes_bytes(const ditch_kv_pages *p) { return pool_codes_bytes(p); }
+uint64_t ditch_hip_kv_pages_scales_bytes(const ditch_kv_pages *p) { return pool_scales_bytes(p); }
+
+int32_t ditch_hip_kv_pages_append_device(ditch_hip *h, const ditch_kv_pages *p, uint32_t layer,
+                                         const ditch_kv_batch *b, int32_t dtype, const ditch_kv_rows *k,
+                                         const ditch_kv_rows *v, const ditch_kv_rope *rope, const ditch_kv_rows *q,
+                                         const ditch_kv_rows *q_out, uint64_t heads, void *stream) {
+    return guarded(h, [&] {
+        const PoolView pv = pool_view(p, layer);
+        const BatchView bv = batch_view(b, pv);
+        const RowsView kr = rows_view(k, b->n_rows, (uint64_t)pv.kv_heads * pv.hd, dtype, "kv append: keys");
+        const RowsView vr = rows_view(v, b->n_rows, (uint64_t)pv.kv_heads * pv.vd, dtype, "kv append: values");
+        DITCH_CHECK(!q == !q_out, DITCH_INVALID_ARGUMENT, "kv append: q and q_out come together");
+        RowsView qr{}, qo{};
+        if (q) {
+            DITCH_CHECK(heads >= 1 && heads <= 65535, DITCH_INVALID_ARGUMENT, "kv append: 1 to 65535 query heads");
+            qr = rows_view(q, b->n_rows, heads * pv.hd, dtype, "kv append: queries");
+            qo = rows_view(q_out, b->n_rows, heads * pv.hd, dtype, "kv append: rotated queries");
+            DITCH_CHECK(qr.data != qo.data || qr.stride == qo.stride, DITCH_INVALID_ARGUMENT,
+                        "kv append: queries rotated in place keep their stride");
+        }
+        RopeView rv{nullptr, nullptr, 0, DITCH_ROPE_NEOX};
+        if (rope) {
+            DITCH_CHECK(rope->style == DITCH_ROPE_NEOX || rope->style == DITCH_ROPE_GPTJ, DITCH_INVALID_ARGUMENT,
+                        "kv append: rotation style");
+            DITCH_CHECK((uint64_t)rope->half * 2 <= (uint64_t)pv.hd, DITCH_INVALID_ARGUMENT,
+                        "kv append: more rotated coordinates than the head has");
+            DITCH_CHECK(rope->half == 0 || bv.n_seqs == 0 ||
+                            (rope->cos_table && rope->sin_table && rope->len >= (uint64_t)bv.max_len),
+                        DITCH_INVALID_ARGUMENT, "kv append: rotation tables missing or shorter than max_len");
+            rv = RopeView{rope->cos_table, rope->sin_table, (int32_t)rope->half, rope->style};
+        }
+        OnDevice on(h->device);
+        launch_pages_append(pv, bv, dtype, kr, vr, rv, q ? &qr : nullptr, q ? &qo : nullptr, (int)heads,
+                            stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+int32_t ditch_hip_kv_pages_read_device(ditch_hip *h, const ditch_kv_pages *p, uint32_t layer, const ditch_kv_batch *b,
+                                       int32_t dtype, const ditch_kv_rows *k, const ditch_kv_rows *v, void *stream) {
+    return guarded(h, [&] {
+        const PoolView pv = pool_view(p, layer);
+        const BatchView bv = batch_view(b, pv);
+        const RowsView kr = rows_view(k, b->n_rows, (uint64_t)pv.kv_heads * pv.hd, dtype, "kv read: keys");
+        const RowsView vr = rows_view(v, b->n_rows, (uint64_t)pv.kv_heads * pv.vd, dtype, "kv read: values");
+        OnDevice on(h->device);
+        launch_pages_read(pv, bv, dtype, kr, vr, stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+// The shapes of an attention call that its workspace and its launch share.
+static void attention_shape(const ditch_kv_pages *p, const ditch_kv_batch *b, uint64_t heads, uint32_t window,
+                            uint32_t sinks, uint32_t layer, PoolView &pv, BatchView &bv) {
+    pv = pool_view(p, layer);
+    bv = batch_view(b, pv);
+    DITCH_CHECK(heads >= 1 && heads <= 65535 && heads % pv.kv_heads == 0, DITCH_INVALID_ARGUMENT,
+                "kv attention: query heads not a multiple of the KV heads (or above 65535)");
+    DITCH_CHECK(window <= (uint32_t)INT32_MAX && sinks <= (uint32_t)INT32_MAX, DITCH_INVALID_ARGUMENT,
+                "kv attention: window or sinks above 2^31");
+}
+
+uint64_t ditch_hip_kv_pages_attention_workspace(const ditch_kv_pages *p, const ditch_kv_batch *b, uint64_t heads,
+                                                int32_t dtype, uint32_t window, uint32_t sinks) {
+    try {
+        PoolView pv;
+        BatchView bv;
+        attention_shape(p, b, heads, window, sinks, 0, pv, bv);
+        return pages_attention_workspace(pv, bv, (int)heads, dtype, window, sinks);
+    } catch (...) {
+        return 0;  // the call itself says why
+    }
+}
+
+int32_t ditch_hip_kv_pages_attention_device(ditch_hip *h, const ditch_kv_pages *p, uint32_t layer,
+                                            const ditch_kv_batch *b, int32_t dtype, const ditch_kv_rows *out,
+                                            const ditch_kv_rows *q, uint64_t heads, float scale, uint32_t window,
+                                            uint32_t sinks, void *ws, uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        PagesAttention a{};
+        attention_shape(p, b, heads, window, sinks, layer, a.p, a.b);
+        a.q = rows_view(q, b->n_rows, heads * a.p.hd, dtype, "kv attention: queries");
+        a.out = rows_view(out, b->n_rows, heads * a.p.vd, dtype, "kv attention: output");
+        a.dtype = dtype;
+        a.heads = (int32_t)heads;
+        a.scale = scale;
+        a.window = (int32_t)window;
+        a.sinks = (int32_t)sinks;
+        const size_t need = pages_attention_workspace(a.p, a.b, a.heads, dtype, window, sinks);
+        DITCH_CHECK(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), DITCH_INVALID_ARGUMENT,
+                    "kv attention: workspace missing, misaligned or shorter than "
+                    "ditch_hip_kv_pages_attention_workspace");
+        OnDevice on(h->device);
+        launch_pages_attention(a, ws, (size_t)ws_bytes, stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, int32_t *d_table_out,
+                                       int32_t *d_spare_out, const int32_t *d_table, uint64_t table_stride,
+                                       const int32_t *d_parents, const int32_t *d_spare, const uint32_t *d_lens,
+                                       uint64_t n_groups, uint64_t beams, void *stream) {
+    return guarded(h, [&] {
+        (void)pool_view(p, 0);
+        if (n_groups == 0) return;
+        DITCH_CHECK(beams >= 1 && beams <= 64 && n_groups <= (uint64_t)1 << 20, DITCH_INVALID_ARGUMENT,
+                    "kv fork: 1 to 64 beams, up to 2^20 groups");
+        DITCH_CHECK(table_stride >= 1 && table_stride <= (uint64_t)INT32_MAX, DITCH_INVALID_ARGUMENT,
+                    "kv fork: table stride");
+        DITCH_CHECK(d_table_out && d_spare_out && d_table && d_parents && d_spare && d_lens, DITCH_INVALID_ARGUMENT,
+                    "kv fork: NULL argument");
+        DITCH_CHECK(d_table_out != d_table && d_spare_out != d_spare, DITCH_INVALID_ARGUMENT,
+                    "kv fork: the tables and spare pages are not reordered in place");
+        OnDevice on(h->device);
+        launch_pages_fork(p, d_table_out, d_spare_out, d_table, (int64_t)table_stride, d_parents, d_spare, d_lens,
+                          (int64_t)n_groups, (int64_t)beams, stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+static bool beam_shape_ok(uint64_t prompts, uint64_t beams, uint64_t vocab, uint64_t k) {
+    return prompts <= (uint64_t)1 << 16 && beams >= 1 && beams <= 64 && vocab >= 1 && vocab <= (uint64_t)INT32_MAX &&
+           k >= 1 && k <= 128 && k <= beams * vocab;
+}
+
+uint64_t ditch_hip_beam_select_workspace(uint64_t n_prompts, uint64_t beams, uint64_t vocab, uint64_t k) {
+    if (n_prompts == 0 || !beam_shape_ok(n_prompts, beams, vocab, k)) return 0;
+    return beam_select_workspace((int64_t)n_prompts, (int64_t)beams, (int64_t)vocab, (int64_t)k);
+}
+
+int32_t ditch_hip_beam_select_device(ditch_hip *h, float *d_scores, int32_t *d_parents, uint32_t *d_tokens,
+                                     const float *d_logits, const float *d_prev, uint64_t n_prompts, uint64_t beams,
+                                     uint64_t vocab, uint64_t k, void *ws, uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        if (n_prompts == 0) return;
+        DITCH_CHECK(beam_shape_ok(n_prompts, beams, vocab, k), DITCH_INVALID_ARGUMENT,
+                    "beam select: 1 to 64 beams, 1 to 128 of the beams' continuations, up to 65536 prompts");
+        DITCH_CHECK(d_scores && d_parents && d_tokens && d_logits && d_prev, DITCH_INVALID_ARGUMENT,
+                    "beam select: NULL argument");
+        DITCH_CHECK(ws && (uintptr_t)ws % 16 == 0 &&
+                        ws_bytes >= beam_select_workspace((int64_t)n_prompts, (int64_t)beams, (int64_t)vocab, (int64_t)k),
+                    DITCH_INVALID_ARGUMENT, "beam select: workspace missing, misaligned or shorter than "
+                                            "ditch_hip_beam_select_workspace");
+        OnDevice on(h->device);
+        launch_beam_select(d_scores, d_parents, d_tokens, d_logits, d_prev, (int64_t)n_prompts, (int64_t)beams,
+                           (int64_t)vocab, (int64_t)k, ws, (size_t)ws_bytes, stream ? (hipStream_t)stream : h->stream);
+    });
 }
 
 // ---------------------------------------------------------------------------

@@ -24,6 +24,10 @@ def _p(a):
     return None if a is None else a.ctypes.data_as(ctypes.c_void_p)
 
 
+def _ref(a):
+    return None if a is None else ctypes.byref(a)
+
+
 def _f32(a):
     return np.ascontiguousarray(a, dtype=np.float32)
 
@@ -202,6 +206,75 @@ class Device:
 
     def klRows_device(self, d_kl, d_base, d_trial, n, vocab, stream=None):
         self.check(self.lib.ditch_hip_klRows_device(self.h, d_kl, d_base, d_trial, n, vocab, stream))
+
+    # paged 8-bit keys and values, the beam step ---------------------------------
+
+    @staticmethod
+    def kv_pages(codes, codes_bytes, scales, scales_bytes, kind, layers, n_pages, page_tokens, kv_heads, head_dim,
+                 v_head_dim=None):
+        """The descriptor of a pool of pages in device memory (ditch_kv_pages);
+        kind: "int8" or "e4m3". Keep the buffers as long as it is used."""
+        return abi.KvPages(codes, codes_bytes, scales, scales_bytes, abi.KV_KIND[kind], layers, n_pages, page_tokens,
+                           kv_heads, head_dim, head_dim if v_head_dim is None else v_head_dim)
+
+    def kv_pages_bytes(self, pages):
+        """(bytes of the codes, bytes of the scales) of a pool; zeros for a shape that is refused."""
+        return (self.lib.ditch_hip_kv_pages_codes_bytes(ctypes.byref(pages)),
+                self.lib.ditch_hip_kv_pages_scales_bytes(ctypes.byref(pages)))
+
+    @staticmethod
+    def kv_batch(table, table_stride, starts, pos, n_seqs, n_rows, max_rows, max_len):
+        """The descriptor of several sequences' rows (ditch_kv_batch; device pointers)."""
+        return abi.KvBatch(table, table_stride, n_seqs, starts, pos, n_rows, max_rows, max_len)
+
+    @staticmethod
+    def kv_rows(data, nbytes, stride):
+        """The descriptor of a row buffer (ditch_kv_rows; `stride` in elements)."""
+        return abi.KvRows(data, nbytes, stride)
+
+    @staticmethod
+    def kv_rope(cos_t, sin_t, length, half, style="neox"):
+        """The descriptor of rotation tables [length][half] in device memory (ditch_kv_rope)."""
+        return abi.KvRope(cos_t, sin_t, length, half, abi.ROPE_NEOX if style == "neox" else abi.ROPE_GPTJ)
+
+    def kv_pages_append(self, pages, layer, batch, dtype, k, v, rope=None, q=None, q_out=None, heads=0, stream=None):
+        """Keys (rotated) and values into the pages, the queries rotated
+        (ditch_hip_kv_pages_append_device); dtype: "f32", "f16" or "bf16"."""
+        self.check(self.lib.ditch_hip_kv_pages_append_device(
+            self.h, _ref(pages), layer, _ref(batch), abi.ROW_DTYPE[dtype], _ref(k), _ref(v), _ref(rope), _ref(q),
+            _ref(q_out), heads, stream))
+
+    def kv_pages_read(self, pages, layer, batch, dtype, k, v, stream=None):
+        """The cached keys and values of the batch's positions as rows (ditch_hip_kv_pages_read_device)."""
+        self.check(self.lib.ditch_hip_kv_pages_read_device(self.h, _ref(pages), layer, _ref(batch),
+                                                           abi.ROW_DTYPE[dtype], _ref(k), _ref(v), stream))
+
+    def kv_pages_attention_workspace(self, pages, batch, heads, dtype, window=0, sinks=0):
+        return self.lib.ditch_hip_kv_pages_attention_workspace(_ref(pages), _ref(batch), heads, abi.ROW_DTYPE[dtype],
+                                                               window, sinks)
+
+    def kv_pages_attention(self, pages, layer, batch, dtype, out, q, heads, scale, ws, ws_bytes, window=0, sinks=0,
+                           stream=None):
+        """Attention of the batch's rows over their cached sequences (ditch_hip_kv_pages_attention_device)."""
+        self.check(self.lib.ditch_hip_kv_pages_attention_device(
+            self.h, _ref(pages), layer, _ref(batch), abi.ROW_DTYPE[dtype], _ref(out), _ref(q), heads, scale, window,
+            sinks, ws, ws_bytes, stream))
+
+    def kv_pages_fork(self, pages, d_table_out, d_spare_out, d_table, table_stride, d_parents, d_spare, d_lens,
+                      n_groups, beams, stream=None):
+        """The beams' tables and last pages by their parents (ditch_hip_kv_pages_fork_device)."""
+        self.check(self.lib.ditch_hip_kv_pages_fork_device(self.h, _ref(pages), d_table_out, d_spare_out, d_table,
+                                                           table_stride, d_parents, d_spare, d_lens, n_groups, beams,
+                                                           stream))
+
+    def beam_select_workspace(self, n_prompts, beams, vocab, k):
+        return self.lib.ditch_hip_beam_select_workspace(n_prompts, beams, vocab, k)
+
+    def beam_select(self, d_scores, d_parents, d_tokens, d_logits, d_prev, n_prompts, beams, vocab, k, ws, ws_bytes,
+                    stream=None):
+        """The k best continuations of each prompt's beams (ditch_hip_beam_select_device)."""
+        self.check(self.lib.ditch_hip_beam_select_device(self.h, d_scores, d_parents, d_tokens, d_logits, d_prev,
+                                                         n_prompts, beams, vocab, k, ws, ws_bytes, stream))
 
 
 class Tensor:

@@ -601,6 +601,170 @@ int32_t ditch_hip_generate(ditch_hip_model *m, ditch_hip_kv_cache *c,
                            uint64_t *out_lens, float *first_logits);
 
 /* ------------------------------------------------------------------------ */
+/* Paged 8-bit keys and values, and the beam step (no reference counterpart:
+ * the reference's KvCache, model.zig:2586-2724, is f32 and contiguous). For
+ * contexts longer than ditch_hip_kv_cache_create's 1024 positions, at a
+ * quarter of its bytes: keys and values live in pages of 8-bit codes that the
+ * caller owns, sequences are lists of pages, and a scale belongs to each
+ * (page, KV head), one for its keys and one for its values. All entries
+ * work on device memory, are enqueued on `stream` (NULL = the context
+ * stream) and neither wait, allocate nor keep anything: calls on different
+ * streams, or captured into graphs, share nothing but what the caller
+ * hands to both.                                                           */
+
+/* Code formats: value = code * scale of its (page, head). INT8: codes
+ * -127..127, scale = largest |value| * 1/127 (both f32, rounded). E4M3: OCP
+ * FP8 (no infinities), scale = largest |value| * 1/448. Values round to the
+ * nearest code, ties to even.                                              */
+enum { DITCH_KV_INT8 = 0, DITCH_KV_E4M3 = 1 };
+
+/* The pool. codes: [layers][n_pages][kv_heads][page_tokens * (dk + dv)], a
+ * head's keys in front of its values, 16-byte aligned; dk and dv are
+ * head_dim and v_head_dim rounded up to multiples of 64 (the dims added hold
+ * zeros). scales: f32 [layers][n_pages][kv_heads][2] (keys, values). The
+ * order within a head's page is that of the matrix cores' operands:
+ *   keys:   per 16 tokens, per 64 dims: [4][16 tokens][16 dims]
+ *   values: per 32 tokens, per 32 dims: [4 g][16 dims d][2 h][8 j],
+ *           dim 16 h + d, token 16 (j / 4) + 4 g + j % 4
+ * page_tokens: 32, 64, 128 or 256. Head dims up to 256, with dk = dv or 192
+ * and 128; others are Unsupported. A pool needs no clearing: append clears
+ * what it starts to fill. Buffers shorter than the shape are refused.      */
+typedef struct ditch_kv_pages {
+    void *codes;
+    uint64_t codes_bytes;
+    float *scales;
+    uint64_t scales_bytes;
+    int32_t kind;          /* DITCH_KV_*                                     */
+    uint32_t layers;
+    uint32_t n_pages;
+    uint32_t page_tokens;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t v_head_dim;
+} ditch_kv_pages;
+/* Bytes of the pool's two buffers (0 for a shape that is refused).         */
+uint64_t ditch_hip_kv_pages_codes_bytes(const ditch_kv_pages *p);
+uint64_t ditch_hip_kv_pages_scales_bytes(const ditch_kv_pages *p);
+
+/* Rows of several sequences, one after the other: sequence b's are rows
+ * starts[b] .. starts[b + 1] of the call's row buffers, at its positions
+ * pos[b], pos[b] + 1, ...; its position t lies in page table[b *
+ * table_stride + t / page_tokens]. table, starts ([n_seqs + 1]) and pos are
+ * device memory; the counts are the caller's: n_rows rows in the buffers,
+ * max_rows the most of one sequence, max_len the longest pos + rows. They
+ * are bounds that the device holds the arrays to: rows past n_rows,
+ * max_rows or max_len, and pages outside the pool, are neither read nor
+ * written (a query that would attend to such a page, or lies past max_len,
+ * gets NaN; one past max_rows or not in any sequence keeps its output).
+ * Two sequences may share pages; append to a shared page only after
+ * ditch_hip_kv_pages_fork_device or a copy of its own.                     */
+typedef struct ditch_kv_batch {
+    const int32_t *table;
+    uint32_t table_stride;
+    uint32_t n_seqs;
+    const uint32_t *starts;
+    const uint32_t *pos;
+    uint64_t n_rows;
+    uint32_t max_rows;
+    uint32_t max_len;
+} ditch_kv_batch;
+
+/* A row buffer: n_rows rows of heads * dim elements (DITCH_F32, DITCH_F16 or
+ * DITCH_BF16, the call's dtype), `stride` elements from row to row, `bytes`
+ * long. Shorter buffers are refused.                                       */
+typedef struct ditch_kv_rows {
+    void *data;
+    uint64_t bytes;
+    uint64_t stride;
+} ditch_kv_rows;
+
+/* Position rotation (compute.zig:85, 119; ditch_hip_ropeRows): the first
+ * 2 * half coordinates of a head by cos_table / sin_table [len][half]
+ * (device memory, len >= max_len), style DITCH_ROPE_NEOX or GPTJ.          */
+typedef struct ditch_kv_rope {
+    const float *cos_table;
+    const float *sin_table;
+    uint64_t len;
+    uint32_t half;
+    int32_t style;
+} ditch_kv_rope;
+
+/* Appends keys k [kv_heads * head_dim] and values v [kv_heads * v_head_dim]
+ * to `layer`: the keys rotated to their positions (rope; NULL: as they are),
+ * both rounded once, from the 64-bit rotation, to codes. The tokens of a
+ * page that lie before its sequence's first new row stay: where the new
+ * rows need a larger scale, their codes are rounded again to it; every
+ * other token of the page is dead and may be written. A NaN or an infinity
+ * makes the page's scale NaN (and every key or value of that head's page
+ * with it) until the page is filled anew from its first token. With q and
+ * q_out (both or neither; they may be the same rows) the queries [heads *
+ * head_dim] are rotated too.                                               */
+int32_t ditch_hip_kv_pages_append_device(ditch_hip *h, const ditch_kv_pages *p, uint32_t layer,
+                                         const ditch_kv_batch *b, int32_t dtype,
+                                         const ditch_kv_rows *k, const ditch_kv_rows *v,
+                                         const ditch_kv_rope *rope, const ditch_kv_rows *q,
+                                         const ditch_kv_rows *q_out, uint64_t heads,
+                                         void *stream);
+/* The inverse of append: the keys (rotated, as stored) and values of the
+ * batch's positions as rows. Positions whose page lies outside the pool
+ * give NaN.                                                                */
+int32_t ditch_hip_kv_pages_read_device(ditch_hip *h, const ditch_kv_pages *p, uint32_t layer,
+                                       const ditch_kv_batch *b, int32_t dtype,
+                                       const ditch_kv_rows *k, const ditch_kv_rows *v,
+                                       void *stream);
+/* Attention of the batch's rows (their keys already appended): out [heads *
+ * v_head_dim] = sum_j softmax_j(scale * q . k_j) v_j over the row's own
+ * sequence, key positions j <= t for a row at position t; with window > 0
+ * only t - window < j and the first `sinks` positions. Query head i reads
+ * KV head i / (heads / kv_heads). f32 rows are exact to about f32 rounding;
+ * 16-bit ones use softmax weights of 11 bits, sums are f32 throughout.
+ * `ws` is device scratch of ditch_hip_kv_pages_attention_workspace bytes
+ * (may be 0; its contents do not matter, calls that overlap need one each). */
+uint64_t ditch_hip_kv_pages_attention_workspace(const ditch_kv_pages *p, const ditch_kv_batch *b,
+                                                uint64_t heads, int32_t dtype, uint32_t window,
+                                                uint32_t sinks);
+int32_t ditch_hip_kv_pages_attention_device(ditch_hip *h, const ditch_kv_pages *p,
+                                            uint32_t layer, const ditch_kv_batch *b,
+                                            int32_t dtype, const ditch_kv_rows *out,
+                                            const ditch_kv_rows *q, uint64_t heads, float scale,
+                                            uint32_t window, uint32_t sinks, void *ws,
+                                            uint64_t ws_bytes, void *stream);
+/* Reorders the states of n_groups groups of `beams` sequences, sequence c of
+ * a group continuing its parent parents[c] (0 .. beams - 1, within the
+ * group; any other value: c itself), each group at the one length lens[g].
+ * Per table row: the pages before the length's page are the parent's
+ * (shared), those behind it stay the row's own. A partly filled last page
+ * goes to the parent's first child; the further children copy it (every
+ * layer, codes and scales) into their spare page spare[c] and find in
+ * spare_out[c] a page that a childless sequence of the group left free:
+ * pages in use and spare ones stay equally many. A length that ends with a
+ * page copies nothing. table / table_out are [n_groups * beams]
+ * [table_stride] and must differ, spare / spare_out [n_groups * beams]
+ * likewise. Pages outside the pool are neither read nor written.           */
+int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, int32_t *d_table_out,
+                                       int32_t *d_spare_out, const int32_t *d_table,
+                                       uint64_t table_stride, const int32_t *d_parents,
+                                       const int32_t *d_spare, const uint32_t *d_lens,
+                                       uint64_t n_groups, uint64_t beams, void *stream);
+
+/* The beam step: of each prompt's beams x vocab continuations, scored
+ * d_prev[prompt][beam] + log_softmax(d_logits[prompt][beam])[token], the k
+ * best, highest first, the lower (beam, token) first among equals: scores
+ * f32 [n_prompts][k], parents (beam) and tokens. Scores are formed in 64
+ * bits. A beam whose previous score is -infinity comes after every finite
+ * one; a beam without probabilities (a NaN or +infinity among its logits,
+ * or nothing above -infinity; a NaN previous score) scores NaN and comes
+ * last. 1 <= beams <= 64, 1 <= k <= 128 and k <= beams * vocab. `ws`:
+ * ditch_hip_beam_select_workspace bytes, as for the attention.             */
+uint64_t ditch_hip_beam_select_workspace(uint64_t n_prompts, uint64_t beams, uint64_t vocab,
+                                         uint64_t k);
+int32_t ditch_hip_beam_select_device(ditch_hip *h, float *d_scores, int32_t *d_parents,
+                                     uint32_t *d_tokens, const float *d_logits,
+                                     const float *d_prev, uint64_t n_prompts, uint64_t beams,
+                                     uint64_t vocab, uint64_t k, void *ws, uint64_t ws_bytes,
+                                     void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Rank-k edit, `none` mode (abliterate.zig:264-280): a = V^T W ([k][cols]),
  * b = -weight * V ([rows][k]) for directions v [k][rows]. Host buffers.    */
 int32_t ditch_hip_edit_delta(ditch_hip *h, float *a, float *b,
