@@ -1,0 +1,209 @@
+// pages_attention.h — what the attention kernels over pages of 8-bit keys and
+// values share (pages_attention.hip, pages_chunk.hip).
+//
+// Mathematics. For a query q, keys k_j = ks c_j (ks: the scale of the key's
+// page and head, c: codes) and values v_j = vs e_j:
+//   out = sum_j exp(s_j) vs_j e_j / sum_j exp(s_j),  s_j = scale ks_j (q . c_j)
+// in one pass with a running maximum. The value scale goes into the
+// exponent, w_j = 2^(s_j log2(e) + log2(vs_j) - m), so the accumulator sums
+// w_j e_j with plain codes, and the denominator adds a granule's w times
+// 1 / vs: one multiplication for a granule's eight weights a lane.
+//
+// Codes of both kinds are exact in f16 (int8: 8 bits of 11; e4m3: 4 bits, the
+// least 2^-9), so both products run on v_mfma_f32_16x16x32_f16 with exact
+// cache operands. A query is scaled by a power of two that takes its largest
+// coordinate to [2^14, 2^15): what f16's smallest steps drop is below
+// 2^-39 of it. 16-bit queries enter as one f16 term (exact for f16, and for
+// bf16's 8 bits), f32 ones as two (22 bits). Weights enter as one RNE f16
+// (2^-12 of their value, below the output's own rounding of at least 2^-12)
+// or, for f32 rows, as two terms.
+#pragma once
+#include "pages.h"
+
+namespace ditch {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Weights are held relative to the running maximum, times 2^W_UP, and the
+// maximum moves only when one would pass 2^W_MOST: f16 ends at 2^16, and
+// its steps below 2^-14 are then 2^-36 of the largest weight.
+constexpr float W_UP = 12.f, W_MOST = 15.f;
+constexpr float M_NONE = -3e38f;  // the maximum over no keys
+
+// A value scale with log2 outside of this goes its own way (see granule_scales).
+constexpr float BIAS_PLAIN = 40.f;
+
+__device__ __forceinline__ floatx4 mfma_f16(half8 a, half8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// The f16 values of 8 codes.
+template <int KIND>
+__device__ __forceinline__ half8 codes_f16(uint32_t lo, uint32_t hi) {
+    u32x4 r;
+    if constexpr (KIND == DITCH_KV_INT8) {
+        // 0x64uu is 1024 + uu in f16; uu = code + 128
+        lo ^= 0x80808080u;
+        hi ^= 0x80808080u;
+        r[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u);
+        r[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u);
+        r[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u);
+        r[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u);
+        return __builtin_bit_cast(half8, r) - (_Float16)1152.f;
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+        return __builtin_bit_cast(half8, r);
+    }
+}
+
+// The largest / the sum over the four lanes (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float max_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A query tile's operands: lane (g, c) holds query c's dims 64 p + 16 g + 0..7
+// (step 0) and + 8..15 (step 1) of every 64-dim unit p, in TERMS f16 terms,
+// and the power of two that undoes the query's scaling.
+template <int KP, int TERMS>
+struct QueryTile {
+    half8 f[KP][2][TERMS];
+    float down;
+};
+
+// x: the query's head (NULL: zeros), hd its dims.
+template <typename T, int KP, int TERMS>
+__device__ __forceinline__ void load_query(QueryTile<KP, TERMS> &q, const T *x, int hd, int g) {
+    float v[KP][16];
+    float most = 0.f;
+#pragma unroll
+    for (int p = 0; p < KP; p++) {
+        const int d0 = 64 * p + 16 * g;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            v[p][j] = x && d0 + j < hd ? (float)x[d0 + j] : 0.f;
+            most = fmaxf(most, fabsf(v[p][j]));
+        }
+    }
+    most = max_groups(most);
+    // 2^up takes the largest to [2^14, 2^15) (from a subnormal: as far as f32 goes)
+    const int up = most > 0.f && most <= 3.4028234663852886e38f ? 14 - (int)((__float_as_uint(most) >> 23) - 127) : 0;
+#pragma unroll
+    for (int p = 0; p < KP; p++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = ldexpf(v[p][8 * s + j], up);
+                const _Float16 hi = (_Float16)y;
+                q.f[p][s][0][j] = hi;
+                if constexpr (TERMS == 2) q.f[p][s][1][j] = (_Float16)(y - (float)hi);
+            }
+    q.down = ldexpf(1.f, -up);
+}
+
+// The keys of a 16-token tile (kb: its KP 16-byte units a lane) times the queries.
+template <int KIND, int KP, int TERMS>
+__device__ __forceinline__ floatx4 scores(const u32x4 *kb, const QueryTile<KP, TERMS> &q) {
+    floatx4 s{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < KP; p++) {
+        const half8 k0 = codes_f16<KIND>(kb[p][0], kb[p][1]), k1 = codes_f16<KIND>(kb[p][2], kb[p][3]);
+#pragma unroll
+        for (int t = 0; t < TERMS; t++) {
+            s = mfma_f16(k0, q.f[p][0][t], s);
+            s = mfma_f16(k1, q.f[p][1][t], s);
+        }
+    }
+    return s;
+}
+
+// 8 weights as the operand of the values' product.
+template <int TERMS>
+struct Weights {
+    half8 f[TERMS];
+};
+template <int TERMS>
+__device__ __forceinline__ void weight_terms(Weights<TERMS> &w, const float (&x)[8]) {
+    u32x4 hi;
+    if constexpr (TERMS == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            hi[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{x[2 * j], x[2 * j + 1]}, half2_t));
+        w.f[0] = __builtin_bit_cast(half8, hi);
+    } else {
+        u32x4 lo;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // toward zero: the second term holds what is left
+            const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x[2 * j], x[2 * j + 1]));
+            hi[j] = __builtin_bit_cast(uint32_t, h);
+            lo[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * j] - (float)h[0], x[2 * j + 1] - (float)h[1]));
+        }
+        w.f[0] = __builtin_bit_cast(half8, hi);
+        w.f[1] = __builtin_bit_cast(half8, lo);
+    }
+}
+
+// A granule's scales as the loops use them. A value scale far from 1 (or
+// none: zero) would leave the weights' range in the sum of the denominator,
+// which then adds exp(s_j) itself (`odd`); at zero the values add nothing
+// and `skip` leaves their product out.
+struct GranuleScales {
+    float key, bias, inverse;
+};
+__device__ __forceinline__ GranuleScales granule_scales(float ks, float vs) {
+    const bool zero = fabsf(vs) < 1.17549435e-38f;  // (subnormal: the logarithm takes it for zero)
+    return {ks, zero ? 0.f : __builtin_amdgcn_logf(vs), zero ? 0.f : 1.f / vs};
+}
+
+// The rows of a query tile: 16 consecutive (row, head of the KV head's
+// group) pairs of one sequence and KV head; lane column c holds pair 16 tile + c.
+struct TileRows {
+    int t_lo, t_hi;  // positions of its first and last live row
+    int granules;    // granules that any of them sees
+    int sink_end;    // the first granules: 0 .. sink_end
+    int skip;        // added to the index of the further ones
+};
+__device__ __forceinline__ TileRows tile_rows(const SeqRows &r, int first_row, int last_row, int window, int sinks) {
+    TileRows t;
+    t.t_lo = r.pos + first_row;
+    t.t_hi = r.pos + (last_row < r.live ? last_row : r.live - 1);
+    const int end = t.t_hi / GRANULE + 1;
+    const int first = window && t.t_lo - window + 1 > 0 ? (t.t_lo - window + 1) / GRANULE : 0;
+    const int sg = sinks > 0 && first > 0 ? (sinks - 1) / GRANULE + 1 : 0;
+    t.sink_end = sg < first ? sg : first;
+    t.skip = first - t.sink_end;
+    t.granules = t.sink_end + end - first;
+    return t;
+}
+__device__ __forceinline__ int granule_index(const TileRows &t, int k) { return k < t.sink_end ? k : k + t.skip; }
+// Every token of granule gi is visible to every live row of the tile.
+__device__ __forceinline__ bool granule_full(const TileRows &t, int gi, int window, int sinks) {
+    const int a = gi * GRANULE, z = a + GRANULE - 1;
+    return z <= t.t_lo && (!window || a > t.t_hi - window || z < sinks);
+}
+__device__ __forceinline__ bool token_seen(int j, int t, int window, int sinks) {
+    return j <= t && (!window || t - j < window || j < sinks);
+}
+
+// pages_chunk.hip: many rows a sequence
+bool pages_chunk_takes(const PagesAttention &a);
+void launch_pages_chunk(const PagesAttention &a, hipStream_t s);
+
+}  // namespace ditch

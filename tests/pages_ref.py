@@ -140,12 +140,13 @@ def sequence(pool, layer, row, n):
 
 
 def attention(pool, layer, table, starts, pos, q, scale, window=0, sinks=0):
-    """f64 (out [n][heads][vd], bound scale): per output the weighted mean of |v|, the largest score's sum of
-    |q k| and the spread of the scores, which the tests' tolerances are made of."""
+    """f64 out [n][heads][vd] and what the tests' tolerances are made of: per output the weighted mean of |v|, per
+    head the largest score's sum of |q k|, the spread of the scores, and the largest code's value under the key that
+    weighs most."""
     n, heads = q.shape[:2]
     group = heads // pool.kv_heads
     out = np.full((n, heads, pool.vd), np.nan)
-    mass, size, spread = np.zeros((n, heads, pool.vd)), np.zeros((n, heads, 1)), np.zeros((n, heads, 1))
+    mass, size, spread, top = np.zeros((n, heads, pool.vd)), *(np.zeros((n, heads, 1)) for _ in range(3))
     for b in range(len(pos)):
         for i in range(int(starts[b + 1]) - int(starts[b])):
             r, t = int(starts[b]) + i, int(pos[b]) + i
@@ -153,6 +154,7 @@ def attention(pool, layer, table, starts, pos, q, scale, window=0, sinks=0):
             j = np.arange(t + 1)
             seen = (t - j < window) | (j < sinks) if window else j <= t
             k, v = k[:, seen], v[:, seen]
+            vs = np.stack([pool.scales[layer, max(table[b, x], 0) % pool.n_pages, :, 1] for x in j[seen] // pool.page], 1)
             for h in range(heads):
                 kk, vv, qq = k[h // group], v[h // group], q[r, h].astype(np.float64)
                 s = kk @ qq * scale
@@ -163,7 +165,8 @@ def attention(pool, layer, table, starts, pos, q, scale, window=0, sinks=0):
                 out[r, h], mass[r, h] = w @ vv, w @ np.abs(vv)
                 size[r, h] = (np.abs(kk) @ np.abs(qq)).max() * abs(scale)
                 spread[r, h] = s.max() - s.min()
-    return out, mass, size, spread
+                top[r, h] = (w * vs[h // group]).max() * MOST[pool.kind]
+    return out, mass, size, spread, top
 
 
 def fork(table, parents, spare, lens, page, beams):
