@@ -86,20 +86,32 @@ struct QueryTile {
     float down;
 };
 
-// x: the query's head (NULL: zeros), hd its dims.
-template <typename T, int KP, int TERMS>
-__device__ __forceinline__ void load_query(QueryTile<KP, TERMS> &q, const T *x, int hd, int g) {
+// The lane's coordinates of a query as loaded. x: the query's head (NULL: zeros), hd its dims.
+template <int KP>
+struct RawQuery {
     float v[KP][16];
-    float most = 0.f;
+};
+template <typename T, int KP>
+__device__ __forceinline__ void load_query(RawQuery<KP> &q, const T *x, int hd, int g) {
 #pragma unroll
     for (int p = 0; p < KP; p++) {
         const int d0 = 64 * p + 16 * g;
+        if (x && d0 + 16 <= hd) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            v[p][j] = x && d0 + j < hd ? (float)x[d0 + j] : 0.f;
-            most = fmaxf(most, fabsf(v[p][j]));
+            for (int j = 0; j < 16; j++) q.v[p][j] = (float)x[d0 + j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) q.v[p][j] = x && d0 + j < hd ? (float)x[d0 + j] : 0.f;
         }
     }
+}
+template <int KP, int TERMS>
+__device__ __forceinline__ void query_terms(QueryTile<KP, TERMS> &q, const RawQuery<KP> &raw) {
+    float most = 0.f;
+#pragma unroll
+    for (int p = 0; p < KP; p++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) most = fmaxf(most, fabsf(raw.v[p][j]));
     most = max_groups(most);
     // 2^up takes the largest to [2^14, 2^15) (from a subnormal: as far as f32 goes)
     const int up = most > 0.f && most <= 3.4028234663852886e38f ? 14 - (int)((__float_as_uint(most) >> 23) - 127) : 0;
@@ -109,7 +121,7 @@ __device__ __forceinline__ void load_query(QueryTile<KP, TERMS> &q, const T *x, 
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float y = ldexpf(v[p][8 * s + j], up);
+                const float y = ldexpf(raw.v[p][8 * s + j], up);
                 const _Float16 hi = (_Float16)y;
                 q.f[p][s][0][j] = hi;
                 if constexpr (TERMS == 2) q.f[p][s][1][j] = (_Float16)(y - (float)hi);

@@ -18,8 +18,11 @@
 
 namespace ditch {
 
+constexpr int MOST_SPLITS = 256;
+
 struct RowsPlan {
     int tiles, splits, cols;  // query tiles of a (sequence, KV head); workgroups a tile; queries a tile
+    int waves;                // of a workgroup: 4 or 8
     float *sums, *stats;      // [item][cols][DV], [item][cols][2]: splits > 1
 };
 
@@ -27,7 +30,7 @@ template <typename T, int KIND, int DK, int DV, int NW>
 __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, RowsPlan plan) {
     constexpr int KP = DK / 64, VU = DV / 32, TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr int OS = DV + 4;
-    __shared__ __attribute__((aligned(16))) float o_s[NW][16][OS];
+    extern __shared__ __attribute__((aligned(16))) float o_s[];  // [NW][cols][OS]
     __shared__ float m_s[NW][16], l_s[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     int64_t blk = blockIdx.x;
@@ -55,12 +58,13 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     const bool mine = row < r.live;
     const int t = mine ? r.pos + row : tr.t_hi;  // the column's position
 
-    QueryTile<KP, TERMS> q;
-    load_query(q, mine ? (const T *)a.q.data + (int64_t)(r.row + row) * a.q.stride +
+    RawQuery<KP> raw;
+    load_query(raw, mine ? (const T *)a.q.data + (int64_t)(r.row + row) * a.q.stride +
                              (int64_t)(h * group + qi % group) * a.p.hd
                        : (const T *)nullptr,
                a.p.hd, g);
-    const float cq = a.scale * 1.4426950408889634f * q.down;
+    QueryTile<KP, TERMS> q;
+    float cq = 0.f;
 
     floatx4 o[DV / 16];
 #pragma unroll
@@ -134,25 +138,26 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     };
 
     // the wave's granules k0 + wave, + NW, ...: the pages and scales of 64 of
-    // them at a time, one a lane, the codes one granule ahead
+    // them at a time, one a lane, the codes one granule ahead. The first
+    // codes are asked for before anything waits for the queries and scales.
     const int mine_n = k1 - k0 > wave ? (k1 - k0 - wave + NW - 1) / NW : 0;
+    if (mine_n == 0) query_terms(q, raw);
     for (int b = 0; b < mine_n; b += 64) {
         const int n = mine_n - b < 64 ? mine_n - b : 64;
-        int gi_l = 0, id_l = 0;
-        GranuleScales sc_l{0.f, 0.f, 1.f};
-        if (lane < n) {
-            gi_l = granule_index(tr, k0 + wave + NW * (b + lane));
-            id_l = page_of(a.b, a.p, seq, gi_l / per);
-            float2 sc = make_float2(NAN, NAN);
-            if (id_l >= 0) sc = *(const float2 *)(a.p.scales + ((int64_t)id_l * a.p.kv_heads + h) * 2);
-            else id_l = 0;  // page 0's codes under scales of NaN
-            sc_l = granule_scales(sc.x, sc.y);
-        }
+        const int gi_l = granule_index(tr, k0 + wave + NW * (b + (lane < n ? lane : 0)));
+        const int id_l = page_of(a.b, a.p, seq, gi_l / per), in_l = id_l < 0 ? 0 : id_l;
         u32x4 ka[2 * KP], va[VU], kb[2 * KP], vb[VU];
         auto at = [&](float x, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
-        auto id_at = [&](int i) { return __builtin_amdgcn_readlane(id_l, i); };
+        auto id_at = [&](int i) { return __builtin_amdgcn_readlane(in_l, i); };
         auto gi_at = [&](int i) { return __builtin_amdgcn_readlane(gi_l, i); };
         load(ka, va, id_at(0), gi_at(0));
+        const float2 sc = *(const float2 *)(a.p.scales + ((int64_t)in_l * a.p.kv_heads + h) * 2);
+        if (b == 0) {
+            query_terms(q, raw);
+            cq = a.scale * 1.4426950408889634f * q.down;
+        }
+        // a page outside the pool: page 0's codes under scales of NaN
+        const GranuleScales sc_l = granule_scales(id_l < 0 ? NAN : sc.x, id_l < 0 ? NAN : sc.y);
         for (int i = 0; i < n; i += 2) {
             if (i + 1 < n) load(kb, vb, id_at(i + 1), gi_at(i + 1));
             compute(ka, va, gi_at(i), GranuleScales{at(sc_l.key, i), at(sc_l.bias, i), at(sc_l.inverse, i)});
@@ -170,7 +175,8 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
         l_s[wave][c] = l;
     }
 #pragma unroll
-    for (int d = 0; d < DV / 16; d++) *(floatx4 *)&o_s[wave][c][16 * d + 4 * g] = o[d];
+    for (int d = 0; d < DV / 16; d++)
+        if (c < plan.cols) *(floatx4 *)&o_s[(wave * plan.cols + c) * OS + 16 * d + 4 * g] = o[d];
     __syncthreads();
     const int64_t item = ((((int64_t)seq * a.p.kv_heads + h) * plan.tiles + tile) * plan.splits + split) * plan.cols;
     for (int e = tid; e < plan.cols * (DV / 4); e += NW * 64) {
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
 #pragma unroll
         for (int w = 0; w < NW; w++) {
             const float f = __builtin_amdgcn_exp2f(m_s[w][cc] - mm);
-            sum += *(const floatx4 *)&o_s[w][cc][d] * f;
+            sum += *(const floatx4 *)&o_s[(w * plan.cols + cc) * OS + d] * f;
             den += l_s[w][cc] * f;
         }
         if (plan.splits > 1) {
@@ -198,29 +204,53 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     }
 }
 
-// The splits of a tile joined: a workgroup a tile.
+// The splits of a query joined: a workgroup a query of a tile. Each group of
+// dv / 4 threads (4 dims a thread) adds every 256 / (dv / 4)-th split, eight
+// in flight; the groups' sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsPlan plan) {
-    const int64_t blk = blockIdx.x;
-    const int tile = (int)(blk % plan.tiles), h = (int)(blk / plan.tiles % a.p.kv_heads),
-              seq = (int)(blk / plan.tiles / a.p.kv_heads);
+    __shared__ float f_s[MOST_SPLITS], part[8];
+    __shared__ __attribute__((aligned(16))) float o_s[256 * 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int64_t blk = blockIdx.x;
+    const int cc = (int)(blk % plan.cols);
+    blk /= plan.cols;
+    const int64_t item = blk * plan.splits * plan.cols + cc;
+    const int tile = (int)(blk % plan.tiles);
+    blk /= plan.tiles;
+    const int h = (int)(blk % a.p.kv_heads), seq = (int)(blk / a.p.kv_heads);
+    // the splits' maxima, factors and denominators
+    const bool has = tid < plan.splits;
+    const float2 st = has ? *(const float2 *)(plan.stats + (item + (int64_t)tid * plan.cols) * 2) : make_float2(M_NONE, 0.f);
     const SeqRows r = seq_rows(a.b, seq);
-    const int group = a.heads / a.p.kv_heads;
-    const int64_t item = blk * plan.splits * plan.cols;
-    for (int e = threadIdx.x; e < plan.cols * a.p.vd; e += 256) {
-        const int cc = e / a.p.vd, d = e % a.p.vd, qq = tile * 16 + cc, i = qq / group;
-        if (i >= r.live) break;
-        float mm = M_NONE, num = 0.f, den = 0.f;
-        for (int s = 0; s < plan.splits; s++) mm = fmaxf(mm, plan.stats[(item + (int64_t)s * plan.cols + cc) * 2]);
-        for (int s = 0; s < plan.splits; s++) {
-            const int64_t at = item + (int64_t)s * plan.cols + cc;
-            const float f = __builtin_amdgcn_exp2f(plan.stats[at * 2] - mm);
-            num += plan.sums[at * a.p.dv + d] * f;
-            den += plan.stats[at * 2 + 1] * f;
-        }
-        ((T *)a.out.data)[(int64_t)(r.row + i) * a.out.stride + (int64_t)(h * group + qq % group) * a.p.vd + d] =
-            (T)(num / den);
+    const int group = a.heads / a.p.kv_heads, qq = tile * 16 + cc, i = qq / group;
+    if (i >= r.live) return;
+    float m = st.x;
+    for (int w = 32; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+    if (lane == 0) part[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const float f = __builtin_amdgcn_exp2f(st.x - m);
+    if (has) f_s[tid] = f;
+    float l = has ? st.y * f : 0.f;
+    for (int w = 32; w > 0; w >>= 1) l += __shfl_xor(l, w, 64);
+    if (lane == 0) part[4 + wave] = l;
+    __syncthreads();
+    const int quads = a.p.dv / 4, groups = 256 / quads, mine = tid / quads, d = tid % quads * 4;
+    floatx4 o{0.f, 0.f, 0.f, 0.f};
+    if (mine < groups) {
+        const float *p = plan.sums + item * a.p.dv + d;
+        const int64_t step = (int64_t)plan.cols * a.p.dv;
+#pragma unroll 8
+        for (int s = mine; s < plan.splits; s += groups) o += *(const floatx4 *)(p + s * step) * f_s[s];
+        *(floatx4 *)&o_s[mine * a.p.dv + d] = o;
     }
+    __syncthreads();
+    if (tid >= a.p.vd) return;
+    float num = 0.f;
+    for (int w = 0; w < groups; w++) num += o_s[w * a.p.dv + tid];
+    ((T *)a.out.data)[(int64_t)(r.row + i) * a.out.stride + (int64_t)(h * group + qq % group) * a.p.vd + tid] =
+        (T)(num / (part[4] + part[5] + part[6] + part[7]));
 }
 
 // ---------------------------------------------------------------------------
@@ -236,10 +266,20 @@ static RowsPlan rows_plan(const PoolView &p, const BatchView &b, int heads, uint
     int64_t keys = b.max_len;
     if (window) keys = std::min<int64_t>(keys, (int64_t)window + 16 + sinks + 2 * GRANULE);
     const int64_t granules = (keys + GRANULE - 1) / GRANULE;
-    const int64_t blocks = (int64_t)b.n_seqs * p.kv_heads * plan.tiles;
-    int64_t splits = (1024 + blocks - 1) / blocks;
-    splits = std::min(splits, (granules + 7) / 8);
-    plan.splits = (int)std::max<int64_t>(splits, 1);
+    const int64_t items = (int64_t)b.n_seqs * p.kv_heads * plan.tiles;
+    // Waves. 2048 (two a SIMD) saturate the memory: 64 sequences of up to 8192
+    // tokens of 8 heads of 128 take 137 us with 512 tiles of 4 waves, 139 us
+    // with twice the waves. A tile's first 8 waves share a workgroup, more go
+    // to further workgroups and need the join, about 4 us; a granule takes a
+    // wave about 0.4 us where latency counts, so up to 12 granules a wave one
+    // workgroup is ahead (36 granules of a window, 96 tiles: 10.9 us against
+    // 13.7 split; 4063 granules, 4 tiles: 34 us split). Four waves where the
+    // registers of larger heads allow no more.
+    const int64_t waves = std::min((2048 + items - 1) / items, granules);
+    plan.waves = waves <= 4 || p.dk > 128 ? 4 : 8;
+    plan.splits = 1;
+    if (waves > plan.waves && granules > 12 * plan.waves)
+        plan.splits = (int)std::min<int64_t>((waves + plan.waves - 1) / plan.waves, MOST_SPLITS);
     return plan;
 }
 
@@ -251,10 +291,17 @@ size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int head
     return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 2) * 4;
 }
 
+template <typename T, int KIND, int DK, int DV, int NW>
+static void rows_waves(const PagesAttention &a, const RowsPlan &plan, unsigned blocks, hipStream_t s) {
+    hipLaunchKernelGGL((pages_rows_kernel<T, KIND, DK, DV, NW>), dim3(blocks), dim3(NW * 64),
+                       (unsigned)(NW * plan.cols * (DV + 4) * 4), s, a, plan);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
 template <typename T, int KIND, int DK, int DV>
 static void rows_dims(const PagesAttention &a, const RowsPlan &plan, unsigned blocks, hipStream_t s) {
-    hipLaunchKernelGGL((pages_rows_kernel<T, KIND, DK, DV, 4>), dim3(blocks), dim3(256), 0, s, a, plan);
-    DITCH_TRY_HIP(hipGetLastError());
+    if (plan.waves == 4) rows_waves<T, KIND, DK, DV, 4>(a, plan, blocks, s);
+    else if constexpr (DK <= 128) rows_waves<T, KIND, DK, DV, 8>(a, plan, blocks, s);
 }
 
 template <typename T, int KIND>
@@ -269,12 +316,12 @@ static void rows_kind(const PagesAttention &a, const RowsPlan &plan, unsigned bl
 template <typename T>
 static void rows_typed(const PagesAttention &a, const RowsPlan &plan, hipStream_t s) {
     const int64_t tiles = (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles;
-    DITCH_CHECK(tiles * plan.splits < ((int64_t)1 << 24), DITCH_INVALID_ARGUMENT,
+    DITCH_CHECK(tiles * std::max(plan.splits, plan.cols) < ((int64_t)1 << 24), DITCH_INVALID_ARGUMENT,
                 "kv attention: more work than one launch holds");
     if (a.p.kind == DITCH_KV_INT8) rows_kind<T, DITCH_KV_INT8>(a, plan, (unsigned)(tiles * plan.splits), s);
     else rows_kind<T, DITCH_KV_E4M3>(a, plan, (unsigned)(tiles * plan.splits), s);
     if (plan.splits > 1) {
-        hipLaunchKernelGGL((pages_join_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, s, a, plan);
+        hipLaunchKernelGGL((pages_join_kernel<T>), dim3((unsigned)(tiles * plan.cols)), dim3(256), 0, s, a, plan);
         DITCH_TRY_HIP(hipGetLastError());
     }
 }
