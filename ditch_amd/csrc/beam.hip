@@ -1,114 +1,457 @@
 // beam.hip — the beam step: the k best continuations over beams and vocabulary.
+//
+// score(beam, token) = prev[beam] + x[beam][token] - log sum exp x[beam]. Within
+// a beam the order is that of the logits, so one pass over them is enough: a
+// workgroup takes a chunk of a row into registers, forms its maximum, the sum
+// of exponentials relative to it, and its k best logits; a second kernel joins
+// the chunks of a prompt's beams, forms the scores in 64 bits and takes the k
+// best of beams x chunks x k.
+//
+// The k best of a wave's part: with the maxima of its 128 half lanes, any
+// threshold that k of them reach is reached by the k best, and by few
+// others; it is found by bisection with ballots. What reaches it goes to a
+// list, or, should that be more than the list holds (many equal logits, the
+// best in few lanes), exactly the k best do, by bisection over the elements.
 #include "pages.h"
 
 namespace ditch {
 
-// An order of f64 scores as unsigned keys: larger key = better, NaN last.
+constexpr int BEAM_MOST_K = 128, BEAM_MOST_BEAMS = 64;
+constexpr int LIST = 256;          // candidates of a wave
+constexpr uint32_t NO_TOKEN = ~0u;  // an unused candidate
+
+// An order of logits as unsigned keys: larger key = larger logit, NaN last
+// (0), both zeros the same.
+__device__ __forceinline__ uint32_t logit_key(float x) {
+    if (!(x == x)) return 0;
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
 __device__ __forceinline__ uint64_t score_key(double x) {
     if (!(x == x)) return 0;
-    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b >> 63 ? ~b : b | ((uint64_t)1 << 63);
 }
+
+// e^d for d <= 0, within about an ulp: 2^n 2^f with d log2(e) = n + f
+__device__ __forceinline__ float exp_below(float d) {
+    d = d < -150.f ? -150.f : d;  // (a NaN stays)
+    const float n = rintf(d * 1.44269504f);
+    float f = __builtin_fmaf(d, 1.44269502162933349609375f, -n);  // log2(e) in two parts
+    f = __builtin_fmaf(d, 1.92596299112661746887e-8f, f);
+    return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
+
+struct Candidate {
+    float x;
+    uint32_t token;
+};
 
 struct BeamArgs {
     float *scores;
     int32_t *parents;
     uint32_t *tokens;
     const float *logits, *prev;
-    double *lse;  // [prompts][beams]
-    int32_t beams, k;
+    Candidate *list;  // [rows][chunks][k]
+    double *stats;    // [rows][chunks][2]: maximum, sum of exponentials relative to it
+    int32_t beams, k, chunks;
     int64_t vocab;
 };
 
-// log sum exp of a row: the f32 maximum, f64 sum
-__global__ __launch_bounds__(1024) void beam_lse_kernel(BeamArgs a) {
-    __shared__ double part[16];
-    const float *x = a.logits + (int64_t)blockIdx.x * a.vocab;
-    const int tid = threadIdx.x;
-    float m = -INFINITY;
-    for (int64_t i = tid; i < a.vocab; i += 1024) m = fmaxf(m, x[i]);
+// A workgroup of 4 waves a chunk of 256 R quads of a row.
+template <int R>
+__global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
+    __shared__ Candidate list[4][LIST];
+    __shared__ int count_s[4];
+    __shared__ float m_s[4];
+    __shared__ double sum_s[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x / a.chunks;
+    const int chunk = (int)(blockIdx.x % a.chunks), k = a.k;
+    const float *x = a.logits + row * a.vocab;
+    // quads at 16-byte addresses: quad q holds tokens 4 q - shift + 0..3
+    const int shift = (int)((uintptr_t)x / 4 % 4), V = (int)a.vocab;
+    const int64_t q0 = ((int64_t)chunk * 4 + wave) * R * 64 + lane;
+    const int64_t t0 = q0 * 4 - shift;  // the lane's first token; quad r's is 256 r further
+    float v[R][4];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int64_t t = t0 + 256 * r;
+        if (t >= 0 && t + 4 <= V) {
+            const float4 f = *(const float4 *)(x + t);
+            v[r][0] = f.x;
+            v[r][1] = f.y;
+            v[r][2] = f.z;
+            v[r][3] = f.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[r][j] = t + j >= 0 && t + j < V ? x[t + j] : -INFINITY;
+        }
+    }
+    auto valid = [&](int r, int j) {
+        const int64_t t = t0 + 256 * r + j;
+        return t >= 0 && t < V;
+    };
+    // the half lanes' maxima, the wave's, and its sum
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) top[r >= R / 2] = fmaxf(top[r >= R / 2], v[r][j]);
+    float m = fmaxf(top[0], top[1]);
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((tid & 63) == 0) part[tid >> 6] = m;
-    __syncthreads();
-    for (int w = 0; w < 16; w++) m = fmaxf(m, (float)part[w]);
-    __syncthreads();
     double sum = 0;
-    for (int64_t i = tid; i < a.vocab; i += 1024) sum += (double)expf(x[i] - m);
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((tid & 63) == 0) part[tid >> 6] = sum;
-    __syncthreads();
-    if (tid == 0) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = exp_below(v[r][j] - m);
+        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+    }
+    // (a wave of -infinities or past the row has no sum; a NaN shows in it)
+    bool nan = false;
+    if (m == -INFINITY) {
         sum = 0;
-        for (int w = 0; w < 16; w++) sum += part[w];
-        a.lse[blockIdx.x] = (double)m + log(sum);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) nan |= v[r][j] != v[r][j];
+        if (nan) sum = NAN;
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+
+    // the wave's tokens, and how many of them the list needs
+    const int64_t first = ((int64_t)chunk * 4 + wave) * R * 256 - shift;
+    const int64_t lo = first < 0 ? 0 : first, hi = first + R * 256 < V ? first + R * 256 : V;
+    const int have = hi > lo ? (int)(hi - lo) : 0, need = have < k ? have : k;
+    int count = 0;
+    bool done = need == 0;
+    if (!done && need == k) {
+        const uint32_t k0 = logit_key(top[0]), k1 = logit_key(top[1]);
+        uint32_t a0 = k0 < k1 ? k0 : k1, b0 = k0 < k1 ? k1 : k0;
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t u = __shfl_xor(a0, o, 64), w = __shfl_xor(b0, o, 64);
+            a0 = u < a0 ? u : a0;
+            b0 = w > b0 ? w : b0;
+        }
+        // at `low` all 128 half lanes reach the threshold; `high` is the largest
+        uint32_t low = a0, high = b0;
+        while (low < high) {
+            const uint32_t mid = low + (high - low + 1) / 2;
+            const int c = __popcll(__ballot(k0 >= mid)) + __popcll(__ballot(k1 >= mid));
+            if (c >= k) {
+                low = mid;
+                if (c <= k + k / 4 + 2) break;
+            } else high = mid - 1;
+        }
+        // (low's logit; the key of a half lane without one is that of -infinity)
+        const float tau = low >> 31 ? __uint_as_float(low & 0x7fffffffu) : __uint_as_float(~low);
+        done = true;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool in = v[r][j] >= tau && valid(r, j);
+                const uint64_t b = __ballot(in);
+                if (b) {
+                    const int at = count + __popcll(b & (((uint64_t)1 << lane) - 1));
+                    if (in && at < LIST) list[wave][at] = Candidate{v[r][j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
+                    count += __popcll(b);
+                }
+            }
+        done = count >= k && count <= LIST;
+    }
+    if (!done) {
+        // exactly the `need` best: the largest key that as many reach, those
+        // above it, and the first equal ones (read again: the registers are
+        // not indexed at run time)
+        uint32_t low = 0, high = ~0u;
+        auto logit = [&](int r, int j, bool &in) {
+            const int64_t t = t0 + 256 * r + j;
+            in = t >= 0 && t < V;
+            return in ? x[t] : 0.f;
+        };
+        auto reach = [&](uint32_t key) {
+            int c = 0;
+#pragma unroll 1
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    bool in;
+                    const float f = logit(r, j, in);
+                    c += __popcll(__ballot(in && logit_key(f) >= key));
+                }
+            return c;
+        };
+        while (low < high) {
+            const uint32_t mid = low + (high - low) / 2 + 1;
+            if (reach(mid) >= need) low = mid;
+            else high = mid - 1;
+        }
+        const int above = low == ~0u ? 0 : reach(low + 1);
+        int equal = need - above, put = 0;
+#pragma unroll 1
+        for (int r = 0; r < R; r++) {
+            // index order: lane after lane, each lane's four
+            uint64_t bg[4], be[4];
+            float f[4];
+            int eq = 0, gt = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bool in;
+                f[j] = logit(r, j, in);
+                const uint32_t key = logit_key(f[j]);
+                bg[j] = __ballot(in && key > low);
+                be[j] = __ballot(in && key == low);
+                eq += __popcll(be[j]);
+                gt += __popcll(bg[j]);
+            }
+            const uint64_t bit = (uint64_t)1 << lane, before = bit - 1;
+            int e = 0, g = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                e += __popcll(be[j] & before);
+                g += __popcll(bg[j] & before);
+            }
+            const int take = eq < equal ? eq : equal;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool is_e = be[j] & bit, is_g = bg[j] & bit;
+                const Candidate c{f[j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
+                if (is_g) list[wave][put + g] = c;
+                if (is_e && e < take) list[wave][put + gt + e] = c;
+                g += is_g;
+                e += is_e;
+            }
+            put += gt + take;
+            equal -= take;
+        }
+        count = need;
+    }
+    if (lane == 0) {
+        count_s[wave] = count;
+        m_s[wave] = m;
+        sum_s[wave] = sum;
+    }
+    __syncthreads();
+    // the workgroup's k best by their ranks among its waves' candidates
+    const int n0 = count_s[0], n1 = count_s[1], n2 = count_s[2], n3 = count_s[3], n = n0 + n1 + n2 + n3;
+    Candidate *out = a.list + (int64_t)blockIdx.x * k;
+    for (int e = tid; e < n; e += 256) {
+        const int w = e < n0 ? 0 : e < n0 + n1 ? 1 : e < n0 + n1 + n2 ? 2 : 3;
+        const Candidate c = list[w][e - (w > 0 ? n0 : 0) - (w > 1 ? n1 : 0) - (w > 2 ? n2 : 0)];
+        const uint32_t key = logit_key(c.x);
+        int rank = 0;
+        for (int u = 0; u < 4; u++)
+            for (int i = 0; i < count_s[u]; i++) {
+                const Candidate o = list[u][i];
+                const uint32_t ok = logit_key(o.x);
+                rank += ok > key || (ok == key && o.token < c.token);
+            }
+        if (rank < k) out[rank] = c;
+    }
+    for (int e = n + tid; e < k; e += 256) out[e] = Candidate{0.f, NO_TOKEN};
+    if (tid == 0) {
+        const float mm = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+        double total = 0;
+        for (int w = 0; w < 4; w++)
+            total += m_s[w] == -INFINITY ? sum_s[w] : sum_s[w] * exp((double)m_s[w] - (double)mm);
+        a.stats[(int64_t)blockIdx.x * 2] = mm;
+        a.stats[(int64_t)blockIdx.x * 2 + 1] = total;
     }
 }
 
-// k times the best continuation behind the last one
-__global__ __launch_bounds__(1024) void beam_pick_kernel(BeamArgs a) {
-    __shared__ uint64_t key_s[16];
-    __shared__ int64_t at_s[16];
-    const int tid = threadIdx.x;
-    const int64_t prompt = blockIdx.x, n = a.beams * a.vocab;
-    uint64_t last = ~(uint64_t)0;
-    int64_t last_at = -1;
-    for (int j = 0; j < a.k; j++) {
-        uint64_t best = 0;
-        int64_t at = n;
-        for (int64_t i = tid; i < n; i += 1024) {
-            const int b = (int)(i / a.vocab);
-            const double s = (double)a.prev[prompt * a.beams + b] +
-                             ((double)a.logits[prompt * n + i] - a.lse[prompt * a.beams + b]);
-            const uint64_t key = score_key(s);
-            if ((key < last || (key == last && i > last_at)) && (at == n || key > best)) {
-                best = key;
-                at = i;
-            }
+// A workgroup a prompt.
+constexpr int JOIN = 1024, HELD = 4;  // threads; candidates a thread holds in registers
+__global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
+    __shared__ double lse_s[BEAM_MOST_BEAMS], prev_s[BEAM_MOST_BEAMS];
+    __shared__ uint64_t lo_s[16], hi_s[16];
+    __shared__ int count_s[2][16];
+    __shared__ int put;
+    __shared__ uint64_t key_s[BEAM_MOST_K], tie_s[BEAM_MOST_K];
+    __shared__ uint32_t token_s[BEAM_MOST_K];
+    __shared__ float score_s[BEAM_MOST_K];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
+    const int64_t row0 = (int64_t)blockIdx.x * a.beams;
+    for (int b = wave; b < a.beams; b += JOIN / 64) {
+        double m = -INFINITY, sum = 0;
+        const double *st = a.stats + (row0 + b) * a.chunks * 2;
+        for (int c = lane; c < a.chunks; c += 64) m = fmax(m, st[2 * c]);
+        for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+        for (int c = lane; c < a.chunks; c += 64) {
+            const double cm = st[2 * c], cs = st[2 * c + 1];
+            sum += cm == -INFINITY ? cs : cs * exp(cm - m);
         }
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t ok = __shfl_xor(best, o, 64);
-            const int64_t oa = __shfl_xor(at, o, 64);
-            if (oa < n && (at == n || ok > best || (ok == best && oa < at))) {
-                best = ok;
-                at = oa;
-            }
-        }
-        if ((tid & 63) == 0) {
-            key_s[tid >> 6] = best;
-            at_s[tid >> 6] = at;
-        }
-        __syncthreads();
-        best = key_s[0];
-        at = at_s[0];
-        for (int w = 1; w < 16; w++)
-            if (at_s[w] < n && (at == n || key_s[w] > best || (key_s[w] == best && at_s[w] < at))) {
-                best = key_s[w];
-                at = at_s[w];
-            }
-        __syncthreads();
-        last = best;
-        last_at = at;
-        if (tid == 0) {
-            const int b = (int)(at / a.vocab);
-            a.parents[prompt * a.k + j] = b;
-            a.tokens[prompt * a.k + j] = (uint32_t)(at % a.vocab);
-            a.scores[prompt * a.k + j] = (float)((double)a.prev[prompt * a.beams + b] +
-                                                 ((double)a.logits[prompt * n + at] - a.lse[prompt * a.beams + b]));
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (lane == 0) {
+            lse_s[b] = m == -INFINITY || m == INFINITY ? NAN : m + log(sum);
+            prev_s[b] = (double)a.prev[row0 + b];
         }
     }
+    if (tid == 0) put = 0;
+    __syncthreads();
+
+    const int per = a.chunks * k;
+    const int64_t n = (int64_t)a.beams * per;
+    const Candidate *list = a.list + row0 * per;
+    struct Item {
+        uint64_t key, tie;  // tie: beam, then the logit, inverted: smaller first
+        uint32_t token;
+        float score;
+    };
+    auto item = [&](int64_t e) {
+        const Candidate c = list[e];
+        const int b = (int)(e / per);
+        const double s = prev_s[b] + ((double)c.x - lse_s[b]);
+        return Item{score_key(s), (uint64_t)b << 32 | (uint32_t)~logit_key(c.x), c.token, (float)s};
+    };
+    Item held[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; j++) {
+        held[j] = Item{0, 0, NO_TOKEN, 0.f};
+        if (tid + (int64_t)JOIN * j < n) held[j] = item(tid + (int64_t)JOIN * j);
+    }
+    auto each = [&](auto &&f) {
+#pragma unroll
+        for (int j = 0; j < HELD; j++)
+            if (held[j].token != NO_TOKEN) f(held[j]);
+        for (int64_t e = tid + (int64_t)JOIN * HELD; e < n; e += JOIN) {
+            const Item it = item(e);
+            if (it.token != NO_TOKEN) f(it);
+        }
+    };
+    int turn = 0;
+    // how many candidates the predicate takes, over the workgroup
+    auto count = [&](auto &&takes) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < HELD; j++) c += __popcll(__ballot(held[j].token != NO_TOKEN && takes(held[j])));
+        for (int64_t e = (int64_t)JOIN * HELD; e < n; e += JOIN) {
+            Item it{0, 0, NO_TOKEN, 0.f};
+            if (e + tid < n) it = item(e + tid);
+            c += __popcll(__ballot(it.token != NO_TOKEN && takes(it)));
+        }
+        if (lane == 0) count_s[turn][wave] = c;
+        __syncthreads();
+        c = 0;
+#pragma unroll
+        for (int w = 0; w < JOIN / 64; w++) c += count_s[turn][w];
+        turn ^= 1;
+        return c;
+    };
+    // the k-th largest score: between the least of the threads' largest (as
+    // many threads as have candidates, or k, reach it) and the largest
+    uint64_t low = ~(uint64_t)0, high = 0;
+    {
+        uint64_t mine = 0;
+        bool any = false;
+        each([&](const Item &it) {
+            mine = it.key > mine ? it.key : mine;
+            any = true;
+        });
+        low = any ? mine : low;
+        high = mine;
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t u = __shfl_xor(low, o, 64), w = __shfl_xor(high, o, 64);
+            low = u < low ? u : low;
+            high = w > high ? w : high;
+        }
+        if (lane == 0) {
+            lo_s[wave] = low;
+            hi_s[wave] = high;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < JOIN / 64; w++) {
+            low = lo_s[w] < low ? lo_s[w] : low;
+            high = hi_s[w] > high ? hi_s[w] : high;
+        }
+    }
+    if (count([&](const Item &it) { return it.key >= low; }) < k) low = 0;
+    int reach = 0;
+    while (low < high) {
+        const uint64_t mid = low + (high - low) / 2 + 1;
+        const int c = count([&](const Item &it) { return it.key >= mid; });
+        if (c >= k) {
+            low = mid;
+            reach = c;
+            if (c == k) break;
+        } else high = mid - 1;
+    }
+    // among equal scores the lowest beams, in a beam the largest logits, among equal logits the lowest tokens
+    uint64_t tie = ~(uint64_t)0;
+    uint32_t token = ~0u;
+    if (reach != k) {
+        int need = k - count([&](const Item &it) { return it.key > low; });
+        uint64_t l = 0, h = ((uint64_t)BEAM_MOST_BEAMS << 32) - 1;
+        while (l < h) {
+            const uint64_t mid = l + (h - l) / 2;
+            if (count([&](const Item &it) { return it.key == low && it.tie <= mid; }) >= need) h = mid;
+            else l = mid + 1;
+        }
+        tie = l;
+        need -= count([&](const Item &it) { return it.key == low && it.tie < tie; });
+        uint32_t tl = 0, th = (uint32_t)a.vocab - 1;
+        while (tl < th) {
+            const uint32_t mid = tl + (th - tl) / 2;
+            if (count([&](const Item &it) { return it.key == low && it.tie == tie && it.token <= mid; }) >= need) th = mid;
+            else tl = mid + 1;
+        }
+        token = tl;
+    }
+    each([&](const Item &it) {
+        if (it.key > low || (it.key == low && (it.tie < tie || (it.tie == tie && it.token <= token)))) {
+            const int at = atomicAdd(&put, 1);
+            if (at < k) {
+                key_s[at] = it.key;
+                tie_s[at] = it.tie;
+                token_s[at] = it.token;
+                score_s[at] = it.score;
+            }
+        }
+    });
+    __syncthreads();
+    // exactly k, in any order: each goes to its rank
+    if (tid < k) {
+        const uint64_t key = key_s[tid], t = tie_s[tid];
+        const uint32_t tok = token_s[tid];
+        int rank = 0;
+        for (int i = 0; i < k; i++)
+            rank += key_s[i] > key || (key_s[i] == key && (tie_s[i] < t || (tie_s[i] == t && token_s[i] < tok)));
+        const int64_t o = (int64_t)blockIdx.x * k + rank;
+        a.scores[o] = score_s[tid];
+        a.parents[o] = (int32_t)(t >> 32);
+        a.tokens[o] = tok;
+    }
+}
+
+// Chunks of 8192 logits; of 16384 once they fill the chip (their lists are
+// half as many, and so is the bisection's share).
+static int beam_quads(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)1024 * 16384 ? 16 : 8; }
+static int64_t beam_chunks(int64_t rows, int64_t vocab) {
+    const int64_t per = beam_quads(rows, vocab) * 1024;
+    return (vocab + 3 + per - 1) / per;  // (a row may start 3 tokens into its first quad)
 }
 
 size_t beam_select_workspace(int64_t prompts, int64_t beams, int64_t vocab, int64_t k) {
-    return (size_t)(prompts * beams) * sizeof(double);
+    const int64_t chunks = beam_chunks(prompts * beams, vocab);
+    return (size_t)(prompts * beams * chunks) * (k * sizeof(Candidate) + 2 * sizeof(double));
 }
 
 void launch_beam_select(float *scores, int32_t *parents, uint32_t *tokens, const float *logits, const float *prev,
                         int64_t prompts, int64_t beams, int64_t vocab, int64_t k, void *ws, size_t ws_bytes,
                         hipStream_t s) {
-    const BeamArgs a{scores, parents, tokens, logits, prev, (double *)ws, (int32_t)beams, (int32_t)k, vocab};
-    hipLaunchKernelGGL(beam_lse_kernel, dim3((unsigned)(prompts * beams)), dim3(1024), 0, s, a);
+    const int64_t rows = prompts * beams, chunks = beam_chunks(rows, vocab);
+    DITCH_CHECK(rows * chunks < (int64_t)1 << 24, DITCH_INVALID_ARGUMENT, "beam select: more logits than one launch holds");
+    double *stats = (double *)ws;
+    const BeamArgs a{scores, parents, tokens, logits, prev, (Candidate *)(stats + rows * chunks * 2), stats,
+                     (int32_t)beams, (int32_t)k, (int32_t)chunks, vocab};
+    if (beam_quads(rows, vocab) == 16)
+        hipLaunchKernelGGL(beam_chunk_kernel<16>, dim3((unsigned)(rows * chunks)), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL(beam_chunk_kernel<8>, dim3((unsigned)(rows * chunks)), dim3(256), 0, s, a);
     DITCH_TRY_HIP(hipGetLastError());
-    hipLaunchKernelGGL(beam_pick_kernel, dim3((unsigned)prompts), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)prompts), dim3(JOIN), 0, s, a);
     DITCH_TRY_HIP(hipGetLastError());
 }
 

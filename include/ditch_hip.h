@@ -749,9 +749,10 @@ int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, in
 
 /* The beam step: of each prompt's beams x vocab continuations, scored
  * d_prev[prompt][beam] + log_softmax(d_logits[prompt][beam])[token], the k
- * best, highest first, the lower (beam, token) first among equals: scores
- * f32 [n_prompts][k], parents (beam) and tokens. Scores are formed in 64
- * bits. A beam whose previous score is -infinity comes after every finite
+ * best, highest first: scores f32 [n_prompts][k], parents (beam) and tokens.
+ * A beam's continuations are in the order of its logits, equal ones by the
+ * lower token; beams are compared by scores formed in 64 bits, the lower
+ * beam first among equals. A beam whose previous score is -infinity comes after every finite
  * one; a beam without probabilities (a NaN or +infinity among its logits,
  * or nothing above -infinity; a NaN previous score) scores NaN and comes
  * last. 1 <= beams <= 64, 1 <= k <= 128 and k <= beams * vocab. `ws`:

@@ -1,9 +1,10 @@
 """The beam step against its definition in 64 bits.
 
-The kernel's log sum exp adds f32 exponentials (each within 2^-22 of its
-value) in 64 bits, so a score is within 2^-22 + 2^-24 * |score| of the exact
-one; the choice is compared for equality with inputs whose scores are
-further apart than that, or tie exactly."""
+The kernel forms d = logit - maximum in f32 (off by 2^-24 |d| at most) and
+e^d within 2^-22, adds four in f32 (2 * 2^-24) and the rest in 64 bits: the log
+sum exp is off by the mean of (2^-24 |d| + 2^-21) weighted with e^d. A score
+adds its rounding to f32, 2^-24 of it. The choice is compared for equality,
+with inputs whose scores are further apart than that, or tie exactly."""
 import numpy as np
 import pytest
 
@@ -14,16 +15,20 @@ pytestmark = pytest.mark.gpu
 
 
 def _plain(logits, prev, k):
-    """logits [prompts][beams][vocab], prev [prompts][beams]: scores, parents, tokens [prompts][k]."""
+    """logits [prompts][beams][vocab], prev [prompts][beams]: scores, parents, tokens, bounds [prompts][k]."""
     x = logits.astype(np.float64)
     with np.errstate(all="ignore"):
         m = x.max(-1, keepdims=True)
-        total = prev.astype(np.float64)[..., None] + (x - (m + np.log(np.exp(x - m).sum(-1, keepdims=True))))
+        e = np.exp(x - m)
+        total = prev.astype(np.float64)[..., None] + (x - (m + np.log(e.sum(-1, keepdims=True))))
+        off = np.where(e > 0, np.abs(x - m), 0) * 2.0 ** -24 + 2.0 ** -21
+        off = ((off * e).sum(-1) / e.sum(-1)).reshape(len(x), -1)
     out = []
-    for t in total.reshape(len(x), -1):
-        key = np.where(np.isnan(t), -np.inf, t)
-        order = np.lexsort((np.arange(t.size), -key, np.isnan(t)))[:k]
-        out.append((t[order], order // x.shape[2], order % x.shape[2]))
+    for p, t in enumerate(total.reshape(len(x), -1)):
+        beam, token, logit = np.arange(t.size) // x.shape[2], np.arange(t.size) % x.shape[2], x[p].reshape(-1)
+        order = np.lexsort((token, -np.where(np.isnan(logit), -np.inf, logit), np.isnan(logit), beam,
+                            -np.where(np.isnan(t), -np.inf, t), np.isnan(t)))[:k]
+        out.append((t[order], beam[order], token[order], off[p][beam[order]]))
     return tuple(np.stack(a) for a in zip(*out))
 
 
@@ -47,13 +52,13 @@ def _select(dev, logits, prev, k, stream=None):
 
 def _check(dev, logits, prev, k):
     s, p, t = _select(dev, logits, prev, k)
-    ws, wp, wt = _plain(logits, prev, k)
+    ws, wp, wt, off = _plain(logits, prev, k)
     np.testing.assert_array_equal(p, wp)
     np.testing.assert_array_equal(t, wt)
     np.testing.assert_array_equal(np.isnan(s), np.isnan(ws))
     fine = np.isfinite(ws)
     np.testing.assert_array_equal(s[~fine & ~np.isnan(ws)], ws[~fine & ~np.isnan(ws)])
-    assert (np.abs(s[fine] - ws[fine]) <= 2.0 ** -22 + 2.0 ** -24 * np.abs(ws[fine])).all()
+    assert (np.abs(s[fine] - ws[fine]) <= off[fine] + 2.0 ** -24 * np.abs(ws[fine])).all()
 
 
 SHAPES = [(1, 1, 1, 1), (1, 4, 151936, 8), (3, 8, 1000, 16), (2, 1, 4097, 1), (5, 3, 17, 51), (2, 64, 300, 128),
