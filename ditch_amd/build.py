@@ -44,7 +44,8 @@ EXTRA = {"gemm_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disab
          "gemm_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "gemm_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"],
          "gemm_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-         "pages_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+         "pages_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "pages_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 # sources compiled more than once: (object name, extra flags) per object

@@ -145,18 +145,24 @@ __device__ __forceinline__ floatx4 scores(const u32x4 *kb, const QueryTile<KP, T
     return s;
 }
 
-// 8 weights as the operand of the values' product.
+// 8 weights as the operand of the values' product, and their sum: of one
+// term what the product really uses, so that a weight's rounding is the same
+// above and below.
 template <int TERMS>
 struct Weights {
     half8 f[TERMS];
 };
 template <int TERMS>
-__device__ __forceinline__ void weight_terms(Weights<TERMS> &w, const float (&x)[8]) {
+__device__ __forceinline__ float weight_terms(Weights<TERMS> &w, const float (&x)[8]) {
     u32x4 hi;
+    float sum = 0.f;
     if constexpr (TERMS == 1) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            hi[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{x[2 * j], x[2 * j + 1]}, half2_t));
+        for (int j = 0; j < 4; j++) {
+            const half2_t h = __builtin_convertvector(floatx2{x[2 * j], x[2 * j + 1]}, half2_t);
+            hi[j] = __builtin_bit_cast(uint32_t, h);
+            sum = __builtin_amdgcn_fdot2(h, half2_t{(_Float16)1.f, (_Float16)1.f}, sum, false);
+        }
         w.f[0] = __builtin_bit_cast(half8, hi);
     } else {
         u32x4 lo;
@@ -166,22 +172,27 @@ __device__ __forceinline__ void weight_terms(Weights<TERMS> &w, const float (&x)
             const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x[2 * j], x[2 * j + 1]));
             hi[j] = __builtin_bit_cast(uint32_t, h);
             lo[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * j] - (float)h[0], x[2 * j + 1] - (float)h[1]));
+            sum += x[2 * j] + x[2 * j + 1];
         }
         w.f[0] = __builtin_bit_cast(half8, hi);
         w.f[1] = __builtin_bit_cast(half8, lo);
     }
+    return sum;
 }
 
-// A granule's scales as the loops use them. A value scale far from 1 (or
-// none: zero) would leave the weights' range in the sum of the denominator,
-// which then adds exp(s_j) itself (`odd`); at zero the values add nothing
-// and `skip` leaves their product out.
+// A granule's scales as the loops use them. A value scale far from 1 would
+// take the denominator's part out of the weights' range, a NaN would reach
+// rows that see none of the granule, and zero has no logarithm: such a
+// granule is `odd` (see odd_granule).
 struct GranuleScales {
     float key, bias, inverse;
 };
 __device__ __forceinline__ GranuleScales granule_scales(float ks, float vs) {
     const bool zero = fabsf(vs) < 1.17549435e-38f;  // (subnormal: the logarithm takes it for zero)
     return {ks, zero ? 0.f : __builtin_amdgcn_logf(vs), zero ? 0.f : 1.f / vs};
+}
+__device__ __forceinline__ bool granule_odd(const GranuleScales &sc) {
+    return sc.inverse == 0.f || !(fabsf(sc.bias) <= BIAS_PLAIN) || !(fabsf(sc.key) <= 3.4028234663852886e38f);
 }
 
 // The rows of a query tile: 16 consecutive (row, head of the KV head's
@@ -210,12 +221,76 @@ __device__ __forceinline__ bool granule_full(const TileRows &t, int gi, int wind
     const int a = gi * GRANULE, z = a + GRANULE - 1;
     return z <= t.t_lo && (!window || a > t.t_hi - window || z < sinks);
 }
-__device__ __forceinline__ bool token_seen(int j, int t, int window, int sinks) {
-    return j <= t && (!window || t - j < window || j < sinks);
+// What a column sees: the tokens first .. first + span (its own position) and
+// those of the first `sinks` that lie before them.
+struct Seen {
+    int first;
+    uint32_t span;
+    int sinks;
+};
+__device__ __forceinline__ Seen seen_from(int t, int window, int sinks) {
+    const int first = window && t - window + 1 > 0 ? t - window + 1 : 0;
+    return {first, (uint32_t)(t - first), sinks < first ? sinks : first};
+}
+__device__ __forceinline__ bool token_seen(int j, const Seen &s) { return (uint32_t)(j - s.first) <= s.span || j < s.sinks; }
+
+// The exponents of a granule's weights for one query tile, less the running
+// maximum: s0, s1 the scores' products (tokens 4 g + i and 16 + 4 g + i of the
+// granule), ck and add what takes them there.
+__device__ __forceinline__ void granule_exponents(float (&w)[8], floatx4 s0, floatx4 s1, float ck, float add) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = __builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], ck, add);
+}
+// Tokens that the column does not see; j0 the lane's first token.
+__device__ __forceinline__ void granule_mask(float (&w)[8], int j0, const Seen &seen) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (!token_seen(j0 + (j < 4 ? j : 12 + j), seen)) w[j] = -INFINITY;
+}
+// (v_max3 itself: fmaxf would quiet each operand first. A NaN is passed over.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+__device__ __forceinline__ float most_of(const float (&w)[8]) {
+    return max3(max3(w[0], w[1], w[2]), max3(w[3], w[4], w[5]), max3(w[6], w[7], w[7]));
+}
+// Moves the running maximum m to the exponents' largest where that passes
+// W_MOST; returns the factor of what was added up under the old one.
+__device__ __forceinline__ float move_maximum(float (&w)[8], floatx4 s0, floatx4 s1, float ck, float bias, bool full, int j0,
+                                              const Seen &seen, float &m) {
+    granule_exponents(w, s0, s1, ck, bias);
+    if (!full) granule_mask(w, j0, seen);
+    const float next = fmaxf(m, max_groups(most_of(w))), f = __builtin_amdgcn_exp2f(m - next);
+    m = next;
+    granule_exponents(w, s0, s1, ck, bias + (W_UP - m));
+    if (!full) granule_mask(w, j0, seen);
+    return f;
+}
+// An odd granule's part of the denominator, from the scores alone: the
+// product's weights then add nothing to it (inverse 0), and under a value
+// scale of zero there are none.
+__device__ __forceinline__ float odd_granule(float (&w)[8], const GranuleScales &sc) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        sum += w[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[j] - sc.bias);
+        if (sc.inverse == 0.f) w[j] = -INFINITY;
+    }
+    return sum;
+}
+// The weights, and their sum.
+template <int TERMS>
+__device__ __forceinline__ float granule_weights(Weights<TERMS> &wt, const float (&w)[8]) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_exp2f(w[j]);
+    return weight_terms<TERMS>(wt, x);
 }
 
 // pages_chunk.hip: many rows a sequence
-bool pages_chunk_takes(const PagesAttention &a);
+bool pages_chunk_takes(const PoolView &p, const BatchView &b, int heads, int32_t dtype);
 void launch_pages_chunk(const PagesAttention &a, hipStream_t s);
 
 }  // namespace ditch

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     const TileRows tr = tile_rows(r, first_row, last_row, a.window, a.sinks);
     const int qi = tile * 16 + c, row = qi / group;
     const bool mine = row < r.live;
-    const int t = mine ? r.pos + row : tr.t_hi;  // the column's position
+    const Seen seen = seen_from(mine ? r.pos + row : tr.t_hi, a.window, a.sinks);
 
     RawQuery<KP> raw;
     load_query(raw, mine ? (const T *)a.q.data + (int64_t)(r.row + row) * a.q.stride +
@@ -88,47 +88,24 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     auto compute = [&](const u32x4 (&kb)[2 * KP], const u32x4 (&vb)[VU], int gi, const GranuleScales &sc) {
         const floatx4 s0 = scores<KIND, KP, TERMS>(kb, q), s1 = scores<KIND, KP, TERMS>(kb + KP, q);
         const float ck = cq * sc.key;
-        float x[8], w[8];
         const bool full = granule_full(tr, gi, a.window, a.sinks);
         const int j0 = gi * GRANULE + 4 * g;
-        auto weigh = [&](float add) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = __builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], ck, add);
-            if (!full)
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (!token_seen(j0 + (j < 4 ? j : 12 + j), t, a.window, a.sinks)) w[j] = -INFINITY;
-        };
-        weigh(sc.bias + (W_UP - m));
-        float most = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
-        if (__any(most > W_MOST)) {
-            weigh(sc.bias);
-            most = max_groups(fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7]))));
-            const float next = fmaxf(m, most), f = __builtin_amdgcn_exp2f(m - next);
-            m = next;
+        float w[8];
+        granule_exponents(w, s0, s1, ck, sc.bias + (W_UP - m));
+        if (!full) granule_mask(w, j0, seen);
+        if (__any(most_of(w) > W_MOST)) {
+            const float f = move_maximum(w, s0, s1, ck, sc.bias, full, j0, seen, m);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DV / 16; d++) o[d] *= f;
-            weigh(sc.bias + (W_UP - m));
         }
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] = __builtin_amdgcn_exp2f(w[j]);
-            sum += x[j];
+        float inverse = sc.inverse;
+        if (granule_odd(sc)) {
+            l += odd_granule(w, sc);
+            inverse = 0.f;
         }
-        if (fabsf(sc.bias) > BIAS_PLAIN) {
-            // a value scale far from 1: the denominator from the scores alone
-            sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) sum += __builtin_amdgcn_exp2f(w[j] - sc.bias);
-        } else if (sc.inverse != 0.f) {
-            sum = sum == 0.f ? 0.f : sum * sc.inverse;
-        }
-        l += sum;
-        if (sc.inverse == 0.f) return;  // values of scale zero
         Weights<TERMS> wt;
-        weight_terms(wt, x);
+        l += granule_weights<TERMS>(wt, w) * inverse;
 #pragma unroll
         for (int d = 0; d < DV / 16; d++) {
             const half8 v = codes_f16<KIND>(vb[d / 2][d % 2 * 2], vb[d / 2][d % 2 * 2 + 1]);
@@ -285,7 +262,7 @@ static RowsPlan rows_plan(const PoolView &p, const BatchView &b, int heads, uint
 
 size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int heads, int32_t dtype, uint32_t window,
                                  uint32_t sinks) {
-    if (b.n_seqs == 0) return 0;
+    if (b.n_seqs == 0 || pages_chunk_takes(p, b, heads, dtype)) return 0;
     const RowsPlan plan = rows_plan(p, b, heads, window, sinks);
     if (plan.splits == 1) return 0;
     return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 2) * 4;
@@ -328,6 +305,7 @@ static void rows_typed(const PagesAttention &a, const RowsPlan &plan, hipStream_
 
 void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, hipStream_t s) {
     if (a.b.n_seqs == 0) return;
+    if (pages_chunk_takes(a.p, a.b, a.heads, a.dtype)) return launch_pages_chunk(a, s);
     RowsPlan plan = rows_plan(a.p, a.b, a.heads, (uint32_t)a.window, (uint32_t)a.sinks);
     if (plan.splits > 1) {
         plan.stats = (float *)ws;
