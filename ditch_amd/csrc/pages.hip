@@ -1,5 +1,6 @@
 // pages.hip — pages of 8-bit keys and values: appending rows (with the
 // position rotation), reading them back, and reordering the beams' states.
+#include <algorithm>
 #include <string>
 
 #include "pages.h"
@@ -153,6 +154,16 @@ __device__ __forceinline__ float code_value(uint8_t c) {
 
 // ---------------------------------------------------------------------------
 // append
+//
+// The new tokens of a (page, head), keys or values, belong to one workgroup.
+// It forms every value in 64 bits twice: for the largest, which gives the
+// scale, and, the rows by then in the caches, for the codes, which it puts in
+// the page's order in LDS; whole granules go out, and the one that holds
+// tokens of before came in first. (Staging the values themselves needs four to
+// eight times the LDS and took 233 us where this takes APPEND_US: 24 sequences
+// of up to 500 f32 rows of 8 heads of 128 and 32 query heads, 360 MB.)
+
+constexpr int TILE = 16384;  // codes staged (the page in parts where it has more)
 
 struct AppendArgs {
     PoolView p;
@@ -161,41 +172,170 @@ struct AppendArgs {
     RopeView rope;
     int32_t slots;   // pages that a sequence's rows can touch
     int32_t heads;   // query heads (0: no queries)
+    int32_t q_parts; // workgroups a query row
     int64_t kv_blocks;
 };
 
-// A workgroup per (sequence, touched page, head, keys or values), then one
-// per query row.
+// Four consecutive elements, or as many as `n` of them.
+template <typename T>
+__device__ __forceinline__ void load4(float (&v)[4], const T *p, bool whole, int n) {
+    if (whole) {
+        typedef T vec __attribute__((ext_vector_type(4)));
+        const vec x = *(const vec *)p;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = (float)x[j];
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = j < n ? (float)p[j] : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&v)[4], bool whole, int n) {
+    if (whole) {
+        typedef T vec __attribute__((ext_vector_type(4)));
+        vec x;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = (T)v[j];
+        *(vec *)p = x;
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < n) p[j] = (T)v[j];
+}
+// Rows of quads of T that may be moved whole.
+template <typename T>
+__device__ __forceinline__ bool quads_ok(const RowsView &r, int dim) {
+    return dim % 4 == 0 && r.stride % 4 == 0 && (uintptr_t)r.data % (4 * sizeof(T)) == 0;
+}
+
+// One query row's heads [part, + q_parts, ...) rotated; four pairs a thread.
+template <typename T>
+__device__ __forceinline__ void rotate_queries(const AppendArgs &a, const SeqRows &r, int i, int part) {
+    const T *src = (const T *)a.q.data + (int64_t)(r.row + i) * a.q.stride;
+    T *dst = (T *)a.q_out.data + (int64_t)(r.row + i) * a.q_out.stride;
+    const int half = a.rope.half, hd = a.p.hd;
+    const float *c = a.rope.cos_t + (int64_t)(r.pos + i) * half, *s = a.rope.sin_t + (int64_t)(r.pos + i) * half;
+    const bool fours = half % 4 == 0 && quads_ok<T>(a.q, hd) && quads_ok<T>(a.q_out, hd);
+    const int n_pairs = (half + 3) / 4, n_rest = (hd - 2 * half + 3) / 4, per = n_pairs + n_rest;
+    const bool table = half % 4 == 0 && ((uintptr_t)a.rope.cos_t | (uintptr_t)a.rope.sin_t) % 16 == 0;
+    for (int e = part * 256 + threadIdx.x; e < a.heads * per; e += a.q_parts * 256) {
+        const int h = e / per, j = e % per;
+        const T *x = src + (int64_t)h * hd;
+        T *y = dst + (int64_t)h * hd;
+        float u[4], w[4];
+        if (j >= n_pairs) {
+            const int d = 2 * half + (j - n_pairs) * 4;
+            load4(u, x + d, fours, hd - d);
+            store4(y + d, u, fours, hd - d);
+            continue;
+        }
+        const int i0 = 4 * j, n = half - i0;
+        float cc[4], ss[4];
+        load4(cc, c + i0, table, n);
+        load4(ss, s + i0, table, n);
+        if (a.rope.style == DITCH_ROPE_NEOX) {
+            load4(u, x + i0, fours, n);
+            load4(w, x + half + i0, fours, n);
+            float yu[4], yw[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                const double p = u[z], q = w[z], co = cc[z], si = ss[z];
+                yu[z] = (float)(p * co - q * si);
+                yw[z] = (float)(q * co + p * si);
+            }
+            store4(y + i0, yu, fours, n);
+            store4(y + half + i0, yw, fours, n);
+        } else {
+            load4(u, x + 2 * i0, fours, 2 * n);
+            load4(w, x + 2 * i0 + 4, fours, 2 * n - 4);
+            float yu[4], yw[4];
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                const double p = u[2 * z], q = u[2 * z + 1], co = cc[z], si = ss[z];
+                yu[2 * z] = (float)(p * co - q * si);
+                yu[2 * z + 1] = (float)(q * co + p * si);
+                const double p2 = w[2 * z], q2 = w[2 * z + 1], co2 = cc[2 + z], si2 = ss[2 + z];
+                yw[2 * z] = (float)(p2 * co2 - q2 * si2);
+                yw[2 * z + 1] = (float)(q2 * co2 + p2 * si2);
+            }
+            store4(y + 2 * i0, yu, fours, 2 * n);
+            store4(y + 2 * i0 + 4, yw, fours, 2 * n - 4);
+        }
+    }
+}
+
+// Calls f(t, d, n, y) for the values y[0..n) of every new token t in [z0, z1)
+// and dims d, d + 1, ..: keys, rotated. x: the rows (token 0's), at: token 0's
+// position.
+template <typename T, typename F>
+__device__ __forceinline__ void each_key(const T *x, int64_t stride, bool quads, int z0, int z1, int D, const RopeView &rope,
+                                         int64_t at, F &&f) {
+    const int half = rope.half;
+    if (half % 4 == 0 && quads) {
+        const int pairs = half / 4, per = pairs + (D - 2 * half) / 4;
+        const bool table = ((uintptr_t)rope.cos_t | (uintptr_t)rope.sin_t) % 16 == 0, neox = rope.style == DITCH_ROPE_NEOX;
+        for (int e = threadIdx.x; e < (z1 - z0) * per; e += 256) {
+            const int t = z0 + e / per, j = e % per;
+            const T *row = x + (int64_t)t * stride;
+            float u[4], w[4];
+            if (j >= pairs) {
+                const int d = 2 * half + (j - pairs) * 4;
+                load4(u, row + d, true, 4);
+                const double y[4] = {u[0], u[1], u[2], u[3]};
+                f(t, d, 4, y);
+                continue;
+            }
+            const int i0 = 4 * j, du = neox ? i0 : 2 * i0, dw = neox ? half + i0 : 2 * i0 + 4;
+            float cc[4], ss[4];
+            load4(u, row + du, true, 4);
+            load4(w, row + dw, true, 4);
+            load4(cc, rope.cos_t + (at + t) * half + i0, table, 4);
+            load4(ss, rope.sin_t + (at + t) * half + i0, table, 4);
+            double yu[4], yw[4];
+            if (neox) {
+#pragma unroll
+                for (int z = 0; z < 4; z++) {
+                    const double p = u[z], q = w[z], co = cc[z], si = ss[z];
+                    yu[z] = p * co - q * si;
+                    yw[z] = q * co + p * si;
+                }
+            } else {
+#pragma unroll
+                for (int z = 0; z < 4; z++) {
+                    const float *v = z < 2 ? u : w;
+                    double *y = z < 2 ? yu : yw;
+                    const double p = v[z % 2 * 2], q = v[z % 2 * 2 + 1], co = cc[z], si = ss[z];
+                    y[z % 2 * 2] = p * co - q * si;
+                    y[z % 2 * 2 + 1] = q * co + p * si;
+                }
+            }
+            f(t, du, 4, yu);
+            f(t, dw, 4, yw);
+        }
+    } else {
+        for (int e = threadIdx.x; e < (z1 - z0) * D; e += 256) {
+            const int t = z0 + e / D, d = e % D;
+            const int64_t row = (at + t) * half;
+            const double y[4] = {rotated(x + (int64_t)t * stride, d, half, rope.style, rope.cos_t + row, rope.sin_t + row)};
+            f(t, d, 1, y);
+        }
+    }
+}
+
+// A workgroup per (sequence, touched page, head, keys or values), then those
+// of the query rows.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
     __shared__ double part[4];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[TILE];
     const int tid = threadIdx.x;
     int64_t blk = blockIdx.x;
     if (blk >= a.kv_blocks) {
         blk -= a.kv_blocks;
+        const int q_part = (int)(blk % a.q_parts);
+        blk /= a.q_parts;
         const int seq = (int)(blk / a.b.max_rows), i = (int)(blk % a.b.max_rows);
         const SeqRows r = seq_rows(a.b, seq);
-        if (i >= r.live) return;
-        const T *src = (const T *)a.q.data + (r.row + i) * a.q.stride;
-        T *dst = (T *)a.q_out.data + (r.row + i) * a.q_out.stride;
-        const int half = a.rope.half, hd = a.p.hd;
-        const float *c = a.rope.cos_t + (int64_t)(r.pos + i) * half, *s = a.rope.sin_t + (int64_t)(r.pos + i) * half;
-        // a pair a thread: the rows may be the same
-        const int pairs = half, rest = hd - 2 * half, per = pairs + rest;
-        for (int e = tid; e < a.heads * per; e += 256) {
-            const int h = e / per, j = e % per;
-            const T *x = src + (int64_t)h * hd;
-            T *y = dst + (int64_t)h * hd;
-            if (j >= pairs) {
-                y[pairs + j] = x[pairs + j];
-                continue;
-            }
-            const int d0 = a.rope.style == DITCH_ROPE_NEOX ? j : 2 * j;
-            const int d1 = a.rope.style == DITCH_ROPE_NEOX ? j + half : 2 * j + 1;
-            const double y0 = rotated(x, d0, half, a.rope.style, c, s), y1 = rotated(x, d1, half, a.rope.style, c, s);
-            y[d0] = (T)(float)y0;
-            y[d1] = (T)(float)y1;
-        }
+        if (i < r.live) rotate_queries<T>(a, r, i, q_part);
         return;
     }
     const int which = (int)(blk & 1);
@@ -210,50 +350,102 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
     const int id = page_of(a.b, a.p, seq, page_index);
     if (id < 0) return;
     const int lo = r.pos > t0 ? r.pos - t0 : 0, hi = end - t0 < a.p.page ? end - t0 : a.p.page;  // new tokens [lo, hi)
-    const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk, half = which ? 0 : a.rope.half;
+    const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk;
     const RowsView &rv = which ? a.v : a.k;
-    const T *rows = (const T *)rv.data + (int64_t)(r.row + t0 + lo - r.pos) * rv.stride + (int64_t)h * D;
-    const float *ct = a.rope.cos_t, *st = a.rope.sin_t;
-    auto value = [&](int t, int d) -> double {  // new token lo + t
-        const int64_t at = (int64_t)(t0 + lo + t) * half;
-        return rotated(rows + t * rv.stride, d, half, a.rope.style, ct + at, st + at);
-    };
+    const T *rows = (const T *)rv.data + (int64_t)(r.row + t0 - r.pos) * rv.stride + (int64_t)h * D;  // token 0's
+    float *sp = a.p.scales + ((int64_t)id * a.p.kv_heads + h) * 2 + which;
+    const float before = lo > 0 ? *sp : 0.f;
+    const bool quads = quads_ok<T>(rv, D);
+
     double most = 0;
     bool bad = false;
-    for (int e = tid; e < (hi - lo) * D; e += 256) {
-        const double y = fabs(value(e / D, e % D));
-        bad |= !(y <= 3.4028234663852886e38);
-        most = fmax(most, y);
+    auto largest = [&](double y) {
+        bad |= !(fabs(y) <= 3.4028234663852886e38);
+        most = fmax(most, fabs(y));
+    };
+    if (which == 0) {
+        each_key(rows, rv.stride, quads, lo, hi, D, a.rope, t0, [&](int t, int d, int n, const double *y) {
+            for (int j = 0; j < n; j++) largest(y[j]);
+        });
+    } else if (quads) {
+        const int per = D / 4;
+        for (int e = tid; e < (hi - lo) * per; e += 256) {
+            float v[4];
+            load4(v, rows + (int64_t)(lo + e / per) * rv.stride + e % per * 4, true, 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) largest((double)v[j]);
+        }
+    } else {
+        for (int e = tid; e < (hi - lo) * D; e += 256) largest((double)(float)rows[(int64_t)(lo + e / D) * rv.stride + e % D]);
     }
     if (bad) most = INFINITY;
     for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
     if ((tid & 63) == 0) part[tid >> 6] = most;
     __syncthreads();
     most = fmax(fmax(part[0], part[1]), fmax(part[2], part[3]));
-    float *sp = a.p.scales + ((int64_t)id * a.p.kv_heads + h) * 2 + which;
-    const float before = lo > 0 ? *sp : 0.f;
-    __syncthreads();  // every thread has read it
     float after = __fmul_rn((float)most, 1.f / code_most(KIND));
     after = before > after ? before : after;
     const bool poison = !(before <= 3.4028234663852886e38f) || !(after <= 3.4028234663852886e38f);
     if (poison) after = NAN;
-    if (tid == 0) *sp = after;
+    if (tid == 0) *sp = after;  // (every thread has read it: the barrier above)
     const double inverse = after > 0.f ? 1.0 / (double)after : 0.0;
+    const bool grown = lo > 0 && after > before;
+    const double f = grown ? (double)before * inverse : 0.0;
     uint8_t *codes = a.p.codes + ((int64_t)id * a.p.kv_heads + h) * a.p.page_bytes + (which ? (int64_t)a.p.page * a.p.dk : 0);
-    // the tokens that stay, to the new scale
-    if (lo > 0 && after > before) {
-        const double f = (double)before * inverse;
-        for (int e = tid; e < lo * DP; e += 256) {
-            const int o = which ? value_offset(e / DP, e % DP, DP) : key_offset(e / DP, e % DP, DP);
-            codes[o] = nearest_code<KIND>((double)code_value<KIND>(codes[o]) * f);
+
+    // the granules to write: from the first that changes to the end of the one
+    // that holds the last new token (what it has behind that, zeros where the
+    // new tokens start it, is dead)
+    const int room = DP <= 64 ? 256 : DP <= 128 ? 128 : 64, CT = room < a.p.page ? room : a.p.page;
+    const int z_first = grown ? 0 : lo / GRANULE * GRANULE, z_last = (hi + GRANULE - 1) / GRANULE * GRANULE;
+    for (int c0 = z_first; c0 < z_last; c0 += CT) {
+        const int c1 = c0 + CT < z_last ? c0 + CT : z_last, n0 = c0 > lo ? c0 : lo, n1 = c1 < hi ? c1 : hi;
+        uint4 *page = (uint4 *)(codes + (int64_t)c0 * DP);
+        for (int u = tid; u < (c1 - c0) * DP / 16; u += 256) {
+            union {
+                uint4 q;
+                uint8_t b[16];
+            } w;
+            w.q = make_uint4(0, 0, 0, 0);
+            if (c0 + u * 16 / (GRANULE * DP) * GRANULE < lo) {  // the granule holds tokens of before
+                w.q = page[u];
+                if (grown) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) w.b[j] = nearest_code<KIND>((double)code_value<KIND>(w.b[j]) * f);
+                }
+            }
+            ((uint4 *)tile)[u] = w.q;
         }
-    }
-    // the new ones, and zeros up to the end of a granule that they start
-    const int fill = hi % GRANULE && hi / GRANULE * GRANULE >= lo ? (hi / GRANULE + 1) * GRANULE : hi;
-    for (int e = tid; e < (fill - lo) * DP; e += 256) {
-        const int t = e / DP, d = e % DP;
-        const int o = which ? value_offset(lo + t, d, DP) : key_offset(lo + t, d, DP);
-        codes[o] = t < hi - lo && d < D && !poison ? nearest_code<KIND>(value(t, d) * inverse) : 0;
+        __syncthreads();
+        auto code = [&](double y) { return (uint32_t)(poison ? 0 : nearest_code<KIND>(y * inverse)); };
+        if (which == 0) {
+            each_key(rows, rv.stride, quads, n0, n1, D, a.rope, t0, [&](int t, int d, int n, const double *y) {
+                uint8_t *at = tile + key_offset(t - c0, d, DP);
+                if (n == 4) *(uint32_t *)at = code(y[0]) | code(y[1]) << 8 | code(y[2]) << 16 | code(y[3]) << 24;
+                else *at = (uint8_t)code(y[0]);
+            });
+        } else {
+            // a dim of four tokens that lie next to each other in the page
+            const int q0 = n0 / 4, q1 = (n1 + 3) / 4;
+            for (int e = tid; e < (q1 - q0) * D; e += 256) {
+                const int t = (q0 + e / D) * 4, d = e % D;
+                uint32_t c[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = t + j >= n0 && t + j < n1;
+                    c[j] = in ? code((double)(float)rows[(int64_t)(t + j) * rv.stride + d]) : 0;
+                }
+                uint8_t *at = tile + value_offset(t - c0, d, DP);
+                if (t >= n0 && t + 4 <= n1) *(uint32_t *)at = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (t + j >= n0 && t + j < n1) at[j] = (uint8_t)c[j];
+            }
+        }
+        __syncthreads();
+        for (int u = tid; u < (c1 - c0) * DP / 16; u += 256) page[u] = ((const uint4 *)tile)[u];
+        __syncthreads();
     }
 }
 
@@ -269,10 +461,13 @@ static void append_typed(const AppendArgs &a, unsigned blocks, hipStream_t s) {
 void launch_pages_append(const PoolView &p, const BatchView &b, int32_t dtype, const RowsView &k, const RowsView &v,
                          const RopeView &rope, const RowsView *q, const RowsView *q_out, int heads, hipStream_t s) {
     if (b.n_seqs == 0) return;
-    AppendArgs a{p, b, k, v, q ? *q : RowsView{}, q ? *q_out : RowsView{}, rope, 0, q ? heads : 0, 0};
+    AppendArgs a{p, b, k, v, q ? *q : RowsView{}, q ? *q_out : RowsView{}, rope, 0, q ? heads : 0, 1, 0};
     a.slots = (b.max_rows + p.page - 2) / p.page + 1;
     a.kv_blocks = (int64_t)b.n_seqs * a.slots * p.kv_heads * 2;
-    const unsigned blocks = grid_blocks(a.kv_blocks + (q ? (int64_t)b.n_seqs * b.max_rows : 0), "kv append");
+    // a row's heads over several workgroups until the rows fill the chip
+    const int64_t rows = (int64_t)b.n_seqs * b.max_rows;
+    if (q && rows < 1024) a.q_parts = (int)std::min<int64_t>((int64_t)heads * ((p.hd + 7) / 8 + 255) / 256 + 1, 1024 / rows + 1);
+    const unsigned blocks = grid_blocks(a.kv_blocks + (q ? rows * a.q_parts : 0), "kv append");
     if (dtype == DITCH_F32) append_typed<float>(a, blocks, s);
     else if (dtype == DITCH_F16) append_typed<_Float16>(a, blocks, s);
     else append_typed<__bf16>(a, blocks, s);
@@ -285,30 +480,59 @@ struct ReadArgs {
     PoolView p;
     BatchView b;
     RowsView k, v;
+    int32_t granules;  // that a sequence's rows can touch
 };
 
+// A workgroup per (sequence, granule, head, keys or values): its units
+// decoded into LDS rows, which go out as rows.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
+    __shared__ __attribute__((aligned(16))) float tile[GRANULE * 260];
+    const int tid = threadIdx.x;
     int64_t blk = blockIdx.x;
-    const int seq = (int)(blk / a.b.max_rows), i = (int)(blk % a.b.max_rows);
+    const int which = (int)(blk & 1);
+    blk >>= 1;
+    const int h = (int)(blk % a.p.kv_heads);
+    blk /= a.p.kv_heads;
+    const int slot = (int)(blk % a.granules), seq = (int)(blk / a.granules);
     const SeqRows r = seq_rows(a.b, seq);
-    if (i >= r.live) return;
-    const int pos = r.pos + i, id = page_of(a.b, a.p, seq, pos >> a.p.page_shift), t = pos & (a.p.page - 1);
-    for (int which = 0; which < 2; which++) {
-        const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk;
-        const RowsView &rv = which ? a.v : a.k;
-        T *row = (T *)rv.data + (int64_t)(r.row + i) * rv.stride;
-        for (int e = threadIdx.x; e < a.p.kv_heads * D; e += 256) {
-            const int h = e / D, d = e % D;
-            float x = NAN;
-            if (id >= 0) {
-                const int64_t ph = (int64_t)id * a.p.kv_heads + h;
-                const uint8_t *codes = a.p.codes + ph * a.p.page_bytes + (which ? (int64_t)a.p.page * a.p.dk : 0);
-                x = code_value<KIND>(codes[which ? value_offset(t, d, DP) : key_offset(t, d, DP)]) *
-                    a.p.scales[ph * 2 + which];
-            }
-            row[e] = (T)x;
+    const int gi = r.pos / GRANULE + slot, t0 = gi * GRANULE, end = r.pos + r.live;
+    if (r.live == 0 || t0 >= end) return;
+    const int id = page_of(a.b, a.p, seq, t0 >> a.p.page_shift);
+    const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk, S = DP + 4;
+    const float scale = id < 0 ? NAN : a.p.scales[((int64_t)id * a.p.kv_heads + h) * 2 + which];
+    const int lo = r.pos > t0 ? r.pos - t0 : 0, hi = end - t0 < GRANULE ? end - t0 : GRANULE;
+    const uint8_t *codes = a.p.codes + ((int64_t)(id < 0 ? 0 : id) * a.p.kv_heads + h) * a.p.page_bytes +
+                           (which ? (int64_t)a.p.page * a.p.dk : 0) + (int64_t)(t0 & (a.p.page - 1)) * DP;
+    for (int u = tid; u < 2 * DP; u += 256) {  // GRANULE * DP / 16 units
+        union {
+            uint4 q;
+            uint8_t b[16];
+        } w;
+        w.q = *(const uint4 *)(codes + u * 16);
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = id < 0 ? NAN : code_value<KIND>(w.b[j]) * scale;
+        if (which == 0) {
+            const int t = u / (DP / 64 * 64) * 16 + u % 16, d = u / 64 % (DP / 64) * 64 + u / 16 % 4 * 16;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *(float4 *)&tile[t * S + d + j] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        } else {
+            const int d = u / 64 * 32 + u % 16, t = u / 16 % 4 * 4;
+#pragma unroll
+            for (int j = 0; j < 16; j++) tile[(t + (j & 4 ? 16 : 0) + (j & 3)) * S + d + (j & 8 ? 16 : 0)] = x[j];
         }
+    }
+    __syncthreads();
+    const RowsView &rv = which ? a.v : a.k;
+    T *rows = (T *)rv.data + (int64_t)(r.row + t0 - r.pos) * rv.stride + (int64_t)h * D;
+    const bool quads = quads_ok<T>(rv, D);
+    const int per = (D + 3) / 4;
+    for (int e = tid; e < (hi - lo) * per; e += 256) {
+        const int t = lo + e / per, d = e % per * 4;
+        const float4 f = *(const float4 *)&tile[t * S + d];
+        const float v[4] = {f.x, f.y, f.z, f.w};
+        store4(rows + (int64_t)t * rv.stride + d, v, quads, D - d);
     }
 }
 
@@ -324,8 +548,8 @@ static void read_typed(const ReadArgs &a, unsigned blocks, hipStream_t s) {
 void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, const RowsView &k, const RowsView &v,
                        hipStream_t s) {
     if (b.n_seqs == 0) return;
-    const ReadArgs a{p, b, k, v};
-    const unsigned blocks = grid_blocks((int64_t)b.n_seqs * b.max_rows, "kv read");
+    ReadArgs a{p, b, k, v, (b.max_rows + GRANULE - 2) / GRANULE + 1};
+    const unsigned blocks = grid_blocks((int64_t)b.n_seqs * a.granules * p.kv_heads * 2, "kv read");
     if (dtype == DITCH_F32) read_typed<float>(a, blocks, s);
     else if (dtype == DITCH_F16) read_typed<_Float16>(a, blocks, s);
     else read_typed<__bf16>(a, blocks, s);
@@ -334,11 +558,14 @@ void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, con
 // ---------------------------------------------------------------------------
 // fork
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+constexpr int FORK_PART = 2048;  // 16-byte words that a workgroup copies
+
 struct ForkArgs {
     uint8_t *codes;
     float *scales;
     int64_t layer_pages, head_bytes;  // pages a layer; bytes of one head's page
-    int32_t page, n_pages, kv_heads;
+    int32_t page, n_pages, kv_heads, parts;  // parts: workgroups a page of a layer
     int32_t *table_out, *spare_out;
     const int32_t *table, *parents, *spare;
     const uint32_t *lens;
@@ -352,8 +579,8 @@ __device__ __forceinline__ int parent_of(const int32_t *parents, int64_t first, 
     return (uint32_t)p < (uint32_t)beams ? p : c;
 }
 
-// A workgroup per (sequence, layer and head); those of the first layer and
-// head write the sequence's table row and spare page too.
+// A workgroup per (sequence, layer, part of the page's heads); the first of a
+// sequence writes its table row and spare page too.
 __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
     const int64_t seq = blockIdx.x, g = seq / a.beams, first = g * a.beams;
     const int c = (int)(seq % a.beams);
@@ -391,22 +618,34 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
         }
     }
     if (!copies || (uint32_t)src >= (uint32_t)a.n_pages || (uint32_t)mine >= (uint32_t)a.n_pages || src == mine) return;
-    const int64_t layer = blockIdx.y / a.kv_heads, h = blockIdx.y % a.kv_heads;
-    const int64_t from = (layer * a.layer_pages + src) * a.kv_heads + h, to = (layer * a.layer_pages + mine) * a.kv_heads + h;
-    const int n = (int)(a.head_bytes / 16);
-    const uint4 *cs = (const uint4 *)(a.codes + from * a.head_bytes);
-    uint4 *cd = (uint4 *)(a.codes + to * a.head_bytes);
-    for (int i = threadIdx.x; i < n; i += 256) cd[i] = cs[i];
-    if (threadIdx.x < 2) a.scales[to * 2 + threadIdx.x] = a.scales[from * 2 + threadIdx.x];
+    // a page's heads lie next to each other: the workgroup's part of them, 8 x 16 bytes a thread in flight
+    const int64_t layer = blockIdx.y / a.parts, piece = blockIdx.y % a.parts;
+    const int64_t from = (layer * a.layer_pages + src) * a.kv_heads, to = (layer * a.layer_pages + mine) * a.kv_heads;
+    const int64_t n = a.kv_heads * a.head_bytes / 16, p0 = piece * FORK_PART, left = n - p0 < FORK_PART ? n - p0 : FORK_PART;
+    const u32x4_t *cs = (const u32x4_t *)(a.codes + from * a.head_bytes) + p0;
+    u32x4_t *cd = (u32x4_t *)(a.codes + to * a.head_bytes) + p0;
+    u32x4_t v[FORK_PART / 256];
+#pragma unroll
+    for (int j = 0; j < FORK_PART / 256; j++) {
+        const int i = threadIdx.x + 256 * j;
+        if (i < left) v[j] = cs[i];
+    }
+#pragma unroll
+    for (int j = 0; j < FORK_PART / 256; j++) {
+        const int i = threadIdx.x + 256 * j;
+        if (i < left) cd[i] = v[j];
+    }
+    if (piece == 0)
+        for (int i = threadIdx.x; i < 2 * a.kv_heads; i += 256) a.scales[to * 2 + i] = a.scales[from * 2 + i];
 }
 
 void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spare_out, const int32_t *table,
                        int64_t table_stride, const int32_t *parents, const int32_t *spare, const uint32_t *lens,
                        int64_t groups, int64_t beams, hipStream_t s) {
     const PoolView v = pool_view(p, 0);
-    const int64_t lh = (int64_t)p->layers * v.kv_heads;
-    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 layers x heads");
-    const ForkArgs a{v.codes, v.scales, v.n_pages, v.page_bytes, v.page, v.n_pages, v.kv_heads, table_out, spare_out,
+    const int64_t parts = (v.kv_heads * v.page_bytes / 16 + FORK_PART - 1) / FORK_PART, lh = p->layers * parts;
+    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 x 32 KB of layers a page");
+    const ForkArgs a{v.codes, v.scales, v.n_pages, v.page_bytes, v.page, v.n_pages, v.kv_heads, (int32_t)parts, table_out, spare_out,
                      table, parents, spare, lens, table_stride, (int32_t)beams};
     hipLaunchKernelGGL(pages_fork_kernel, dim3(grid_blocks(groups * beams, "kv fork"), (unsigned)lh), dim3(256), 0, s, a);
     DITCH_TRY_HIP(hipGetLastError());
