@@ -908,7 +908,7 @@ int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, in
 }
 
 static bool beam_shape_ok(uint64_t prompts, uint64_t beams, uint64_t vocab, uint64_t k) {
-    return prompts <= (uint64_t)1 << 16 && beams >= 1 && beams <= 64 && vocab >= 1 && vocab <= (uint64_t)INT32_MAX &&
+    return prompts <= (uint64_t)1 << 16 && beams >= 1 && beams <= 64 && vocab >= 1 && vocab <= (uint64_t)1 << 30 &&
            k >= 1 && k <= 128 && k <= beams * vocab;
 }
 

@@ -33,15 +33,6 @@ __device__ __forceinline__ uint64_t score_key(double x) {
     return b >> 63 ? ~b : b | ((uint64_t)1 << 63);
 }
 
-// e^d for d <= 0, within about an ulp: 2^n 2^f with d log2(e) = n + f
-__device__ __forceinline__ float exp_below(float d) {
-    d = d < -150.f ? -150.f : d;  // (a NaN stays)
-    const float n = rintf(d * 1.44269504f);
-    float f = __builtin_fmaf(d, 1.44269502162933349609375f, -n);  // log2(e) in two parts
-    f = __builtin_fmaf(d, 1.92596299112661746887e-8f, f);
-    return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
-}
-
 struct Candidate {
     float x;
     uint32_t token;
@@ -53,7 +44,7 @@ struct BeamArgs {
     uint32_t *tokens;
     const float *logits, *prev;
     Candidate *list;  // [rows][chunks][k]
-    double *stats;    // [rows][chunks][2]: maximum, sum of exponentials relative to it
+    double *stats;    // [rows][chunks][4 waves][2]: maximum, sum of exponentials relative to it
     int32_t beams, k, chunks;
     int64_t vocab;
 };
@@ -63,20 +54,18 @@ template <int R>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     __shared__ Candidate list[4][LIST];
     __shared__ int count_s[4];
-    __shared__ float m_s[4];
-    __shared__ double sum_s[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / a.chunks;
     const int chunk = (int)(blockIdx.x % a.chunks), k = a.k;
     const float *x = a.logits + row * a.vocab;
     // quads at 16-byte addresses: quad q holds tokens 4 q - shift + 0..3
+    // (vocab <= 2^30: 32 bits hold the last chunk's end)
     const int shift = (int)((uintptr_t)x / 4 % 4), V = (int)a.vocab;
-    const int64_t q0 = ((int64_t)chunk * 4 + wave) * R * 64 + lane;
-    const int64_t t0 = q0 * 4 - shift;  // the lane's first token; quad r's is 256 r further
+    const int first = (chunk * 4 + wave) * R * 256 - shift, t0 = first + 4 * lane;  // the lane's quad r: from t0 + 256 r
     float v[R][4];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const int64_t t = t0 + 256 * r;
+        const int t = t0 + 256 * r;
         if (t >= 0 && t + 4 <= V) {
             const float4 f = *(const float4 *)(x + t);
             v[r][0] = f.x;
@@ -88,10 +77,6 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
             for (int j = 0; j < 4; j++) v[r][j] = t + j >= 0 && t + j < V ? x[t + j] : -INFINITY;
         }
     }
-    auto valid = [&](int r, int j) {
-        const int64_t t = t0 + 256 * r + j;
-        return t >= 0 && t < V;
-    };
     // the half lanes' maxima, the wave's, and its sum
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -105,7 +90,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     for (int r = 0; r < R; r++) {
         float s[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = exp_below(v[r][j] - m);
+        for (int j = 0; j < 4; j++) s[j] = __builtin_amdgcn_exp2f((v[r][j] - m) * 1.44269504f);
         sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
     }
     // (a wave of -infinities or past the row has no sum; a NaN shows in it)
@@ -121,9 +106,8 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
 
     // the wave's tokens, and how many of them the list needs
-    const int64_t first = ((int64_t)chunk * 4 + wave) * R * 256 - shift;
-    const int64_t lo = first < 0 ? 0 : first, hi = first + R * 256 < V ? first + R * 256 : V;
-    const int have = hi > lo ? (int)(hi - lo) : 0, need = have < k ? have : k;
+    const int lo = first < 0 ? 0 : first, hi = first + R * 256 < V ? first + R * 256 : V;
+    const int have = hi > lo ? hi - lo : 0, need = have < k ? have : k;
     int count = 0;
     bool done = need == 0;
     if (!done && need == k) {
@@ -146,19 +130,23 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         }
         // (low's logit; the key of a half lane without one is that of -infinity)
         const float tau = low >> 31 ? __uint_as_float(low & 0x7fffffffu) : __uint_as_float(~low);
-        done = true;
+        // (a threshold of -infinity would take what pads the row, too)
+        if (tau > -INFINITY) {
 #pragma unroll
-        for (int r = 0; r < R; r++)
+            for (int r = 0; r < R; r++) {
+                uint64_t in[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = v[r][j] >= tau && valid(r, j);
-                const uint64_t b = __ballot(in);
-                if (b) {
-                    const int at = count + __popcll(b & (((uint64_t)1 << lane) - 1));
-                    if (in && at < LIST) list[wave][at] = Candidate{v[r][j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
-                    count += __popcll(b);
+                for (int j = 0; j < 4; j++) in[j] = __ballot(v[r][j] >= tau);
+                if (in[0] | in[1] | in[2] | in[3]) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int at = count + __popcll(in[j] & (((uint64_t)1 << lane) - 1));
+                        if (v[r][j] >= tau && at < LIST) list[wave][at] = Candidate{v[r][j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
+                        count += __popcll(in[j]);
+                    }
                 }
             }
+        }
         done = count >= k && count <= LIST;
     }
     if (!done) {
@@ -167,7 +155,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         // not indexed at run time)
         uint32_t low = 0, high = ~0u;
         auto logit = [&](int r, int j, bool &in) {
-            const int64_t t = t0 + 256 * r + j;
+            const int t = t0 + 256 * r + j;
             in = t >= 0 && t < V;
             return in ? x[t] : 0.f;
         };
@@ -230,8 +218,9 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     }
     if (lane == 0) {
         count_s[wave] = count;
-        m_s[wave] = m;
-        sum_s[wave] = sum;
+        double *st = a.stats + ((int64_t)blockIdx.x * 4 + wave) * 2;
+        st[0] = m;
+        st[1] = sum;
     }
     __syncthreads();
     // the workgroup's k best by their ranks among its waves' candidates
@@ -251,34 +240,27 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         if (rank < k) out[rank] = c;
     }
     for (int e = n + tid; e < k; e += 256) out[e] = Candidate{0.f, NO_TOKEN};
-    if (tid == 0) {
-        const float mm = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-        double total = 0;
-        for (int w = 0; w < 4; w++)
-            total += m_s[w] == -INFINITY ? sum_s[w] : sum_s[w] * exp((double)m_s[w] - (double)mm);
-        a.stats[(int64_t)blockIdx.x * 2] = mm;
-        a.stats[(int64_t)blockIdx.x * 2 + 1] = total;
-    }
 }
 
 // A workgroup a prompt.
 constexpr int JOIN = 1024, HELD = 4;  // threads; candidates a thread holds in registers
+constexpr int NEAR = 256;             // candidates that are ranked against each other
 __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ double lse_s[BEAM_MOST_BEAMS], prev_s[BEAM_MOST_BEAMS];
     __shared__ uint64_t lo_s[16], hi_s[16];
     __shared__ int count_s[2][16];
     __shared__ int put;
-    __shared__ uint64_t key_s[BEAM_MOST_K], tie_s[BEAM_MOST_K];
-    __shared__ uint32_t token_s[BEAM_MOST_K];
-    __shared__ float score_s[BEAM_MOST_K];
+    __shared__ uint64_t key_s[NEAR], tie_s[NEAR];
+    __shared__ uint32_t token_s[NEAR];
+    __shared__ float score_s[NEAR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
     const int64_t row0 = (int64_t)blockIdx.x * a.beams;
     for (int b = wave; b < a.beams; b += JOIN / 64) {
         double m = -INFINITY, sum = 0;
-        const double *st = a.stats + (row0 + b) * a.chunks * 2;
-        for (int c = lane; c < a.chunks; c += 64) m = fmax(m, st[2 * c]);
+        const double *st = a.stats + (row0 + b) * a.chunks * 8;
+        for (int c = lane; c < 4 * a.chunks; c += 64) m = fmax(m, st[2 * c]);
         for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
-        for (int c = lane; c < a.chunks; c += 64) {
+        for (int c = lane; c < 4 * a.chunks; c += 64) {
             const double cm = st[2 * c], cs = st[2 * c + 1];
             sum += cm == -INFINITY ? cs : cs * exp(cm - m);
         }
@@ -375,13 +357,13 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
         if (c >= k) {
             low = mid;
             reach = c;
-            if (c == k) break;
+            if (c <= k + 64) break;  // few enough to rank
         } else high = mid - 1;
     }
-    // among equal scores the lowest beams, in a beam the largest logits, among equal logits the lowest tokens
+    // should more than can be ranked reach it: exactly k; among equal scores the lowest beams, in a beam the largest logits, among equal logits the lowest tokens
     uint64_t tie = ~(uint64_t)0;
     uint32_t token = ~0u;
-    if (reach != k) {
+    if (reach < k || reach > NEAR) {
         int need = k - count([&](const Item &it) { return it.key > low; });
         uint64_t l = 0, h = ((uint64_t)BEAM_MOST_BEAMS << 32) - 1;
         while (l < h) {
@@ -402,7 +384,7 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     each([&](const Item &it) {
         if (it.key > low || (it.key == low && (it.tie < tie || (it.tie == tie && it.token <= token)))) {
             const int at = atomicAdd(&put, 1);
-            if (at < k) {
+            if (at < NEAR) {
                 key_s[at] = it.key;
                 tie_s[at] = it.tie;
                 token_s[at] = it.token;
@@ -411,17 +393,20 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
         }
     });
     __syncthreads();
-    // exactly k, in any order: each goes to its rank
-    if (tid < k) {
+    // k or a few more, in any order: each goes to its rank
+    const int n_near = put < NEAR ? put : NEAR;
+    if (tid < n_near) {
         const uint64_t key = key_s[tid], t = tie_s[tid];
         const uint32_t tok = token_s[tid];
         int rank = 0;
-        for (int i = 0; i < k; i++)
+        for (int i = 0; i < n_near; i++)
             rank += key_s[i] > key || (key_s[i] == key && (tie_s[i] < t || (tie_s[i] == t && token_s[i] < tok)));
-        const int64_t o = (int64_t)blockIdx.x * k + rank;
-        a.scores[o] = score_s[tid];
-        a.parents[o] = (int32_t)(t >> 32);
-        a.tokens[o] = tok;
+        if (rank < k) {
+            const int64_t o = (int64_t)blockIdx.x * k + rank;
+            a.scores[o] = score_s[tid];
+            a.parents[o] = (int32_t)(t >> 32);
+            a.tokens[o] = tok;
+        }
     }
 }
 
@@ -435,7 +420,7 @@ static int64_t beam_chunks(int64_t rows, int64_t vocab) {
 
 size_t beam_select_workspace(int64_t prompts, int64_t beams, int64_t vocab, int64_t k) {
     const int64_t chunks = beam_chunks(prompts * beams, vocab);
-    return (size_t)(prompts * beams * chunks) * (k * sizeof(Candidate) + 2 * sizeof(double));
+    return (size_t)(prompts * beams * chunks) * (k * sizeof(Candidate) + 8 * sizeof(double));
 }
 
 void launch_beam_select(float *scores, int32_t *parents, uint32_t *tokens, const float *logits, const float *prev,
@@ -444,7 +429,7 @@ void launch_beam_select(float *scores, int32_t *parents, uint32_t *tokens, const
     const int64_t rows = prompts * beams, chunks = beam_chunks(rows, vocab);
     DITCH_CHECK(rows * chunks < (int64_t)1 << 24, DITCH_INVALID_ARGUMENT, "beam select: more logits than one launch holds");
     double *stats = (double *)ws;
-    const BeamArgs a{scores, parents, tokens, logits, prev, (Candidate *)(stats + rows * chunks * 2), stats,
+    const BeamArgs a{scores, parents, tokens, logits, prev, (Candidate *)(stats + rows * chunks * 8), stats,
                      (int32_t)beams, (int32_t)k, (int32_t)chunks, vocab};
     if (beam_quads(rows, vocab) == 16)
         hipLaunchKernelGGL(beam_chunk_kernel<16>, dim3((unsigned)(rows * chunks)), dim3(256), 0, s, a);

@@ -160,7 +160,7 @@ __device__ __forceinline__ float code_value(uint8_t c) {
 // scale, and, the rows by then in the caches, for the codes, which it puts in
 // the page's order in LDS; whole granules go out, and the one that holds
 // tokens of before came in first. (Staging the values themselves needs four to
-// eight times the LDS and took 233 us where this takes APPEND_US: 24 sequences
+// eight times the LDS and took 233 us where this takes 85: 24 sequences
 // of up to 500 f32 rows of 8 heads of 128 and 32 query heads, 360 MB.)
 
 constexpr int TILE = 16384;  // codes staged (the page in parts where it has more)
@@ -559,7 +559,10 @@ void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, con
 // fork
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-constexpr int FORK_PART = 2048;  // 16-byte words that a workgroup copies
+// 16-byte words that a workgroup copies: 16 a thread in flight. The last pages
+// of 16 x 8 beams (32 layers of 8 heads of 128, 360 MB moved): 97 us, with 8
+// or fewer a thread 105 to 112.
+constexpr int FORK_PART = 4096;
 
 struct ForkArgs {
     uint8_t *codes;
@@ -573,69 +576,65 @@ struct ForkArgs {
     int32_t beams;
 };
 
-// The parent of the group's sequence c.
-__device__ __forceinline__ int parent_of(const int32_t *parents, int64_t first, int c, int beams) {
-    const int32_t p = parents[first + c];
-    return (uint32_t)p < (uint32_t)beams ? p : c;
-}
-
 // A workgroup per (sequence, layer, part of the page's heads); the first of a
-// sequence writes its table row and spare page too.
+// sequence writes its table row and spare page too. Lane e of every wave holds
+// the parent of the group's sequence e, so the group's state is a few ballots.
 __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
+    const int lane = threadIdx.x & 63;
     const int64_t seq = blockIdx.x, g = seq / a.beams, first = g * a.beams;
     const int c = (int)(seq % a.beams);
+    const int32_t named = lane < a.beams ? a.parents[first + lane] : -1;
     const int64_t len = a.lens[g], full = len / a.page, part = len % a.page;
-    const int p = parent_of(a.parents, first, c, a.beams);
+    const int parent = lane >= a.beams ? -1 : (uint32_t)named < (uint32_t)a.beams ? named : lane;
+    const int p = __builtin_amdgcn_readlane(parent, c);
     const bool has = part && full < a.table_stride;
     // a child before this one has taken the parent's last page over
-    bool copies = false;
-    for (int e = 0; e < c && has; e++) copies |= parent_of(a.parents, first, e, a.beams) == p;
+    const uint64_t before = ((uint64_t)1 << c) - 1;
+    const bool copies = has && (__ballot(parent == p) & before);
+    if (!copies && blockIdx.y) return;
     const int32_t src = has ? a.table[(first + p) * a.table_stride + full] : -1, mine = a.spare[seq];
     if (blockIdx.y == 0) {
+#pragma unroll 1
         for (int64_t j = threadIdx.x; j < a.table_stride; j += 256) {
             int32_t v = a.table[(j < full ? first + p : seq) * a.table_stride + j];
             if (has && j == full) v = copies ? mine : src;
             a.table_out[seq * a.table_stride + j] = v;
         }
-        if (threadIdx.x == 0) {
-            int32_t left = mine;
-            if (copies) {
-                // the n-th copying sequence of the group gets the page of the n-th childless one
-                int nth = 0;
-                for (int e = 0; e < c; e++) {
-                    const int q = parent_of(a.parents, first, e, a.beams);
-                    bool before = false;
-                    for (int f = 0; f < e; f++) before |= parent_of(a.parents, first, f, a.beams) == q;
-                    nth += before;
-                }
-                for (int e = 0; e < a.beams; e++) {
-                    bool child = false;
-                    for (int f = 0; f < a.beams; f++) child |= parent_of(a.parents, first, f, a.beams) == e;
-                    if (!child && nth-- == 0) left = a.table[(first + e) * a.table_stride + full];
-                }
-            }
-            a.spare_out[seq] = left;
+        // the n-th copying sequence of the group gets the page of the n-th childless one
+        bool again = false, child = false;  // lane e: copies too; is a parent
+#pragma unroll 1
+        for (int e = 0; e < a.beams; e++) {
+            const int q = __builtin_amdgcn_readlane(parent, e);
+            again |= e < lane && q == parent;
+            child |= q == lane;
         }
+        const int nth = __popcll(__ballot(again && lane < a.beams) & before);
+        uint64_t free = __ballot(!child && lane < a.beams);
+#pragma unroll 1
+        for (int e = 0; e < nth; e++) free &= free - 1;
+        if (threadIdx.x == 0)
+            a.spare_out[seq] = copies ? a.table[(first + __ffsll((unsigned long long)free) - 1) * a.table_stride + full] : mine;
     }
     if (!copies || (uint32_t)src >= (uint32_t)a.n_pages || (uint32_t)mine >= (uint32_t)a.n_pages || src == mine) return;
-    // a page's heads lie next to each other: the workgroup's part of them, 8 x 16 bytes a thread in flight
+    // a page's heads lie next to each other: the workgroup's part of them
     const int64_t layer = blockIdx.y / a.parts, piece = blockIdx.y % a.parts;
     const int64_t from = (layer * a.layer_pages + src) * a.kv_heads, to = (layer * a.layer_pages + mine) * a.kv_heads;
     const int64_t n = a.kv_heads * a.head_bytes / 16, p0 = piece * FORK_PART, left = n - p0 < FORK_PART ? n - p0 : FORK_PART;
     const u32x4_t *cs = (const u32x4_t *)(a.codes + from * a.head_bytes) + p0;
     u32x4_t *cd = (u32x4_t *)(a.codes + to * a.head_bytes) + p0;
-    u32x4_t v[FORK_PART / 256];
+    const int tid = threadIdx.x;
+    if (left == FORK_PART) {
+        u32x4_t v[FORK_PART / 256];
 #pragma unroll
-    for (int j = 0; j < FORK_PART / 256; j++) {
-        const int i = threadIdx.x + 256 * j;
-        if (i < left) v[j] = cs[i];
-    }
+        for (int j = 0; j < FORK_PART / 256; j++) v[j] = cs[tid + 256 * j];
 #pragma unroll
-    for (int j = 0; j < FORK_PART / 256; j++) {
-        const int i = threadIdx.x + 256 * j;
-        if (i < left) cd[i] = v[j];
+        for (int j = 0; j < FORK_PART / 256; j++) cd[tid + 256 * j] = v[j];
+    } else {
+#pragma unroll 4
+        for (int i = tid; i < left; i += 256) cd[i] = cs[i];
     }
     if (piece == 0)
+#pragma unroll 1
         for (int i = threadIdx.x; i < 2 * a.kv_heads; i += 256) a.scales[to * 2 + i] = a.scales[from * 2 + i];
 }
 
@@ -644,7 +643,7 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
                        int64_t groups, int64_t beams, hipStream_t s) {
     const PoolView v = pool_view(p, 0);
     const int64_t parts = (v.kv_heads * v.page_bytes / 16 + FORK_PART - 1) / FORK_PART, lh = p->layers * parts;
-    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 x 32 KB of layers a page");
+    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 x 64 KB of layers a page");
     const ForkArgs a{v.codes, v.scales, v.n_pages, v.page_bytes, v.page, v.n_pages, v.kv_heads, (int32_t)parts, table_out, spare_out,
                      table, parents, spare, lens, table_stride, (int32_t)beams};
     hipLaunchKernelGGL(pages_fork_kernel, dim3(grid_blocks(groups * beams, "kv fork"), (unsigned)lh), dim3(256), 0, s, a);

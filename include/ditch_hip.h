@@ -755,7 +755,7 @@ int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, in
  * beam first among equals. A beam whose previous score is -infinity comes after every finite
  * one; a beam without probabilities (a NaN or +infinity among its logits,
  * or nothing above -infinity; a NaN previous score) scores NaN and comes
- * last. 1 <= beams <= 64, 1 <= k <= 128 and k <= beams * vocab. `ws`:
+ * last. 1 <= beams <= 64, 1 <= k <= 128, k <= beams * vocab, vocab <= 2^30. `ws`:
  * ditch_hip_beam_select_workspace bytes, as for the attention.             */
 uint64_t ditch_hip_beam_select_workspace(uint64_t n_prompts, uint64_t beams, uint64_t vocab,
                                          uint64_t k);
