@@ -232,6 +232,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         const uint32_t key = logit_key(c.x);
         int rank = 0;
         for (int u = 0; u < 4; u++)
+#pragma unroll 8
             for (int i = 0; i < count_s[u]; i++) {
                 const Candidate o = list[u][i];
                 const uint32_t ok = logit_key(o.x);
@@ -255,11 +256,22 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ float score_s[NEAR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
     const int64_t row0 = (int64_t)blockIdx.x * a.beams;
+    const int per = a.chunks * k;
+    const int64_t n = (int64_t)a.beams * per;
+    const Candidate *list = a.list + row0 * per;
+    Candidate held_c[HELD];  // (asked for before the sums)
+#pragma unroll
+    for (int j = 0; j < HELD; j++) {
+        held_c[j] = Candidate{0.f, NO_TOKEN};
+        if (tid + (int64_t)JOIN * j < n) held_c[j] = list[tid + (int64_t)JOIN * j];
+    }
     for (int b = wave; b < a.beams; b += JOIN / 64) {
-        double m = -INFINITY, sum = 0;
+        double sum = 0;
+        float most = -INFINITY;  // (the maxima are f32)
         const double *st = a.stats + (row0 + b) * a.chunks * 8;
-        for (int c = lane; c < 4 * a.chunks; c += 64) m = fmax(m, st[2 * c]);
-        for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+        for (int c = lane; c < 4 * a.chunks; c += 64) most = fmaxf(most, (float)st[2 * c]);
+        for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+        const double m = most;
         for (int c = lane; c < 4 * a.chunks; c += 64) {
             const double cm = st[2 * c], cs = st[2 * c + 1];
             sum += cm == -INFINITY ? cs : cs * exp(cm - m);
@@ -273,16 +285,12 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     if (tid == 0) put = 0;
     __syncthreads();
 
-    const int per = a.chunks * k;
-    const int64_t n = (int64_t)a.beams * per;
-    const Candidate *list = a.list + row0 * per;
     struct Item {
         uint64_t key, tie;  // tie: beam, then the logit, inverted: smaller first
         uint32_t token;
         float score;
     };
-    auto item = [&](int64_t e) {
-        const Candidate c = list[e];
+    auto item = [&](int64_t e, Candidate c) {
         const int b = (int)(e / per);
         const double s = prev_s[b] + ((double)c.x - lse_s[b]);
         return Item{score_key(s), (uint64_t)b << 32 | (uint32_t)~logit_key(c.x), c.token, (float)s};
@@ -291,14 +299,14 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
 #pragma unroll
     for (int j = 0; j < HELD; j++) {
         held[j] = Item{0, 0, NO_TOKEN, 0.f};
-        if (tid + (int64_t)JOIN * j < n) held[j] = item(tid + (int64_t)JOIN * j);
+        if (held_c[j].token != NO_TOKEN) held[j] = item(tid + (int64_t)JOIN * j, held_c[j]);
     }
     auto each = [&](auto &&f) {
 #pragma unroll
         for (int j = 0; j < HELD; j++)
             if (held[j].token != NO_TOKEN) f(held[j]);
         for (int64_t e = tid + (int64_t)JOIN * HELD; e < n; e += JOIN) {
-            const Item it = item(e);
+            const Item it = item(e, list[e]);
             if (it.token != NO_TOKEN) f(it);
         }
     };
@@ -310,7 +318,7 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
         for (int j = 0; j < HELD; j++) c += __popcll(__ballot(held[j].token != NO_TOKEN && takes(held[j])));
         for (int64_t e = (int64_t)JOIN * HELD; e < n; e += JOIN) {
             Item it{0, 0, NO_TOKEN, 0.f};
-            if (e + tid < n) it = item(e + tid);
+            if (e + tid < n) it = item(e + tid, list[e + tid]);
             c += __popcll(__ballot(it.token != NO_TOKEN && takes(it)));
         }
         if (lane == 0) count_s[turn][wave] = c;
@@ -357,7 +365,7 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
         if (c >= k) {
             low = mid;
             reach = c;
-            if (c <= k + 64) break;  // few enough to rank
+            if (c <= k + k / 2 + 8) break;  // few enough to rank
         } else high = mid - 1;
     }
     // should more than can be ranked reach it: exactly k; among equal scores the lowest beams, in a beam the largest logits, among equal logits the lowest tokens
@@ -398,9 +406,15 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     if (tid < n_near) {
         const uint64_t key = key_s[tid], t = tie_s[tid];
         const uint32_t tok = token_s[tid];
-        int rank = 0;
-        for (int i = 0; i < n_near; i++)
-            rank += key_s[i] > key || (key_s[i] == key && (tie_s[i] < t || (tie_s[i] == t && token_s[i] < tok)));
+        int rank = 0, same = 0;
+#pragma unroll 8
+        for (int i = 0; i < n_near; i++) {
+            rank += key_s[i] > key;
+            same += key_s[i] == key;
+        }
+        if (same > 1)
+            for (int i = 0; i < n_near; i++)
+                rank += key_s[i] == key && (tie_s[i] < t || (tie_s[i] == t && token_s[i] < tok));
         if (rank < k) {
             const int64_t o = (int64_t)blockIdx.x * k + rank;
             a.scores[o] = score_s[tid];
