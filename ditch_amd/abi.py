@@ -258,6 +258,7 @@ PROTOTYPES = {
     "ditch_hip_forward_cached": (I32, [P, P, P, P, U64, P, U64, P, U64]),
     "ditch_hip_sampler_init": (I32, [P, U64, FLT, U64, FLT]),
     "ditch_hip_pick_tokens_device": (I32, [P, P, P, U64, U64, P, P]),
+    "ditch_hip_kv_cache_create_pages": (P, [P, U32, U32, I32, U32, U32, U32]),
     "ditch_hip_kv_pages_codes_bytes": (U64, [P]),
     "ditch_hip_kv_pages_scales_bytes": (U64, [P]),
     "ditch_hip_kv_pages_append_device": (I32, [P, P, U32, P, I32, P, P, P, P, P, U64, P]),

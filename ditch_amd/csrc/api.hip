@@ -24,6 +24,8 @@ void model_edit_batch(ditch_hip_model *m, const ditch_edit_target *targets, uint
 void model_edit_ex(ditch_hip_model *m, int layer, int slot, int expert, const float *v, uint64_t k, float weight,
                    int mode, int64_t lora_rank, uint64_t seed, int ablate);
 ditch_hip_kv_cache *kv_cache_create(ditch_hip_model *m, int64_t B, int64_t T);
+ditch_hip_kv_cache *kv_cache_create_pages(ditch_hip_model *m, int64_t B, int64_t T, int32_t kind, uint32_t page,
+                                          uint32_t window, uint32_t sinks);
 ditch_hip_model *model_load(ditch_hip *h, const char *path, uint64_t expert_cache);
 void generate(ditch_hip_model *m, ditch_hip_kv_cache *kc, const uint32_t *tokens, const uint64_t *lens, int64_t B,
               int64_t max_new, const uint32_t *eos, int64_t n_eos, ditch_sampler *smp, uint32_t *out_tokens,
@@ -31,7 +33,8 @@ void generate(ditch_hip_model *m, ditch_hip_kv_cache *kc, const uint32_t *tokens
 uint64_t model_bytes(const ditch_hip_model *m);
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
-                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc = nullptr);
+                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc = nullptr,
+                   int64_t max_rows = 0);
 
 // Device buffer owned for the duration of one call.
 struct Tmp {
@@ -714,6 +717,17 @@ ditch_hip_kv_cache *ditch_hip_kv_cache_create(ditch_hip_model *m, uint32_t n_pro
     if (!m) return nullptr;
     ditch_hip_kv_cache *c = nullptr;
     int32_t rc = guarded(m->h, [&] { c = kv_cache_create(m, (int64_t)n_prompts, (int64_t)max_len); });
+    return rc == DITCH_OK ? c : nullptr;
+}
+
+ditch_hip_kv_cache *ditch_hip_kv_cache_create_pages(ditch_hip_model *m, uint32_t n_prompts, uint32_t max_len,
+                                                    int32_t kind, uint32_t page_tokens, uint32_t window,
+                                                    uint32_t sinks) {
+    if (!m) return nullptr;
+    ditch_hip_kv_cache *c = nullptr;
+    int32_t rc = guarded(m->h, [&] {
+        c = kv_cache_create_pages(m, (int64_t)n_prompts, (int64_t)max_len, kind, page_tokens, window, sinks);
+    });
     return rc == DITCH_OK ? c : nullptr;
 }
 

@@ -19,7 +19,7 @@ namespace ditch {
 
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
-                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc);
+                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows);
 
 constexpr int PICK_MAXK = 256;  // Sampler.max_top_k
 constexpr int PICK_ROWS = 256;  // rows per launch: their draws travel in the arguments
@@ -256,11 +256,12 @@ void generate(ditch_hip_model *m, ditch_hip_kv_cache *kc, const uint32_t *tokens
     DITCH_CHECK(max_new >= 1, DITCH_INVALID_ARGUMENT, "generate: max_new_tokens must be at least 1");
     const int64_t V = (int64_t)c.vocab;
     const uint64_t rows_embed = m->embed.ok() ? (uint64_t)m->embed.t->v.rows : 0;
-    int64_t total = 0;
+    int64_t total = 0, longest = 0;
     for (int64_t b = 0; b < B; b++) {
         DITCH_CHECK(lens[b] >= 1 && (int64_t)lens[b] <= kc->T, DITCH_INVALID_ARGUMENT,
                     "generate: a prompt is empty or longer than the KV cache");
         total += (int64_t)lens[b];
+        longest = (int64_t)lens[b] > longest ? (int64_t)lens[b] : longest;
     }
     for (int64_t i = 0; i < total; i++)
         DITCH_CHECK(tokens[i] < rows_embed, DITCH_INVALID_ARGUMENT, "generate: token id outside the embedding table");
@@ -282,7 +283,7 @@ void generate(ditch_hip_model *m, ditch_hip_kv_cache *kc, const uint32_t *tokens
     DITCH_TRY_HIP(hipMemcpyAsync(dt, tokens, total * 4, hipMemcpyHostToDevice, s));
     DITCH_TRY_HIP(hipMemcpyAsync(dr, rows.data(), total * sizeof(ditch_row), hipMemcpyHostToDevice, s));
     DITCH_TRY_HIP(hipMemcpyAsync(dl, last.data(), B * 8, hipMemcpyHostToDevice, s));
-    model_forward(m, dt, dr, total, kc->B, kc->T, nullptr, 0, nullptr, dl, B, dlog, kc);
+    model_forward(m, dt, dr, total, kc->B, kc->T, nullptr, 0, nullptr, dl, B, dlog, kc, longest);
     launch_pick(dp, dlog, B, V, smp, s);
     std::vector<uint32_t> picked(B), ids;
     DITCH_TRY_HIP(hipMemcpyAsync(picked.data(), dp, B * 4, hipMemcpyDeviceToHost, s));
@@ -324,7 +325,7 @@ void generate(ditch_hip_model *m, ditch_hip_kv_cache *kc, const uint32_t *tokens
         DITCH_TRY_HIP(hipMemcpyAsync(dt, step_tok.data(), n * 4, hipMemcpyHostToDevice, s));
         DITCH_TRY_HIP(hipMemcpyAsync(dr, step_rows.data(), n * sizeof(ditch_row), hipMemcpyHostToDevice, s));
         DITCH_TRY_HIP(hipMemcpyAsync(dl, step_lr.data(), n * 8, hipMemcpyHostToDevice, s));
-        model_forward(m, dt, dr, n, kc->B, kc->T, nullptr, 0, nullptr, dl, n, dlog, kc);
+        model_forward(m, dt, dr, n, kc->B, kc->T, nullptr, 0, nullptr, dl, n, dlog, kc, 1);
         launch_pick(dp, dlog, n, V, smp, s);
         DITCH_TRY_HIP(hipMemcpyAsync(picked.data(), dp, n * 4, hipMemcpyDeviceToHost, s));
         DITCH_TRY_HIP(hipStreamSynchronize(s));

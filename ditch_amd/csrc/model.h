@@ -161,6 +161,13 @@ struct ditch_hip_kv_cache {
     ditch_hip_model *m = nullptr;
     int64_t B = 0, T = 0, kvd = 0, layers = 0;
     float *k = nullptr, *v = nullptr;
+    // in pages of 8-bit codes instead (ditch_hip_kv_cache_create_pages): every
+    // prompt's own pages in order, and the rows of the call at hand
+    ditch_kv_pages pages{};
+    uint32_t window = 0, sinks = 0;
+    int64_t cols = 0;  // pages a prompt
+    ditch::DevBuf codes, scales, table, starts, pos, ws;
+    bool paged() const { return pages.n_pages != 0; }
     ~ditch_hip_kv_cache();
 };
 

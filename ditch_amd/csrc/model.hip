@@ -13,6 +13,7 @@
 #include "gemm_few.h"
 #include "tiled.h"
 #include "model.h"
+#include "pages.h"
 
 namespace ditch {
 
@@ -1419,14 +1420,15 @@ static void moe_forward(ditch_hip_model *m, Layer &L, float *x, const float *h, 
 // wrote (decode steps after a prefill).
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
-                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc) {
+                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows) {
     const ditch_model_config &c = m->c;
     hipStream_t s = m->h->stream;
     if (n <= 0) return;
     DITCH_CHECK(m->embed.ok(), DITCH_INVALID_ARGUMENT, "forward: no embedding");
     int64_t hidden = (int64_t)c.hidden;
     DITCH_CHECK(B > 0 && T > 0 && B <= (int64_t)INT32_MAX, DITCH_INVALID_ARGUMENT, "forward: KV cache shape");
-    DITCH_CHECK(T <= ATT_MAXK, DITCH_UNSUPPORTED, "forward: positions beyond 1024 per prompt");
+    const bool paged = pc && pc->paged();
+    DITCH_CHECK(paged || T <= ATT_MAXK, DITCH_UNSUPPORTED, "forward: positions beyond 1024 per prompt");
     int64_t nh = (int64_t)c.heads, nkv = c.mla ? nh : (int64_t)c.kv_heads, hd = (int64_t)c.head_dim;
     int64_t vd = c.mla ? (int64_t)c.v_head_dim : hd;
     DITCH_CHECK(hd <= 512, DITCH_UNSUPPORTED, "forward: head_dim above 512");
@@ -1440,6 +1442,23 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
                     "forward: the KV cache belongs to another model or shape");
     }
     float *kc = pc ? pc->k : m->kc.get<float>(B * T * kvd), *vc = pc ? pc->v : m->vc.get<float>(B * T * kvd);
+    // a paged cache: the rows as its batch (see launch_rows_batch), and its attention's workspace
+    BatchView batch{};
+    PagesAttention pa{};
+    if (paged) {
+        const ditch_kv_batch kb{pc->table.get<int32_t>(0), (uint32_t)pc->cols, (uint32_t)B, pc->starts.get<uint32_t>(0),
+                                pc->pos.get<uint32_t>(0), (uint64_t)n, (uint32_t)std::min(max_rows ? max_rows : n, T), (uint32_t)T};
+        pa.p = pool_view(&pc->pages, 0);
+        pa.b = batch = batch_view(&kb, pa.p);
+        pa.dtype = DITCH_F32;
+        pa.heads = (int32_t)nh;
+        pa.scale = c.attn_scale;
+        pa.window = (int32_t)pc->window;
+        pa.sinks = (int32_t)pc->sinks;
+        pa.few = !max_rows && n <= B;  // one row a prompt, as far as can be told
+        (void)pc->ws.get<uint8_t>(pages_attention_workspace(pa.p, batch, pa.heads, DITCH_F32, pc->window, pc->sinks, pa.few));
+        launch_rows_batch(d_rows, n, B, T, pc->starts.get<uint32_t>(0), pc->pos.get<uint32_t>(0), s);
+    }
     int *dense_flag = m->attn_dense.get<int>(1);  // checked at the first layer that can use it
     bool dense_checked = false;
 
@@ -1534,86 +1553,100 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
             mm_act(m, L.k, kk, hact, n, L.k_bias.p, 0, s);
             mm_act(m, L.v, vv, hact, n, L.v_bias.p, 0, s);
         }
-        if (pc) {  // this layer's slice of the persistent cache
+        if (paged) {
+            if (c.qk_norm) {
+                launch_rmsnorm(q, q, L.q_norm.p, L.q_norm.len, n * nh, hd, c.rms_eps, 0, s);
+                launch_rmsnorm(kk, kk, L.k_norm.p, L.k_norm.len, n * nkv, hd, c.rms_eps, 0, s);
+            }
+            pa.p = pool_view(&pc->pages, (uint32_t)li);
+            pa.q = RowsView{q, qd};
+            pa.out = RowsView{att, nh * vd};
+            const RopeView rope{m->rope_cos, m->rope_sin, (int32_t)(c.rotary_dim / 2), c.rope_style};
+            launch_pages_append(pa.p, batch, DITCH_F32, RowsView{kk, kvd}, RowsView{vv, nkv * vd}, rope, &pa.q, &pa.q,
+                                (int)nh, s);
+            launch_pages_attention(pa, pc->ws.p, pc->ws.bytes, s);
+        } else if (pc) {  // this layer's slice of the persistent cache
             kc = pc->k + li * B * T * kvd;
             vc = pc->v + li * B * T * kvd;
         }
-        // the attention kernels this layer takes; with the whole-prompt kernel
-        // (decided on the device by the dense check) and a whole-head neox
-        // RoPE of head_dim 128 without a query norm, that kernel rotates the
-        // queries as it loads them and the RoPE kernel leaves them alone
-        const bool mfma_attn = attention_mfma_takes(hd, vd, nh / nkv);
-        const bool frag_epi = attn_split_fragments && frags && mfma_attn && (nh * vd) % 128 == 0 &&
-                              frag_only(L.o, n) && !mx_only(L.o, n);
-        const bool row_attn = attention_rows_takes(hd, vd, nh / nkv, n, B, T);
-        const bool prompt_attn = mfma_attn && !row_attn && !frag_epi && attention_prompt_takes(hd, vd, T);
-        const bool q_rope_in_attn = prompt_attn && !c.mla && hd == 128 && c.rotary_dim == 128 &&
-                                    c.rope_style == DITCH_ROPE_NEOX && !c.qk_norm;
-        if (prompt_attn && !dense_checked) {
-            launch_attention_dense_check(d_rows, n, T, B, dense_flag, s);
-            dense_checked = true;
-        }
-        RopeArgs ra{};
-        ra.q = q;
-        ra.k = kk;
-        ra.v = vv;
-        ra.kc = kc;
-        ra.vc = vc;
-        ra.rows = d_rows;
-        ra.cos_t = m->rope_cos;
-        ra.sin_t = m->rope_sin;
-        ra.q_norm = c.qk_norm ? L.q_norm.p : nullptr;
-        ra.k_norm = c.qk_norm ? L.k_norm.p : nullptr;
-        ra.n = n;
-        ra.heads = nh;
-        ra.kv_heads = nkv;
-        ra.hd = hd;
-        ra.rope_off = c.mla ? (int64_t)c.qk_nope_dim : 0;
-        ra.rot = (int64_t)(c.rotary_dim / 2 * 2);
-        ra.half = (int64_t)(c.rotary_dim / 2);
-        ra.rope_len = (int64_t)c.rope_len;
-        ra.T = T;
-        ra.nb = B;
-        ra.kvd = kvd;
-        ra.eps = c.rms_eps;
-        ra.style = c.rope_style;
-        ra.dense = q_rope_in_attn ? dense_flag : nullptr;
-        ra.q_in_attn = q_rope_in_attn ? 1 : 0;
-        if (mla_fused) {
-            MlaCacheArgs ma{q, mla_kvb, mla_kva, kc, vc, d_rows, m->rope_cos, m->rope_sin, nh, hd,
-                            (int64_t)c.qk_nope_dim, (int64_t)c.qk_rope_dim, vd, (int64_t)c.kv_lora_rank, ra.half,
-                            ra.rope_len, T, B, kvd, c.rope_style};
-            hipLaunchKernelGGL(mla_rope_cache_kernel, dim3((unsigned)n), dim3(256), 0, s, ma);
-        } else {
-            // a wave a head (four of 128) until the rows alone fill the CUs
-            const int64_t per = hd == 128 ? 16 : 4, split = n < 256 ? (nh + nkv + per - 1) / per : 1;
-            hipLaunchKernelGGL(qk_rope_cache_kernel, dim3((unsigned)n, (unsigned)split), dim3(256), 0, s, ra);
-        }
-        DITCH_TRY_HIP(hipGetLastError());
-        AttnArgs aa{q, kc, vc, att, d_rows, n, nh, nh / nkv, hd, vd, T, kvd, c.attn_scale, nullptr, 0, B, nullptr};
         Act aact{att, nullptr, 0};
-        // (the kernel's own bf16-fragment epilogue needs 34 KB more LDS a
-        // workgroup, which halves its occupancy: the o product splitting the
-        // f32 rows costs less)
-        if (frag_epi) {
-            aa.ldk = split_ldk(nh * vd);
-            aa.xs = m->atts.get<uint8_t>(split_bytes_ldk(n, aa.ldk, 2));
-            aact = Act{att, aa.xs, aa.ldk};
+        if (!paged) {
+            // the attention kernels this layer takes; with the whole-prompt kernel
+            // (decided on the device by the dense check) and a whole-head neox
+            // RoPE of head_dim 128 without a query norm, that kernel rotates the
+            // queries as it loads them and the RoPE kernel leaves them alone
+            const bool mfma_attn = attention_mfma_takes(hd, vd, nh / nkv);
+            const bool frag_epi = attn_split_fragments && frags && mfma_attn && (nh * vd) % 128 == 0 &&
+                                  frag_only(L.o, n) && !mx_only(L.o, n);
+            const bool row_attn = attention_rows_takes(hd, vd, nh / nkv, n, B, T);
+            const bool prompt_attn = mfma_attn && !row_attn && !frag_epi && attention_prompt_takes(hd, vd, T);
+            const bool q_rope_in_attn = prompt_attn && !c.mla && hd == 128 && c.rotary_dim == 128 &&
+                                        c.rope_style == DITCH_ROPE_NEOX && !c.qk_norm;
+            if (prompt_attn && !dense_checked) {
+                launch_attention_dense_check(d_rows, n, T, B, dense_flag, s);
+                dense_checked = true;
+            }
+            RopeArgs ra{};
+            ra.q = q;
+            ra.k = kk;
+            ra.v = vv;
+            ra.kc = kc;
+            ra.vc = vc;
+            ra.rows = d_rows;
+            ra.cos_t = m->rope_cos;
+            ra.sin_t = m->rope_sin;
+            ra.q_norm = c.qk_norm ? L.q_norm.p : nullptr;
+            ra.k_norm = c.qk_norm ? L.k_norm.p : nullptr;
+            ra.n = n;
+            ra.heads = nh;
+            ra.kv_heads = nkv;
+            ra.hd = hd;
+            ra.rope_off = c.mla ? (int64_t)c.qk_nope_dim : 0;
+            ra.rot = (int64_t)(c.rotary_dim / 2 * 2);
+            ra.half = (int64_t)(c.rotary_dim / 2);
+            ra.rope_len = (int64_t)c.rope_len;
+            ra.T = T;
+            ra.nb = B;
+            ra.kvd = kvd;
+            ra.eps = c.rms_eps;
+            ra.style = c.rope_style;
+            ra.dense = q_rope_in_attn ? dense_flag : nullptr;
+            ra.q_in_attn = q_rope_in_attn ? 1 : 0;
+            if (mla_fused) {
+                MlaCacheArgs ma{q, mla_kvb, mla_kva, kc, vc, d_rows, m->rope_cos, m->rope_sin, nh, hd,
+                                (int64_t)c.qk_nope_dim, (int64_t)c.qk_rope_dim, vd, (int64_t)c.kv_lora_rank, ra.half,
+                                ra.rope_len, T, B, kvd, c.rope_style};
+                hipLaunchKernelGGL(mla_rope_cache_kernel, dim3((unsigned)n), dim3(256), 0, s, ma);
+            } else {
+                // a wave a head (four of 128) until the rows alone fill the CUs
+                const int64_t per = hd == 128 ? 16 : 4, split = n < 256 ? (nh + nkv + per - 1) / per : 1;
+                hipLaunchKernelGGL(qk_rope_cache_kernel, dim3((unsigned)n, (unsigned)split), dim3(256), 0, s, ra);
+            }
+            DITCH_TRY_HIP(hipGetLastError());
+            AttnArgs aa{q, kc, vc, att, d_rows, n, nh, nh / nkv, hd, vd, T, kvd, c.attn_scale, nullptr, 0, B, nullptr};
+            // (the kernel's own bf16-fragment epilogue needs 34 KB more LDS a
+            // workgroup, which halves its occupancy: the o product splitting the
+            // f32 rows costs less)
+            if (frag_epi) {
+                aa.ldk = split_ldk(nh * vd);
+                aa.xs = m->atts.get<uint8_t>(split_bytes_ldk(n, aa.ldk, 2));
+                aact = Act{att, aa.xs, aa.ldk};
+            }
+            if (prompt_attn) aa.dense = dense_flag;
+            // few rows: the row kernel writes the o product's fragments (the f32
+            // rows too when a delta reads them)
+            if (row_attn && few && !few_rows && small_frags(L.o, n) && (nh * vd) % 128 == 0) {
+                aa.ldk = split_ldk(nh * vd);
+                aa.xs = m->atts.get<uint8_t>(split_bytes_ldk(n, aa.ldk, 2));
+                if (L.o.rank == 0) aa.out = nullptr;
+                aact = Act{aa.out, aa.xs, aa.ldk};
+            }
+            if (row_attn) launch_attention_rows(aa, nkv, s);
+            else if (q_rope_in_attn) launch_attention_mfma_rope(aa, AttnRope{m->rope_cos, m->rope_sin, (int64_t)c.rope_len}, nkv, s);
+            else if (mfma_attn) launch_attention_mfma(aa, nkv, s);
+            else hipLaunchKernelGGL(attention_kernel, dim3((unsigned)((n * nh + 3) / 4)), dim3(256), 0, s, aa);
+            DITCH_TRY_HIP(hipGetLastError());
         }
-        if (prompt_attn) aa.dense = dense_flag;
-        // few rows: the row kernel writes the o product's fragments (the f32
-        // rows too when a delta reads them)
-        if (row_attn && few && !few_rows && small_frags(L.o, n) && (nh * vd) % 128 == 0) {
-            aa.ldk = split_ldk(nh * vd);
-            aa.xs = m->atts.get<uint8_t>(split_bytes_ldk(n, aa.ldk, 2));
-            if (L.o.rank == 0) aa.out = nullptr;
-            aact = Act{aa.out, aa.xs, aa.ldk};
-        }
-        if (row_attn) launch_attention_rows(aa, nkv, s);
-        else if (q_rope_in_attn) launch_attention_mfma_rope(aa, AttnRope{m->rope_cos, m->rope_sin, (int64_t)c.rope_len}, nkv, s);
-        else if (mfma_attn) launch_attention_mfma(aa, nkv, s);
-        else hipLaunchKernelGGL(attention_kernel, dim3((unsigned)((n * nh + 3) / 4)), dim3(256), 0, s, aa);
-        DITCH_TRY_HIP(hipGetLastError());
         mm_act(m, L.o, x, aact, n, nullptr, 1, s);  // x += o(att)
         const bool moe_layer = c.n_experts && m->moe_layers[li];
         if (!moe_layer)
@@ -1757,6 +1790,46 @@ ditch_hip_kv_cache::~ditch_hip_kv_cache() {
 }
 
 namespace ditch {
+
+ditch_hip_kv_cache *kv_cache_create_pages(ditch_hip_model *m, int64_t B, int64_t T, int32_t kind, uint32_t page,
+                                          uint32_t window, uint32_t sinks) {
+    const ditch_model_config &c = m->c;
+    hipStream_t s = m->h->stream;
+    DITCH_CHECK(!c.mla, DITCH_UNSUPPORTED, "kv cache: pages of a model with latent attention");
+    DITCH_CHECK(B > 0 && T > 0 && T <= (int64_t)c.rope_len, DITCH_INVALID_ARGUMENT,
+                "kv cache: 1 to rope_len positions and at least one prompt");
+    DITCH_CHECK(window <= (uint32_t)INT32_MAX && sinks <= (uint32_t)INT32_MAX, DITCH_INVALID_ARGUMENT,
+                "kv cache: window or sinks above 2^31");
+    DITCH_CHECK(page == 32 || page == 64 || page == 128 || page == 256, DITCH_INVALID_ARGUMENT,
+                "kv cache: pages of 32, 64, 128 or 256 tokens");
+    const int64_t cols = (T + page - 1) / page;
+    DITCH_CHECK(B <= (int64_t)INT32_MAX / cols, DITCH_INVALID_ARGUMENT, "kv cache: more than 2^31 pages");
+    std::unique_ptr<ditch_hip_kv_cache> kc(new ditch_hip_kv_cache());
+    kc->m = m;
+    kc->B = B;
+    kc->T = T;
+    kc->kvd = (int64_t)(c.kv_heads * c.head_dim);
+    kc->layers = (int64_t)c.layers;
+    kc->cols = cols;
+    kc->window = window;
+    kc->sinks = sinks;
+    ditch_kv_pages &p = kc->pages;
+    p.kind = kind;
+    p.layers = (uint32_t)c.layers;
+    p.n_pages = (uint32_t)(B * cols);
+    p.page_tokens = page;
+    p.kv_heads = (uint32_t)c.kv_heads;
+    p.head_dim = p.v_head_dim = (uint32_t)c.head_dim;
+    p.codes_bytes = pool_codes_bytes(&p);
+    p.scales_bytes = pool_scales_bytes(&p);
+    DITCH_CHECK(p.codes_bytes && c.head_dim <= 256, DITCH_INVALID_ARGUMENT, "kv cache: kind or head_dim");
+    p.codes = kc->codes.get<uint8_t>(p.codes_bytes);
+    p.scales = kc->scales.get<float>(p.scales_bytes / 4);
+    (void)kc->starts.get<uint32_t>(B + 1);
+    (void)kc->pos.get<uint32_t>(B);
+    launch_own_pages(kc->table.get<int32_t>(B * cols), B * cols, s);
+    return kc.release();
+}
 
 ditch_hip_kv_cache *kv_cache_create(ditch_hip_model *m, int64_t B, int64_t T) {
     const ditch_model_config &c = m->c;

@@ -97,6 +97,14 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
                        int64_t table_stride, const int32_t *parents, const int32_t *spare, const uint32_t *lens,
                        int64_t groups, int64_t beams, hipStream_t s);
 
+// The batch of a forward's rows {b, pos}, sorted by prompt and position:
+// starts [B + 1] and pos [B]; a prompt whose rows are not consecutive gets
+// the position max_len, past which nothing is appended and outputs are NaN.
+void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *pos,
+                       hipStream_t s);
+// table [B][cols] = b cols + j
+void launch_own_pages(int32_t *table, int64_t n, hipStream_t s);
+
 // pages_attention.hip
 struct PagesAttention {
     PoolView p;
@@ -105,9 +113,10 @@ struct PagesAttention {
     int32_t dtype, heads;
     float scale;
     int32_t window, sinks;
+    int32_t few;  // max_rows is a bound that few sequences reach: the few-row kernel
 };
 size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int heads, int32_t dtype, uint32_t window,
-                                 uint32_t sinks);
+                                 uint32_t sinks, int few = 0);
 void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, hipStream_t s);
 
 // beam.hip

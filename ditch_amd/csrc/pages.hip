@@ -135,14 +135,20 @@ __device__ __forceinline__ double rotated(const T *x, int d, int half, int style
 template <int KIND>
 __device__ __forceinline__ uint8_t nearest_code(double y) {
     constexpr double most = KIND == DITCH_KV_INT8 ? 127.0 : 448.0;
-    y = fmin(fmax(y, -most), most);
-    if constexpr (KIND == DITCH_KV_INT8) return (uint8_t)(int8_t)(int)rint(y);
-    // e4m3: 3 bits behind the leading one, the least step 2^-9
-    int e = (int)((__double_as_longlong(y) >> 52) & 0x7ff) - 1023;
-    e = e < -6 ? -6 : e;
-    const double up = __longlong_as_double((int64_t)(1023 + 3 - e) << 52);
-    const double down = __longlong_as_double((int64_t)(1023 - 3 + e) << 52);
-    const float v = (float)(rint(y * up) * down);  // a code's value: the conversion is exact
+    if constexpr (KIND == DITCH_KV_INT8) return (uint8_t)(int8_t)(int)rint(fmin(fmax(y, -most), most));
+    // e4m3: 3 bits behind the leading one, the least step 2^-9. Through f32
+    // and the conversion instruction the value is rounded twice, which differs
+    // from once only where the f32 value is half way between two codes (its
+    // low 20 bits say so above 2^-6): there, and below, in 64 bits.
+    float v = fminf(fmaxf((float)y, (float)-most), (float)most);
+    if ((__float_as_uint(v) & 0xfffffu) == 0x80000u || fabsf(v) < 0.015625f) {
+        y = fmin(fmax(y, -most), most);
+        int e = (int)((__double_as_longlong(y) >> 52) & 0x7ff) - 1023;
+        e = e < -6 ? -6 : e;
+        const double up = __longlong_as_double((int64_t)(1023 + 3 - e) << 52);
+        const double down = __longlong_as_double((int64_t)(1023 - 3 + e) << 52);
+        v = (float)(rint(y * up) * down);  // a code's value: the conversion is exact
+    }
     return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff);
 }
 
@@ -217,6 +223,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs &a, const SeqRow
     const bool fours = half % 4 == 0 && quads_ok<T>(a.q, hd) && quads_ok<T>(a.q_out, hd);
     const int n_pairs = (half + 3) / 4, n_rest = (hd - 2 * half + 3) / 4, per = n_pairs + n_rest;
     const bool table = half % 4 == 0 && ((uintptr_t)a.rope.cos_t | (uintptr_t)a.rope.sin_t) % 16 == 0;
+#pragma unroll 2
     for (int e = part * 256 + threadIdx.x; e < a.heads * per; e += a.q_parts * 256) {
         const int h = e / per, j = e % per;
         const T *x = src + (int64_t)h * hd;
@@ -369,6 +376,7 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
         });
     } else if (quads) {
         const int per = D / 4;
+#pragma unroll 2
         for (int e = tid; e < (hi - lo) * per; e += 256) {
             float v[4];
             load4(v, rows + (int64_t)(lo + e / per) * rv.stride + e % per * 4, true, 4);
@@ -427,6 +435,7 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
         } else {
             // a dim of four tokens that lie next to each other in the page
             const int q0 = n0 / 4, q1 = (n1 + 3) / 4;
+#pragma unroll 2
             for (int e = tid; e < (q1 - q0) * D; e += 256) {
                 const int t = (q0 + e / D) * 4, d = e % D;
                 uint32_t c[4];
@@ -647,6 +656,50 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
     const ForkArgs a{v.codes, v.scales, v.n_pages, v.page_bytes, v.page, v.n_pages, v.kv_heads, (int32_t)parts, table_out, spare_out,
                      table, parents, spare, lens, table_stride, (int32_t)beams};
     hipLaunchKernelGGL(pages_fork_kernel, dim3(grid_blocks(groups * beams, "kv fork"), (unsigned)lh), dim3(256), 0, s, a);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
+// ---------------------------------------------------------------------------
+// a model's own cache in pages
+
+// A wave a prompt: its first row, and whether its rows follow each other.
+__global__ __launch_bounds__(64) void rows_batch_kernel(const ditch_row *rows, uint32_t n, uint32_t B, uint32_t max_len,
+                                                        uint32_t *starts, uint32_t *pos) {
+    const uint32_t b = blockIdx.x, lane = threadIdx.x;
+    auto first_of = [&](uint32_t p) {
+        uint32_t lo = 0, hi = n;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (rows[mid].b < p) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const uint32_t s = first_of(b), e = b < B ? first_of(b + 1) : s;
+    if (lane == 0) starts[b] = s;
+    if (b == B) return;
+    const uint32_t p = s < e ? rows[s].pos : 0;
+    bool bad = false;
+    for (uint32_t i = s + lane; i < e; i += 64) bad |= rows[i].b != b || rows[i].pos != p + (i - s);
+    if (__any(bad)) {
+        if (lane == 0) pos[b] = max_len;
+    } else if (lane == 0) pos[b] = p;
+}
+
+__global__ __launch_bounds__(256) void own_pages_kernel(int32_t *table, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) table[i] = (int32_t)i;
+}
+
+void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *pos,
+                       hipStream_t s) {
+    hipLaunchKernelGGL(rows_batch_kernel, dim3((unsigned)(B + 1)), dim3(64), 0, s, rows, (uint32_t)n, (uint32_t)B,
+                       (uint32_t)max_len, starts, pos);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
+void launch_own_pages(int32_t *table, int64_t n, hipStream_t s) {
+    hipLaunchKernelGGL(own_pages_kernel, dim3(grid_blocks((n + 255) / 256, "kv cache")), dim3(256), 0, s, table, n);
     DITCH_TRY_HIP(hipGetLastError());
 }
 

@@ -261,8 +261,8 @@ static RowsPlan rows_plan(const PoolView &p, const BatchView &b, int heads, uint
 }
 
 size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int heads, int32_t dtype, uint32_t window,
-                                 uint32_t sinks) {
-    if (b.n_seqs == 0 || pages_chunk_takes(p, b, heads, dtype)) return 0;
+                                 uint32_t sinks, int few) {
+    if (b.n_seqs == 0 || (!few && pages_chunk_takes(p, b, heads, dtype))) return 0;
     const RowsPlan plan = rows_plan(p, b, heads, window, sinks);
     if (plan.splits == 1) return 0;
     return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 2) * 4;
@@ -305,7 +305,7 @@ static void rows_typed(const PagesAttention &a, const RowsPlan &plan, hipStream_
 
 void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, hipStream_t s) {
     if (a.b.n_seqs == 0) return;
-    if (pages_chunk_takes(a.p, a.b, a.heads, a.dtype)) return launch_pages_chunk(a, s);
+    if (!a.few && pages_chunk_takes(a.p, a.b, a.heads, a.dtype)) return launch_pages_chunk(a, s);
     RowsPlan plan = rows_plan(a.p, a.b, a.heads, (uint32_t)a.window, (uint32_t)a.sinks);
     if (plan.splits > 1) {
         plan.stats = (float *)ws;

@@ -483,6 +483,16 @@ class Model:
             raise DeviceError(abi.DEVICE_FAILED, self.dev.lib.ditch_hip_last_error(self.dev.h).decode())
         return c
 
+    def kv_cache_pages(self, n_prompts, max_len, kind="int8", page_tokens=64, window=0, sinks=0):
+        """kv_cache in pages of 8-bit codes (ditch_hip_kv_cache_create_pages),
+        max_len up to the model's rope_len; a window with the first `sinks`
+        positions visible, or 0 for all."""
+        c = self.dev.lib.ditch_hip_kv_cache_create_pages(self.h, n_prompts, max_len, abi.KV_KIND[kind], page_tokens,
+                                                         window, sinks)
+        if not c:
+            raise DeviceError(abi.DEVICE_FAILED, self.dev.lib.ditch_hip_last_error(self.dev.h).decode())
+        return c
+
     def kv_cache_free(self, c):
         self.dev.lib.ditch_hip_kv_cache_free(c)
 

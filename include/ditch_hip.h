@@ -765,6 +765,20 @@ int32_t ditch_hip_beam_select_device(ditch_hip *h, float *d_scores, int32_t *d_p
                                      uint64_t vocab, uint64_t k, void *ws, uint64_t ws_bytes,
                                      void *stream);
 
+/* ditch_hip_kv_cache_create with such pages of the model's own: the cache for
+ * ditch_hip_forward_cached and ditch_hip_generate in 8 bits (kind DITCH_KV_*,
+ * page_tokens as in ditch_kv_pages), for max_len up to the model's rope_len,
+ * past 1024 positions too; with window > 0 every layer attends to the last
+ * `window` positions and the first `sinks`. Every layer then appends, rotates
+ * and attends through the entries above. The rows of a call are a prompt's
+ * after the other's, each prompt's at consecutive positions (as generate
+ * passes them; rows of a prompt that are not give NaN). Models with latent
+ * attention are Unsupported. Freed by ditch_hip_kv_cache_free.             */
+ditch_hip_kv_cache *ditch_hip_kv_cache_create_pages(ditch_hip_model *m, uint32_t n_prompts,
+                                                    uint32_t max_len, int32_t kind,
+                                                    uint32_t page_tokens, uint32_t window,
+                                                    uint32_t sinks);
+
 /* ------------------------------------------------------------------------ */
 /* Rank-k edit, `none` mode (abliterate.zig:264-280): a = V^T W ([k][cols]),
  * b = -weight * V ([rows][k]) for directions v [k][rows]. Host buffers.    */
