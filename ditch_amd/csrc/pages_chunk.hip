@@ -22,6 +22,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
     constexpr int KP = DK / 64, VU = DV / 32, TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr int UNITS = 2 * KP + VU;              // of a granule's codes, 1 KB each
     constexpr int PER = (UNITS + NW - 1) / NW;      // of a granule, a wave
+    constexpr bool EVEN = UNITS % NW == 0;
     extern __shared__ __attribute__((aligned(16))) u32x4 ops[];  // [RING][2 UNITS][64]
     __shared__ int32_t id_s[META];
     __shared__ float key_s[META], bias_s[META], inverse_s[META];
@@ -98,14 +99,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int u = wave + i * NW;
-            if (u < UNITS) raw[i] = *(const u32x4 *)(u < 2 * KP ? kp + u * 1024 : vp + (u - 2 * KP) * 1024);
+            // (known when compiled where the waves share the units evenly: no branch in the loop)
+            const bool keys = 2 * KP % NW == 0 ? i < 2 * KP / NW : u < 2 * KP;
+            if (EVEN || u < UNITS) raw[i] = *(const u32x4 *)(keys ? kp + u * 1024 : vp + (u - 2 * KP) * 1024);
         }
     };
     auto store = [&](const u32x4 (&raw)[PER], int slot) {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int u = wave + i * NW;
-            if (u < UNITS) {
+            if (EVEN || u < UNITS) {
                 u32x4 *to = ops + ((slot * UNITS + u) * 2) * 64 + lane;
                 to[0] = __builtin_bit_cast(u32x4, codes_f16<KIND>(raw[i][0], raw[i][1]));
                 to[64] = __builtin_bit_cast(u32x4, codes_f16<KIND>(raw[i][2], raw[i][3]));
