@@ -241,9 +241,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 // against 51 us with 5 x 1500 rows under a window.
 constexpr int CHUNK_TILES = 2, CHUNK_WAVES = 4;
 
+// A workgroup here walks all of its keys by itself, so it takes enough of them
+// to fill the chip; the few-row kernel, in tiles of 16 queries, splits the keys
+// instead and is ahead below that. Both measured (int8, 32 heads of 128 over 8,
+// bf16, us few-row / chunk): 1024 tiles of 16 (512 rows, 4000 cached) 102 / 135,
+// 2048 (1024 rows, 2000 cached) 124 / 98, 2048 (8 x 128 rows, 1000 cached)
+// 63 / 50, 4096 (32 x 64 rows, 200 cached) 69 / 36; 14 heads of 64 over 2: 896
+// tiles 41 / 75, 1792 tiles 18 / 20. Under 64 queries a head half of a
+// workgroup's lanes hold none.
 bool pages_chunk_takes(const PoolView &p, const BatchView &b, int heads, int32_t dtype) {
     const int64_t queries = (int64_t)b.max_rows * (heads / p.kv_heads);
-    return queries >= 64;
+    return queries >= 64 && (int64_t)b.n_seqs * p.kv_heads * ((queries + 15) / 16) >= 1536;
 }
 
 template <typename T, int KIND, int DK, int DV>

@@ -382,37 +382,47 @@ ATTENTION = [
 ]
 
 
+# the bound that the call gives for a sequence's rows: what there are, or one
+# that thousands of workgroups find nothing behind (the chunk kernel's choice)
+BOUNDS = (None, 50000)
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("case", range(len(ATTENTION)))
-def test_attention(dev, case):
+def test_attention(dev, case, bound):
     kind, dtype, heads, kvh, hd, vd, page, seqs, window, sinks = ATTENTION[case]
     rng = np.random.default_rng(case)
     cols = max(-(-(r + p) // page) for r, p in seqs) + 1
     pool = _filled(rng, kind, 2, len(seqs) * cols + 2, page, kvh, hd, vd)
     _check_attention(dev, pool, _tables(rng, pool, len(seqs), cols), seqs, heads, dtype, window, sinks, layer=1,
-                     size=2.0, seed=case, stride=case % 3 * 4 + case % 2)
+                     size=2.0, seed=case, stride=case % 3 * 4 + case % 2, max_rows=bound)
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,pos,heads,kvh", [(1, 4500, 4, 1), (1, 9000, 2, 2), (2, 3000, 8, 1)])
-def test_long_contexts(dev, dtype, rows, pos, heads, kvh):
+def test_long_contexts(dev, dtype, rows, pos, heads, kvh, bound):
     """Lengths whose keys are split over workgroups and joined."""
     rng = np.random.default_rng(pos)
     cols = -(-(rows + pos) // 64)
     pool = _filled(rng, "int8", 1, cols + 2, 64, kvh, 64, 64)
-    _check_attention(dev, pool, _tables(rng, pool, 1, cols), [(rows, pos)], heads, dtype, size=3.0, seed=pos)
+    _check_attention(dev, pool, _tables(rng, pool, 1, cols), [(rows, pos)], heads, dtype, size=3.0, seed=pos,
+                     max_rows=bound)
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("rows", [1, 70])
-def test_scores_far_apart(dev, rows):
+def test_scores_far_apart(dev, rows, bound):
     """Scores of hundreds: one key takes everything, the others' weights underflow to zero."""
     rng = np.random.default_rng(1)
     pool = _filled(rng, "int8", 1, 12, 32, 2, 64, 64)
-    _check_attention(dev, pool, _tables(rng, pool, 1, 12), [(rows, 250)], 4, "f32", size=150.0)
+    _check_attention(dev, pool, _tables(rng, pool, 1, 12), [(rows, 250)], 4, "f32", size=150.0, max_rows=bound)
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("rows", [1, 64])
-def test_scales_of_every_size(dev, kind, rows):
+def test_scales_of_every_size(dev, kind, rows, bound):
     """Pages whose value scales differ by powers of ten, and one with a scale of zero (a page of zeros)."""
     rng = np.random.default_rng(12)
     pool = _filled(rng, kind, 1, 9, 64, 2, 128, 128)
@@ -420,18 +430,19 @@ def test_scales_of_every_size(dev, kind, rows):
     table = _tables(rng, pool, 1, 8)
     pool.scales[0, table[0, 2]] = 0
     pool.codes[0, table[0, 2]] = 0
-    _check_attention(dev, pool, table, [(rows, 400)], 4, "f32", seed=5)
+    _check_attention(dev, pool, table, [(rows, 400)], 4, "f32", seed=5, max_rows=bound)
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_dead_tokens_and_unseen_pages_do_not_matter(dev, dtype):
+def test_dead_tokens_and_unseen_pages_do_not_matter(dev, dtype, bound):
     """NaN scales, pages outside the pool and garbage codes where no query looks: behind the last token, in
     front of the window, in other layers."""
     rng = np.random.default_rng(13)
     pool = _filled(rng, "e4m3", 2, 20, 32, 2, 64, 64)
     table = _tables(rng, pool, 2, 9)
     seqs, window, sinks = [(1, 200), (40, 160)], 40, 3
-    clean = _check_attention(dev, pool, table, seqs, 4, dtype, window, sinks)
+    clean = _check_attention(dev, pool, table, seqs, 4, dtype, window, sinks, max_rows=bound)
     # between the sinks and every window: pages 1 and 2 of both sequences, pages 3 and 4 of the first
     for b in range(2):
         pool.scales[0, table[b, 1]] = np.nan
@@ -442,37 +453,39 @@ def test_dead_tokens_and_unseen_pages_do_not_matter(dev, dtype):
     # the dead tokens of the last page of sequence 0 (position 200 is token 8 of it): large, but codes
     for which in (0, 1):
         pool.codes[0, table[0, 6]][:, pool.off[which][9:]] = 0x7E
-    s = _check_attention(dev, pool, table, seqs, 4, dtype, window, sinks)
+    s = _check_attention(dev, pool, table, seqs, 4, dtype, window, sinks, max_rows=bound)
     np.testing.assert_array_equal(s, clean)
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("rows", [3, 80])
 @pytest.mark.parametrize("which", [0, 1])
-def test_poison_reaches_the_rows_that_see_it_only(dev, rows, which):
+def test_poison_reaches_the_rows_that_see_it_only(dev, rows, which, bound):
     rng = np.random.default_rng(14)
     pool = _filled(rng, "int8", 1, 8, 32, 2, 64, 64)
     table = _tables(rng, pool, 1, 8)
     at = (95 + rows) // 32  # the page that only the last rows see
     pool.scales[0, table[0, at], 1, which] = np.nan
-    got = _check_attention(dev, pool, table, [(rows, 96)], 4, "f32")
+    got = _check_attention(dev, pool, table, [(rows, 96)], 4, "f32", max_rows=bound)
     assert np.isnan(got[-1, 2:]).all() and np.isfinite(got[:, :2]).all()
     if rows > 3:
         assert np.isfinite(got[0]).all()
 
 
+@pytest.mark.parametrize("bound", BOUNDS)
 @pytest.mark.parametrize("rows", [2, 80])
-def test_attention_within_its_bounds(dev, rows):
+def test_attention_within_its_bounds(dev, rows, bound):
     """A visible page outside the pool gives NaN, rows past max_len NaN, rows past max_rows and rows of no sequence
     keep what they held."""
     rng = np.random.default_rng(15)
     pool = _filled(rng, "int8", 1, 8, 32, 1, 64, 64)
     table = np.array([[0, 1, 2, 3, 4, 5], [6, 9999, 7, 0, 1, 2]])
-    got = _check_attention(dev, pool, table, [(rows, 70), (rows, 20)], 2, "f32")
+    got = _check_attention(dev, pool, table, [(rows, 70), (rows, 20)], 2, "f32", max_rows=bound)
     assert np.isfinite(got[:rows]).all() and np.isnan(got[rows + 12:]).all()
     s = Setup(dev, pool, table)
     n = 2 * rows + 5
     q, out = Rows(dev, n, 128, "f32", rng.standard_normal((n, 128))), Rows(dev, n, 128, "f32")
-    s.attention(0, s.batch([0, rows], [70], n_rows=n, max_len=71), "f32", out, q, 2, 0.1)
+    s.attention(0, s.batch([0, rows], [70], n_rows=n, max_len=71, max_rows=bound), "f32", out, q, 2, 0.1)
     dev.sync()
     got = out.get()
     sentinel = out.host[:4].view(np.float32)[0]
@@ -484,7 +497,8 @@ def test_attention_within_its_bounds(dev, rows):
     assert (got[:2] == sentinel).all() and np.isfinite(got[2:1 + rows]).all() and (got[1 + rows:] == sentinel).all()
 
 
-def test_a_query_that_is_not_finite_gives_nan(dev):
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_a_query_that_is_not_finite_gives_nan(dev, bound):
     rng = np.random.default_rng(16)
     pool = _filled(rng, "int8", 1, 4, 64, 1, 64, 64)
     s = Setup(dev, pool, [[0, 1, 2, 3]])
@@ -493,20 +507,21 @@ def test_a_query_that_is_not_finite_gives_nan(dev):
             x = rng.standard_normal((rows, 3, 64))
             x[0, 1, 5] = bad
             q, out = Rows(dev, rows, 192, "f32", x), Rows(dev, rows, 192, "f32")
-            s.attention(0, s.batch([0, rows], [100]), "f32", out, q, 3, 0.125)
+            s.attention(0, s.batch([0, rows], [100], max_rows=bound), "f32", out, q, 3, 0.125)
             dev.sync()
             got = out.get().reshape(rows, 3, 64)
             assert np.isnan(got[0, 1]).all() and np.isfinite(got[:, 0]).all() and np.isfinite(got[:, 2]).all()
             assert np.isfinite(got[1:]).all()
 
 
-def test_queries_of_zero_and_of_extreme_size(dev):
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_queries_of_zero_and_of_extreme_size(dev, bound):
     rng = np.random.default_rng(17)
     pool = _filled(rng, "e4m3", 1, 4, 64, 1, 64, 64)
     for size in (0.0, 1e-30, 1e30):
         pool.scales[0, :, :, 0] = 1e-30 if size > 1 else 0.01
         for rows in (1, 40):
-            _check_attention(dev, pool, np.array([[2, 0, 1, 3]]), [(rows, 90)], 2, "f32", size=size)
+            _check_attention(dev, pool, np.array([[2, 0, 1, 3]]), [(rows, 90)], 2, "f32", size=size, max_rows=bound)
 
 
 # ---------------------------------------------------------------------------
