@@ -863,6 +863,8 @@ static void attention_shape(const ditch_kv_pages *p, const ditch_kv_batch *b, ui
                 "kv attention: query heads not a multiple of the KV heads (or above 65535)");
     DITCH_CHECK(window <= (uint32_t)INT32_MAX && sinks <= (uint32_t)INT32_MAX, DITCH_INVALID_ARGUMENT,
                 "kv attention: window or sinks above 2^31");
+    DITCH_CHECK((int64_t)bv.max_rows * (int64_t)(heads / pv.kv_heads) < (int64_t)1 << 30, DITCH_INVALID_ARGUMENT,
+                "kv attention: max_rows x query heads a KV head above 2^30");
 }
 
 uint64_t ditch_hip_kv_pages_attention_workspace(const ditch_kv_pages *p, const ditch_kv_batch *b, uint64_t heads,

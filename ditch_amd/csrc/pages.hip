@@ -94,6 +94,9 @@ RowsView rows_view(const ditch_kv_rows *r, uint64_t n_rows, uint64_t width, int3
     return RowsView{r->data, (int64_t)r->stride};
 }
 
+// The most rows of a sequence that can have a place in the cache.
+static int32_t most_rows(const BatchView &b) { return std::min(b.max_rows, std::min(b.max_len, b.n_rows)); }
+
 static unsigned grid_blocks(int64_t n, const char *what) {
     // (a launch holds fewer than 2^32 threads, 256 a workgroup)
     DITCH_CHECK(n < ((int64_t)1 << 24), DITCH_INVALID_ARGUMENT, std::string(what) + ": more work than one launch holds");
@@ -338,10 +341,20 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
     int64_t blk = blockIdx.x;
     if (blk >= a.kv_blocks) {
         blk -= a.kv_blocks;
-        const int q_part = (int)(blk % a.q_parts);
-        blk /= a.q_parts;
-        const int seq = (int)(blk / a.b.max_rows), i = (int)(blk % a.b.max_rows);
+        const int q_part = (int)(blk % a.q_parts), row = (int)(blk / a.q_parts);
+        // the row's sequence: the last whose rows start at or before it, 64 candidates at a time
+        int seq = 0, span = a.b.n_seqs;
+        while (span > 1) {
+            const int step = (span + 63) / 64, at = seq + (tid & 63) * step;
+            const uint64_t before = __ballot(at < seq + span && a.b.starts[at < seq + span ? at : seq] <= (uint32_t)row);
+            if (!before) return;
+            const int last = 63 - __builtin_clzll(before), end = seq + span;
+            seq += last * step;
+            span = end - seq < step ? end - seq : step;
+        }
         const SeqRows r = seq_rows(a.b, seq);
+        const int i = row - r.row;
+        if (i < 0) return;
         if (i < r.live) rotate_queries<T>(a, r, i, q_part);
         return;
     }
@@ -471,10 +484,11 @@ void launch_pages_append(const PoolView &p, const BatchView &b, int32_t dtype, c
                          const RopeView &rope, const RowsView *q, const RowsView *q_out, int heads, hipStream_t s) {
     if (b.n_seqs == 0) return;
     AppendArgs a{p, b, k, v, q ? *q : RowsView{}, q ? *q_out : RowsView{}, rope, 0, q ? heads : 0, 1, 0};
-    a.slots = (b.max_rows + p.page - 2) / p.page + 1;
+    a.b.max_rows = most_rows(b);
+    a.slots = (a.b.max_rows + p.page - 2) / p.page + 1;
     a.kv_blocks = (int64_t)b.n_seqs * a.slots * p.kv_heads * 2;
     // a row's heads over several workgroups until the rows fill the chip
-    const int64_t rows = (int64_t)b.n_seqs * b.max_rows;
+    const int64_t rows = b.n_rows;
     if (q && rows < 1024) a.q_parts = (int)std::min<int64_t>((int64_t)heads * ((p.hd + 7) / 8 + 255) / 256 + 1, 1024 / rows + 1);
     const unsigned blocks = grid_blocks(a.kv_blocks + (q ? rows * a.q_parts : 0), "kv append");
     if (dtype == DITCH_F32) append_typed<float>(a, blocks, s);
@@ -557,7 +571,9 @@ static void read_typed(const ReadArgs &a, unsigned blocks, hipStream_t s) {
 void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, const RowsView &k, const RowsView &v,
                        hipStream_t s) {
     if (b.n_seqs == 0) return;
-    ReadArgs a{p, b, k, v, (b.max_rows + GRANULE - 2) / GRANULE + 1};
+    ReadArgs a{p, b, k, v, 0};
+    a.b.max_rows = most_rows(b);
+    a.granules = (a.b.max_rows + GRANULE - 2) / GRANULE + 1;
     const unsigned blocks = grid_blocks((int64_t)b.n_seqs * a.granules * p.kv_heads * 2, "kv read");
     if (dtype == DITCH_F32) read_typed<float>(a, blocks, s);
     else if (dtype == DITCH_F16) read_typed<_Float16>(a, blocks, s);

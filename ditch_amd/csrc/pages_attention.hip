@@ -308,8 +308,8 @@ void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, 
     if (!a.few && pages_chunk_takes(a.p, a.b, a.heads, a.dtype)) return launch_pages_chunk(a, s);
     RowsPlan plan = rows_plan(a.p, a.b, a.heads, (uint32_t)a.window, (uint32_t)a.sinks);
     if (plan.splits > 1) {
-        plan.stats = (float *)ws;
-        plan.sums = plan.stats + (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles * plan.splits * plan.cols * 2;
+        plan.sums = (float *)ws;
+        plan.stats = plan.sums + (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles * plan.splits * plan.cols * a.p.dv;
     }
     if (a.dtype == DITCH_F32) rows_typed<float>(a, plan, s);
     else if (a.dtype == DITCH_F16) rows_typed<_Float16>(a, plan, s);

@@ -148,6 +148,8 @@ APPEND = [
     ("int8", "bf16", 3, 3, 256, 256, 256, 0, "neox", [(1, 255), (17, 250), (300, 4)]),
     ("e4m3", "f16", 3, 1, 1, 1, 32, 0, "neox", [(5, 30)]),
     ("int8", "f32", 6, 3, 30, 30, 64, 30, "gptj", [(97, 63), (1, 0)]),
+    ("e4m3", "bf16", 2, 1, 160, 160, 64, 160, "neox", [(1, 7), (100, 40)]),
+    ("int8", "bf16", 3, 1, 64, 64, 32, 64, "neox", [(b % 3, 11 * b % 90) for b in range(200)]),
 ]
 
 
@@ -255,6 +257,64 @@ def test_values_of_zero_and_of_extreme_size(dev):
             dev.kv_pages_append(s.pages, 0, s.batch([0, 9], [0]), "f32", k.desc, v.desc)
             touched = ref.append(pool, 0, np.array([[0]]), [0, 9], [0], k.x.reshape(9, 1, 64), v.x.reshape(9, 1, 64))
             _compare_pools(s.download(), pool, touched, 0)
+
+
+def test_bounds_far_above_what_there_is(dev):
+    """max_rows and max_len up to their limits cost nothing but idle workgroups, or are refused."""
+    rng = np.random.default_rng(18)
+    pool = ref.Pool("int8", 1, 3, 32, 1, 64)
+    s = Setup(dev, pool, [[2, 0, 1]])
+    k = Rows(dev, 5, 64, "f32", rng.standard_normal((5, 64)))
+    out = Rows(dev, 5, 64, "f32")
+    for bound in (1 << 10, (1 << 31) - 1):
+        b = s.batch([0, 5], [30], max_rows=bound, max_len=96)
+        dev.kv_pages_append(s.pages, 0, b, "f32", k.desc, k.desc)
+        touched = ref.append(pool, 0, np.array([[2, 0, 1]]), [0, 5], [30], k.x.reshape(5, 1, 64), k.x.reshape(5, 1, 64))
+        got = s.download()
+        for (page, h), live in touched.items():
+            lo = 30 if page == 2 else 0
+            np.testing.assert_array_equal(got.codes[0, page, h][got.off[0][lo:live]],
+                                          pool.codes[0, page, h][pool.off[0][lo:live]])
+        dev.kv_pages_read(s.pages, 0, b, "f32", out.desc, out.desc)
+        dev.sync()
+        if bound > 1 << 30:
+            with pytest.raises(DeviceError, match="max_rows"):
+                s.attention(0, b, "f32", out, k, 1, 0.1)
+
+
+def test_offsets_past_32_bits(dev):
+    """The same calls on pages at the start of a small pool and at the end of one of 4.7 GB: the same bytes."""
+    rng = np.random.default_rng(19)
+    heads, kvh, hd, page, cols = 16, 8, 128, 64, 3
+    small = ref.Pool("e4m3", 1, 8, page, kvh, hd)
+    n_big = 36000
+    codes, scales = hipmem.Buffer(n_big * kvh * small.bytes), hipmem.Buffer(n_big * kvh * 8)
+    x = [rng.standard_normal((150, h * hd)) for h in (kvh, kvh, heads)]
+    results = []
+    for first, n_pages in ((0, 8), (n_big - 8, n_big)):
+        table = np.array([[5, 1, 3], [2, 7, 6]], dtype=np.int32) + first
+        s = Setup(dev, small, table)
+        if first:
+            s.pages = dev.kv_pages(codes.ptr.value, codes.nbytes, scales.ptr.value, scales.nbytes, "e4m3", 1, n_pages,
+                                   page, kvh, hd)
+        b = s.batch([0, 100, 150], [0, 0])
+        k, v, q = (Rows(dev, 150, a.shape[1], "bf16", a) for a in x)
+        out, ko, vo = Rows(dev, 150, heads * hd, "bf16"), Rows(dev, 150, kvh * hd, "f32"), Rows(dev, 150, kvh * hd, "f32")
+        dev.kv_pages_append(s.pages, 0, b, "bf16", k.desc, v.desc)
+        s.attention(0, b, "bf16", out, q, heads, 0.1)
+        # the second sequence continues the first: its copy of the last page goes to a spare one
+        d = [hipmem.Buffer.from_array(np.array(a, dtype=np.int32)) for a in ([0, 0], [first, first + 4], [100])]
+        t_out, s_out = hipmem.Buffer.from_array(table * 0), hipmem.Buffer.from_array(table[:, 0] * 0)
+        dev.kv_pages_fork(s.pages, t_out.ptr, s_out.ptr, s.d_table.ptr, cols, d[0].ptr, d[1].ptr, d[2].ptr, 1, 2)
+        b2 = s.batch([0, 100, 150], [0, 50])
+        b2.table = t_out.ptr.value
+        dev.kv_pages_read(s.pages, 0, b2, "f32", ko.desc, vo.desc)
+        dev.sync()
+        results.append((out.get(), ko.get(), vo.get(), t_out.download(np.int32, (2, cols)) - first,
+                        s_out.download(np.int32, (2,)) - first))
+        assert results[-1][3][1, 1] == 4 and np.array_equal(results[-1][1][100:], results[-1][1][50:100])
+    for a, b in zip(*results):
+        np.testing.assert_array_equal(a, b)
 
 
 def test_append_within_its_bounds(dev):
@@ -379,6 +439,10 @@ ATTENTION = [
     ("e4m3", "f16", 2, 1, 256, 256, 64, [(90, 20)], 0, 0),
     ("int8", "f32", 3, 3, 192, 128, 64, [(100, 1)], 30, 2),
     ("int8", "bf16", 7, 1, 80, 80, 128, [(140, 300), (1, 20)], 128, 4),
+    # the largest heads, every column of a tile a query
+    ("int8", "f32", 16, 1, 256, 256, 64, [(1, 90), (2, 40)], 0, 0),
+    ("e4m3", "bf16", 32, 1, 160, 160, 64, [(1, 200)], 0, 0),
+    ("e4m3", "f32", 20, 1, 192, 128, 32, [(2, 70)], 50, 1),
 ]
 
 
