@@ -584,10 +584,10 @@ void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, con
 // fork
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-// 16-byte words that a workgroup copies: 16 a thread in flight. The last pages
-// of 16 x 8 beams (32 layers of 8 heads of 128, 360 MB moved): 97 us, with 8
-// or fewer a thread 105 to 112.
-constexpr int FORK_PART = 4096;
+// 16-byte words that a workgroup copies: 32 a thread in flight. The last pages
+// of 16 x 8 beams (32 layers of 8 heads of 128, 360 MB moved): 92 us, with 16
+// a thread 102, with 8 or fewer 105 to 112.
+constexpr int FORK_PART = 8192;
 
 struct ForkArgs {
     uint8_t *codes;
@@ -668,7 +668,7 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
                        int64_t groups, int64_t beams, hipStream_t s) {
     const PoolView v = pool_view(p, 0);
     const int64_t parts = (v.kv_heads * v.page_bytes / 16 + FORK_PART - 1) / FORK_PART, lh = p->layers * parts;
-    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 x 64 KB of layers a page");
+    DITCH_CHECK(lh <= 65535, DITCH_INVALID_ARGUMENT, "kv fork: more than 65535 x 128 KB of layers a page");
     const ForkArgs a{v.codes, v.scales, v.n_pages, v.page_bytes, v.page, v.n_pages, v.kv_heads, (int32_t)parts, table_out, spare_out,
                      table, parents, spare, lens, table_stride, (int32_t)beams};
     hipLaunchKernelGGL(pages_fork_kernel, dim3(grid_blocks(groups * beams, "kv fork"), (unsigned)lh), dim3(256), 0, s, a);
