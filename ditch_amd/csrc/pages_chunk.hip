@@ -6,10 +6,18 @@
 // any of them sees granule by granule. A granule's codes are converted to f16
 // once, into LDS in operand order (each lane's 16 codes become two 16-byte
 // operand entries of the same lane: no bank conflicts either way), two
-// granules ahead of their use (and asked for four ahead), and every wave reads each operand once for its
-// QT tiles. The scores of the next granule are formed in one straight run of
-// code with the weights and values of this one, so that the matrix cores
-// work while the vector units exponentiate.
+// granules ahead of their use (and asked for three ahead), and every wave
+// reads each operand once for its QT tiles. The scores of the next granule are
+// formed in one straight run of code with the weights and values of this one,
+// so that the matrix cores work while the vector units exponentiate.
+//
+// 2 x 2048 bf16 rows over 2048 cached tokens (32 heads of 128 over 8, e4m3):
+// 206 GF in 232 to 237 us, 870 to 890 TFLOP/s, where a large f16 product
+// reaches 1109. No unit is full (matrix cores 36 % of the cycles, vector issue 50 %, LDS under
+// half): what bounds it is the order within a wave, products, then maxima and
+// exponentials, then products, with two waves a SIMD to fill each other's
+// gaps. f32 rows take two terms on both products: 5 x up to 1500 rows of 14
+// heads of 64 under a window of 512 take 46 us.
 #include "pages_attention.h"
 
 namespace ditch {
@@ -90,9 +98,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
     const int per = a.p.page / GRANULE;
     const int64_t head_stride = (int64_t)a.p.kv_heads * a.p.page_bytes;
     const uint8_t *base = a.p.codes + (int64_t)h * a.p.page_bytes + lane * 16;
-    // the wave's share of a granule's codes on their way, of two granules
-    u32x4 raw_a[PER], raw_b[PER];
-    auto fetch = [&](u32x4 (&raw)[PER], int b, int k) {
+    u32x4 raw[PER];  // the wave's share of a granule's codes on their way
+    auto fetch = [&](int b, int k) {
         const int64_t at = granule_index(tr, b + k) & (per - 1);
         const uint8_t *p = base + __builtin_amdgcn_readfirstlane(id_s[k]) * head_stride;
         const uint8_t *kp = p + at * (GRANULE * DK), *vp = p + (int64_t)a.p.page * DK + at * (GRANULE * DV);
@@ -104,7 +111,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
             if (EVEN || u < UNITS) raw[i] = *(const u32x4 *)(keys ? kp + u * 1024 : vp + (u - 2 * KP) * 1024);
         }
     };
-    auto store = [&](const u32x4 (&raw)[PER], int slot) {
+    auto store = [&](int slot) {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int u = wave + i * NW;
@@ -162,17 +169,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
             inverse_s[e] = gs.inverse;
         }
         __syncthreads();
-        fetch(raw_a, b, 0);
-        fetch(raw_b, b, n > 1 ? 1 : 0);
-        store(raw_a, 0);
-        store(raw_b, 1);
-        fetch(raw_a, b, n > 2 ? 2 : 0);
-        fetch(raw_b, b, n > 3 ? 3 : 0);
+        fetch(b, 0);
+        store(0);
+        fetch(b, n > 1 ? 1 : 0);
+        store(1);
+        fetch(b, n > 2 ? 2 : 0);
         __syncthreads();
         form_scores(0);
         int slot = 0;
-        // granule k: granule k + 2 to LDS, k + 4 on its way
-        auto step = [&](u32x4 (&raw)[PER], int k) {
+        // granule k: granule k + 2 to LDS, k + 3 on its way
+#pragma unroll 1
+        for (int k = 0; k < n; k++) {
             const int next = slot == RING - 1 ? 0 : slot + 1, after = next == RING - 1 ? 0 : next + 1;
             const int gi = granule_index(tr, b + k), a0 = gi * GRANULE, z0 = a0 + GRANULE - 1;
             auto uniform = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
@@ -205,17 +212,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
                 inverse = 0.f;
             }
             // one straight run: behind the batch's last granules the scores and
-            // the copies are of whatever is there, and not used
+            // the copies are of whatever is there, and not used. The wave that
+            // feeds the matrix cores goes first: 235 -> 232 us and, of two
+            // terms, 49 -> 46 us (the calls above)
+            __builtin_amdgcn_s_setprio(1);
             form_scores(next);
-            store(raw, after);
-            fetch(raw, b, k + 4 < n ? k + 4 : n - 1);
+            store(after);
+            fetch(b, k + 3 < n ? k + 3 : n - 1);
             add_values(slot, w, inverse);
+            __builtin_amdgcn_s_setprio(0);
             __syncthreads();
             slot = next;
-        };
-        for (int k = 0; k < n; k += 2) {
-            step(raw_a, k);
-            if (k + 1 < n) step(raw_b, k + 1);
         }
     }
 
@@ -236,9 +243,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 // ---------------------------------------------------------------------------
 
 // Two tiles a wave, four waves: with 2 x 2048 rows over 2048 cached tokens (32
-// heads of 128 over 8, bf16, e4m3) 270 us; three tiles a wave 324 us and four
-// 491 us, with one wave a SIMD left; eight waves 275 us there, but 77 us
-// against 51 us with 5 x 1500 rows under a window.
+// heads of 128 over 8, bf16, e4m3) 232 to 237 us; three tiles a wave 316 us, with one
+// wave a SIMD left; eight waves 242 us there, but 78 us against 46 us with
+// 5 x 1500 rows under a window; registers for three waves a SIMD (19 of them
+// spilled) 323 us.
 constexpr int CHUNK_TILES = 2, CHUNK_WAVES = 4;
 
 // A workgroup here walks all of its keys by itself, so it takes enough of them

@@ -656,6 +656,7 @@ uint64_t ditch_hip_kv_pages_scales_bytes(const ditch_kv_pages *p);
  * max_rows or max_len, and pages outside the pool, are neither read nor
  * written (a query that would attend to such a page, or lies past max_len,
  * gets NaN; one past max_rows or not in any sequence keeps its output).
+ * max_rows times the query heads of a KV head stays below 2^30.
  * Two sequences may share pages; append to a shared page only after
  * ditch_hip_kv_pages_fork_device or a copy of its own.                     */
 typedef struct ditch_kv_batch {
