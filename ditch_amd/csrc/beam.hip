@@ -13,11 +13,10 @@
 // list, or, should that be more than the list holds (many equal logits, the
 // best in few lanes), exactly the k best do, by bisection over the elements.
 //
-// Bound by the read of the logits: 64 prompts of 8 beams over 128 256 tokens
-// (263 MB), 16 best: 64 us, 4.1 TB/s, of the 5.1 that a large copy reaches; the
-// exponentials, comparisons and the search take the rest, as a lane holds 64
-// logits and a SIMD few waves. Loads past the caches did not change it, half the
-// chunk took 82 us.
+// 64 prompts of 8 beams over 128 256 tokens (263 MB), 16 best: 64 us, 4.1 TB/s,
+// of the 5.1 that a large copy reaches: vector issue, 77 % of the cycles
+// (exponentials, maxima, the search), is what keeps it from there. Loads past
+// the caches did not change it; half the chunk took 82 us.
 #include "pages.h"
 
 namespace ditch {
@@ -249,9 +248,9 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     for (int e = n + tid; e < k; e += 256) out[e] = Candidate{0.f, NO_TOKEN};
 }
 
-// A workgroup a prompt: 10 us, a chain of three searches and a ranking over
-// beams x chunks x k candidates (1 prompt of 4 beams over 151 936 tokens takes
-// 17 us for both kernels).
+// A workgroup a prompt: 10 us, bound by its chain: the beams' statistics, the
+// candidates' scores, the search for the k-th of them, the ranking (1 prompt of
+// 4 beams over 151 936 tokens takes 17 us for both kernels).
 constexpr int JOIN = 1024, HELD = 4;  // threads; candidates a thread holds in registers
 constexpr int NEAR = 256;             // candidates that are ranked against each other
 __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {

@@ -13,11 +13,11 @@
 //
 // 2 x 2048 bf16 rows over 2048 cached tokens (32 heads of 128 over 8, e4m3):
 // 206 GF in 232 to 237 us, 870 to 890 TFLOP/s, where a large f16 product
-// reaches 1109. No unit is full (matrix cores 36 % of the cycles, vector issue 50 %, LDS under
-// half): what bounds it is the order within a wave, products, then maxima and
-// exponentials, then products, with two waves a SIMD to fill each other's
-// gaps. f32 rows take two terms on both products: 5 x up to 1500 rows of 14
-// heads of 64 under a window of 512 take 46 us.
+// reaches 1109. No unit is full (matrix cores 36 % of the cycles, vector issue
+// 52 %, LDS 30 %): what bounds it is the order within a wave, products, then
+// maxima and exponentials, then products, with two waves a SIMD to fill each
+// other's gaps. f32 rows take two terms on both products: 5 x up to 1500 rows
+// of 14 heads of 64 under a window of 512 take 46 us.
 #include "pages_attention.h"
 
 namespace ditch {
