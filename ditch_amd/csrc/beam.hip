@@ -30,7 +30,15 @@ constexpr uint32_t NO_TOKEN = ~0u;  // an unused candidate
 __device__ __forceinline__ uint32_t logit_key(float x) {
     if (!(x == x)) return 0;
     const uint32_t b = __float_as_uint(x + 0.f);
-    return b >> 31 ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_logit(uint32_t key) {
+    return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+// A candidate as one number: the larger goes first, among equal logits the
+// lower token.
+__device__ __forceinline__ uint64_t candidate_rank(float x, uint32_t token) {
+    return (uint64_t)logit_key(x) << 32 | ~token;
 }
 __device__ __forceinline__ uint64_t score_key(double x) {
     if (!(x == x)) return 0;
@@ -57,7 +65,7 @@ struct BeamArgs {
 // A workgroup of 4 waves a chunk of 256 R quads of a row.
 template <int R>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
-    __shared__ Candidate list[4][LIST];
+    __shared__ uint64_t list[4][LIST];
     __shared__ int count_s[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / a.chunks;
@@ -134,7 +142,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
             } else high = mid - 1;
         }
         // (low's logit; the key of a half lane without one is that of -infinity)
-        const float tau = low >> 31 ? __uint_as_float(low & 0x7fffffffu) : __uint_as_float(~low);
+        const float tau = key_logit(low);
         // (a threshold of -infinity would take what pads the row, too)
         if (tau > -INFINITY) {
 #pragma unroll
@@ -144,11 +152,14 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
                 for (int j = 0; j < 4; j++) in[j] = __ballot(v[r][j] >= tau);
                 if (in[0] | in[1] | in[2] | in[3]) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int at = count + __popcll(in[j] & (((uint64_t)1 << lane) - 1));
-                        if (v[r][j] >= tau && at < LIST) list[wave][at] = Candidate{v[r][j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
-                        count += __popcll(in[j]);
-                    }
+                    for (int j = 0; j < 4; j++)
+                        if (in[j]) {
+                            const int at = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in[j] >> 32),
+                                                                          __builtin_amdgcn_mbcnt_lo((uint32_t)in[j], count));
+                            if (v[r][j] >= tau && at < LIST)
+                                list[wave][at] = candidate_rank(v[r][j], (uint32_t)(t0 + 256 * r + j));
+                            count += __popcll(in[j]);
+                        }
                 }
             }
         }
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const bool is_e = be[j] & bit, is_g = bg[j] & bit;
-                const Candidate c{f[j] + 0.f, (uint32_t)(t0 + 256 * r + j)};
+                const uint64_t c = candidate_rank(f[j], (uint32_t)(t0 + 256 * r + j));
                 if (is_g) list[wave][put + g] = c;
                 if (is_e && e < take) list[wave][put + gt + e] = c;
                 g += is_g;
@@ -233,17 +244,12 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     Candidate *out = a.list + (int64_t)blockIdx.x * k;
     for (int e = tid; e < n; e += 256) {
         const int w = e < n0 ? 0 : e < n0 + n1 ? 1 : e < n0 + n1 + n2 ? 2 : 3;
-        const Candidate c = list[w][e - (w > 0 ? n0 : 0) - (w > 1 ? n1 : 0) - (w > 2 ? n2 : 0)];
-        const uint32_t key = logit_key(c.x);
+        const uint64_t c = list[w][e - (w > 0 ? n0 : 0) - (w > 1 ? n1 : 0) - (w > 2 ? n2 : 0)];
         int rank = 0;
         for (int u = 0; u < 4; u++)
 #pragma unroll 8
-            for (int i = 0; i < count_s[u]; i++) {
-                const Candidate o = list[u][i];
-                const uint32_t ok = logit_key(o.x);
-                rank += ok > key || (ok == key && o.token < c.token);
-            }
-        if (rank < k) out[rank] = c;
+            for (int i = 0; i < count_s[u]; i++) rank += list[u][i] > c;
+        if (rank < k) out[rank] = Candidate{key_logit((uint32_t)(c >> 32)), ~(uint32_t)c};
     }
     for (int e = n + tid; e < k; e += 256) out[e] = Candidate{0.f, NO_TOKEN};
 }
