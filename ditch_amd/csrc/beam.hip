@@ -13,10 +13,11 @@
 // list, or, should that be more than the list holds (many equal logits, the
 // best in few lanes), exactly the k best do, by bisection over the elements.
 //
-// 64 prompts of 8 beams over 128 256 tokens (263 MB), 16 best: 64 us, 4.1 TB/s,
-// of the 5.1 that a large copy reaches: vector issue, 77 % of the cycles
-// (exponentials, maxima, the search), is what keeps it from there. Loads past
-// the caches did not change it; half the chunk took 82 us.
+// 64 prompts of 8 beams over 128 256 tokens (263 MB), 16 best: 45 us, 5.8 TB/s
+// (a large copy: 5.1; some of it is still cached), and 8 us for the join; 1 prompt of 4 beams over 151 936
+// tokens 14 us for both kernels. Vector issue comes next: a candidate's place
+// in the list and its rank are few operations each (with twice as many the
+// kernel took 62 us). Loads past the caches and half the chunk changed nothing.
 #include "pages.h"
 
 namespace ditch {
@@ -254,10 +255,11 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     for (int e = n + tid; e < k; e += 256) out[e] = Candidate{0.f, NO_TOKEN};
 }
 
-// A workgroup a prompt: 10 us, bound by its chain: the beams' statistics, the
-// candidates' scores, the search for the k-th of them, the ranking (1 prompt of
-// 4 beams over 151 936 tokens takes 17 us for both kernels).
-constexpr int JOIN = 1024, HELD = 4;  // threads; candidates a thread holds in registers
+// A workgroup a prompt: 8 us, bound by its chain: the beams' statistics, the
+// candidates' scores, the search for the k-th of them (five turns of some 900
+// cycles), the ranking. Every wave of a SIMD repeats the steps between, so 1024
+// threads took 1.4 us more; with 256 the beams' statistics queue up (2 us more).
+constexpr uint32_t JOIN = 512, HELD = 8;  // threads; candidates a thread holds in registers
 constexpr int NEAR = 256;             // candidates that are ranked against each other
 __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ double lse_s[BEAM_MOST_BEAMS], prev_s[BEAM_MOST_BEAMS];
@@ -269,30 +271,32 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ float score_s[NEAR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
     const int64_t row0 = (int64_t)blockIdx.x * a.beams;
-    const int per = a.chunks * k;
-    const int64_t n = (int64_t)a.beams * per;
-    const Candidate *list = a.list + row0 * per;
+    const uint32_t per = (uint32_t)a.chunks * k, n = a.beams * per;  // (2^30 and a few at most)
+    const Candidate *list = a.list + (size_t)row0 * per;
     Candidate held_c[HELD];  // (asked for before the sums)
 #pragma unroll
     for (int j = 0; j < HELD; j++) {
         held_c[j] = Candidate{0.f, NO_TOKEN};
-        if (tid + (int64_t)JOIN * j < n) held_c[j] = list[tid + (int64_t)JOIN * j];
+        if (tid + JOIN * j < n) held_c[j] = list[tid + JOIN * j];
     }
     for (int b = wave; b < a.beams; b += JOIN / 64) {
         double sum = 0;
-        float most = -INFINITY;  // (the maxima are f32)
+        float most;  // (the maxima are f32)
         const double *st = a.stats + (row0 + b) * a.chunks * 8;
-        for (int c = lane; c < 4 * a.chunks; c += 64) most = fmaxf(most, (float)st[2 * c]);
+        // (a lane's first part stays in registers, as few have a second)
+        const double2 one = lane < 4 * a.chunks ? *(const double2 *)(st + 2 * lane) : make_double2(-INFINITY, 0);
+        const float prev = a.prev[row0 + b];
+        most = (float)one.x;
+        for (int c = lane + 64; c < 4 * a.chunks; c += 64) most = fmaxf(most, (float)st[2 * c]);
         for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
         const double m = most;
-        for (int c = lane; c < 4 * a.chunks; c += 64) {
-            const double cm = st[2 * c], cs = st[2 * c + 1];
-            sum += cm == -INFINITY ? cs : cs * exp(cm - m);
-        }
+        auto add = [&](double cm, double cs) { sum += cm == -INFINITY ? cs : cs * exp(cm - m); };
+        add(one.x, one.y);
+        for (int c = lane + 64; c < 4 * a.chunks; c += 64) add(st[2 * c], st[2 * c + 1]);
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if (lane == 0) {
             lse_s[b] = m == -INFINITY || m == INFINITY ? NAN : m + log(sum);
-            prev_s[b] = (double)a.prev[row0 + b];
+            prev_s[b] = (double)prev;
         }
     }
     if (tid == 0) put = 0;
@@ -303,7 +307,7 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
         uint32_t token;
         float score;
     };
-    auto item = [&](int64_t e, Candidate c) {
+    auto item = [&](uint32_t e, Candidate c) {
         const int b = (int)(e / per);
         const double s = prev_s[b] + ((double)c.x - lse_s[b]);
         return Item{score_key(s), (uint64_t)b << 32 | (uint32_t)~logit_key(c.x), c.token, (float)s};
@@ -312,13 +316,13 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
 #pragma unroll
     for (int j = 0; j < HELD; j++) {
         held[j] = Item{0, 0, NO_TOKEN, 0.f};
-        if (held_c[j].token != NO_TOKEN) held[j] = item(tid + (int64_t)JOIN * j, held_c[j]);
+        if (JOIN * j < n && held_c[j].token != NO_TOKEN) held[j] = item(tid + JOIN * j, held_c[j]);
     }
     auto each = [&](auto &&f) {
 #pragma unroll
         for (int j = 0; j < HELD; j++)
-            if (held[j].token != NO_TOKEN) f(held[j]);
-        for (int64_t e = tid + (int64_t)JOIN * HELD; e < n; e += JOIN) {
+            if (JOIN * j < n && held[j].token != NO_TOKEN) f(held[j]);
+        for (uint32_t e = tid + JOIN * HELD; e < n; e += JOIN) {
             const Item it = item(e, list[e]);
             if (it.token != NO_TOKEN) f(it);
         }
@@ -328,8 +332,9 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     auto count = [&](auto &&takes) {
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < HELD; j++) c += __popcll(__ballot(held[j].token != NO_TOKEN && takes(held[j])));
-        for (int64_t e = (int64_t)JOIN * HELD; e < n; e += JOIN) {
+        for (int j = 0; j < HELD; j++)  // (the waves' time is their number of operations: none for empty places)
+            if (JOIN * j < n) c += __popcll(__ballot(held[j].token != NO_TOKEN && takes(held[j])));
+        for (uint32_t e = JOIN * HELD; e < n; e += JOIN) {
             Item it{0, 0, NO_TOKEN, 0.f};
             if (e + tid < n) it = item(e + tid, list[e + tid]);
             c += __popcll(__ballot(it.token != NO_TOKEN && takes(it)));
