@@ -515,7 +515,7 @@ struct ReadArgs {
 // 75 MB, in 23 us; a row of 64 sequences 10 us.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
-    __shared__ __attribute__((aligned(16))) float tile[GRANULE * 260];
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [GRANULE][DP + 4]
     const int tid = threadIdx.x;
     int64_t blk = blockIdx.x;
     const int which = (int)(blk & 1);
@@ -566,10 +566,11 @@ __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
 
 template <typename T>
 static void read_typed(const ReadArgs &a, unsigned blocks, hipStream_t s) {
+    const unsigned lds = GRANULE * (std::max(a.p.dk, a.p.dv) + 4) * 4;
     if (a.p.kind == DITCH_KV_INT8)
-        hipLaunchKernelGGL((pages_read_kernel<T, DITCH_KV_INT8>), dim3(blocks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((pages_read_kernel<T, DITCH_KV_INT8>), dim3(blocks), dim3(256), lds, s, a);
     else
-        hipLaunchKernelGGL((pages_read_kernel<T, DITCH_KV_E4M3>), dim3(blocks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((pages_read_kernel<T, DITCH_KV_E4M3>), dim3(blocks), dim3(256), lds, s, a);
     DITCH_TRY_HIP(hipGetLastError());
 }
 
