@@ -134,25 +134,43 @@ __device__ __forceinline__ double rotated(const T *x, int d, int half, int style
     return second ? xb * cc + xa * ss : xa * cc - xb * ss;
 }
 
-// The code nearest to y (ties to even), y within the code's range after the clamp.
+// The codes nearest to y (ties to even; a scale below f32's normal range can
+// leave a y past the largest code: that one). Four at a time: the conversions
+// and their checks are what an append computes.
 template <int KIND>
-__device__ __forceinline__ uint8_t nearest_code(double y) {
-    constexpr double most = KIND == DITCH_KV_INT8 ? 127.0 : 448.0;
-    if constexpr (KIND == DITCH_KV_INT8) return (uint8_t)(int8_t)(int)rint(fmin(fmax(y, -most), most));
-    // e4m3: 3 bits behind the leading one, the least step 2^-9. Through f32
-    // and the conversion instruction the value is rounded twice, which differs
-    // from once only where the f32 value is half way between two codes (its
-    // low 20 bits say so above 2^-6): there, and below, in 64 bits.
-    float v = fminf(fmaxf((float)y, (float)-most), (float)most);
-    if ((__float_as_uint(v) & 0xfffffu) == 0x80000u || fabsf(v) < 0.015625f) {
-        y = fmin(fmax(y, -most), most);
-        int e = (int)((__double_as_longlong(y) >> 52) & 0x7ff) - 1023;
-        e = e < -6 ? -6 : e;
-        const double up = __longlong_as_double((int64_t)(1023 + 3 - e) << 52);
-        const double down = __longlong_as_double((int64_t)(1023 - 3 + e) << 52);
-        v = (float)(rint(y * up) * down);  // a code's value: the conversion is exact
+__device__ __forceinline__ uint32_t nearest_codes(const double (&y)[4]) {
+    if constexpr (KIND == DITCH_KV_INT8) {
+        int c[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) c[j] = min(max((int)rint(y[j]), -127), 127);
+        return (c[0] & 0xff) | (c[1] & 0xff) << 8 | (c[2] & 0xff) << 16 | (uint32_t)c[3] << 24;
+    } else {
+        // e4m3: 3 bits behind the leading one, the least step 2^-9. Through f32
+        // and the conversion instruction the value is rounded twice, which differs
+        // from once only where the f32 value is half way between two codes (its
+        // low 20 bits say so above 2^-6): there, and below, in 64 bits.
+        float v[4];
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = __builtin_amdgcn_fmed3f((float)y[j], -448.f, 448.f);
+            odd |= (__float_as_uint(v[j]) & 0xfffffu) == 0x80000u || fabsf(v[j]) < 0.015625f;
+        }
+        if (odd) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double z = fmin(fmax(y[j], -448.0), 448.0);
+                int e = (int)((__double_as_longlong(z) >> 52) & 0x7ff) - 1023;
+                e = e < -6 ? -6 : e;
+                const double up = __longlong_as_double((int64_t)(1023 + 3 - e) << 52);
+                const double down = __longlong_as_double((int64_t)(1023 - 3 + e) << 52);
+                v[j] = (float)(rint(z * up) * down);  // a code's value: the conversion is exact
+            }
+        }
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true);
+        return (uint32_t)r;
     }
-    return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff);
 }
 
 template <int KIND>
@@ -171,9 +189,11 @@ __device__ __forceinline__ float code_value(uint8_t c) {
 // tokens of before came in first. (Staging the values themselves needs four to
 // eight times the LDS and took 233 us where this takes 85: 24 sequences
 // of up to 500 f32 rows of 8 heads of 128 and 32 query heads.) That call moves
-// 314 MB, 239 of them the queries: 83 us, 3.8 TB/s. One row for each of 64
-// sequences takes 7 us, the latency of a chain of table, scale, the page's
-// codes of before (rounded again where the scale grows) and the stores.
+// 314 MB, 239 of them the queries: 79 us, 4.0 TB/s; the keys and values alone
+// take half of that, bound by the operations of the conversions in 64 bits. One
+// row for each of 64 sequences takes 7 us, the latency of a chain of table,
+// scale, the page's codes of before (rounded again where the scale grows) and
+// the stores.
 
 constexpr int TILE = 16384;  // codes staged (the page in parts where it has more)
 
@@ -336,8 +356,10 @@ __device__ __forceinline__ void each_key(const T *x, int64_t stride, bool quads,
 
 // A workgroup per (sequence, touched page, head, keys or values), then those
 // of the query rows.
+// Five waves a SIMD: four, with two registers more, took 7 us longer for the
+// 24 sequences above; six and eight, which spill, 2 and 14 us.
 template <typename T, int KIND>
-__global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5))) void pages_append_kernel(AppendArgs a) {
     __shared__ double part[4];
     __shared__ __attribute__((aligned(16))) uint8_t tile[TILE];
     const int tid = threadIdx.x;
@@ -386,6 +408,11 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
         bad |= !(fabs(y) <= 3.4028234663852886e38);
         most = fmax(most, fabs(y));
     };
+    float most_value = 0;  // (a value is an f32: no rotation)
+    auto largest_value = [&](float y) {
+        bad |= !(fabsf(y) <= 3.4028234663852886e38f);
+        most_value = fmaxf(most_value, fabsf(y));
+    };
     if (which == 0) {
         each_key(rows, rv.stride, quads, lo, hi, D, a.rope, t0, [&](int t, int d, int n, const double *y) {
             for (int j = 0; j < n; j++) largest(y[j]);
@@ -397,11 +424,12 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
             float v[4];
             load4(v, rows + (int64_t)(lo + e / per) * rv.stride + e % per * 4, true, 4);
 #pragma unroll
-            for (int j = 0; j < 4; j++) largest((double)v[j]);
+            for (int j = 0; j < 4; j++) largest_value(v[j]);
         }
     } else {
-        for (int e = tid; e < (hi - lo) * D; e += 256) largest((double)(float)rows[(int64_t)(lo + e / D) * rv.stride + e % D]);
+        for (int e = tid; e < (hi - lo) * D; e += 256) largest_value((float)rows[(int64_t)(lo + e / D) * rv.stride + e % D]);
     }
+    if (which) most = (double)most_value;
     if (bad) most = INFINITY;
     for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
     if ((tid & 63) == 0) part[tid >> 6] = most;
@@ -429,24 +457,33 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
             union {
                 uint4 q;
                 uint8_t b[16];
+                uint32_t d[4];
             } w;
             w.q = make_uint4(0, 0, 0, 0);
             if (c0 + u * 16 / (GRANULE * DP) * GRANULE < lo) {  // the granule holds tokens of before
                 w.q = page[u];
                 if (grown) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) w.b[j] = nearest_code<KIND>((double)code_value<KIND>(w.b[j]) * f);
+                    for (int j = 0; j < 4; j++) {
+                        double y[4];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) y[z] = (double)code_value<KIND>(w.b[4 * j + z]) * f;
+                        w.d[j] = nearest_codes<KIND>(y);
+                    }
                 }
             }
             ((uint4 *)tile)[u] = w.q;
         }
         __syncthreads();
-        auto code = [&](double y) { return (uint32_t)(poison ? 0 : nearest_code<KIND>(y * inverse)); };
+        auto code = [&](const double (&y)[4]) {
+            const double z[4] = {y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse};
+            return poison ? 0u : nearest_codes<KIND>(z);
+        };
         if (which == 0) {
             each_key(rows, rv.stride, quads, n0, n1, D, a.rope, t0, [&](int t, int d, int n, const double *y) {
                 uint8_t *at = tile + key_offset(t - c0, d, DP);
-                if (n == 4) *(uint32_t *)at = code(y[0]) | code(y[1]) << 8 | code(y[2]) << 16 | code(y[3]) << 24;
-                else *at = (uint8_t)code(y[0]);
+                if (n == 4) *(uint32_t *)at = code({y[0], y[1], y[2], y[3]});
+                else *at = (uint8_t)code({y[0], 0.0, 0.0, 0.0});
             });
         } else {
             // a dim of four tokens that lie next to each other in the page
@@ -454,18 +491,19 @@ __global__ __launch_bounds__(256) void pages_append_kernel(AppendArgs a) {
 #pragma unroll 2
             for (int e = tid; e < (q1 - q0) * D; e += 256) {
                 const int t = (q0 + e / D) * 4, d = e % D;
-                uint32_t c[4];
+                double y[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const bool in = t + j >= n0 && t + j < n1;
-                    c[j] = in ? code((double)(float)rows[(int64_t)(t + j) * rv.stride + d]) : 0;
+                    y[j] = in ? (double)(float)rows[(int64_t)(t + j) * rv.stride + d] : 0.0;
                 }
+                const uint32_t c = code(y);
                 uint8_t *at = tile + value_offset(t - c0, d, DP);
-                if (t >= n0 && t + 4 <= n1) *(uint32_t *)at = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+                if (t >= n0 && t + 4 <= n1) *(uint32_t *)at = c;
                 else
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        if (t + j >= n0 && t + j < n1) at[j] = (uint8_t)c[j];
+                        if (t + j >= n0 && t + j < n1) at[j] = (uint8_t)(c >> 8 * j);
             }
         }
         __syncthreads();
@@ -512,7 +550,7 @@ struct ReadArgs {
 // A workgroup per (sequence, granule, head, keys or values): its units
 // decoded into LDS rows, which go out as rows: both sides of the transposition
 // in 16-byte accesses. Bound by the memory: 7291 f32 rows of 8 heads of 128,
-// 75 MB, in 23 us; a row of 64 sequences 10 us.
+// 75 MB, in 20 us; up to 64 of 64 sequences 9 us.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
     extern __shared__ __attribute__((aligned(16))) float tile[];  // [GRANULE][DP + 4]
