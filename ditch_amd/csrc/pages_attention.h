@@ -7,7 +7,11 @@
 // in one pass with a running maximum. The value scale goes into the
 // exponent, w_j = 2^(s_j log2(e) + log2(vs_j) - m), so the accumulator sums
 // w_j e_j with plain codes, and the denominator adds a granule's w times
-// 1 / vs: one multiplication for a granule's eight weights a lane.
+// 1 / vs: one multiplication for a granule's eight weights a lane. The maximum
+// is that of the weights, scale included, so the denominator relative to it
+// spans what the scales do, 2^-126 to 2^127: it is held in 64 bits (32 would
+// end at infinity where the first pages' values are below about 2^-113, and
+// stay there when the maximum moves on).
 //
 // Codes of both kinds are exact in f16 (int8: 8 bits of 11; e4m3: 4 bits, the
 // least 2^-9), so both products run on v_mfma_f32_16x16x32_f16 with exact
@@ -63,18 +67,21 @@ __device__ __forceinline__ half8 codes_f16(uint32_t lo, uint32_t hi) {
     }
 }
 
-// The largest / the sum over the four lanes (l, l ^ 16, l ^ 32, l ^ 48).
+// The largest over the four lanes (l, l ^ 16, l ^ 32, l ^ 48), the sum.
 __device__ __forceinline__ float max_groups(float x) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float sum_groups(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+__device__ __forceinline__ double sum_groups(double x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+// 2^t past f32's range.
+__device__ __forceinline__ double exp2_wide(float t) {
+    const double h = (double)__builtin_amdgcn_exp2f(0.5f * t);
+    return h * h;
 }
 
 // A query tile's operands: lane (g, c) holds query c's dims 64 p + 16 g + 0..7
@@ -183,13 +190,14 @@ __device__ __forceinline__ float weight_terms(Weights<TERMS> &w, const float (&x
 // A granule's scales as the loops use them. A value scale far from 1 would
 // take the denominator's part out of the weights' range, a NaN would reach
 // rows that see none of the granule, and zero has no logarithm: such a
-// granule is `odd` (see odd_granule).
+// granule is `odd` (see odd_granule). Zero goes by the least scale there is,
+// so that it moves the maximum past no other's weights.
 struct GranuleScales {
     float key, bias, inverse;
 };
 __device__ __forceinline__ GranuleScales granule_scales(float ks, float vs) {
     const bool zero = fabsf(vs) < 1.17549435e-38f;  // (subnormal: the logarithm takes it for zero)
-    return {ks, zero ? 0.f : __builtin_amdgcn_logf(vs), zero ? 0.f : 1.f / vs};
+    return {ks, zero ? -126.f : __builtin_amdgcn_logf(vs), zero ? 0.f : 1.f / vs};
 }
 __device__ __forceinline__ bool granule_odd(const GranuleScales &sc) {
     return sc.inverse == 0.f || !(fabsf(sc.bias) <= BIAS_PLAIN) || !(fabsf(sc.key) <= 3.4028234663852886e38f);
@@ -257,25 +265,25 @@ __device__ __forceinline__ float most_of(const float (&w)[8]) {
     return max3(max3(w[0], w[1], w[2]), max3(w[3], w[4], w[5]), max3(w[6], w[7], w[7]));
 }
 // Moves the running maximum m to the exponents' largest where that passes
-// W_MOST; returns the factor of what was added up under the old one.
+// W_MOST; returns the root of the factor of what was added up under the old one.
 __device__ __forceinline__ float move_maximum(float (&w)[8], floatx4 s0, floatx4 s1, float ck, float bias, bool full, int j0,
                                               const Seen &seen, float &m) {
     granule_exponents(w, s0, s1, ck, bias);
     if (!full) granule_mask(w, j0, seen);
-    const float next = fmaxf(m, max_groups(most_of(w))), f = __builtin_amdgcn_exp2f(m - next);
+    const float next = fmaxf(m, max_groups(most_of(w))), root = __builtin_amdgcn_exp2f(0.5f * (m - next));
     m = next;
     granule_exponents(w, s0, s1, ck, bias + (W_UP - m));
     if (!full) granule_mask(w, j0, seen);
-    return f;
+    return root;
 }
 // An odd granule's part of the denominator, from the scores alone: the
 // product's weights then add nothing to it (inverse 0), and under a value
 // scale of zero there are none.
-__device__ __forceinline__ float odd_granule(float (&w)[8], const GranuleScales &sc) {
-    float sum = 0.f;
+__device__ __forceinline__ double odd_granule(float (&w)[8], const GranuleScales &sc) {
+    double sum = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        sum += w[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[j] - sc.bias);
+        sum += w[j] == -INFINITY ? 0.0 : exp2_wide(w[j] - sc.bias);
         if (sc.inverse == 0.f) w[j] = -INFINITY;
     }
     return sum;

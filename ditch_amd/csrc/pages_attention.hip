@@ -30,7 +30,8 @@ constexpr int MOST_SPLITS = 256;
 struct RowsPlan {
     int tiles, splits, cols;  // query tiles of a (sequence, KV head); workgroups a tile; queries a tile
     int waves;                // of a workgroup: 4 or 8
-    float *sums, *stats;      // [item][cols][DV], [item][cols][2]: splits > 1
+    float *sums;              // [item][cols][DV]: splits > 1
+    double *stats;            // [item][cols][2]: the maximum, the denominator relative to it
 };
 
 template <typename T, int KIND, int DK, int DV, int NW>
@@ -38,7 +39,8 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     constexpr int KP = DK / 64, VU = DV / 32, TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr int OS = DV + 4;
     extern __shared__ __attribute__((aligned(16))) float o_s[];  // [NW][cols][OS]
-    __shared__ float m_s[NW][16], l_s[NW][16];
+    __shared__ float m_s[NW][16];
+    __shared__ double l_s[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     int64_t blk = blockIdx.x;
     const int split = (int)(blk % plan.splits);
@@ -76,7 +78,8 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     floatx4 o[DV / 16];
 #pragma unroll
     for (int d = 0; d < DV / 16; d++) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float m = M_NONE, l = 0.f;
+    float m = M_NONE;
+    double l = 0;
 
     const int k0 = (int)((int64_t)tr.granules * split / plan.splits), k1 = (int)((int64_t)tr.granules * (split + 1) / plan.splits);
     const int per = a.p.page / GRANULE;
@@ -102,9 +105,9 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
         if (!full) granule_mask(w, j0, seen);
         if (__any(most_of(w) > W_MOST)) {
             const float f = move_maximum(w, s0, s1, ck, sc.bias, full, j0, seen, m);
-            l *= f;
+            l *= (double)f * f;
 #pragma unroll
-            for (int d = 0; d < DV / 16; d++) o[d] *= f;
+            for (int d = 0; d < DV / 16; d++) o[d] *= f * f;
         }
         float inverse = sc.inverse;
         if (granule_odd(sc)) {
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
             inverse = 0.f;
         }
         Weights<TERMS> wt;
-        l += granule_weights<TERMS>(wt, w) * inverse;
+        l += (double)(granule_weights<TERMS>(wt, w) * inverse);
 #pragma unroll
         for (int d = 0; d < DV / 16; d++) {
             const half8 v = codes_f16<KIND>(vb[d / 2][d % 2 * 2], vb[d / 2][d % 2 * 2 + 1]);
@@ -170,20 +173,21 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
 #pragma unroll
         for (int w = 0; w < NW; w++) mm = fmaxf(mm, m_s[w][cc]);
         floatx4 sum{0.f, 0.f, 0.f, 0.f};
-        float den = 0.f;
+        double den = 0;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = __builtin_amdgcn_exp2f(m_s[w][cc] - mm);
-            sum += *(const floatx4 *)&o_s[(w * plan.cols + cc) * OS + d] * f;
-            den += l_s[w][cc] * f;
+            const float f = __builtin_amdgcn_exp2f(0.5f * (m_s[w][cc] - mm));
+            sum += *(const floatx4 *)&o_s[(w * plan.cols + cc) * OS + d] * (f * f);
+            den += l_s[w][cc] * ((double)f * f);
         }
         if (plan.splits > 1) {
             *(floatx4 *)(plan.sums + (item + cc) * DV + d) = sum;
-            if (d == 0) *(float2 *)(plan.stats + (item + cc) * 2) = make_float2(mm, den);
+            if (d == 0) *(double2 *)(plan.stats + (item + cc) * 2) = make_double2((double)mm, den);
         } else {
+            const double norm = 1.0 / den;
             T *out = (T *)a.out.data + (int64_t)(r.row + i) * a.out.stride + (int64_t)(h * group + qq % group) * a.p.vd;
             for (int j = 0; j < 4; j++)
-                if (d + j < a.p.vd) out[d + j] = (T)(sum[j] / den);
+                if (d + j < a.p.vd) out[d + j] = (T)(float)((double)sum[j] * norm);
         }
     }
 }
@@ -193,7 +197,8 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
 // in flight; the groups' sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsPlan plan) {
-    __shared__ float f_s[MOST_SPLITS], part[8];
+    __shared__ float f_s[MOST_SPLITS], most_s[4];
+    __shared__ double l_s[4];
     __shared__ __attribute__((aligned(16))) float o_s[256 * 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int64_t blk = blockIdx.x;
@@ -205,20 +210,20 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsP
     const int h = (int)(blk % a.p.kv_heads), seq = (int)(blk / a.p.kv_heads);
     // the splits' maxima, factors and denominators
     const bool has = tid < plan.splits;
-    const float2 st = has ? *(const float2 *)(plan.stats + (item + (int64_t)tid * plan.cols) * 2) : make_float2(M_NONE, 0.f);
+    const double2 st = has ? *(const double2 *)(plan.stats + (item + (int64_t)tid * plan.cols) * 2) : make_double2(M_NONE, 0);
     const SeqRows r = seq_rows(a.b, seq);
     const int group = a.heads / a.p.kv_heads, qq = tile * 16 + cc, i = qq / group;
     if (i >= r.live) return;
-    float m = st.x;
+    float m = (float)st.x;
     for (int w = 32; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
-    if (lane == 0) part[wave] = m;
+    if (lane == 0) most_s[wave] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const float f = __builtin_amdgcn_exp2f(st.x - m);
-    if (has) f_s[tid] = f;
-    float l = has ? st.y * f : 0.f;
+    m = fmaxf(fmaxf(most_s[0], most_s[1]), fmaxf(most_s[2], most_s[3]));
+    const float f = __builtin_amdgcn_exp2f(0.5f * ((float)st.x - m));
+    if (has) f_s[tid] = f * f;
+    double l = has ? st.y * ((double)f * f) : 0;
     for (int w = 32; w > 0; w >>= 1) l += __shfl_xor(l, w, 64);
-    if (lane == 0) part[4 + wave] = l;
+    if (lane == 0) l_s[wave] = l;
     __syncthreads();
     const int quads = a.p.dv / 4, groups = 256 / quads, mine = tid / quads, d = tid % quads * 4;
     floatx4 o{0.f, 0.f, 0.f, 0.f};
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsP
     float num = 0.f;
     for (int w = 0; w < groups; w++) num += o_s[w * a.p.dv + tid];
     ((T *)a.out.data)[(int64_t)(r.row + i) * a.out.stride + (int64_t)(h * group + qq % group) * a.p.vd + tid] =
-        (T)(num / (part[4] + part[5] + part[6] + part[7]));
+        (T)(float)((double)num / ((l_s[0] + l_s[1]) + (l_s[2] + l_s[3])));
 }
 
 // ---------------------------------------------------------------------------
@@ -272,7 +277,7 @@ size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int head
     if (b.n_seqs == 0 || (!few && pages_chunk_takes(p, b, heads, dtype))) return 0;
     const RowsPlan plan = rows_plan(p, b, heads, window, sinks);
     if (plan.splits == 1) return 0;
-    return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 2) * 4;
+    return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 4) * 4;
 }
 
 template <typename T, int KIND, int DK, int DV, int NW>
@@ -316,7 +321,7 @@ void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, 
     RowsPlan plan = rows_plan(a.p, a.b, a.heads, (uint32_t)a.window, (uint32_t)a.sinks);
     if (plan.splits > 1) {
         plan.sums = (float *)ws;
-        plan.stats = plan.sums + (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles * plan.splits * plan.cols * a.p.dv;
+        plan.stats = (double *)(plan.sums + (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles * plan.splits * plan.cols * a.p.dv);
     }
     if (a.dtype == DITCH_F32) rows_typed<float>(a, plan, s);
     else if (a.dtype == DITCH_F16) rows_typed<_Float16>(a, plan, s);

@@ -71,7 +71,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 
     // the wave's tiles
     QueryTile<KP, TERMS> q[QT];
-    float cq[QT], m[QT], l[QT];
+    float cq[QT], m[QT];
+    double l[QT];
     Seen seen[QT];
     int lo[QT], hi[QT];  // positions of each tile's first and last live row
     floatx4 o[QT][DV / 16];
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
         query_terms(q[i], raw);
         cq[i] = a.scale * 1.4426950408889634f * q[i].down;
         m[i] = M_NONE;
-        l[i] = 0.f;
+        l[i] = 0;
 #pragma unroll
         for (int d = 0; d < DV / 16; d++) o[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
         const half8 *v = (const half8 *)(ops + (slot * UNITS + 2 * KP) * 2 * 64) + lane;
         Weights<TERMS> wt[QT];
 #pragma unroll
-        for (int i = 0; i < QT; i++) l[i] += granule_weights<TERMS>(wt[i], w[i]) * inverse;
+        for (int i = 0; i < QT; i++) l[i] += (double)(granule_weights<TERMS>(wt[i], w[i]) * inverse);
 #pragma unroll
         for (int d = 0; d < DV / 16; d++) {
             const half8 x = v[d * 64];
@@ -200,9 +201,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 #pragma unroll
                 for (int i = 0; i < QT; i++) {
                     const float f = move_maximum(w[i], s[i][0], s[i][1], cq[i] * sc.key, sc.bias, full, a0 + 4 * g, seen[i], m[i]);
-                    l[i] *= f;
+                    l[i] *= (double)f * f;
 #pragma unroll
-                    for (int d = 0; d < DV / 16; d++) o[i][d] *= f;
+                    for (int d = 0; d < DV / 16; d++) o[i][d] *= f * f;
                 }
             }
             float inverse = sc.inverse;
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 
 #pragma unroll
     for (int i = 0; i < QT; i++) {
-        const float den = sum_groups(l[i]);
+        const double norm = 1.0 / sum_groups(l[i]);
         const int qi = q0 + (wave * QT + i) * 16 + c, row = qi / group;
         if (row >= r.live) continue;
         T *out = (T *)a.out.data + (int64_t)(r.row + row) * a.out.stride + (int64_t)(h * group + qi % group) * a.p.vd;
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
         for (int d = 0; d < DV / 16; d++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (16 * d + 4 * g + j < a.p.vd) out[16 * d + 4 * g + j] = (T)(o[i][d][j] / den);
+                if (16 * d + 4 * g + j < a.p.vd) out[16 * d + 4 * g + j] = (T)(float)((double)o[i][d][j] * norm);
     }
 }
 

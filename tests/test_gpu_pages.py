@@ -843,3 +843,68 @@ def test_refusals(dev):
     attend(batch=changed(b, max_rows=0))
     got = s.download()
     np.testing.assert_array_equal(got.codes, pool.codes)
+
+
+# ---------------------------------------------------------------------------
+# value scales of any size next to each other
+
+def _check_scales(dev, pool, table, seqs, heads, dtype, bound, seed=3):
+    """Attention against 64 bits, relative to the outputs themselves however small they are. On top of what the head
+    of this file adds up: the logarithm of a value scale is off by 2^-23 of itself, and as much again for each of the
+    two sums it goes into, a weight then by less than 2^-21 max |log2 scale|; of 16-bit rows a granule's part of the
+    denominator comes from its f16 weights where its scale is at most 2^6 below the largest of those before it, which
+    is n * 2^-31 of the whole."""
+    rng = np.random.default_rng(seed)
+    s = Setup(dev, pool, table)
+    rows, pos = [r for r, _ in seqs], [p for _, p in seqs]
+    starts, n = _starts(rows), sum(rows)
+    keys = max(r + p for r, p in seqs)
+    q = Rows(dev, n, heads * pool.hd, dtype, rng.standard_normal((n, heads * pool.hd)))
+    out = Rows(dev, n, heads * pool.vd, dtype)
+    scale = pool.hd ** -0.5
+    s.attention(0, s.batch(starts, pos, max_rows=bound), dtype, out, q, heads, scale)
+    dev.sync()
+    got = out.get().reshape(n, heads, pool.vd)
+    want, mass, size, spread, top = ref.attention(pool, 0, table, starts, pos, q.x.reshape(n, heads, pool.hd), scale)
+    vs = pool.scales[0, :, :, 1]
+    bias = np.abs(np.log2(vs[vs > 0])).max()
+    d = (ref.padded(pool.hd) / 32 + 8) * 2.0 ** -23 * size + 2.0 ** -22 * spread + 2.0 ** -21 * bias
+    tol = (2 * d + (keys / 256 + 16) * 2.0 ** -23) * mass + keys * 2.0 ** -36 * top + 2.0 ** -149
+    if dtype != "f32":
+        info = torch.finfo(TORCH[dtype])
+        tol += 2.0 ** -12 * mass + (keys * 2.0 ** -31 + info.eps / 2 * 1.01) * np.abs(want) + info.smallest_normal * info.eps / 2
+    worst = np.max(np.abs(got - want) / tol)
+    assert worst <= 1, worst
+
+
+# rows and position of one sequence: one workgroup a tile, a chunk, keys split over workgroups
+REACHES = [(1, 400), (64, 400), (1, 4500)]
+
+
+def _scaled(kind, pos, first, rest, page=64):
+    rng = np.random.default_rng(pos)
+    cols = -(-(pos + 64) // page)
+    pool = _filled(rng, kind, 1, cols, page, 1, 64, 64)
+    table = _tables(rng, pool, 1, cols)
+    pool.scales[0, :, :, 1] *= np.where(np.arange(cols) == table[0, 0], first, rest)[:, None]
+    return pool, table
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
+@pytest.mark.parametrize("reach", REACHES)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("first,rest", [(1e-35, 1.0), (1e-32, 1.0), (1.0, 1e-35), (1e-35, 1e-35), (1e-35, 1e30),
+                                        (1e30, 1e-35), (1e-20, 1.0)])
+def test_value_scales_at_the_ends_of_the_range(dev, first, rest, dtype, reach, bound):
+    pool, table = _scaled("int8", reach[1], first, rest)
+    _check_scales(dev, pool, table, [reach], 4, dtype, bound)
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
+@pytest.mark.parametrize("reach", REACHES)
+@pytest.mark.parametrize("rest", [1.0, 1e-33])
+def test_a_page_of_zeros_in_front(dev, rest, reach, bound):
+    pool, table = _scaled("e4m3", reach[1], rest, rest)
+    pool.scales[0, table[0, 0]] = 0
+    pool.codes[0, table[0, 0]] = 0
+    _check_scales(dev, pool, table, [reach], 4, "f32", bound)
