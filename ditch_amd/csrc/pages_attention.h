@@ -38,8 +38,15 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float W_UP = 12.f, W_MOST = 15.f;
 constexpr float M_NONE = -3e38f;  // the maximum over no keys
 
-// A value scale with log2 outside of this goes its own way (see granule_scales).
+// A value scale with log2 outside of this, or this far below that of the
+// largest scale walked before it, goes its own way (see granule_scales). Of
+// one-term weights the denominator sums what f16 leaves, off by 2^-25 a key,
+// so that n keys of a scale 2^-NEAR of the one that the maximum holds to 2^12
+// are off by n 2^(NEAR - 37) of the whole: 2^-13 at 2^18 keys. Two terms sum
+// the weights in f32: they end at 2^-126.
 constexpr float BIAS_PLAIN = 40.f;
+template <int TERMS>
+constexpr float BIAS_NEAR = TERMS == 1 ? 6.f : 60.f;
 
 __device__ __forceinline__ floatx4 mfma_f16(half8 a, half8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -188,19 +195,26 @@ __device__ __forceinline__ float weight_terms(Weights<TERMS> &w, const float (&x
 }
 
 // A granule's scales as the loops use them. A value scale far from 1 would
-// take the denominator's part out of the weights' range, a NaN would reach
-// rows that see none of the granule, and zero has no logarithm: such a
-// granule is `odd` (see odd_granule). Zero goes by the least scale there is,
-// so that it moves the maximum past no other's weights.
+// take the denominator's part out of the weights' range, and so would one far
+// below the others; a NaN would reach rows that see none of the granule, and
+// zero has no logarithm: such a granule is `odd` (see odd_granule), by itself
+// with an inverse of 0. Zero goes below the least scale there is, so that it
+// moves the maximum past no other's weights.
+constexpr float BIAS_ZERO = -127.f;
 struct GranuleScales {
     float key, bias, inverse;
 };
 __device__ __forceinline__ GranuleScales granule_scales(float ks, float vs) {
     const bool zero = fabsf(vs) < 1.17549435e-38f;  // (subnormal: the logarithm takes it for zero)
-    return {ks, zero ? -126.f : __builtin_amdgcn_logf(vs), zero ? 0.f : 1.f / vs};
+    const float bias = zero ? BIAS_ZERO : __builtin_amdgcn_logf(vs);
+    const bool plain = fabsf(bias) <= BIAS_PLAIN && fabsf(ks) <= 3.4028234663852886e38f;
+    return {ks, bias, plain ? 1.f / vs : 0.f};
 }
-__device__ __forceinline__ bool granule_odd(const GranuleScales &sc) {
-    return sc.inverse == 0.f || !(fabsf(sc.bias) <= BIAS_PLAIN) || !(fabsf(sc.key) <= 3.4028234663852886e38f);
+// (top: the largest bias so far, this granule's included)
+template <int TERMS>
+__device__ __forceinline__ bool granule_odd(const GranuleScales &sc, float &top) {
+    top = fmaxf(top, sc.bias);
+    return sc.inverse == 0.f || sc.bias < top - BIAS_NEAR<TERMS>;
 }
 
 // The rows of a query tile: 16 consecutive (row, head of the KV head's
@@ -284,7 +298,7 @@ __device__ __forceinline__ double odd_granule(float (&w)[8], const GranuleScales
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         sum += w[j] == -INFINITY ? 0.0 : exp2_wide(w[j] - sc.bias);
-        if (sc.inverse == 0.f) w[j] = -INFINITY;
+        if (sc.bias == BIAS_ZERO) w[j] = -INFINITY;
     }
     return sum;
 }

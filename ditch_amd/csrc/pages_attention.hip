@@ -78,7 +78,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     floatx4 o[DV / 16];
 #pragma unroll
     for (int d = 0; d < DV / 16; d++) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float m = M_NONE;
+    float m = M_NONE, top = -INFINITY;
     double l = 0;
 
     const int k0 = (int)((int64_t)tr.granules * split / plan.splits), k1 = (int)((int64_t)tr.granules * (split + 1) / plan.splits);
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
             for (int d = 0; d < DV / 16; d++) o[d] *= f * f;
         }
         float inverse = sc.inverse;
-        if (granule_odd(sc)) {
+        if (granule_odd<TERMS>(sc, top)) {
             l += odd_granule(w, sc);
             inverse = 0.f;
         }

@@ -72,6 +72,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
     // the wave's tiles
     QueryTile<KP, TERMS> q[QT];
     float cq[QT], m[QT];
+    float top = -INFINITY;
     double l[QT];
     Seen seen[QT];
     int lo[QT], hi[QT];  // positions of each tile's first and last live row
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
                 }
             }
             float inverse = sc.inverse;
-            if (granule_odd(sc)) {
+            if (granule_odd<TERMS>(sc, top)) {
 #pragma unroll
                 for (int i = 0; i < QT; i++) l[i] += odd_granule(w[i], sc);
                 inverse = 0.f;

@@ -718,7 +718,8 @@ int32_t ditch_hip_kv_pages_read_device(ditch_hip *h, const ditch_kv_pages *p, ui
  * sequence, key positions j <= t for a row at position t; with window > 0
  * only t - window < j and the first `sinks` positions. Query head i reads
  * KV head i / (heads / kv_heads). f32 rows are exact to about f32 rounding;
- * 16-bit ones use softmax weights of 11 bits, sums are f32 throughout.
+ * 16-bit ones use softmax weights of 11 bits. Sums of values are f32, those
+ * of weights 64 bits wide, whatever the pages' scales are.
  * `ws` is device scratch of ditch_hip_kv_pages_attention_workspace bytes
  * (may be 0; its contents do not matter, calls that overlap need one each). */
 uint64_t ditch_hip_kv_pages_attention_workspace(const ditch_kv_pages *p, const ditch_kv_batch *b,

@@ -908,3 +908,31 @@ def test_a_page_of_zeros_in_front(dev, rest, reach, bound):
     pool.scales[0, table[0, 0]] = 0
     pool.codes[0, table[0, 0]] = 0
     _check_scales(dev, pool, table, [reach], 4, "f32", bound)
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
+@pytest.mark.parametrize("reach", REACHES)
+@pytest.mark.parametrize("kind,dtype", [("int8", "bf16"), ("e4m3", "f16"), ("int8", "f32")])
+@pytest.mark.parametrize("apart", [7, 20, 33, 43])
+@pytest.mark.parametrize("large_first", [True, False])
+def test_value_scales_far_apart(dev, large_first, apart, kind, dtype, reach, bound):
+    """One page of large values and the others 2^-apart of it, in front of them or behind."""
+    low = 2.0 ** -apart
+    pool, table = _scaled(kind, reach[1], 1.0 if large_first else low, low)
+    if not large_first:
+        pool.scales[0, table[0, reach[1] // 64 - 1], :, 1] /= np.float32(low)
+    _check_scales(dev, pool, table, [reach], 4, dtype, bound)
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 64])
+def test_scales_of_every_size_in_16_bits(dev, kind, dtype, rows, bound):
+    rng = np.random.default_rng(12)
+    pool = _filled(rng, kind, 1, 9, 64, 2, 128, 128)
+    pool.scales[0, :, :, 1] *= 10.0 ** rng.integers(-8 if dtype == "f16" else -6, 1 if dtype == "f16" else 7, (9, 2))
+    table = _tables(rng, pool, 1, 8)
+    pool.scales[0, table[0, 2]] = 0
+    pool.codes[0, table[0, 2]] = 0
+    _check_scales(dev, pool, table, [(rows, 400)], 4, dtype, bound)
