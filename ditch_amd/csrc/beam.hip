@@ -5,7 +5,9 @@
 // workgroup takes a chunk of a row into registers, forms its maximum, the sum
 // of exponentials relative to it, and its k best logits; a second kernel joins
 // the chunks of a prompt's beams, forms the scores in 64 bits and takes the k
-// best of beams x chunks x k.
+// best of beams x chunks x k. A row is cut by its tokens, whatever its address,
+// and summed in units of 2048 whatever the chunks: equal rows have equal sums,
+// to the bit, in every beam and every batch, so that equal scores stay ties.
 //
 // The k best of a wave's part: with the maxima of its 128 half lanes, any
 // threshold that k of them reach is reached by the k best, and by few
@@ -58,10 +60,14 @@ struct BeamArgs {
     uint32_t *tokens;
     const float *logits, *prev;
     Candidate *list;  // [rows][chunks][k]
-    double *stats;    // [rows][chunks][4 waves][2]: maximum, sum of exponentials relative to it
-    int32_t beams, k, chunks;
+    double *stats;    // [rows][units][2]: maximum, sum of exponentials relative to it
+    int32_t beams, k, chunks, units;  // units: of 2048 tokens, those of a row's chunks
     int64_t vocab;
 };
+
+// (rows start at any multiple of 4 bytes)
+typedef float quad_t __attribute__((ext_vector_type(4), aligned(4)));
+constexpr int UNIT = 8;  // quads a lane of a unit
 
 // A workgroup of 4 waves a chunk of 256 R quads of a row.
 template <int R>
@@ -72,56 +78,60 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
     const int64_t row = blockIdx.x / a.chunks;
     const int chunk = (int)(blockIdx.x % a.chunks), k = a.k;
     const float *x = a.logits + row * a.vocab;
-    // quads at 16-byte addresses: quad q holds tokens 4 q - shift + 0..3
     // (vocab <= 2^30: 32 bits hold the last chunk's end)
-    const int shift = (int)((uintptr_t)x / 4 % 4), V = (int)a.vocab;
-    const int first = (chunk * 4 + wave) * R * 256 - shift, t0 = first + 4 * lane;  // the lane's quad r: from t0 + 256 r
+    const int V = (int)a.vocab;
+    const int first = (chunk * 4 + wave) * R * 256, t0 = first + 4 * lane;  // the lane's quad r: from t0 + 256 r
     float v[R][4];
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const int t = t0 + 256 * r;
-        if (t >= 0 && t + 4 <= V) {
-            const float4 f = *(const float4 *)(x + t);
-            v[r][0] = f.x;
-            v[r][1] = f.y;
-            v[r][2] = f.z;
-            v[r][3] = f.w;
+        if (t + 4 <= V) {
+            const quad_t f = *(const quad_t *)(x + t);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[r][j] = f[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[r][j] = t + j >= 0 && t + j < V ? x[t + j] : -INFINITY;
+            for (int j = 0; j < 4; j++) v[r][j] = t + j < V ? x[t + j] : -INFINITY;
         }
     }
-    // the half lanes' maxima, the wave's, and its sum
+    // the half lanes' maxima, and each unit's maximum and sum
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int j = 0; j < 4; j++) top[r >= R / 2] = fmaxf(top[r >= R / 2], v[r][j]);
-    float m = fmaxf(top[0], top[1]);
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    double sum = 0;
+    double *st = a.stats + (row * a.units + (chunk * 4 + wave) * (R / UNIT)) * 2;
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        float s[4];
+    for (int u = 0; u < R / UNIT; u++) {
+        float m = R == UNIT ? fmaxf(top[0], top[1]) : top[u];
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        double sum = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = __builtin_amdgcn_exp2f((v[r][j] - m) * 1.44269504f);
-        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+        for (int r = UNIT * u; r < UNIT * (u + 1); r++) {
+            float s[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[j] = __builtin_amdgcn_exp2f((v[r][j] - m) * 1.44269504f);
+            sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+        }
+        // (a unit of -infinities or past the row has no sum; a NaN shows in it)
+        if (m == -INFINITY) {
+            bool nan = false;
+#pragma unroll
+            for (int r = UNIT * u; r < UNIT * (u + 1); r++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) nan |= v[r][j] != v[r][j];
+            sum = nan ? NAN : 0;
+        }
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (lane == 0) {
+            st[2 * u] = m;
+            st[2 * u + 1] = sum;
+        }
     }
-    // (a wave of -infinities or past the row has no sum; a NaN shows in it)
-    bool nan = false;
-    if (m == -INFINITY) {
-        sum = 0;
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) nan |= v[r][j] != v[r][j];
-        if (nan) sum = NAN;
-    }
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
 
     // the wave's tokens, and how many of them the list needs
-    const int lo = first < 0 ? 0 : first, hi = first + R * 256 < V ? first + R * 256 : V;
-    const int have = hi > lo ? hi - lo : 0, need = have < k ? have : k;
+    const int hi = first + R * 256 < V ? first + R * 256 : V;
+    const int have = hi > first ? hi - first : 0, need = have < k ? have : k;
     int count = 0;
     bool done = need == 0;
     if (!done && need == k) {
@@ -173,7 +183,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         uint32_t low = 0, high = ~0u;
         auto logit = [&](int r, int j, bool &in) {
             const int t = t0 + 256 * r + j;
-            in = t >= 0 && t < V;
+            in = t < V;
             return in ? x[t] : 0.f;
         };
         auto reach = [&](uint32_t key) {
@@ -233,12 +243,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamArgs a) {
         }
         count = need;
     }
-    if (lane == 0) {
-        count_s[wave] = count;
-        double *st = a.stats + ((int64_t)blockIdx.x * 4 + wave) * 2;
-        st[0] = m;
-        st[1] = sum;
-    }
+    if (lane == 0) count_s[wave] = count;
     __syncthreads();
     // the workgroup's k best by their ranks among its waves' candidates
     const int n0 = count_s[0], n1 = count_s[1], n2 = count_s[2], n3 = count_s[3], n = n0 + n1 + n2 + n3;
@@ -282,17 +287,17 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
     for (int b = wave; b < a.beams; b += JOIN / 64) {
         double sum = 0;
         float most;  // (the maxima are f32)
-        const double *st = a.stats + (row0 + b) * a.chunks * 8;
+        const double *st = a.stats + (row0 + b) * a.units * 2;
         // (a lane's first part stays in registers, as few have a second)
-        const double2 one = lane < 4 * a.chunks ? *(const double2 *)(st + 2 * lane) : make_double2(-INFINITY, 0);
+        const double2 one = lane < a.units ? *(const double2 *)(st + 2 * lane) : make_double2(-INFINITY, 0);
         const float prev = a.prev[row0 + b];
         most = (float)one.x;
-        for (int c = lane + 64; c < 4 * a.chunks; c += 64) most = fmaxf(most, (float)st[2 * c]);
+        for (int c = lane + 64; c < a.units; c += 64) most = fmaxf(most, (float)st[2 * c]);
         for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
         const double m = most;
         auto add = [&](double cm, double cs) { sum += cm == -INFINITY ? cs : cs * exp(cm - m); };
         add(one.x, one.y);
-        for (int c = lane + 64; c < 4 * a.chunks; c += 64) add(st[2 * c], st[2 * c + 1]);
+        for (int c = lane + 64; c < a.units; c += 64) add(st[2 * c], st[2 * c + 1]);
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if (lane == 0) {
             lse_s[b] = m == -INFINITY || m == INFINITY ? NAN : m + log(sum);
@@ -447,22 +452,23 @@ __global__ __launch_bounds__(JOIN) void beam_join_kernel(BeamArgs a) {
 static int beam_quads(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)1024 * 16384 ? 16 : 8; }
 static int64_t beam_chunks(int64_t rows, int64_t vocab) {
     const int64_t per = beam_quads(rows, vocab) * 1024;
-    return (vocab + 3 + per - 1) / per;  // (a row may start 3 tokens into its first quad)
+    return (vocab + per - 1) / per;
 }
+static int64_t beam_units(int64_t rows, int64_t vocab) { return beam_chunks(rows, vocab) * 4 * beam_quads(rows, vocab) / UNIT; }
 
 size_t beam_select_workspace(int64_t prompts, int64_t beams, int64_t vocab, int64_t k) {
-    const int64_t chunks = beam_chunks(prompts * beams, vocab);
-    return (size_t)(prompts * beams * chunks) * (k * sizeof(Candidate) + 8 * sizeof(double));
+    const int64_t rows = prompts * beams;
+    return (size_t)rows * (beam_chunks(rows, vocab) * k * sizeof(Candidate) + beam_units(rows, vocab) * 2 * sizeof(double));
 }
 
 void launch_beam_select(float *scores, int32_t *parents, uint32_t *tokens, const float *logits, const float *prev,
                         int64_t prompts, int64_t beams, int64_t vocab, int64_t k, void *ws, size_t ws_bytes,
                         hipStream_t s) {
-    const int64_t rows = prompts * beams, chunks = beam_chunks(rows, vocab);
+    const int64_t rows = prompts * beams, chunks = beam_chunks(rows, vocab), units = beam_units(rows, vocab);
     DITCH_CHECK(rows * chunks < (int64_t)1 << 24, DITCH_INVALID_ARGUMENT, "beam select: more logits than one launch holds");
     double *stats = (double *)ws;
-    const BeamArgs a{scores, parents, tokens, logits, prev, (Candidate *)(stats + rows * chunks * 8), stats,
-                     (int32_t)beams, (int32_t)k, (int32_t)chunks, vocab};
+    const BeamArgs a{scores, parents, tokens, logits, prev, (Candidate *)(stats + rows * units * 2), stats,
+                     (int32_t)beams, (int32_t)k, (int32_t)chunks, (int32_t)units, vocab};
     if (beam_quads(rows, vocab) == 16)
         hipLaunchKernelGGL(beam_chunk_kernel<16>, dim3((unsigned)(rows * chunks)), dim3(256), 0, s, a);
     else

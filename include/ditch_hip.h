@@ -754,7 +754,10 @@ int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, in
  * best, highest first: scores f32 [n_prompts][k], parents (beam) and tokens.
  * A beam's continuations are in the order of its logits, equal ones by the
  * lower token; beams are compared by scores formed in 64 bits, the lower
- * beam first among equals. A beam whose previous score is -infinity comes after every finite
+ * beam first among equals. The log sum exp in them adds f32 exponentials (off
+ * by some 2^-21) in an order that is the row's own: equal rows under equal
+ * previous scores tie, wherever they lie and whatever else the call
+ * holds. A beam whose previous score is -infinity comes after every finite
  * one; a beam without probabilities (a NaN or +infinity among its logits,
  * or nothing above -infinity; a NaN previous score) scores NaN and comes
  * last. 1 <= beams <= 64, 1 <= k <= 128, k <= beams * vocab, vocab <= 2^30. `ws`:

@@ -149,3 +149,34 @@ def test_refusals(dev):
     with pytest.raises(DeviceError):
         dev.beam_select(16, 16, None, 16, 16, 1, 2, 100, 4, 16, need)
     dev.beam_select(16, 16, 16, 16, 16, 0, 2, 100, 4, 16, need)  # no prompts: nothing to do
+
+
+@pytest.mark.parametrize("prompts,beams,vocab,k", [(3, 4, 4097, 8), (2, 8, 50257, 16), (1, 6, 1001, 128),
+                                                   (90, 4, 50257, 5), (1, 64, 30, 60)])
+def test_equal_beams_tie(dev, prompts, beams, vocab, k):
+    """Beams with the same random logits and the same previous scores, their rows at every alignment: the lower first."""
+    rng = np.random.default_rng(vocab)
+    row = rng.standard_normal((prompts, 1, vocab)).astype(np.float32) * 3
+    _check(dev, np.repeat(row, beams, 1), np.full((prompts, beams), -1.25, dtype=np.float32), k)
+
+
+def test_a_prompt_alone_and_in_a_batch(dev):
+    """The same bits for a prompt by itself, in a batch of the larger chunks, and at every address."""
+    rng = np.random.default_rng(10)
+    n, beams, vocab, k = 84, 4, 50257, 6
+    x = rng.standard_normal((n, beams, vocab)).astype(np.float32) * 2
+    prev = -rng.uniform(0, 5, (n, beams)).astype(np.float32)
+    whole = _select(dev, x, prev, k)
+    for p in (0, 1, 2, 41, 83):
+        for got, want in zip(_select(dev, x[p:p + 1], prev[p:p + 1], k), whole):
+            np.testing.assert_array_equal(got[0], want[p])
+    need = dev.beam_select_workspace(1, beams, vocab, k)
+    ws, pb = hipmem.Buffer(need), hipmem.Buffer.from_array(prev[5])
+    for shift in range(4):
+        b = hipmem.Buffer.from_array(np.concatenate([np.zeros(shift, np.float32), x[5].ravel()]))
+        outs = [hipmem.Buffer(k * 4) for _ in range(3)]
+        dev.beam_select(outs[0].ptr, outs[1].ptr, outs[2].ptr, b.ptr.value + 4 * shift, pb.ptr, 1, beams, vocab, k,
+                        ws.ptr.value, need)
+        hipmem.synchronize()
+        for got, want in zip(outs, whole):
+            np.testing.assert_array_equal(got.download(np.int32, (k,)), want[5].view(np.int32))
