@@ -1449,7 +1449,7 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
         const ditch_kv_batch kb{pc->table.get<int32_t>(0), (uint32_t)pc->cols, (uint32_t)B, pc->starts.get<uint32_t>(0),
                                 pc->pos.get<uint32_t>(0), (uint64_t)n, (uint32_t)std::min(max_rows ? max_rows : n, T), (uint32_t)T};
         pa.p = pool_view(&pc->pages, 0);
-        pa.b = batch = batch_view(&kb, pa.p);
+        batch = batch_view(&kb, pa.p);
         pa.dtype = DITCH_F32;
         pa.heads = (int32_t)nh;
         pa.scale = c.attn_scale;
@@ -1457,7 +1457,9 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
         pa.sinks = (int32_t)pc->sinks;
         pa.few = !max_rows && n <= B;  // one row a prompt, as far as can be told
         (void)pc->ws.get<uint8_t>(pages_attention_workspace(pa.p, batch, pa.heads, DITCH_F32, pc->window, pc->sinks, pa.few));
-        launch_rows_batch(d_rows, n, B, T, pc->starts.get<uint32_t>(0), pc->pos.get<uint32_t>(0), s);
+        batch.ends = kb.starts + B;
+        batch.rows = d_rows;
+        pa.b = batch;
     }
     int *dense_flag = m->attn_dense.get<int>(1);  // checked at the first layer that can use it
     bool dense_checked = false;
@@ -1467,6 +1469,9 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
     else
         hipLaunchKernelGGL(embed_kernel, dim3(grid_for(n * hidden)), dim3(256), 0, s, x, m->embed.t->v, d_tokens, n);
     DITCH_TRY_HIP(hipGetLastError());
+    if (paged)
+        launch_rows_batch(d_rows, n, B, T, pc->starts.get<uint32_t>(0), pc->starts.get<uint32_t>(0) + B,
+                          pc->pos.get<uint32_t>(0), x, hidden, s);
     auto capture = [&](int64_t entry) {
         if (!d_res || n_capture == 0) return;
         hipLaunchKernelGGL(capture_kernel, dim3(grid_for(n_capture * hidden)), dim3(256), 0, s,
@@ -1825,7 +1830,7 @@ ditch_hip_kv_cache *kv_cache_create_pages(ditch_hip_model *m, int64_t B, int64_t
     DITCH_CHECK(p.codes_bytes && c.head_dim <= 256, DITCH_INVALID_ARGUMENT, "kv cache: kind or head_dim");
     p.codes = kc->codes.get<uint8_t>(p.codes_bytes);
     p.scales = kc->scales.get<float>(p.scales_bytes / 4);
-    (void)kc->starts.get<uint32_t>(B + 1);
+    (void)kc->starts.get<uint32_t>(2 * B);  // starts and ends
     (void)kc->pos.get<uint32_t>(B);
     launch_own_pages(kc->table.get<int32_t>(B * cols), B * cols, s);
     return kc.release();

@@ -16,10 +16,13 @@ struct PoolView {
     int32_t dk, dv;      // as stored: rounded up to multiples of 64
 };
 
-// The batch (ditch_kv_batch), checked on the host as far as it can be.
+// The batch (ditch_kv_batch), checked on the host as far as it can be; or a
+// forward's, whose sequences lie in any order: `ends` are then its own, and
+// `rows` (else NULL) say whose a row is.
 struct BatchView {
     const int32_t *table;
-    const uint32_t *starts, *pos;
+    const uint32_t *starts, *ends, *pos;
+    const ditch_row *rows;
     int64_t table_stride;
     int32_t n_seqs, n_rows, max_rows, max_len;
 };
@@ -41,7 +44,7 @@ struct SeqRows {
 };
 
 __device__ __forceinline__ SeqRows seq_rows(const BatchView &b, int s) {
-    const uint32_t lo = b.starts[s], hi = b.starts[s + 1], pos = b.pos[s];
+    const uint32_t lo = b.starts[s], hi = b.ends[s], pos = b.pos[s];
     SeqRows r{0, 0, 0, 0};
     if (lo >= (uint32_t)b.n_rows || hi <= lo) return r;
     uint32_t n = hi - lo;
@@ -97,11 +100,12 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
                        int64_t table_stride, const int32_t *parents, const int32_t *spare, const uint32_t *lens,
                        int64_t groups, int64_t beams, hipStream_t s);
 
-// The batch of a forward's rows {b, pos}, sorted by prompt and position:
-// starts [B + 1] and pos [B]; a prompt whose rows are not consecutive gets
-// the position max_len, past which nothing is appended and outputs are NaN.
-void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *pos,
-                       hipStream_t s);
+// The batch of a forward's rows {b, pos}, each prompt's one after the other, the
+// prompts in any order: starts, ends and pos [B]. A prompt whose rows do not
+// lie so gets the position max_len, past which nothing is appended; its rows,
+// and those of prompts from B on, become NaN in x [n][hidden].
+void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *ends,
+                       uint32_t *pos, float *x, int64_t hidden, hipStream_t s);
 // table [B][cols] = b cols + j
 void launch_own_pages(int32_t *table, int64_t n, hipStream_t s);
 

@@ -67,8 +67,8 @@ BatchView batch_view(const ditch_kv_batch *b, const PoolView &p) {
     DITCH_CHECK(b->n_rows <= (uint64_t)INT32_MAX && b->n_seqs <= (uint32_t)INT32_MAX &&
                     b->max_rows <= (uint32_t)INT32_MAX && b->max_len <= (uint32_t)INT32_MAX - 256,
                 DITCH_INVALID_ARGUMENT, "kv pages: more rows, sequences or positions than 2^31");
-    BatchView v{b->table, b->starts, b->pos, (int64_t)b->table_stride, (int32_t)b->n_seqs, (int32_t)b->n_rows,
-                (int32_t)b->max_rows, (int32_t)b->max_len};
+    BatchView v{b->table, b->starts, b->starts ? b->starts + 1 : nullptr, b->pos, nullptr, (int64_t)b->table_stride,
+                (int32_t)b->n_seqs, (int32_t)b->n_rows, (int32_t)b->max_rows, (int32_t)b->max_len};
     if (v.n_seqs == 0 || v.n_rows == 0 || v.max_rows == 0 || v.max_len == 0) {
         v.n_seqs = 0;
         return v;
@@ -369,6 +369,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5))) void p
         const int q_part = (int)(blk % a.q_parts), row = (int)(blk / a.q_parts);
         // the row's sequence: the last whose rows start at or before it, 64 candidates at a time
         int seq = 0, span = a.b.n_seqs;
+        if (a.b.rows) {
+            const uint32_t of = a.b.rows[row].b;
+            if (of >= (uint32_t)a.b.n_seqs) return;
+            seq = (int)of;
+            span = 1;
+        }
         while (span > 1) {
             const int step = (span + 63) / 64, at = seq + (tid & 63) * step;
             const uint64_t before = __ballot(at < seq + span && a.b.starts[at < seq + span ? at : seq] <= (uint32_t)row);
@@ -722,28 +728,63 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
 // ---------------------------------------------------------------------------
 // a model's own cache in pages
 
-// A wave a prompt: its first row, and whether its rows follow each other.
-__global__ __launch_bounds__(64) void rows_batch_kernel(const ditch_row *rows, uint32_t n, uint32_t B, uint32_t max_len,
-                                                        uint32_t *starts, uint32_t *pos) {
-    const uint32_t b = blockIdx.x, lane = threadIdx.x;
-    auto first_of = [&](uint32_t p) {
-        uint32_t lo = 0, hi = n;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (rows[mid].b < p) lo = mid + 1;
-            else hi = mid;
-        }
-        return lo;
-    };
-    const uint32_t s = first_of(b), e = b < B ? first_of(b + 1) : s;
-    if (lane == 0) starts[b] = s;
-    if (b == B) return;
-    const uint32_t p = s < e ? rows[s].pos : 0;
-    bool bad = false;
-    for (uint32_t i = s + lane; i < e; i += 64) bad |= rows[i].b != b || rows[i].pos != p + (i - s);
-    if (__any(bad)) {
-        if (lane == 0) pos[b] = max_len;
-    } else if (lane == 0) pos[b] = p;
+// A workgroup a prompt, one more for the rows of no prompt: it looks all rows
+// over once. A prompt's rows follow each other if they are as many as lie
+// between its first and its last, and all as far from their indexes.
+constexpr int ROWS_BATCH = 1024;
+__global__ __launch_bounds__(ROWS_BATCH) void rows_batch_kernel(const ditch_row *rows, uint32_t n, uint32_t B, uint32_t max_len,
+                                                                uint32_t *starts, uint32_t *ends, uint32_t *pos, float *x,
+                                                                int64_t hidden) {
+    __shared__ uint32_t part[5][ROWS_BATCH / 64];
+    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    auto mine = [&](uint32_t of) { return b < B ? of == b : of >= B; };
+    // its first and last row, their number, the least and largest distance of a position from its index
+    uint32_t lo = ~0u, hi = 0, many = 0, near = ~0u, far = 0;
+#pragma unroll 4
+    for (uint32_t i = tid; i < n; i += ROWS_BATCH) {
+        const ditch_row r = rows[i];
+        if (!mine(r.b)) continue;
+        const uint32_t d = r.pos - i;
+        lo = i < lo ? i : lo;
+        hi = i;
+        many++;
+        near = d < near ? d : near;
+        far = d > far ? d : far;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor(lo, o, 64));
+        hi = max(hi, (uint32_t)__shfl_xor(hi, o, 64));
+        many += __shfl_xor(many, o, 64);
+        near = min(near, (uint32_t)__shfl_xor(near, o, 64));
+        far = max(far, (uint32_t)__shfl_xor(far, o, 64));
+    }
+    if (lane == 0) {
+        part[0][wave] = lo;
+        part[1][wave] = hi;
+        part[2][wave] = many;
+        part[3][wave] = near;
+        part[4][wave] = far;
+    }
+    __syncthreads();
+    lo = near = ~0u;
+    hi = many = far = 0;
+    for (int w = 0; w < ROWS_BATCH / 64; w++) {
+        lo = min(lo, part[0][w]);
+        hi = max(hi, part[1][w]);
+        many += part[2][w];
+        near = min(near, part[3][w]);
+        far = max(far, part[4][w]);
+    }
+    const bool ok = b < B && many && hi - lo + 1 == many && near == far;
+    if (tid == 0 && b < B) {
+        starts[b] = many ? lo : 0;
+        ends[b] = ok ? hi + 1 : 0;
+        pos[b] = ok ? near + lo : max_len;
+    }
+    if (ok || !many) return;
+    for (uint32_t i = wave; i < n; i += ROWS_BATCH / 64)
+        if (mine(rows[i].b))
+            for (int64_t d = lane; d < hidden; d += 64) x[i * hidden + d] = NAN;
 }
 
 __global__ __launch_bounds__(256) void own_pages_kernel(int32_t *table, int64_t n) {
@@ -751,10 +792,10 @@ __global__ __launch_bounds__(256) void own_pages_kernel(int32_t *table, int64_t 
     if (i < n) table[i] = (int32_t)i;
 }
 
-void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *pos,
-                       hipStream_t s) {
-    hipLaunchKernelGGL(rows_batch_kernel, dim3((unsigned)(B + 1)), dim3(64), 0, s, rows, (uint32_t)n, (uint32_t)B,
-                       (uint32_t)max_len, starts, pos);
+void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *ends,
+                       uint32_t *pos, float *x, int64_t hidden, hipStream_t s) {
+    hipLaunchKernelGGL(rows_batch_kernel, dim3((unsigned)(B + 1)), dim3(ROWS_BATCH), 0, s, rows, (uint32_t)n, (uint32_t)B,
+                       (uint32_t)max_len, starts, ends, pos, x, hidden);
     DITCH_TRY_HIP(hipGetLastError());
 }
 

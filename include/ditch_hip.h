@@ -776,8 +776,10 @@ int32_t ditch_hip_beam_select_device(ditch_hip *h, float *d_scores, int32_t *d_p
  * past 1024 positions too; with window > 0 every layer attends to the last
  * `window` positions and the first `sinks`. Every layer then appends, rotates
  * and attends through the entries above. The rows of a call are a prompt's
- * after the other's, each prompt's at consecutive positions (as generate
- * passes them; rows of a prompt that are not give NaN). Models with latent
+ * after the other's, the prompts in any order, each prompt's at consecutive
+ * positions. All rows of a prompt that are not so give NaN and none of them is
+ * appended; rows of prompts from n_prompts on and at positions from max_len on
+ * give NaN too. Models with latent
  * attention are Unsupported. Freed by ditch_hip_kv_cache_free.             */
 ditch_hip_kv_cache *ditch_hip_kv_cache_create_pages(ditch_hip_model *m, uint32_t n_prompts,
                                                     uint32_t max_len, int32_t kind,

@@ -171,3 +171,45 @@ def test_refused_caches(dev):
     finally:
         m.free()
         latent.free()
+
+
+def _orders():
+    whole = [[(0, p) for p in range(5)], [(1, p) for p in range(40)], [(2, 0)], [(3, p) for p in range(3)]]
+    mixed = [(b, p) for p in range(3) for b in (0, 1)]
+    return [
+        # rows, those that have to come out as the sorted rows do (the others: NaN)
+        (sum(whole[::-1], []), lambda b, p: True),
+        (whole[2] + whole[0] + whole[3] + whole[1], lambda b, p: True),
+        (mixed + whole[2], lambda b, p: b == 2),
+        (whole[1] + [(0, 0), (2, 0), (0, 1)], lambda b, p: b in (1, 2)),
+        ([(7, 0)] + whole[1] + [(4, 0), ((1 << 32) - 1, 2)] + whole[0], lambda b, p: b in (0, 1)),
+        (whole[3] + whole[3][:1] + whole[0], lambda b, p: b == 0),
+        (whole[0][:3] + [(0, 4), (1, 0)], lambda b, p: b == 1),
+        (whole[0] + [(1, p) for p in range(48, 53)], lambda b, p: b == 0),
+        (whole[0] + [(1, (1 << 32) - 1), (1, 0)], lambda b, p: b == 0),
+    ]
+
+
+@pytest.mark.parametrize("case", range(len(_orders())))
+def test_prompts_in_any_order(dev, case):
+    """Prompts one after the other in any order give what the sorted ones do; rows of a prompt that do not follow each
+    other, of no prompt, or past the cache give NaN and leave the others alone."""
+    rows, fine = _orders()[case]
+    spec = mg.dense("bf16", hidden=128, inter=128, heads=4, kv_heads=2, head_dim=64, layers=2, vocab=100, seed=8)
+    m = Model(dev, spec)
+    a, b = m.kv_cache_pages(4, 50, page_tokens=32), m.kv_cache_pages(4, 50, page_tokens=32)
+    token = {(x, y): (7 * x + 13 * y) % 100 for x, y in rows}
+    good = sorted(r for r in set(rows) if fine(*r) and r[1] < 50)
+    try:
+        want = dict(zip(good, _cached(dev, m, a, [token[r] for r in good], good, np.arange(len(good)), 100)))
+        for turn in range(2):  # (what the first left in the buffers must not show in the second)
+            got = _cached(dev, m, b, [token[r] for r in rows], rows, np.arange(len(rows)), 100)
+            for r, g in zip(rows, got):
+                if r in want:
+                    assert np.abs(g - want[r]).max() <= 1e-5 * np.abs(want[r]).max(), r
+                else:
+                    assert np.isnan(g).all(), r
+    finally:
+        m.kv_cache_free(a)
+        m.kv_cache_free(b)
+        m.free()
