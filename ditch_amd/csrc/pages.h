@@ -103,7 +103,8 @@ void launch_pages_fork(const ditch_kv_pages *p, int32_t *table_out, int32_t *spa
 // The batch of a forward's rows {b, pos}, each prompt's one after the other, the
 // prompts in any order: starts, ends and pos [B]. A prompt whose rows do not
 // lie so gets the position max_len, past which nothing is appended; its rows,
-// and those of prompts from B on, become NaN in x [n][hidden].
+// those at such positions and those of prompts from B on become NaN in x
+// [n][hidden].
 void launch_rows_batch(const ditch_row *rows, int64_t n, int64_t B, int64_t max_len, uint32_t *starts, uint32_t *ends,
                        uint32_t *pos, float *x, int64_t hidden, hipStream_t s);
 // table [B][cols] = b cols + j

@@ -781,9 +781,10 @@ __global__ __launch_bounds__(ROWS_BATCH) void rows_batch_kernel(const ditch_row 
         ends[b] = ok ? hi + 1 : 0;
         pos[b] = ok ? near + lo : max_len;
     }
-    if (ok || !many) return;
+    // (the last: of one that ends within the cache every row has a place)
+    if (!many || (ok && near + hi < max_len && near + lo <= near + hi)) return;
     for (uint32_t i = wave; i < n; i += ROWS_BATCH / 64)
-        if (mine(rows[i].b))
+        if (mine(rows[i].b) && !(ok && rows[i].pos < max_len))
             for (int64_t d = lane; d < hidden; d += 64) x[i * hidden + d] = NAN;
 }
 

@@ -187,6 +187,7 @@ def _orders():
         (whole[0][:3] + [(0, 4), (1, 0)], lambda b, p: b == 1),
         (whole[0] + [(1, p) for p in range(48, 53)], lambda b, p: b == 0),
         (whole[0] + [(1, (1 << 32) - 1), (1, 0)], lambda b, p: b == 0),
+        (whole[3] + [(0, p) for p in range(70)] + whole[2], lambda b, p: True),
     ]
 
 
