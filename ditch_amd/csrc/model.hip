@@ -1456,10 +1456,11 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
         pa.window = (int32_t)pc->window;
         pa.sinks = (int32_t)pc->sinks;
         pa.few = !max_rows && n <= B;  // one row a prompt, as far as can be told
-        (void)pc->ws.get<uint8_t>(pages_attention_workspace(pa.p, batch, pa.heads, DITCH_F32, pc->window, pc->sinks, pa.few));
         batch.ends = kb.starts + B;
         batch.rows = d_rows;
+        batch.by_rows = !max_rows;
         pa.b = batch;
+        (void)pc->ws.get<uint8_t>(pages_attention_workspace(pa.p, batch, pa.heads, DITCH_F32, pc->window, pc->sinks, pa.few));
     }
     int *dense_flag = m->attn_dense.get<int>(1);  // checked at the first layer that can use it
     bool dense_checked = false;

@@ -18,13 +18,16 @@ struct PoolView {
 
 // The batch (ditch_kv_batch), checked on the host as far as it can be; or a
 // forward's, whose sequences lie in any order: `ends` are then its own, and
-// `rows` (else NULL) say whose a row is.
+// `rows` (else NULL) say whose a row is. Where max_rows is no more than the
+// number of rows (by_rows), a grid of sequences x max_rows grows with its
+// square; launches may then have workgroups for the rows instead, of which
+// the first row of a tile or page finds work.
 struct BatchView {
     const int32_t *table;
     const uint32_t *starts, *ends, *pos;
     const ditch_row *rows;
     int64_t table_stride;
-    int32_t n_seqs, n_rows, max_rows, max_len;
+    int32_t n_seqs, n_rows, max_rows, max_len, by_rows;
 };
 
 struct RowsView {
@@ -58,6 +61,17 @@ __device__ __forceinline__ SeqRows seq_rows(const BatchView &b, int s) {
         r.pos = (int32_t)pos;
     }
     return r;
+}
+
+// The sequence of row `row` of a batch with `rows`, and the row's place in it;
+// -1 for none.
+__device__ __forceinline__ int32_t row_place(const BatchView &b, int row, int &seq, SeqRows &r) {
+    const uint32_t of = b.rows[row].b;
+    if (of >= (uint32_t)b.n_seqs) return -1;
+    seq = (int)of;
+    r = seq_rows(b, seq);
+    const int i = row - r.row;
+    return i >= 0 && i < r.n ? i : -1;
 }
 
 // The page that holds position page_index * page .. of sequence s; -1 when
@@ -118,7 +132,7 @@ struct PagesAttention {
     int32_t dtype, heads;
     float scale;
     int32_t window, sinks;
-    int32_t few;  // max_rows is a bound that few sequences reach: the few-row kernel
+    int32_t few;  // one row a sequence, as far as can be told: the few-row kernel
 };
 size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int heads, int32_t dtype, uint32_t window,
                                  uint32_t sinks, int few = 0);

@@ -68,7 +68,7 @@ BatchView batch_view(const ditch_kv_batch *b, const PoolView &p) {
                     b->max_rows <= (uint32_t)INT32_MAX && b->max_len <= (uint32_t)INT32_MAX - 256,
                 DITCH_INVALID_ARGUMENT, "kv pages: more rows, sequences or positions than 2^31");
     BatchView v{b->table, b->starts, b->starts ? b->starts + 1 : nullptr, b->pos, nullptr, (int64_t)b->table_stride,
-                (int32_t)b->n_seqs, (int32_t)b->n_rows, (int32_t)b->max_rows, (int32_t)b->max_len};
+                (int32_t)b->n_seqs, (int32_t)b->n_rows, (int32_t)b->max_rows, (int32_t)b->max_len, 0};
     if (v.n_seqs == 0 || v.n_rows == 0 || v.max_rows == 0 || v.max_len == 0) {
         v.n_seqs = 0;
         return v;
@@ -202,7 +202,7 @@ struct AppendArgs {
     BatchView b;
     RowsView k, v, q, q_out;
     RopeView rope;
-    int32_t slots;   // pages that a sequence's rows can touch
+    int32_t slots;   // pages that a sequence's rows can touch (0: workgroups for the rows)
     int32_t heads;   // query heads (0: no queries)
     int32_t q_parts; // workgroups a query row
     int64_t kv_blocks;
@@ -393,9 +393,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5))) void p
     blk >>= 1;
     const int h = (int)(blk % a.p.kv_heads);
     blk /= a.p.kv_heads;
-    const int slot = (int)(blk % a.slots), seq = (int)(blk / a.slots);
-    const SeqRows r = seq_rows(a.b, seq);
-    const int page_index = (r.pos >> a.p.page_shift) + slot, t0 = page_index << a.p.page_shift;
+    int seq, page_index;
+    SeqRows r;
+    if (a.slots) {
+        seq = (int)(blk / a.slots);
+        r = seq_rows(a.b, seq);
+        page_index = (r.pos >> a.p.page_shift) + (int)(blk % a.slots);
+    } else {
+        const int i = row_place(a.b, (int)blk, seq, r);
+        // (the page's first new row)
+        if (i < 0 || i >= r.live || (i > 0 && ((r.pos + i) & (a.p.page - 1)))) return;
+        page_index = (r.pos + i) >> a.p.page_shift;
+    }
+    const int t0 = page_index << a.p.page_shift;
     const int end = r.pos + r.live;
     if (r.live == 0 || t0 >= end) return;
     const int id = page_of(a.b, a.p, seq, page_index);
@@ -533,7 +543,8 @@ void launch_pages_append(const PoolView &p, const BatchView &b, int32_t dtype, c
     AppendArgs a{p, b, k, v, q ? *q : RowsView{}, q ? *q_out : RowsView{}, rope, 0, q ? heads : 0, 1, 0};
     a.b.max_rows = most_rows(b);
     a.slots = (a.b.max_rows + p.page - 2) / p.page + 1;
-    a.kv_blocks = (int64_t)b.n_seqs * a.slots * p.kv_heads * 2;
+    if (b.by_rows && b.n_rows < (int64_t)b.n_seqs * a.slots) a.slots = 0;
+    a.kv_blocks = (a.slots ? (int64_t)b.n_seqs * a.slots : b.n_rows) * p.kv_heads * 2;
     // a row's heads over several workgroups until the rows fill the chip
     const int64_t rows = b.n_rows;
     if (q && rows < 1024) a.q_parts = (int)std::min<int64_t>((int64_t)heads * ((p.hd + 7) / 8 + 255) / 256 + 1, 1024 / rows + 1);

@@ -29,10 +29,29 @@ constexpr int MOST_SPLITS = 256;
 
 struct RowsPlan {
     int tiles, splits, cols;  // query tiles of a (sequence, KV head); workgroups a tile; queries a tile
+    int by_rows;              // tiles are those that can start in a row, and rows go in place of sequences
     int waves;                // of a workgroup: 4 or 8
     float *sums;              // [item][cols][DV]: splits > 1
     double *stats;            // [item][cols][2]: the maximum, the denominator relative to it
 };
+
+// Whose tile workgroup `blk` of a split has; false for none.
+__device__ __forceinline__ bool place_tile(const PagesAttention &a, const RowsPlan &plan, int64_t blk, int &tile, int &h, int &seq,
+                                           SeqRows &r) {
+    const int u = (int)(blk % plan.tiles);
+    blk /= plan.tiles;
+    h = (int)(blk % a.p.kv_heads);
+    const int at = (int)(blk / a.p.kv_heads), group = a.heads / a.p.kv_heads;
+    if (!plan.by_rows) {
+        tile = u;
+        seq = at;
+        r = seq_rows(a.b, seq);
+        return tile * 16 / group < r.n;
+    }
+    const int i = row_place(a.b, at, seq, r);
+    tile = (i * group + 15) / 16 + u;
+    return i >= 0 && tile * 16 < (i + 1) * group;
+}
 
 template <typename T, int KIND, int DK, int DV, int NW>
 __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, RowsPlan plan) {
@@ -42,16 +61,12 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     __shared__ float m_s[NW][16];
     __shared__ double l_s[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    int64_t blk = blockIdx.x;
-    const int split = (int)(blk % plan.splits);
-    blk /= plan.splits;
-    const int tile = (int)(blk % plan.tiles);
-    blk /= plan.tiles;
-    const int h = (int)(blk % a.p.kv_heads), seq = (int)(blk / a.p.kv_heads);
-    const SeqRows r = seq_rows(a.b, seq);
+    const int split = (int)(blockIdx.x % plan.splits);
+    int tile, h, seq;
+    SeqRows r;
+    if (!place_tile(a, plan, blockIdx.x / plan.splits, tile, h, seq, r)) return;
     const int group = a.heads / a.p.kv_heads;
     const int first_row = tile * 16 / group, last_row = (tile * 16 + 15) / group;
-    if (first_row >= r.n) return;
     // rows past max_len
     if (split == 0 && last_row >= r.live) {
         for (int e = tid; e < 16 * a.p.vd; e += NW * 64) {
@@ -165,7 +180,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     for (int d = 0; d < DV / 16; d++)
         if (c < plan.cols) *(floatx4 *)&o_s[(wave * plan.cols + c) * OS + 16 * d + 4 * g] = o[d];
     __syncthreads();
-    const int64_t item = ((((int64_t)seq * a.p.kv_heads + h) * plan.tiles + tile) * plan.splits + split) * plan.cols;
+    const int64_t item = (int64_t)blockIdx.x * plan.cols;
     for (int e = tid; e < plan.cols * (DV / 4); e += NW * 64) {
         const int cc = e / (DV / 4), d = e % (DV / 4) * 4, qq = tile * 16 + cc, i = qq / group;
         if (i >= r.live) continue;
@@ -201,17 +216,15 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsP
     __shared__ double l_s[4];
     __shared__ __attribute__((aligned(16))) float o_s[256 * 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t blk = blockIdx.x;
-    const int cc = (int)(blk % plan.cols);
-    blk /= plan.cols;
+    const int64_t blk = blockIdx.x / plan.cols;
+    const int cc = (int)(blockIdx.x % plan.cols);
     const int64_t item = blk * plan.splits * plan.cols + cc;
-    const int tile = (int)(blk % plan.tiles);
-    blk /= plan.tiles;
-    const int h = (int)(blk % a.p.kv_heads), seq = (int)(blk / a.p.kv_heads);
     // the splits' maxima, factors and denominators
     const bool has = tid < plan.splits;
     const double2 st = has ? *(const double2 *)(plan.stats + (item + (int64_t)tid * plan.cols) * 2) : make_double2(M_NONE, 0);
-    const SeqRows r = seq_rows(a.b, seq);
+    int tile, h, seq;
+    SeqRows r;
+    if (!place_tile(a, plan, blk, tile, h, seq, r)) return;
     const int group = a.heads / a.p.kv_heads, qq = tile * 16 + cc, i = qq / group;
     if (i >= r.live) return;
     float m = (float)st.x;
@@ -245,6 +258,10 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PagesAttention a, RowsP
 // ---------------------------------------------------------------------------
 // the plan
 
+static int64_t plan_items(const PoolView &p, const BatchView &b, const RowsPlan &plan) {
+    return (int64_t)(plan.by_rows ? b.n_rows : b.n_seqs) * p.kv_heads * plan.tiles;
+}
+
 static RowsPlan rows_plan(const PoolView &p, const BatchView &b, int heads, uint32_t window, uint32_t sinks) {
     const int group = heads / p.kv_heads;
     RowsPlan plan{};
@@ -255,7 +272,11 @@ static RowsPlan rows_plan(const PoolView &p, const BatchView &b, int heads, uint
     int64_t keys = b.max_len;
     if (window) keys = std::min<int64_t>(keys, (int64_t)window + 16 + sinks + 2 * GRANULE);
     const int64_t granules = (keys + GRANULE - 1) / GRANULE;
-    const int64_t items = (int64_t)b.n_seqs * p.kv_heads * plan.tiles;
+    if (b.by_rows && (int64_t)b.n_rows * ((group + 15) / 16) < (int64_t)b.n_seqs * plan.tiles) {
+        plan.by_rows = 1;
+        plan.tiles = (group + 15) / 16;
+    }
+    const int64_t items = plan_items(p, b, plan);
     // Waves. 2048 (two a SIMD) saturate the memory: 64 sequences of up to 8192
     // tokens of 8 heads of 128 take 137 us with 512 tiles of 4 waves, 139 us
     // with twice the waves. A tile's first 8 waves share a workgroup, more go
@@ -277,7 +298,7 @@ size_t pages_attention_workspace(const PoolView &p, const BatchView &b, int head
     if (b.n_seqs == 0 || (!few && pages_chunk_takes(p, b, heads, dtype))) return 0;
     const RowsPlan plan = rows_plan(p, b, heads, window, sinks);
     if (plan.splits == 1) return 0;
-    return (size_t)b.n_seqs * p.kv_heads * plan.tiles * plan.splits * plan.cols * (p.dv + 4) * 4;
+    return (size_t)plan_items(p, b, plan) * plan.splits * plan.cols * (p.dv + 4) * 4;
 }
 
 template <typename T, int KIND, int DK, int DV, int NW>
@@ -304,8 +325,8 @@ static void rows_kind(const PagesAttention &a, const RowsPlan &plan, unsigned bl
 
 template <typename T>
 static void rows_typed(const PagesAttention &a, const RowsPlan &plan, hipStream_t s) {
-    const int64_t tiles = (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles;
-    DITCH_CHECK(tiles * std::max(plan.splits, plan.cols) < ((int64_t)1 << 24), DITCH_INVALID_ARGUMENT,
+    const int64_t tiles = plan_items(a.p, a.b, plan);
+    DITCH_CHECK(tiles * (plan.splits > 1 ? std::max(plan.splits, plan.cols) : 1) < ((int64_t)1 << 24), DITCH_INVALID_ARGUMENT,
                 "kv attention: more work than one launch holds");
     if (a.p.kind == DITCH_KV_INT8) rows_kind<T, DITCH_KV_INT8>(a, plan, (unsigned)(tiles * plan.splits), s);
     else rows_kind<T, DITCH_KV_E4M3>(a, plan, (unsigned)(tiles * plan.splits), s);
@@ -321,7 +342,7 @@ void launch_pages_attention(const PagesAttention &a, void *ws, size_t ws_bytes, 
     RowsPlan plan = rows_plan(a.p, a.b, a.heads, (uint32_t)a.window, (uint32_t)a.sinks);
     if (plan.splits > 1) {
         plan.sums = (float *)ws;
-        plan.stats = (double *)(plan.sums + (int64_t)a.b.n_seqs * a.p.kv_heads * plan.tiles * plan.splits * plan.cols * a.p.dv);
+        plan.stats = (double *)(plan.sums + plan_items(a.p, a.b, plan) * plan.splits * plan.cols * a.p.dv);
     }
     if (a.dtype == DITCH_F32) rows_typed<float>(a, plan, s);
     else if (a.dtype == DITCH_F16) rows_typed<_Float16>(a, plan, s);

@@ -38,23 +38,35 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
     // Workgroups go to the 8 XCDs in turn. Each XCD takes whole heads, four at
     // a time (their keys and values share its L2), and the tiles with the most
     // keys first, so that the short ones fill the end.
-    const int heads = a.b.n_seqs * a.p.kv_heads;
-    int head, rank;
-    if (heads >= 8) {
-        const int x = (int)(blockIdx.x % 8), j = (int)(blockIdx.x / 8);
-        const int h0 = (int)((int64_t)heads * x / 8), h1 = (int)((int64_t)heads * (x + 1) / 8);
-        const int set = j / (4 * tiles), first = h0 + 4 * set, many = h1 - first < 4 ? h1 - first : 4;
-        if (many <= 0 || j - 4 * set * tiles >= many * tiles) return;
-        head = first + (j - 4 * set * tiles) % many;
-        rank = (j - 4 * set * tiles) / many;
-    } else {
-        head = (int)(blockIdx.x % heads);
-        rank = (int)(blockIdx.x / heads);
-    }
-    const int h = head % a.p.kv_heads, seq = head / a.p.kv_heads, tile = tiles - 1 - rank;
-    const SeqRows r = seq_rows(a.b, seq);
-    const int group = a.heads / a.p.kv_heads;
+    // (tiles 0: workgroups for the rows, the longest sequences' ends first)
     constexpr int QUERIES = 16 * QT * NW;
+    const int heads = a.b.n_seqs * a.p.kv_heads, group = a.heads / a.p.kv_heads;
+    int h, seq, tile;
+    SeqRows r;
+    if (tiles == 0) {
+        const int per = (group + QUERIES - 1) / QUERIES;
+        h = (int)(blockIdx.x % a.p.kv_heads);
+        const int at = (int)(blockIdx.x / a.p.kv_heads), i = row_place(a.b, a.b.n_rows - 1 - at / per, seq, r);
+        tile = (i * group + QUERIES - 1) / QUERIES + at % per;
+        if (i < 0 || tile * QUERIES >= (i + 1) * group) return;
+    } else {
+        int head, rank;
+        if (heads >= 8) {
+            const int x = (int)(blockIdx.x % 8), j = (int)(blockIdx.x / 8);
+            const int h0 = (int)((int64_t)heads * x / 8), h1 = (int)((int64_t)heads * (x + 1) / 8);
+            const int set = j / (4 * tiles), first = h0 + 4 * set, many = h1 - first < 4 ? h1 - first : 4;
+            if (many <= 0 || j - 4 * set * tiles >= many * tiles) return;
+            head = first + (j - 4 * set * tiles) % many;
+            rank = (j - 4 * set * tiles) / many;
+        } else {
+            head = (int)(blockIdx.x % heads);
+            rank = (int)(blockIdx.x / heads);
+        }
+        h = head % a.p.kv_heads;
+        seq = head / a.p.kv_heads;
+        tile = tiles - 1 - rank;
+        r = seq_rows(a.b, seq);
+    }
     const int q0 = tile * QUERIES;  // the workgroup's first query
     if (q0 / group >= r.n) return;
     const int first_row = q0 / group, last_row = (q0 + QUERIES - 1) / group;
@@ -268,9 +280,13 @@ template <typename T, int KIND, int DK, int DV>
 static void chunk_dims(const PagesAttention &a, hipStream_t s) {
     constexpr int LDS = RING * (2 * (DK / 64) + DV / 32) * 2048;
     const int per = 16 * CHUNK_TILES * CHUNK_WAVES;
-    const int64_t queries = (int64_t)a.b.max_rows * (a.heads / a.p.kv_heads), tiles = (queries + per - 1) / per;
-    const int64_t heads = (int64_t)a.b.n_seqs * a.p.kv_heads;
-    const int64_t blocks = heads >= 8 ? (heads + 7) / 8 * 8 * tiles : heads * tiles;
+    const int64_t group = a.heads / a.p.kv_heads, queries = a.b.max_rows * group, heads = (int64_t)a.b.n_seqs * a.p.kv_heads;
+    int64_t tiles = (queries + per - 1) / per, blocks = heads >= 8 ? (heads + 7) / 8 * 8 * tiles : heads * tiles;
+    const int64_t by_rows = a.b.n_rows * ((group + per - 1) / per) * a.p.kv_heads;
+    if (a.b.by_rows && by_rows < blocks) {
+        tiles = 0;
+        blocks = by_rows;
+    }
     DITCH_CHECK(blocks < ((int64_t)1 << 24) && queries < ((int64_t)1 << 30), DITCH_INVALID_ARGUMENT, "kv attention: more work than one launch holds");
     auto *kernel = pages_chunk_kernel<T, KIND, DK, DV, CHUNK_TILES, CHUNK_WAVES>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(CHUNK_WAVES * 64), LDS, s, a, (int)tiles);

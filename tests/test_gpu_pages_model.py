@@ -214,3 +214,64 @@ def test_prompts_in_any_order(dev, case):
         m.kv_cache_free(a)
         m.kv_cache_free(b)
         m.free()
+
+
+MANY = [
+    # heads, kv_heads, prompts, max_len, the calls: (prompt, rows) in the order of their rows
+    (4, 1, 40, 300, [[(0, 20), (7, 1), (3, 13), (39, 2)], [(b, 1) for b in range(39, -1, -1)], [(7, 33), (0, 2)]]),
+    (5, 1, 20, 100, [[(19, 4), (2, 7), (3, 1)], [(3, 1), (2, 1), (19, 3)]]),
+    (20, 1, 33, 70, [[(5, 3), (4, 30)], [(b, 1) for b in range(33)], [(32, 2), (0, 1), (9, 5)]]),
+    # more rows than prompts, a few of them in one prompt
+    (4, 2, 300, 400, [[(b, 1) for b in range(299)] + [(299, 170)], [(299, 40)] + [(b, 1) for b in range(290)]]),
+    # keys split over workgroups
+    (4, 1, 3, 4000, [[(0, 1200), (1, 10)], [(2, 1), (0, 2)], [(0, 1), (1, 1)], [(0, 3)]]),
+]
+
+
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_rows_of_some_of_many_prompts(dev, case):
+    """Calls whose rows are those of few prompts or of many, no bound on a prompt's rows given, against the plain
+    forward."""
+    heads, kvh, prompts, max_len, calls = MANY[case]
+    spec = mg.dense("bf16", hidden=128, inter=128, heads=heads, kv_heads=kvh, head_dim=64, layers=1, vocab=100, seed=case)
+    spec.config["rope_len"] = max(max_len, spec.config["rope_len"])
+    m = Model(dev, spec)
+    cache = m.kv_cache_pages(prompts, max_len, page_tokens=32)
+    plain = Plain(dev, spec, prompts, max_len, "int8", 32, 0, 0)
+    rng = np.random.default_rng(case)
+    pos = np.zeros(prompts, dtype=np.int64)
+    try:
+        for call in calls:
+            rows = [(b, int(pos[b]) + i) for b, n in call for i in range(n)]
+            tokens = rng.integers(0, 100, len(rows))
+            got = _cached(dev, m, cache, tokens, rows, np.arange(len(rows)), 100)
+            order = sorted(range(len(rows)), key=lambda i: rows[i])
+            counts = np.bincount([b for b, _ in rows], minlength=prompts)
+            want = plain.forward(tokens[order], np.concatenate([[0], np.cumsum(counts)]), pos)
+            assert np.abs(got[order] - want).max() <= TOLERANCE["int8"] * np.abs(want).max()
+            pos += counts
+    finally:
+        m.kv_cache_free(cache)
+        m.free()
+
+
+def test_a_step_of_thousands_of_prompts(dev):
+    """A row for each of 2048 prompts with room for 2048 positions, and one for each of a few: the same logits."""
+    spec = mg.dense("bf16", hidden=128, inter=128, heads=16, kv_heads=1, head_dim=64, layers=1, vocab=100, seed=9)
+    spec.config["rope_len"] = 2048
+    m = Model(dev, spec)
+    n, some = 2048, [0, 1, 63, 700, 2047]
+    big, small = m.kv_cache_pages(n, 2048, page_tokens=32), m.kv_cache_pages(len(some), 2048, page_tokens=32)
+    rng = np.random.default_rng(3)
+    try:
+        for step in range(3):
+            tokens, order = rng.integers(0, 100, n), rng.permutation(n)
+            got = np.empty((n, 100), dtype=np.float32)
+            got[order] = _cached(dev, m, big, tokens[order], [(b, step) for b in order], np.arange(n), 100)
+            want = _cached(dev, m, small, tokens[some], [(i, step) for i in range(len(some))], np.arange(len(some)), 100)
+            assert np.isfinite(got).all()
+            assert np.abs(got[some] - want).max() <= TOLERANCE["int8"] * np.abs(want).max()
+    finally:
+        m.kv_cache_free(big)
+        m.kv_cache_free(small)
+        m.free()
