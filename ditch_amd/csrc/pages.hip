@@ -405,15 +405,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5))) void p
         if (i < 0 || i >= r.live || (i > 0 && ((r.pos + i) & (a.p.page - 1)))) return;
         page_index = (r.pos + i) >> a.p.page_shift;
     }
-    const int t0 = page_index << a.p.page_shift;
     const int end = r.pos + r.live;
-    if (r.live == 0 || t0 >= end) return;
+    // (by the page: its first position may lie past 2^31)
+    if (r.live == 0 || page_index > (end - 1) >> a.p.page_shift) return;
+    const int t0 = page_index << a.p.page_shift;
     const int id = page_of(a.b, a.p, seq, page_index);
     if (id < 0) return;
     const int lo = r.pos > t0 ? r.pos - t0 : 0, hi = end - t0 < a.p.page ? end - t0 : a.p.page;  // new tokens [lo, hi)
     const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk;
     const RowsView &rv = which ? a.v : a.k;
-    const T *rows = (const T *)rv.data + (int64_t)(r.row + t0 - r.pos) * rv.stride + (int64_t)h * D;  // token 0's
+    const T *rows = (const T *)rv.data + (int64_t)(r.row + (t0 - r.pos)) * rv.stride + (int64_t)h * D;  // token 0's
     float *sp = a.p.scales + ((int64_t)id * a.p.kv_heads + h) * 2 + which;
     const float before = lo > 0 ? *sp : 0.f;
     const bool quads = quads_ok<T>(rv, D);
@@ -579,8 +580,9 @@ __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
     blk /= a.p.kv_heads;
     const int slot = (int)(blk % a.granules), seq = (int)(blk / a.granules);
     const SeqRows r = seq_rows(a.b, seq);
-    const int gi = r.pos / GRANULE + slot, t0 = gi * GRANULE, end = r.pos + r.live;
-    if (r.live == 0 || t0 >= end) return;
+    const int gi = r.pos / GRANULE + slot, end = r.pos + r.live;
+    if (r.live == 0 || gi > (end - 1) / GRANULE) return;
+    const int t0 = gi * GRANULE;
     const int id = page_of(a.b, a.p, seq, t0 >> a.p.page_shift);
     const int D = which ? a.p.vd : a.p.hd, DP = which ? a.p.dv : a.p.dk, S = DP + 4;
     const float scale = id < 0 ? NAN : a.p.scales[((int64_t)id * a.p.kv_heads + h) * 2 + which];
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
     }
     __syncthreads();
     const RowsView &rv = which ? a.v : a.k;
-    T *rows = (T *)rv.data + (int64_t)(r.row + t0 - r.pos) * rv.stride + (int64_t)h * D;
+    T *rows = (T *)rv.data + (int64_t)(r.row + (t0 - r.pos)) * rv.stride + (int64_t)h * D;
     const bool quads = quads_ok<T>(rv, D);
     const int per = (D + 3) / 4;
     for (int e = tid; e < (hi - lo) * per; e += 256) {

@@ -936,3 +936,38 @@ def test_scales_of_every_size_in_16_bits(dev, kind, dtype, rows, bound):
     pool.scales[0, table[0, 2]] = 0
     pool.codes[0, table[0, 2]] = 0
     _check_scales(dev, pool, table, [(rows, 400)], 4, dtype, bound)
+
+
+def test_the_last_positions(dev):
+    """Positions up to the most that a batch may have, rows that run past them, pages named behind them: what lies
+    there is as it was, and the rows' attention is that of the same page at the start of a sequence."""
+    rng = np.random.default_rng(20)
+    most, page, n = (1 << 31) - 257, 256, 700
+    pool = ref.Pool("int8", 1, 8, page, 1, 64)
+    table = np.full((1, most // page + 65), 5, dtype=np.int32)  # (page 5: where no row belongs)
+    table[0, :most // page] = -1
+    pos = most - 100
+    table[0, pos // page] = 2
+    s = Setup(dev, pool, table)
+    k, v = (Rows(dev, n, 64, "f32", rng.standard_normal((n, 64))) for _ in range(2))
+    b = s.batch([0, n], [pos], max_len=most)
+    dev.kv_pages_append(s.pages, 0, b, "f32", k.desc, v.desc)
+    touched = ref.append(pool, 0, table, [0, 100], [pos], k.x.reshape(n, 1, 64), v.x.reshape(n, 1, 64))
+    _compare_pools(s.download(), pool, touched, 0)
+    ko, vo = Rows(dev, n, 64, "f32"), Rows(dev, n, 64, "f32")
+    dev.kv_pages_read(s.pages, 0, b, "f32", ko.desc, vo.desc)
+    q, far = Rows(dev, n, 128, "f32", rng.standard_normal((n, 128))), Rows(dev, n, 128, "f32")
+    s.attention(0, b, "f32", far, q, 2, 0.1, window=64)
+    dev.sync()
+    wk, wv = ref.sequence(pool, 0, [2], page)
+    in_page = pos % page
+    for got, want in ((ko.get(), wk), (vo.get(), wv)):
+        np.testing.assert_array_equal(got[:100], want[0, in_page:in_page + 100].astype(np.float32))
+        assert (got[100:] == np.full(4, 0x77, np.uint8).view(np.float32)).all()
+    near_s = Setup(dev, pool, [[2]])
+    near = Rows(dev, n, 128, "f32")
+    near_s.attention(0, near_s.batch([0, n], [in_page], max_len=in_page + 100), "f32", near, q, 2, 0.1, window=64)
+    dev.sync()
+    far, near = far.get(), near.get()
+    assert np.isfinite(far[:100]).all() and np.isnan(far[100:]).all()
+    np.testing.assert_array_equal(far, near)
