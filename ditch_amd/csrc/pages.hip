@@ -703,9 +703,15 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
         if (threadIdx.x == 0)
             a.spare_out[seq] = copies ? a.table[(first + __ffsll((unsigned long long)free) - 1) * a.table_stride + full] : mine;
     }
-    if (!copies || (uint32_t)src >= (uint32_t)a.n_pages || (uint32_t)mine >= (uint32_t)a.n_pages || src == mine) return;
+    if (!copies || (uint32_t)mine >= (uint32_t)a.n_pages || src == mine) return;
     // a page's heads lie next to each other: the workgroup's part of them
     const int64_t layer = blockIdx.y / a.parts, piece = blockIdx.y % a.parts;
+    if ((uint32_t)src >= (uint32_t)a.n_pages) {  // no page to copy: NaN, as where it is looked for
+        if (piece == 0)
+            for (int i = threadIdx.x; i < 2 * a.kv_heads; i += 256)
+                a.scales[(layer * a.layer_pages + mine) * a.kv_heads * 2 + i] = NAN;
+        return;
+    }
     const int64_t from = (layer * a.layer_pages + src) * a.kv_heads, to = (layer * a.layer_pages + mine) * a.kv_heads;
     const int64_t n = a.kv_heads * a.head_bytes / 16, p0 = piece * FORK_PART, left = n - p0 < FORK_PART ? n - p0 : FORK_PART;
     const u32x4_t *cs = (const u32x4_t *)(a.codes + from * a.head_bytes) + p0;

@@ -739,10 +739,12 @@ int32_t ditch_hip_kv_pages_attention_device(ditch_hip *h, const ditch_kv_pages *
  * goes to the parent's first child; the further children copy it (every
  * layer, codes and scales) into their spare page spare[c] and find in
  * spare_out[c] a page that a childless sequence of the group left free:
- * pages in use and spare ones stay equally many. A length that ends with a
- * page copies nothing. table / table_out are [n_groups * beams]
+ * last pages in use and spare ones stay equally many. (Of a childless
+ * sequence's full pages the call says nothing: those that no row of table_out
+ * names are free.) A length that ends with a page copies nothing. table / table_out are [n_groups * beams]
  * [table_stride] and must differ, spare / spare_out [n_groups * beams]
- * likewise. Pages outside the pool are neither read nor written.           */
+ * likewise. Pages outside the pool are neither read nor written; a copy of one
+ * gets scales of NaN, so that rows that see it give NaN as the parent's do. */
 int32_t ditch_hip_kv_pages_fork_device(ditch_hip *h, const ditch_kv_pages *p, int32_t *d_table_out,
                                        int32_t *d_spare_out, const int32_t *d_table,
                                        uint64_t table_stride, const int32_t *d_parents,

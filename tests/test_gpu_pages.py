@@ -971,3 +971,33 @@ def test_the_last_positions(dev):
     far, near = far.get(), near.get()
     assert np.isfinite(far[:100]).all() and np.isnan(far[100:]).all()
     np.testing.assert_array_equal(far, near)
+
+
+@pytest.mark.parametrize("parents,copier,spare", [([0, 0], 1, [2, 3]), ([1, 1], 1, [2, 3]), ([1, 1, 1], 2, [4, 2, 3])])
+def test_a_copy_of_a_page_outside_the_pool_is_nan(dev, parents, copier, spare):
+    """The child's copy has nothing in it that could pass for the parent's tokens; the codes stay."""
+    beams = len(parents)
+    pool = ref.Pool("int8", 2, 6, 32, 3, 64)
+    pool.codes[:] = np.random.default_rng(3).integers(0, 256, pool.codes.shape)
+    table = np.array([[0, -5], [1, 900], [0, 5]], dtype=np.int32)[:beams]
+    spare = np.array(spare, dtype=np.int32)
+    s = Setup(dev, pool, table)
+    d = [hipmem.Buffer.from_array(np.asarray(x)) for x in (np.asarray(parents, np.int32), spare, np.array([40], np.uint32),
+                                                           table * 0, spare * 0)]
+    dev.kv_pages_fork(s.pages, d[3].ptr, d[4].ptr, s.d_table.ptr, 2, d[0].ptr, d[1].ptr, d[2].ptr, 1, beams)
+    got = s.download()
+    t, sp, copies = ref.fork(table, np.asarray(parents), spare, [40], 32, beams)
+    np.testing.assert_array_equal(d[3].download(np.int32, table.shape), t)
+    np.testing.assert_array_equal(d[4].download(np.int32, spare.shape), sp)
+    np.testing.assert_array_equal(got.codes, pool.codes)
+    assert t[copier, 1] == spare[copier]
+    for _, dst in copies:
+        pool.scales[:, dst] = np.nan
+    np.testing.assert_array_equal(got.scales, pool.scales)
+    s.table = t
+    s.d_table = hipmem.Buffer.from_array(t)
+    q, out = Rows(dev, beams, 192, "f32", np.ones((beams, 192))), Rows(dev, beams, 192, "f32")
+    s.attention(0, s.batch(np.arange(beams + 1), [39] * beams), "f32", out, q, 3, 0.1)
+    dev.sync()
+    out = out.get()
+    assert np.isnan(out[[c for c in range(beams) if parents[c] < 2]]).all()
