@@ -546,9 +546,10 @@ void launch_pages_append(const PoolView &p, const BatchView &b, int32_t dtype, c
     a.slots = (a.b.max_rows + p.page - 2) / p.page + 1;
     if (b.by_rows && b.n_rows < (int64_t)b.n_seqs * a.slots) a.slots = 0;
     a.kv_blocks = (a.slots ? (int64_t)b.n_seqs * a.slots : b.n_rows) * p.kv_heads * 2;
-    // a row's heads over several workgroups until the rows fill the chip
-    const int64_t rows = b.n_rows;
-    if (q && rows < 1024) a.q_parts = (int)std::min<int64_t>((int64_t)heads * ((p.hd + 7) / 8 + 255) / 256 + 1, 1024 / rows + 1);
+    // a row's heads over several workgroups until the rows fill the chip, a
+    // thread a pair of quads or a quad that stays as it is (see rotate_queries)
+    const int64_t rows = b.n_rows, quads = (rope.half + 3) / 4 + (p.hd - 2 * rope.half + 3) / 4;
+    if (q && rows < 1024) a.q_parts = (int)std::min<int64_t>((heads * quads + 255) / 256, 1024 / rows + 1);
     const unsigned blocks = grid_blocks(a.kv_blocks + (q ? rows * a.q_parts : 0), "kv append");
     if (dtype == DITCH_F32) append_typed<float>(a, blocks, s);
     else if (dtype == DITCH_F16) append_typed<_Float16>(a, blocks, s);

@@ -1001,3 +1001,24 @@ def test_a_copy_of_a_page_outside_the_pool_is_nan(dev, parents, copier, spare):
     dev.sync()
     out = out.get()
     assert np.isnan(out[[c for c in range(beams) if parents[c] < 2]]).all()
+
+
+@pytest.mark.parametrize("heads,hd,half,style", [(48, 256, 128, "neox"), (33, 100, 20, "gptj"), (40, 128, 0, "neox")])
+def test_many_query_heads_of_few_rows(dev, heads, hd, half, style):
+    """A row's heads over several workgroups, and over one that takes more than its threads hold at once."""
+    rng = np.random.default_rng(heads)
+    pool = ref.Pool("int8", 1, 2, 64, 1, hd)
+    s = Setup(dev, pool, [[1, 0]])
+    cos, sin = _rope(rng, 64, max(half, 1))
+    dc, ds = hipmem.Buffer.from_array(cos), hipmem.Buffer.from_array(sin)
+    for rows in (1, 3):
+        k = Rows(dev, rows, hd, "f32", rng.standard_normal((rows, hd)))
+        q, q_out = Rows(dev, rows, heads * hd, "f32", rng.standard_normal((rows, heads * hd))), Rows(dev, rows, heads * hd, "f32")
+        dev.kv_pages_append(s.pages, 0, s.batch([0, rows], [60 - rows]), "f32", k.desc, k.desc,
+                            rope=dev.kv_rope(dc.ptr.value, ds.ptr.value, 64, half, style), q=q.desc, q_out=q_out.desc,
+                            heads=heads)
+        dev.sync()
+        want = q.x.reshape(rows, heads, hd).astype(np.float64)
+        if half:
+            want = ref.rotate(want, np.arange(60 - rows, 60), cos, sin, style)
+        np.testing.assert_array_equal(q_out.get().reshape(rows, heads, hd), want.astype(np.float32))
