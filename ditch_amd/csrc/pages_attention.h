@@ -37,6 +37,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // its steps below 2^-14 are then 2^-36 of the largest weight.
 constexpr float W_UP = 12.f, W_MOST = 15.f;
 constexpr float M_NONE = -3e38f;  // the maximum over no keys
+// From here on the steps of a maximum (1/2 and more) are no longer small beside
+// W_MOST - W_UP: exponents are then formed as the maximum was, rounded
+// before it is taken off, so that none is above it.
+constexpr float M_FAR = 4194304.f;
 
 // A value scale with log2 outside of this, or this far below that of the
 // largest scale walked before it, goes its own way (see granule_scales). Of
@@ -263,6 +267,14 @@ __device__ __forceinline__ void granule_exponents(float (&w)[8], floatx4 s0, flo
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j] = __builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], ck, add);
 }
+// The same relative to a maximum past M_FAR.
+__device__ __forceinline__ void far_exponents(float (&w)[8], floatx4 s0, floatx4 s1, float ck, float bias, float m) {
+    granule_exponents(w, s0, s1, ck, bias);
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = (w[j] - m) + W_UP;
+}
+// A column of the wave has such a maximum.
+__device__ __forceinline__ bool maximum_far(float m) { return __any(fabsf(m) > M_FAR && m != M_NONE); }
 // Tokens that the column does not see; j0 the lane's first token.
 __device__ __forceinline__ void granule_mask(float (&w)[8], int j0, const Seen &seen) {
 #pragma unroll
@@ -286,7 +298,7 @@ __device__ __forceinline__ float move_maximum(float (&w)[8], floatx4 s0, floatx4
     if (!full) granule_mask(w, j0, seen);
     const float next = fmaxf(m, max_groups(most_of(w))), root = __builtin_amdgcn_exp2f(0.5f * (m - next));
     m = next;
-    granule_exponents(w, s0, s1, ck, bias + (W_UP - m));
+    far_exponents(w, s0, s1, ck, bias, m);
     if (!full) granule_mask(w, j0, seen);
     return root;
 }

@@ -95,6 +95,7 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
     for (int d = 0; d < DV / 16; d++) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = M_NONE, top = -INFINITY;
     double l = 0;
+    bool far = false;
 
     const int k0 = (int)((int64_t)tr.granules * split / plan.splits), k1 = (int)((int64_t)tr.granules * (split + 1) / plan.splits);
     const int per = a.p.page / GRANULE;
@@ -117,9 +118,13 @@ __global__ __launch_bounds__(NW * 64) void pages_rows_kernel(PagesAttention a, R
         const int j0 = gi * GRANULE + 4 * g;
         float w[8];
         granule_exponents(w, s0, s1, ck, sc.bias + (W_UP - m));
-        if (!full) granule_mask(w, j0, seen);
+        if (!full || far) {
+            if (far) far_exponents(w, s0, s1, ck, sc.bias, m);
+            if (!full) granule_mask(w, j0, seen);
+        }
         if (__any(most_of(w) > W_MOST)) {
             const float f = move_maximum(w, s0, s1, ck, sc.bias, full, j0, seen, m);
+            far = maximum_far(m);
             l *= (double)f * f;
 #pragma unroll
             for (int d = 0; d < DV / 16; d++) o[d] *= f * f;

@@ -85,6 +85,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
     QueryTile<KP, TERMS> q[QT];
     float cq[QT], m[QT];
     float top = -INFINITY;
+    bool far = false;
     double l[QT];
     Seen seen[QT];
     int lo[QT], hi[QT];  // positions of each tile's first and last live row
@@ -205,15 +206,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
                 full &= z0 <= lo[i] && (!a.window || a0 > hi[i] - a.window || z0 < a.sinks);
                 granule_exponents(w[i], s[i][0], s[i][1], cq[i] * sc.key, sc.bias + (W_UP - m[i]));
             }
-            if (!full)
+            if (!full || far)
 #pragma unroll
-                for (int i = 0; i < QT; i++) granule_mask(w[i], a0 + 4 * g, seen[i]);
+                for (int i = 0; i < QT; i++) {
+                    if (far) far_exponents(w[i], s[i][0], s[i][1], cq[i] * sc.key, sc.bias, m[i]);
+                    if (!full) granule_mask(w[i], a0 + 4 * g, seen[i]);
+                }
 #pragma unroll
             for (int i = 0; i < QT; i++) more |= most_of(w[i]) > W_MOST;
             if (__any(more)) {
+                far = false;
 #pragma unroll
                 for (int i = 0; i < QT; i++) {
                     const float f = move_maximum(w[i], s[i][0], s[i][1], cq[i] * sc.key, sc.bias, full, a0 + 4 * g, seen[i], m[i]);
+                    far |= maximum_far(m[i]);
                     l[i] *= (double)f * f;
 #pragma unroll
                     for (int d = 0; d < DV / 16; d++) o[i][d] *= f * f;

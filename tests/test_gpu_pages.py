@@ -1022,3 +1022,38 @@ def test_many_query_heads_of_few_rows(dev, heads, hd, half, style):
         if half:
             want = ref.rotate(want, np.arange(60 - rows, 60), cos, sin, style)
         np.testing.assert_array_equal(q_out.get().reshape(rows, heads, hd), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("bound", BOUNDS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("reach", REACHES)
+def test_scores_past_the_exponents_steps(dev, reach, size, dtype, bound):
+    """Scores so large that f32 holds them in steps of a weight's whole range and more: where the largest lies further
+    ahead of the others than they are off (d of the head of this file, and 200 for weights that vanish), its value
+    comes out; elsewhere a mean of values."""
+    rng = np.random.default_rng(22)
+    rows, pos = reach
+    cols = -(-(rows + pos) // 64)
+    pool = _filled(rng, "int8", 1, cols, 64, 1, 64, 64)
+    table = _tables(rng, pool, 1, cols)
+    s = Setup(dev, pool, table)
+    q = Rows(dev, rows, 256, dtype, rng.standard_normal((rows, 256)) * size)
+    out = Rows(dev, rows, 256, dtype)
+    s.attention(0, s.batch([0, rows], [pos], max_rows=bound), dtype, out, q, 4, 0.125)
+    dev.sync()
+    got = out.get().reshape(rows, 4, 64)
+    k, v = (x[0] for x in ref.sequence(pool, 0, table[0], rows + pos))
+    eps = 2.0 ** -20 if dtype == "f32" else 2.0 ** -8
+    alone = 0
+    for i in range(rows):
+        n = pos + i + 1
+        scores = q.x[i].reshape(4, 64).astype(np.float64) @ k[:n].T * 0.125
+        off = 10 * 2.0 ** -23 * (np.abs(q.x[i].reshape(4, 64)).astype(np.float64) @ np.abs(k[:n]).T).max(1) * 0.125
+        best, second = scores.argmax(1), np.sort(scores, 1)[:, -2]
+        for h in range(4):
+            assert np.isfinite(got[i, h]).all() and (np.abs(got[i, h]) <= np.abs(v[:n]).max(0) * (1 + eps)).all()
+            if scores[h].max() - second[h] > 2 * off[h] + 200:
+                alone += 1
+                assert (np.abs(got[i, h] - v[best[h]]) <= eps * np.abs(v[best[h]]) + 1e-30).all()
+    assert alone >= 2 * rows
