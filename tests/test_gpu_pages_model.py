@@ -177,7 +177,8 @@ def _orders():
     whole = [[(0, p) for p in range(5)], [(1, p) for p in range(40)], [(2, 0)], [(3, p) for p in range(3)]]
     mixed = [(b, p) for p in range(3) for b in (0, 1)]
     return [
-        # rows, those that have to come out as the sorted rows do (the others: NaN)
+        # rows, those that have to come out as the sorted rows do (the others: NaN; None: whatever the positions in
+        # front of them hold, which nothing was appended to)
         (sum(whole[::-1], []), lambda b, p: True),
         (whole[2] + whole[0] + whole[3] + whole[1], lambda b, p: True),
         (mixed + whole[2], lambda b, p: b == 2),
@@ -185,7 +186,7 @@ def _orders():
         ([(7, 0)] + whole[1] + [(4, 0), ((1 << 32) - 1, 2)] + whole[0], lambda b, p: b in (0, 1)),
         (whole[3] + whole[3][:1] + whole[0], lambda b, p: b == 0),
         (whole[0][:3] + [(0, 4), (1, 0)], lambda b, p: b == 1),
-        (whole[0] + [(1, p) for p in range(48, 53)], lambda b, p: b == 0),
+        (whole[0] + [(1, p) for p in range(48, 53)], lambda b, p: b == 0 or (None if p < 50 else False)),
         (whole[0] + [(1, (1 << 32) - 1), (1, 0)], lambda b, p: b == 0),
         (whole[3] + [(0, p) for p in range(70)] + whole[2], lambda b, p: True),
     ]
@@ -206,6 +207,8 @@ def test_prompts_in_any_order(dev, case):
         for turn in range(2):  # (what the first left in the buffers must not show in the second)
             got = _cached(dev, m, b, [token[r] for r in rows], rows, np.arange(len(rows)), 100)
             for r, g in zip(rows, got):
+                if fine(*r) is None:
+                    continue
                 if r in want:
                     assert np.abs(g - want[r]).max() <= 1e-5 * np.abs(want[r]).max(), r
                 else:
