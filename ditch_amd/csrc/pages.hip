@@ -568,8 +568,10 @@ struct ReadArgs {
 
 // A workgroup per (sequence, granule, head, keys or values): its units
 // decoded into LDS rows, which go out as rows: both sides of the transposition
-// in 16-byte accesses. Bound by the memory: 7291 f32 rows of 8 heads of 128,
-// 75 MB, in 20 us; up to 64 of 64 sequences 9 us.
+// in 16-byte accesses. 7291 f32 rows of 8 heads of 128, 75 MB, in 20 us, 3.8 TB/s;
+// up to 64 of 64 sequences 9 us: a workgroup's 4 KB are loaded, transposed and
+// stored one after the other, and what the others do meanwhile does not fill
+// the memory.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
     extern __shared__ __attribute__((aligned(16))) float tile[];  // [GRANULE][DP + 4]
@@ -649,8 +651,9 @@ void launch_pages_read(const PoolView &p, const BatchView &b, int32_t dtype, con
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 // 16-byte words that a workgroup copies: 32 a thread in flight. The last pages
-// of 16 x 8 beams (32 layers of 8 heads of 128, 360 MB moved): 92 us, with 16
-// a thread 102, with 8 or fewer 105 to 112.
+// of 16 x 8 beams (32 layers of 8 heads of 128, 368 MB moved): 76 us the
+// kernel; measured in one sitting, 92 us a call, with 16 a thread 102, with 8
+// or fewer 105 to 112.
 constexpr int FORK_PART = 8192;
 
 struct ForkArgs {

@@ -17,7 +17,7 @@
 // 8192 tokens (8 heads of 128, int8, 32 bf16 query heads, 714 MB) take 139 us,
 // 5.1 TB/s, as a large copy does; one sequence of 130 001 (4 heads of 128,
 // 133 MB) 26 us and 5 us for the join. Bound by latency where they are few
-// (500 tokens: 9.5 us): page id, then scales and codes, then two products and
+// (500 tokens: 9.7 us): page id, then scales and codes, then two products and
 // the exponentials between them, a granule after the other.
 #include <algorithm>
 

@@ -12,12 +12,12 @@
 // so that the matrix cores work while the vector units exponentiate.
 //
 // 2 x 2048 bf16 rows over 2048 cached tokens (32 heads of 128 over 8, e4m3):
-// 206 GF in 232 to 237 us, 870 to 890 TFLOP/s, where a large f16 product
-// reaches 1109. No unit is full (matrix cores 36 % of the cycles, vector issue
-// 52 %, LDS 30 %): what bounds it is the order within a wave, products, then
+// 206 GF in 228 to 239 us, 862 to 904 TFLOP/s, where a large f16 product
+// reaches 1109. No unit is full (matrix cores 38 % of the cycles, vector issue
+// 53 %, LDS 31 %): what bounds it is the order within a wave, products, then
 // maxima and exponentials, then products, with two waves a SIMD to fill each
 // other's gaps. f32 rows take two terms on both products: 5 x up to 1500 rows
-// of 14 heads of 64 under a window of 512 take 46 us.
+// of 14 heads of 64 under a window of 512 take 45 us.
 #include "pages_attention.h"
 
 namespace ditch {
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DK <= 1
 // ---------------------------------------------------------------------------
 
 // Two tiles a wave, four waves: with 2 x 2048 rows over 2048 cached tokens (32
-// heads of 128 over 8, bf16, e4m3) 232 to 237 us; three tiles a wave 316 us, with one
+// heads of 128 over 8, bf16, e4m3) 228 to 239 us; three tiles a wave 316 us, with one
 // wave a SIMD left; eight waves 242 us there, but 78 us against 46 us with
 // 5 x 1500 rows under a window; registers for three waves a SIMD (19 of them
 // spilled) 323 us.
@@ -275,7 +275,9 @@ constexpr int CHUNK_TILES = 2, CHUNK_WAVES = 4;
 // bf16, us few-row / chunk): 1024 tiles of 16 (512 rows, 4000 cached) 102 / 135,
 // 2048 (1024 rows, 2000 cached) 124 / 98, 2048 (8 x 128 rows, 1000 cached)
 // 63 / 50, 4096 (32 x 64 rows, 200 cached) 69 / 36; 14 heads of 64 over 2: 896
-// tiles 41 / 75, 1792 tiles 18 / 20. Under 64 queries a head half of a
+// tiles 41 / 75, 1792 tiles 18 / 20 (past the border by so little that the
+// rule, which knows neither the heads' size nor the keys, is 2 us behind).
+// Under 64 queries a head half of a
 // workgroup's lanes hold none.
 bool pages_chunk_takes(const PoolView &p, const BatchView &b, int heads, int32_t dtype) {
     const int64_t queries = (int64_t)b.max_rows * (heads / p.kv_heads);
