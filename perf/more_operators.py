@@ -220,8 +220,10 @@ def _plain_loss(s):
 
 def _plain_kl(s):
     w = _decoded(s.w[0])
-    # the logits in 64 bits: p and q are near each other, and in their difference 32 lose what f32 gradients hold
-    p, q = (torch.matmul(x.double(), w.double().T) for x in (s.x, s.trial))
+    # where f32 gradients are wanted the logits in 64 bits: in the difference of p and q, which are near each other,
+    # 32 lose what the gradients hold
+    t = torch.float64 if s.case["kind"] == "kl_grad" and s.case["dtype"] == "f32" else torch.float32
+    p, q = (torch.matmul(x.to(t), w.to(t).T).double() for x in (s.x, s.trial))
     lse_p, lse_q = _log_sum(p), _log_sum(q)
     p, q = p.sub_(lse_p[:, None]), q.sub_(lse_q[:, None])
     kl = (p.exp() * (p - q)).sum(-1)
