@@ -268,6 +268,20 @@ PROTOTYPES = {
     "ditch_hip_kv_pages_fork_device": (I32, [P, P, P, P, P, U64, P, P, P, U64, U64, P]),
     "ditch_hip_beam_select_workspace": (U64, [U64, U64, U64, U64]),
     "ditch_hip_beam_select_device": (I32, [P, P, P, P, P, P, U64, U64, U64, U64, P, U64, P]),
+    "ditch_hip_head_loss_workspace": (U64, [P, U64, I32]),
+    "ditch_hip_head_loss_device": (I32, [P, P, P, I32, P, U64, P, P, P, U64, P]),
+    "ditch_hip_head_loss_grad_workspace": (U64, [P, U64, I32, I32]),
+    "ditch_hip_head_loss_grad_device": (I32, [P, I32, P, P, P, U64, P, P, P, P, P, U64, P]),
+    "ditch_hip_head_kl_workspace": (U64, [P, U64, I32]),
+    "ditch_hip_head_kl_device": (I32, [P, P, P, P, I32, P, P, U64, P, P, U64, P]),
+    "ditch_hip_head_kl_grad_workspace": (U64, [P, U64, I32]),
+    "ditch_hip_head_kl_grad_device": (I32, [P, I32, P, P, P, U64, P, P, P, P, P, U64, P]),
+    "ditch_hip_glu_rows_workspace": (U64, [P, P, U64, I32]),
+    "ditch_hip_glu_rows_device": (I32, [P, I32, P, P, U64, P, P, U32, P, U64, P]),
+    "ditch_hip_glu_rows_grad_workspace": (U64, [P, P, U64, I32, I32]),
+    "ditch_hip_glu_rows_grad_device": (I32, [P, I32, P, P, P, P, P, U64, P, P, U32, P, U64, P]),
+    "ditch_hip_model_head": (P, [P]),
+    "ditch_hip_forward_hidden_device": (I32, [P, P, P, U64, U32, U32, P, U64, P, U64]),
     "ditch_hip_generate": (I32, [P, P, P, P, U64, U64, P, U64, P, P, P, P]),
     "ditch_hip_edit_delta": (I32, [P, P, P, P, P, U64, FLT]),
     "ditch_hip_model_edit": (I32, [P, I32, I32, I32, P, U64, FLT]),

@@ -11,6 +11,7 @@
 #include "internal.h"
 #include "model.h"
 #include "pages.h"
+#include "rows.h"
 
 namespace ditch {
 void dequant_to_host(ditch_hip *h, void *out, const ditch_weight *w, uint64_t row0, uint64_t nrows);
@@ -34,7 +35,7 @@ uint64_t model_bytes(const ditch_hip_model *m);
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
                    int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc = nullptr,
-                   int64_t max_rows = 0);
+                   int64_t max_rows = 0, float *d_hidden = nullptr);
 
 // Device buffer owned for the duration of one call.
 struct Tmp {
@@ -713,6 +714,35 @@ int32_t ditch_hip_forward_device(ditch_hip_model *m, const uint32_t *d_tokens, c
     });
 }
 
+int32_t ditch_hip_forward_hidden_device(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows,
+                                        uint64_t n, uint32_t n_prompts, uint32_t max_len,
+                                        const uint64_t *d_hidden_rows, uint64_t n_hidden, float *d_hidden,
+                                        uint64_t hidden_bytes) {
+    if (!m) return DITCH_INVALID_ARGUMENT;
+    return guarded(m->h, [&] {
+        DITCH_CHECK(d_tokens && d_rows, DITCH_INVALID_ARGUMENT, "NULL tokens/rows");
+        if (n == 0) return;
+        DITCH_CHECK(n_prompts > 0 && max_len > 0, DITCH_INVALID_ARGUMENT, "forward_hidden: empty KV cache shape");
+        DITCH_CHECK(n_hidden <= (uint64_t)1 << 32 &&
+                        (n_hidden == 0 || (d_hidden_rows && d_hidden && hidden_bytes >= n_hidden * m->c.hidden * 4)),
+                    DITCH_INVALID_ARGUMENT, "forward_hidden: rows or their buffer missing or too short");
+        model_forward(m, d_tokens, d_rows, (int64_t)n, (int64_t)n_prompts, (int64_t)max_len, nullptr, 0, nullptr,
+                      d_hidden_rows, (int64_t)n_hidden, nullptr, nullptr, 0, d_hidden);
+    });
+}
+
+const ditch_hip_tensor *ditch_hip_model_head(ditch_hip_model *m) {
+    if (!m) return nullptr;
+    const ditch_hip_tensor *t = nullptr;
+    const int32_t rc = guarded(m->h, [&] {
+        const Mat &lm = m->lm_head.ok() ? m->lm_head : m->embed;
+        DITCH_CHECK(lm.ok(), DITCH_INVALID_ARGUMENT, "model head: not registered");
+        DITCH_CHECK(lm.rank == 0, DITCH_UNSUPPORTED, "model head: it carries a low-rank delta");
+        t = lm.t;
+    });
+    return rc == DITCH_OK ? t : nullptr;
+}
+
 ditch_hip_kv_cache *ditch_hip_kv_cache_create(ditch_hip_model *m, uint32_t n_prompts, uint32_t max_len) {
     if (!m) return nullptr;
     ditch_hip_kv_cache *c = nullptr;
@@ -949,6 +979,169 @@ int32_t ditch_hip_beam_select_device(ditch_hip *h, float *d_scores, int32_t *d_p
         OnDevice on(h->device);
         launch_beam_select(d_scores, d_parents, d_tokens, d_logits, d_prev, (int64_t)n_prompts, (int64_t)beams,
                            (int64_t)vocab, (int64_t)k, ws, (size_t)ws_bytes, stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Losses of rows against a head, the gated block over rows, their gradients
+
+static constexpr uint64_t ROWS_MOST = (uint64_t)1 << 24;
+static bool rows_call_ok(const ditch_hip_tensor *w, uint64_t n, int32_t dtype) {
+    return w && n <= ROWS_MOST && (dtype == DITCH_F32 || dtype == DITCH_F16 || dtype == DITCH_BF16) &&
+           w->v.rows < (int64_t)1 << 30 && w->v.cols < (int64_t)1 << 24;
+}
+static bool glu_pair_ok(const ditch_hip_tensor *gate, const ditch_hip_tensor *up) {
+    return gate && up && gate->v.tf == up->v.tf && gate->v.rows == up->v.rows && gate->v.cols == up->v.cols;
+}
+static RowsArg rows_arg(const ditch_kv_rows *r, uint64_t n, uint64_t width, int32_t dtype, const char *what) {
+    const RowsView v = rows_view(r, n, width, dtype, what);
+    return RowsArg{v.data, v.stride};
+}
+static void check_rows_call(const ditch_hip_tensor *w, uint64_t n, int32_t dtype, const char *what) {
+    DITCH_CHECK(rows_call_ok(w, n, dtype), DITCH_INVALID_ARGUMENT,
+                std::string(what) + ": NULL weight, rows of another type than f32, f16 or bf16, or over 2^24 of them");
+}
+static void check_rows_ws(void *ws, uint64_t ws_bytes, uint64_t need, const char *what) {
+    DITCH_CHECK(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, DITCH_INVALID_ARGUMENT,
+                std::string(what) + ": workspace missing, misaligned or shorter than its ..._workspace");
+}
+
+uint64_t ditch_hip_head_loss_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype) {
+    return n && rows_call_ok(w, n, dtype) ? head_loss_workspace(w->v, (int64_t)n, dtype) : 0;
+}
+
+int32_t ditch_hip_head_loss_device(ditch_hip *h, float *d_loss, float *d_lse, int32_t dtype, const ditch_kv_rows *x,
+                                   uint64_t n, const ditch_hip_tensor *w, const int32_t *d_targets, void *ws,
+                                   uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(w, n, dtype, "head loss");
+        if (n == 0) return;
+        DITCH_CHECK(d_loss && d_lse && d_targets, DITCH_INVALID_ARGUMENT, "head loss: NULL argument");
+        const RowsArg xa = rows_arg(x, n, w->v.cols, dtype, "head loss: x");
+        check_rows_ws(ws, ws_bytes, head_loss_workspace(w->v, (int64_t)n, dtype), "head loss");
+        OnDevice on(h->device);
+        launch_head_loss(d_loss, d_lse, dtype, xa, (int64_t)n, w->v, d_targets, ws,
+                         stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+uint64_t ditch_hip_head_loss_grad_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype, int32_t want_dw) {
+    return n && rows_call_ok(w, n, dtype) ? head_loss_grad_workspace(w->v, (int64_t)n, dtype, want_dw != 0) : 0;
+}
+
+int32_t ditch_hip_head_loss_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx, const ditch_kv_rows *dw,
+                                        const ditch_kv_rows *x, uint64_t n, const ditch_hip_tensor *w,
+                                        const int32_t *d_targets, const float *d_lse, const float *d_dloss, void *ws,
+                                        uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(w, n, dtype, "head loss gradient");
+        if (n == 0) return;
+        DITCH_CHECK((dx || dw) && d_targets && d_lse && d_dloss, DITCH_INVALID_ARGUMENT,
+                    "head loss gradient: NULL argument");
+        const RowsArg xa = rows_arg(x, n, w->v.cols, dtype, "head loss gradient: x");
+        const RowsArg dxa = dx ? rows_arg(dx, n, w->v.cols, dtype, "head loss gradient: dx") : RowsArg{};
+        const RowsArg dwa = dw ? rows_arg(dw, w->v.rows, w->v.cols, dtype, "head loss gradient: dw") : RowsArg{};
+        check_rows_ws(ws, ws_bytes, head_loss_grad_workspace(w->v, (int64_t)n, dtype, dw != nullptr),
+                      "head loss gradient");
+        OnDevice on(h->device);
+        launch_head_loss_grad(dtype, dxa, dwa, xa, (int64_t)n, w->v, d_targets, d_lse, d_dloss, ws,
+                              stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+uint64_t ditch_hip_head_kl_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype) {
+    return n && rows_call_ok(w, n, dtype) ? head_kl_workspace(w->v, (int64_t)n, dtype) : 0;
+}
+
+int32_t ditch_hip_head_kl_device(ditch_hip *h, float *d_kl, float *d_lse_base, float *d_lse_trial, int32_t dtype,
+                                 const ditch_kv_rows *base, const ditch_kv_rows *trial, uint64_t n,
+                                 const ditch_hip_tensor *w, void *ws, uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(w, n, dtype, "head kl");
+        if (n == 0) return;
+        DITCH_CHECK(d_kl && d_lse_base && d_lse_trial, DITCH_INVALID_ARGUMENT, "head kl: NULL argument");
+        const RowsArg b = rows_arg(base, n, w->v.cols, dtype, "head kl: base");
+        const RowsArg t = rows_arg(trial, n, w->v.cols, dtype, "head kl: trial");
+        check_rows_ws(ws, ws_bytes, head_kl_workspace(w->v, (int64_t)n, dtype), "head kl");
+        OnDevice on(h->device);
+        launch_head_kl(d_kl, d_lse_base, d_lse_trial, dtype, b, t, (int64_t)n, w->v, ws,
+                       stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+uint64_t ditch_hip_head_kl_grad_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype) {
+    return n && rows_call_ok(w, n, dtype) ? head_kl_grad_workspace(w->v, (int64_t)n, dtype) : 0;
+}
+
+int32_t ditch_hip_head_kl_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx, const ditch_kv_rows *base,
+                                      const ditch_kv_rows *trial, uint64_t n, const ditch_hip_tensor *w,
+                                      const float *d_lse_base, const float *d_lse_trial, const float *d_dkl, void *ws,
+                                      uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(w, n, dtype, "head kl gradient");
+        if (n == 0) return;
+        DITCH_CHECK(d_lse_base && d_lse_trial && d_dkl, DITCH_INVALID_ARGUMENT, "head kl gradient: NULL argument");
+        const RowsArg d = rows_arg(dx, n, w->v.cols, dtype, "head kl gradient: dx");
+        const RowsArg b = rows_arg(base, n, w->v.cols, dtype, "head kl gradient: base");
+        const RowsArg t = rows_arg(trial, n, w->v.cols, dtype, "head kl gradient: trial");
+        check_rows_ws(ws, ws_bytes, head_kl_grad_workspace(w->v, (int64_t)n, dtype), "head kl gradient");
+        OnDevice on(h->device);
+        launch_head_kl_grad(dtype, d, b, t, (int64_t)n, w->v, d_lse_base, d_lse_trial, d_dkl, ws,
+                            stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+uint64_t ditch_hip_glu_rows_workspace(const ditch_hip_tensor *gate, const ditch_hip_tensor *up, uint64_t n,
+                                      int32_t dtype) {
+    if (n == 0 || !glu_pair_ok(gate, up) || !rows_call_ok(gate, n, dtype)) return 0;
+    return glu_rows_workspace(gate->v, up->v, (int64_t)n, dtype);
+}
+
+int32_t ditch_hip_glu_rows_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *out, const ditch_kv_rows *x,
+                                  uint64_t n, const ditch_hip_tensor *gate, const ditch_hip_tensor *up, uint32_t act,
+                                  void *ws, uint64_t ws_bytes, void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(gate, n, dtype, "glu rows");
+        DITCH_CHECK(up && act <= 5, DITCH_INVALID_ARGUMENT, "glu rows: NULL up or unknown activation");
+        DITCH_CHECK(glu_pair_ok(gate, up), DITCH_UNSUPPORTED, "glu rows: gate and up differ in format or shape");
+        if (n == 0) return;
+        const RowsArg o = rows_arg(out, n, gate->v.rows, dtype, "glu rows: out");
+        const RowsArg xa = rows_arg(x, n, gate->v.cols, dtype, "glu rows: x");
+        check_rows_ws(ws, ws_bytes, glu_rows_workspace(gate->v, up->v, (int64_t)n, dtype), "glu rows");
+        OnDevice on(h->device);
+        launch_glu_rows(dtype, o, xa, (int64_t)n, gate->v, up->v, act, ws, stream ? (hipStream_t)stream : h->stream);
+    });
+}
+
+uint64_t ditch_hip_glu_rows_grad_workspace(const ditch_hip_tensor *gate, const ditch_hip_tensor *up, uint64_t n,
+                                           int32_t dtype, int32_t want_dw) {
+    if (n == 0 || !glu_pair_ok(gate, up) || !rows_call_ok(gate, n, dtype)) return 0;
+    return glu_rows_grad_workspace(gate->v, up->v, (int64_t)n, dtype, want_dw != 0);
+}
+
+int32_t ditch_hip_glu_rows_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx,
+                                       const ditch_kv_rows *dgate, const ditch_kv_rows *dup, const ditch_kv_rows *dout,
+                                       const ditch_kv_rows *x, uint64_t n, const ditch_hip_tensor *gate,
+                                       const ditch_hip_tensor *up, uint32_t act, void *ws, uint64_t ws_bytes,
+                                       void *stream) {
+    return guarded(h, [&] {
+        check_rows_call(gate, n, dtype, "glu rows gradient");
+        DITCH_CHECK(up && act <= 5, DITCH_INVALID_ARGUMENT, "glu rows gradient: NULL up or unknown activation");
+        DITCH_CHECK(glu_pair_ok(gate, up), DITCH_UNSUPPORTED,
+                    "glu rows gradient: gate and up differ in format or shape");
+        if (n == 0) return;
+        DITCH_CHECK(dx || dgate || dup, DITCH_INVALID_ARGUMENT, "glu rows gradient: no gradient asked for");
+        const uint64_t rows = gate->v.rows, cols = gate->v.cols;
+        const RowsArg dxa = dx ? rows_arg(dx, n, cols, dtype, "glu rows gradient: dx") : RowsArg{};
+        const RowsArg dg = dgate ? rows_arg(dgate, rows, cols, dtype, "glu rows gradient: dgate") : RowsArg{};
+        const RowsArg du = dup ? rows_arg(dup, rows, cols, dtype, "glu rows gradient: dup") : RowsArg{};
+        const RowsArg d = rows_arg(dout, n, rows, dtype, "glu rows gradient: dout");
+        const RowsArg xa = rows_arg(x, n, cols, dtype, "glu rows gradient: x");
+        check_rows_ws(ws, ws_bytes, glu_rows_grad_workspace(gate->v, up->v, (int64_t)n, dtype, dgate || dup),
+                      "glu rows gradient");
+        OnDevice on(h->device);
+        launch_glu_rows_grad(dtype, dxa, dg, du, d, xa, (int64_t)n, gate->v, up->v, act, ws,
+                             stream ? (hipStream_t)stream : h->stream);
     });
 }
 

@@ -19,7 +19,8 @@ namespace ditch {
 
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
-                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows);
+                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows,
+                   float *d_hidden = nullptr);
 
 constexpr int PICK_MAXK = 256;  // Sampler.max_top_k
 constexpr int PICK_ROWS = 256;  // rows per launch: their draws travel in the arguments

@@ -1,0 +1,227 @@
+// glu.hip — the gated block over rows, y = act(x Wg^T) * (x Wu^T), and its
+// gradient.
+//
+// One product over both matrices, their 16-row blocks interleaved, so that a
+// lane holds a gate and the up value beside it: y is formed in registers and is
+// all that is written. Gradient: the same product again, its epilogue reads dy and
+// leaves dg = dy u act'(g) and du = dy act(g) as bf16 terms; then dx = dg Wg +
+// du Wu is one product over both pairs, and dWg = dg^T x, dWu = du^T x.
+#include "rows_gemm.h"
+
+namespace ditch {
+
+// act(g) and its derivative; the activations of ditch_hip_gatedActivation.
+template <int A>
+__device__ __forceinline__ void act_both(float g, float &y, float &dy) {
+    if constexpr (A == 0 || A == 5) {
+        constexpr float c = A == 0 ? 1.f : 1.702f;
+        const float s = __fdiv_rn(1.f, 1.f + expf(-c * g));
+        y = g * s;
+        dy = s * __builtin_fmaf(c * g, 1.f - s, 1.f);
+    } else if constexpr (A == 1) {
+        const float k = 0.7978845608028654f, g2 = g * g;
+        const float t = tanhf(k * __builtin_fmaf(0.044715f * g2, g, g));
+        y = 0.5f * g * (1.f + t);
+        dy = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * k * __builtin_fmaf(3.f * 0.044715f, g2, 1.f);
+    } else if constexpr (A == 2) {
+        const float c = 0.5f * (1.f + erff(g * 0.7071067811865476f));
+        y = g * c;
+        dy = __builtin_fmaf(g * 0.3989422804014327f, expf(-0.5f * g * g), c);
+    } else {
+        const float r = fmaxf(g, 0.f);
+        y = A == 3 ? r : r * r;
+        dy = A == 3 ? (g > 0.f ? 1.f : 0.f) : 2.f * r;
+        if (g != g) y = dy = g;
+    }
+}
+
+// Blocks 2i of m are gate rows, 2i + 1 the same up rows.
+struct EpiGlu {
+    void *out;
+    int64_t stride, n, rows;
+    int32_t dtype, wide;
+    uint32_t act;
+    template <int A, int MI, int NJ>
+    __device__ __forceinline__ void store(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+            if (tok >= n) continue;
+#pragma unroll
+            for (int i = 0; i < MI; i += 2) {
+                const int64_t c = (int64_t)(mb + i) / 2 * 16 + 4 * (lane >> 4);
+                if (c >= rows) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float y, dy;
+                    act_both<A>(acc[i][j][r], y, dy);
+                    v[r] = y * acc[i + 1][j][r];
+                }
+                put_row4(out, dtype, tok * stride + c, rows - c, wide, v);
+            }
+        }
+    }
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        switch (act) {
+        case 0: store<0>(acc, mb, nb, lane); break;
+        case 1: store<1>(acc, mb, nb, lane); break;
+        case 2: store<2>(acc, mb, nb, lane); break;
+        case 3: store<3>(acc, mb, nb, lane); break;
+        case 4: store<4>(acc, mb, nb, lane); break;
+        default: store<5>(acc, mb, nb, lane); break;
+        }
+    }
+};
+
+template <int T>
+struct EpiGluGrad {
+    Planes dg, du;
+    const void *dout;
+    int64_t stride, n, rows;
+    int32_t dtype;
+    uint32_t act;
+    __device__ __forceinline__ float dout_at(int64_t i) const {
+        if (dtype == DITCH_F32) return ((const float *)dout)[i];
+        const uint16_t b = ((const uint16_t *)dout)[i];
+        return dtype == DITCH_F16 ? f16_to_f32_hw(b) : bf16_to_f32(b);
+    }
+    template <int A, int MI, int NJ>
+    __device__ __forceinline__ void store(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (nb + j >= dg.groups) continue;
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < MI; i += 2) {
+                const int wb = (mb + i) / 2;
+                if ((wb >> 1) >= dg.units) continue;
+                const int64_t c = (int64_t)wb * 16 + 4 * (lane >> 4);
+                float a[4], b[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float y, dy;
+                    act_both<A>(acc[i][j][r], y, dy);
+                    const bool in = tok < n && c + r < rows;
+                    const float d = in ? dout_at(tok * stride + c + r) : 0.f;
+                    a[r] = in ? d * acc[i + 1][j][r] * dy : 0.f;
+                    b[r] = in ? d * y : 0.f;
+                }
+                put_grad_terms<T>(dg, wb, nb + j, lane, a);
+                put_grad_terms<T>(du, wb, nb + j, lane, b);
+            }
+        }
+    }
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        switch (act) {
+        case 0: store<0>(acc, mb, nb, lane); break;
+        case 1: store<1>(acc, mb, nb, lane); break;
+        case 2: store<2>(acc, mb, nb, lane); break;
+        case 3: store<3>(acc, mb, nb, lane); break;
+        case 4: store<4>(acc, mb, nb, lane); break;
+        default: store<5>(acc, mb, nb, lane); break;
+        }
+    }
+};
+
+// x and both matrices as planes, one operand after the other.
+struct GluPlan {
+    Planes x, dg, du;
+    char *room[2] = {nullptr, nullptr};
+    int64_t ld = 0;
+    int parts = 1, order = 1;
+    float *part = nullptr;
+    size_t bytes = 0;
+};
+static GluPlan glu_plan(const TileView &w, int64_t n, int32_t dtype, bool grad, void *ws) {
+    GluPlan p;
+    Carver c(ws);
+    const int terms = row_terms(dtype);
+    p.x = row_planes(n, w.cols, terms);
+    p.x.p = c.take(p.x.bytes());
+    if (!weight_is_planes(w))
+        for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows).bytes());
+    if (grad) {
+        for (Planes *d : {&p.dg, &p.du}) {
+            *d = Planes{nullptr, p.x.groups, ceil_div(w.rows, 64) * 2, terms};
+            d->p = c.take(d->bytes());
+        }
+        p.ld = ceil_div(w.cols, 4) * 4;
+        p.parts = rows_parts(ceil_div(w.cols, 16), p.x.groups, p.dg.units / 2);
+        p.part = c.take<float>((size_t)p.parts * n * p.ld);
+        p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
+    }
+    p.bytes = c.at;
+    return p;
+}
+
+size_t glu_rows_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype) {
+    return glu_plan(gate, n, dtype, false, nullptr).bytes;
+}
+size_t glu_rows_grad_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype, bool dw) {
+    return glu_plan(gate, n, dtype, true, nullptr).bytes;
+}
+
+static RowsGemm glu_gemm(const GluPlan &p, const Planes &wg, const Planes &wu) {
+    RowsGemm g;
+    g.a = rows_inner(wg);
+    g.a.paired = 1;
+    g.a.pair = wu.p - wg.p;
+    g.b = rows_inner(p.x);
+    g.stages = (int32_t)(p.x.units / 2);
+    rows_pairs(g, wg, p.x, wg.terms > p.x.terms ? wg.terms : p.x.terms);
+    return g;
+}
+
+void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const TileView &gate, const TileView &up,
+                     uint32_t act, void *ws, hipStream_t s) {
+    const GluPlan p = glu_plan(gate, n, dtype, false, ws);
+    launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
+    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
+    const EpiGlu epi{out.p, out.stride, n, gate.rows, dtype, rows_wide(out.p, out.stride, dtype), act};
+    launch_rows_gemm<false, false>(glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
+}
+
+template <int T>
+static void fill_glu(const GluPlan &p, const RowsGemm &g, int32_t dtype, RowsArg dout, int64_t n, int64_t rows,
+                     uint32_t act, hipStream_t s) {
+    const EpiGluGrad<T> epi{p.dg, p.du, dout.p, dout.stride, n, rows, dtype, act};
+    launch_rows_gemm<false, false>(g, 4 * p.dg.units, p.x.groups, epi, s);
+}
+
+void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
+                          const TileView &gate, const TileView &up, uint32_t act, void *ws, hipStream_t s) {
+    const GluPlan p = glu_plan(gate, n, dtype, true, ws);
+    launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
+    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
+    auto fill = p.x.terms == 1 ? fill_glu<1> : p.x.terms == 2 ? fill_glu<2> : fill_glu<3>;
+    fill(p, glu_gemm(p, wg, wu), dtype, dout, n, gate.rows, act, s);
+    if (dx.p) {
+        RowsGemm g;
+        g.a = rows_outer(wg);
+        g.b = rows_inner(p.dg);
+        g.stages = (int32_t)(p.dg.units / 2);
+        g.parts = p.parts;
+        rows_pairs(g, wg, p.dg, p.order);
+        rows_pairs(g, wu, p.du, p.order);
+        const EpiParts epi{p.part, n * p.ld, p.ld, n, p.ld, 0};
+        launch_rows_gemm<true, false>(g, ceil_div(gate.cols, 16), p.x.groups, epi, s);
+        launch_join_parts(dx.p, dtype, dx.stride, p.part, p.parts, n * p.ld, p.ld, n, gate.cols, s);
+    }
+    const RowsArg dw[2] = {dgate, dup};
+    const Planes *d[2] = {&p.dg, &p.du};
+    for (int i = 0; i < 2; i++) {
+        if (!dw[i].p) continue;
+        RowsGemm g;
+        g.a = rows_outer(p.x);
+        g.b = rows_outer(*d[i]);
+        g.stages = (int32_t)(p.x.groups / 4);
+        rows_pairs(g, p.x, *d[i], p.x.terms);
+        const EpiRows epi{dw[i].p, dw[i].stride, gate.rows, gate.cols, dtype, rows_wide(dw[i].p, dw[i].stride, dtype)};
+        launch_rows_gemm<true, true>(g, ceil_div(gate.cols, 16), ceil_div(gate.rows, 16), epi, s);
+    }
+}
+
+}  // namespace ditch

@@ -1418,9 +1418,12 @@ static void moe_forward(ditch_hip_model *m, Layer &L, float *x, const float *h, 
 // With `pc`, the keys and values of every layer live in that persistent
 // cache (its B x T), so later calls attend to the positions earlier calls
 // wrote (decode steps after a prefill).
+// With `d_hidden`, the rows d_logit_rows after the last norm go there, and
+// their logits are formed only where d_logits is given.
 void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row *d_rows, int64_t n, int64_t B,
                    int64_t T, const uint64_t *d_capture, int64_t n_capture, float *d_res, const uint64_t *d_logit_rows,
-                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows) {
+                   int64_t n_logit, float *d_logits, ditch_hip_kv_cache *pc, int64_t max_rows,
+                   float *d_hidden) {
     const ditch_model_config &c = m->c;
     hipStream_t s = m->h->stream;
     if (n <= 0) return;
@@ -1721,10 +1724,11 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
         }
         capture(li + 1);
     }
-    if (n_logit > 0 && d_logits) {
-        float *hl = m->logit_h.get<float>(n_logit * hidden);
+    if (n_logit > 0 && (d_logits || d_hidden)) {
+        float *hl = d_hidden ? d_hidden : m->logit_h.get<float>(n_logit * hidden);
         launch_rmsnorm(hl, x, m->final_norm.p, m->final_norm.len, n_logit, hidden, c.rms_eps, 0, s,
                        (const int64_t *)d_logit_rows, n);
+        if (!d_logits) return;
         const Mat &lm = m->lm_head.ok() ? m->lm_head : m->embed;
         mm(m, lm, d_logits, hl, n_logit, nullptr, 0, s);
     }

@@ -1,0 +1,93 @@
+// rows.h — products between rows of activations and registered weights in both
+// directions, for the operators that hand back gradients (head.hip, glu.hip).
+//
+// Every operand is brought to one form, planes of bf16 terms in 1 KiB units of
+// 16 rows x 32 columns, the layout in which bf16 tensors are registered:
+// element (row, k) at 16 * (row % 16 + 16 * (k % 32 / 8)) + 2 * (k % 8) of unit
+// [row / 16][k / 32]. A product contracts over the columns of such an operand
+// ("inner") or over its rows ("outer", read through the transposing LDS load),
+// so the same planes serve x W^T, d W and d^T x. bf16 values are one term, f16
+// values exactly two, f32 values exactly three (each term the next 8 bits), FP8,
+// MXFP4 and INT4 weights one (what they decode to), f16 weights two, Q8_0 and
+// f32 weights three. A product of several terms adds the pairs i + j < order.
+#pragma once
+#include "gemm_common.h"
+#include "internal.h"
+
+namespace ditch {
+
+constexpr int ROWS_MAX_SEG = 6;
+
+// Planes of terms: plane e at p + e * plane_bytes().
+struct Planes {
+    char *p = nullptr;
+    int64_t groups = 0, units = 0;  // of 16 rows, of 32 columns
+    int terms = 0;
+    __host__ __device__ int64_t plane_bytes() const { return groups * units * 1024; }
+    size_t bytes() const { return (size_t)terms * plane_bytes(); }
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+inline int row_terms(int32_t dtype) { return dtype == DITCH_BF16 ? 1 : dtype == DITCH_F16 ? 2 : 3; }
+inline size_t row_size(int32_t dtype) { return dtype == DITCH_F32 ? 4 : 2; }
+int weight_terms(const TileView &w);
+
+// Rows of activations: whole stages of 64 in both directions, zeros behind the
+// last row and column.
+inline Planes row_planes(int64_t n, int64_t cols, int terms) {
+    return Planes{nullptr, ceil_div(n, 64) * 4, ceil_div(cols, 64) * 2, terms};
+}
+void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
+                      hipStream_t s);
+// The weight's rows [row0, row0 + rows) as planes: its own tiles where they are
+// that already (nothing launched), else decoded to `room` (row0 a multiple of 16).
+bool weight_is_planes(const TileView &w);
+Planes weight_planes_shape(const TileView &w, int64_t rows);
+Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, hipStream_t s);
+
+// Scratch as one run of the caller's workspace.
+struct Carver {
+    char *base;
+    size_t at = 0;
+    explicit Carver(void *p) : base((char *)p) {}
+    template <typename T = char>
+    T *take(size_t count) {
+        at = (at + 255) & ~(size_t)255;
+        T *r = (T *)(base + at);
+        at += count * sizeof(T);
+        return base ? r : nullptr;
+    }
+};
+
+// out[i][c] = the sum over parts of part[p][i][c], in f32, rounded to dtype.
+void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
+                       int64_t ld, int64_t n, int64_t cols, hipStream_t s);
+
+// head.hip
+struct RowsArg {
+    void *p = nullptr;
+    int64_t stride = 0;
+};
+size_t head_loss_workspace(const TileView &w, int64_t n, int32_t dtype);
+void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t n, const TileView &w,
+                      const int32_t *targets, void *ws, hipStream_t s);
+size_t head_loss_grad_workspace(const TileView &w, int64_t n, int32_t dtype, bool dw);
+void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int64_t n, const TileView &w,
+                           const int32_t *targets, const float *lse, const float *dloss, void *ws, hipStream_t s);
+size_t head_kl_workspace(const TileView &w, int64_t n, int32_t dtype);
+void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype, RowsArg base, RowsArg trial,
+                    int64_t n, const TileView &w, void *ws, hipStream_t s);
+size_t head_kl_grad_workspace(const TileView &w, int64_t n, int32_t dtype);
+void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial, int64_t n, const TileView &w,
+                         const float *lse_base, const float *lse_trial, const float *dkl, void *ws, hipStream_t s);
+
+// glu.hip
+size_t glu_rows_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype);
+void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const TileView &gate, const TileView &up,
+                     uint32_t act, void *ws, hipStream_t s);
+size_t glu_rows_grad_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype, bool dw);
+void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
+                          const TileView &gate, const TileView &up, uint32_t act, void *ws, hipStream_t s);
+
+}  // namespace ditch

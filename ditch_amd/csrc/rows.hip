@@ -1,0 +1,175 @@
+// rows.hip — operands of the products in rows_gemm.h: activations and weights
+// as planes of bf16 terms, and the joining of partial sums.
+#include "rows.h"
+
+#include "tiled.h"
+
+namespace ditch {
+
+int weight_terms(const TileView &w) {
+    switch (w.tf) {
+    case TF_F16: return 2;
+    case TF_F32: case TF_Q8: return 3;
+    default: return 1;
+    }
+}
+
+// v as terms: each but the last the next 8 bits of the remainder (cut, so that
+// no finite value becomes infinite), the last one rounded to nearest even. With
+// as many terms as the type's mantissa has bytes nothing is rounded. Infinities
+// and NaN are all in the first term.
+template <int T>
+__device__ __forceinline__ void to_terms(float v, uint16_t (&t)[T]) {
+    if ((f2u(v) & 0x7f800000u) == 0x7f800000u) {
+        t[0] = (uint16_t)(f2u(v) >> 16) | ((f2u(v) & 0x7fffffu) ? 0x40 : 0);
+#pragma unroll
+        for (int e = 1; e < T; e++) t[e] = 0;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < T; e++) {
+        const uint32_t b = e + 1 < T ? f2u(v) & 0xffff0000u : rne_bits(v);
+        t[e] = (uint16_t)(b >> 16);
+        v = __fsub_rn(v, u2f(b));
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float row_value(const void *x, int64_t i) {
+    if constexpr (DT == DITCH_F32) return ((const float *)x)[i];
+    else if constexpr (DT == DITCH_F16) return f16_to_f32_hw(((const uint16_t *)x)[i]);
+    else return bf16_to_f32(((const uint16_t *)x)[i]);
+}
+
+// A wave a unit: each lane 8 columns of a row, as whole 16-byte words where the
+// rows are aligned to them.
+template <int DT, int T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(Planes out, const void *x, int64_t n, int64_t cols,
+                                                        int64_t stride, int wide) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= out.groups * out.units) return;
+    const int64_t g = unit / out.units, u = unit % out.units;
+    const int64_t row = g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
+    float v[8];
+    uint16_t t[8][T];
+    if (row < n && k + 8 <= cols && wide) {
+        const int64_t at = row * stride + k;
+        if constexpr (DT == DITCH_F32) {
+            const float4 a = *(const float4 *)((const float *)x + at), b = *(const float4 *)((const float *)x + at + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const u32x4 a = *(const u32x4 *)((const uint16_t *)x + at);
+            if constexpr (DT == DITCH_BF16) {
+                *(u32x4 *)(out.p + unit * 1024 + lane * 16) = a;
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = f16_to_f32_hw((uint16_t)(a[j / 2] >> (16 * (j & 1))));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = row < n && k + j < cols ? row_value<DT>(x, row * stride + k + j) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) to_terms<T>(v[j], t[j]);
+#pragma unroll
+    for (int e = 0; e < T; e++) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = (uint32_t)t[2 * j][e] | (uint32_t)t[2 * j + 1][e] << 16;
+        *(u32x4 *)(out.p + e * out.plane_bytes() + unit * 1024 + lane * 16) = w;
+    }
+}
+
+void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
+                      hipStream_t s) {
+    const int64_t units = out.groups * out.units;
+    if (units == 0) return;
+    const int wide = ((uintptr_t)x | (uintptr_t)(stride * (int64_t)row_size(dtype))) % 16 == 0;
+    const dim3 grid((unsigned)ceil_div(units, 4));
+    if (dtype == DITCH_F32)
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F32, 3>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+    else if (dtype == DITCH_F16)
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F16, 2>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+    else
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_BF16, 1>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
+bool weight_is_planes(const TileView &w) { return w.tf == TF_BF16; }
+
+Planes weight_planes_shape(const TileView &w, int64_t rows) {
+    if (weight_is_planes(w)) return Planes{nullptr, ceil_div(rows, 16), w.units_k, 1};
+    return Planes{nullptr, ceil_div(rows, 16), ceil_div(w.cols, 32), weight_terms(w)};
+}
+
+// A wave a unit, each lane 8 columns of a row.
+template <int T>
+__global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView w, int64_t row0) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= out.groups * out.units) return;
+    const int64_t g = unit / out.units, u = unit % out.units;
+    const int64_t row = row0 + g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
+    uint16_t t[8][T];
+    for (int j = 0; j < 8; j++) {
+        uint16_t bits = 0;
+        const float v = row < w.rows && k + j < w.cols ? tiled_element_f32(w, row, k + j, &bits) : 0.f;
+        to_terms<T>(v, t[j]);
+    }
+#pragma unroll
+    for (int e = 0; e < T; e++) {
+        u32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = (uint32_t)t[2 * j][e] | (uint32_t)t[2 * j + 1][e] << 16;
+        *(u32x4 *)(out.p + e * out.plane_bytes() + unit * 1024 + lane * 16) = o;
+    }
+}
+
+Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, hipStream_t s) {
+    Planes out = weight_planes_shape(w, rows);
+    if (weight_is_planes(w)) {
+        out.p = (char *)w.codes + row0 / 16 * w.units_k * 1024;
+        return out;
+    }
+    out.p = room;
+    const dim3 grid((unsigned)ceil_div(out.groups * out.units, 4));
+    if (out.terms == 1) hipLaunchKernelGGL(decode_planes_kernel<1>, grid, dim3(256), 0, s, out, w, row0);
+    else if (out.terms == 2) hipLaunchKernelGGL(decode_planes_kernel<2>, grid, dim3(256), 0, s, out, w, row0);
+    else hipLaunchKernelGGL(decode_planes_kernel<3>, grid, dim3(256), 0, s, out, w, row0);
+    DITCH_TRY_HIP(hipGetLastError());
+    return out;
+}
+
+__device__ __forceinline__ void put_row_value(void *out, int32_t dtype, int64_t i, float v) {
+    if (dtype == DITCH_F32) ((float *)out)[i] = v;
+    else if (dtype == DITCH_F16) ((_Float16 *)out)[i] = (_Float16)v;
+    else ((__bf16 *)out)[i] = (__bf16)v;
+}
+
+__global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtype, int64_t stride, const float *part,
+                                                         int parts, int64_t part_stride, int64_t ld, int64_t n,
+                                                         int64_t cols) {
+    const int64_t per = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n * per) return;
+    const int64_t row = i / per, c = i % per * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < parts; p++) {
+        const float4 v = *(const float4 *)(part + p * part_stride + row * ld + c);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    for (int j = 0; j < 4; j++)
+        if (c + j < cols) put_row_value(out, dtype, row * stride + c + j, v[j]);
+}
+
+void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
+                       int64_t ld, int64_t n, int64_t cols, hipStream_t s) {
+    const int64_t total = n * ceil_div(cols, 4);
+    hipLaunchKernelGGL(join_parts_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, s, out, dtype, stride,
+                       part, parts, part_stride, ld, n, cols);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
+}  // namespace ditch

@@ -1,0 +1,355 @@
+// rows_gemm.h — the product over planes of bf16 terms (rows.h) and what is done
+// with its tiles. Included by the operators that instantiate it.
+//
+// c[m][n] = sum over the pairs of terms and k of a[m][k] b[n][k]. Each operand
+// is inner (its columns are k) or outer (its rows are k). A workgroup computes
+// BM x BN; a stage is 64 k of one pair: whole units are copied global -> LDS, two
+// stage buffers, the next stage on its way while this one is multiplied. Fragments
+// of inner operands are one 16-byte LDS read a lane, those of outer ones two
+// transposing reads (ds_read_b64_tr_b16: lane t of 16 gets column t of four
+// 16-column rows whose quarters the 16 lanes address).
+// v_mfma_f32_16x16x32_bf16 leaves lane l with c[4 (l / 16) + r][l % 16], r =
+// 0..3: four neighbours along m, one n. Every use has what must be contiguous
+// in memory along m.
+//
+// Stages past an operand's end read its last unit again: the other operand's
+// planes hold zeros there. Tiles past an operand's end repeat its last rows and
+// are not stored.
+#pragma once
+#include "rows.h"
+
+namespace ditch {
+
+typedef __attribute__((address_space(3))) void rows_lds_void;
+typedef short rows_short4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) rows_short4 rows_lds_short4;
+
+struct RowsOperand {
+    int64_t ldu = 0;      // units of a 16-row group
+    int64_t pair = 0;     // interleaved: bytes from the first planes to the second's
+    int32_t blocks = 0;   // along the output: 16-row groups (inner), 32-column units (outer); of one of a pair
+    int32_t ks = 0;       // along k: units (inner), groups (outer)
+    int32_t paired = 0;   // blocks 2i and 2i + 1 are block i of the first and of the second planes
+};
+
+struct RowsGemm {
+    RowsOperand a, b;
+    const char *sa[2 * ROWS_MAX_SEG], *sb[2 * ROWS_MAX_SEG];  // the planes of each pair of terms
+    int32_t nseg = 0;
+    int32_t stages = 0;   // of 64 k, of one pair
+    int32_t parts = 1;    // the stages are split over blockIdx.y
+    int32_t tiles_m = 0, tiles_n = 0;
+};
+
+// The pairs of terms i + j < order of two operands' planes.
+inline void rows_pairs(RowsGemm &g, const Planes &a, const Planes &b, int order) {
+    for (int t = 0; t < order; t++)
+        for (int i = 0; i <= t; i++) {
+            const int j = t - i;
+            if (i >= a.terms || j >= b.terms) continue;
+            g.sa[g.nseg] = a.p + i * a.plane_bytes();
+            g.sb[g.nseg++] = b.p + j * b.plane_bytes();
+        }
+}
+inline RowsOperand rows_inner(const Planes &p) {
+    RowsOperand o;
+    o.ldu = p.units;
+    o.blocks = (int32_t)p.groups;
+    o.ks = (int32_t)p.units;
+    return o;
+}
+inline RowsOperand rows_outer(const Planes &p) {
+    RowsOperand o;
+    o.ldu = p.units;
+    o.blocks = (int32_t)p.units;
+    o.ks = (int32_t)p.groups;
+    return o;
+}
+
+// Workgroups an XCD runs at one time (every eighth block) cover a patch of
+// 8 tiles of m and a few of n, so that they share operands in its L2.
+__device__ __forceinline__ void rows_map_tile(int g, int total, int tm, int tn, int &mt, int &nt) {
+    const int xcd = g & 7, j = g >> 3, per = total >> 3, rem = total & 7;
+    const int t = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + j;
+    constexpr int GM = 8;
+    const int width = GM * tn, grp = t / width, first = grp * GM;
+    const int gs = tm - first < GM ? tm - first : GM, r = t - grp * width;
+    mt = first + r % gs;
+    nt = r / gs;
+}
+
+template <bool OUTER>
+__device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int kk, int lane) {
+    if constexpr (!OUTER) {
+        return S[(block * 2 + kk) * 64 + lane];
+    } else {
+        // k 8 g .. +8 of the step for lane group g: unit g / 2, rows 8 (g % 2) .. +8, four a read
+        const int t = lane & 15, g = lane >> 4;
+        const char *p = (const char *)S + (g >> 1) * 1024 + (8 * (g & 1) + (t >> 2) + 16 * ((t & 3) >> 1)) * 16 +
+                        (t & 1) * 8;
+        p += ((block >> 1) * 4 + 2 * kk) * 1024 + (block & 1) * 512;
+        const rows_short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)p);
+        const rows_short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)(p + 64));
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+        return u32x4{l[0], l[1], h[0], h[1]};
+    }
+}
+
+// WGM x WGN waves of MI x NJ blocks of 16 x 16.
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, typename Epi>
+__global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, Epi epi) {
+    constexpr int WAVES = WGM * WGN, BM = WGM * MI, BN = WGN * NJ;  // tile in 16-row blocks
+    static_assert(BM % 2 == 0 && BN % 2 == 0, "whole 32-column units");
+    constexpr int UA = BM * 2, UB = BN * 2, PER = (UA + UB) / WAVES;
+    static_assert((UA + UB) % WAVES == 0, "copies split evenly");
+    // distinct objects: the compiler sees that the copies into one do not touch what is read from the other
+    __shared__ u32x4 S0[(UA + UB) * 64], S1[(UA + UB) * 64];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    int mt, nt;
+    rows_map_tile(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, mt, nt);
+
+    // this wave's copies: where in the planes each begins (the k part is added a stage)
+    const char *unused = nullptr;
+    (void)unused;
+    int64_t off[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int q = wave * PER + j;
+        const bool is_a = q < UA;
+        const RowsOperand &o = is_a ? p.a : p.b;
+        const int l = is_a ? q : q - UA, first = is_a ? mt * BM : nt * BN;
+        if (is_a ? AO : BO) {
+            int u = first / 2 + (l >> 2);
+            u = u < o.blocks ? u : o.blocks - 1;
+            off[j] = (int64_t)u * 1024;
+        } else {
+            int g = first + (l >> 1), second = 0;
+            if (o.paired) {
+                second = g & 1;
+                g >>= 1;
+            }
+            g = g < o.blocks ? g : o.blocks - 1;
+            off[j] = (int64_t)g * o.ldu * 1024 + (second ? o.pair : 0);
+        }
+    }
+    // a linear stage is (stage of 64 k, pair of terms): the pairs of a stage
+    // follow each other, so that what they share is read from near
+    const int total = p.stages * p.nseg;
+    const int first_t = (int)((int64_t)p.stages * blockIdx.y / p.parts) * p.nseg;
+    const int last_t = (int)((int64_t)p.stages * (blockIdx.y + 1) / p.parts) * p.nseg;
+    (void)total;
+    int cs = first_t / p.nseg, seg = 0;  // of the next copy
+    auto copy = [&](u32x4 *S) {
+        const char *ba = p.sa[seg], *bb = p.sb[seg];
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int q = wave * PER + j;
+            const bool is_a = q < UA;
+            const RowsOperand &o = is_a ? p.a : p.b;
+            const int l = is_a ? q : q - UA;
+            const bool outer = is_a ? AO : BO;
+            int k = outer ? 4 * cs + (l & 3) : 2 * cs + (l & 1);
+            k = k < o.ks ? k : o.ks - 1;
+            const char *src = (is_a ? ba : bb) + off[j] + (outer ? k * o.ldu : (int64_t)k) * 1024;
+            __builtin_amdgcn_global_load_lds((const void *)(src + lane * 16), (rows_lds_void *)&S[q * 64], 16, 0, 0);
+        }
+        if (++seg == p.nseg) {
+            seg = 0;
+            cs++;
+        }
+    };
+    floatx4 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    auto step = [&](const u32x4 *S, u32x4 *N, bool more) {
+        if (more) copy(N);
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 *A = S, *B = S + UA * 64;
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            u32x4 a[MI], b[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; j++) b[j] = rows_fragment<BO>(B, wn * NJ + j, kk, lane);
+#pragma unroll
+            for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO>(A, wm * MI + i, kk, lane);
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies have landed
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (first_t < last_t) {
+        copy(S0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        int t = first_t;
+        for (; t + 1 < last_t; t += 2) {
+            step(S0, S1, true);
+            step(S1, S0, t + 2 < last_t);
+        }
+        if (t < last_t) step(S0, S1, false);
+    }
+    epi(acc, mt * BM + wm * MI, nt * BN + wn * NJ, lane);
+}
+
+// ---------------------------------------------------------------------------
+// what is done with the tiles: (mb, nb) = the wave's first blocks
+
+// v as terms of a plane (rows.hip: to_terms; rounded to nearest where one is not enough)
+template <int T>
+__device__ __forceinline__ void grad_terms(float v, uint16_t (&t)[T]) {
+#pragma unroll
+    for (int e = 0; e < T; e++) {
+        const bool cut = e + 1 < T && (f2u(v) & 0x7f800000u) != 0x7f800000u;
+        const uint32_t b = cut ? f2u(v) & 0xffff0000u : is_nan(v) ? 0x7fc00000u : rne_bits(v);
+        t[e] = (uint16_t)(b >> 16);
+        v = cut ? __fsub_rn(v, u2f(b)) : 0.f;
+    }
+}
+
+// Four values along m of block mb (rows of a weight) at token `tok`, to planes
+// [token][weight row]: 8 bytes a lane and term.
+template <int T>
+__device__ __forceinline__ void put_grad_terms(const Planes &d, int64_t mb, int64_t nb, int lane, const float (&v)[4]) {
+    uint16_t t[4][T];
+#pragma unroll
+    for (int r = 0; r < 4; r++) grad_terms<T>(v[r], t[r]);
+    const int q = lane >> 4;
+    char *at = d.p + (nb * d.units + (mb >> 1)) * 1024 + ((lane & 15) + 16 * (2 * (mb & 1) + (q >> 1))) * 16 + (q & 1) * 8;
+#pragma unroll
+    for (int e = 0; e < T; e++) {
+        uint2 w;
+        w.x = (uint32_t)t[0][e] | (uint32_t)t[1][e] << 16;
+        w.y = (uint32_t)t[2][e] | (uint32_t)t[3][e] << 16;
+        *(uint2 *)(at + e * d.plane_bytes()) = w;
+    }
+}
+
+// Partial sums: part[blockIdx.y][n][m], added to where `add`.
+struct EpiParts {
+    float *part;
+    int64_t part_stride, ld;
+    int64_t n, m;
+    int add;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        float *base = part + blockIdx.y * part_stride;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int64_t row = (int64_t)(nb + j) * 16 + (lane & 15);
+            if (row >= n) continue;
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                const int64_t c = (int64_t)(mb + i) * 16 + 4 * (lane >> 4);
+                if (c >= m) continue;
+                float4 *o = (float4 *)(base + row * ld + c);
+                float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+                if (add) {
+                    const float4 w = *o;
+                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                }
+                *o = v;
+            }
+        }
+    }
+};
+
+// Four neighbours of a row as the caller's type.
+__device__ __forceinline__ void put_row4(void *out, int32_t dtype, int64_t at, int64_t left, bool wide,
+                                         const float (&v)[4]) {
+    if (dtype == DITCH_F32) {
+        float *o = (float *)out + at;
+        if (wide && left >= 4) *(float4 *)o = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            for (int r = 0; r < 4; r++)
+                if (r < left) o[r] = v[r];
+        return;
+    }
+    uint16_t h[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        h[r] = dtype == DITCH_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[r]) : __builtin_bit_cast(uint16_t, (__bf16)v[r]);
+    uint16_t *o = (uint16_t *)out + at;
+    if (wide && left >= 4) {
+        uint2 w;
+        w.x = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+        w.y = (uint32_t)h[2] | (uint32_t)h[3] << 16;
+        *(uint2 *)o = w;
+    } else
+        for (int r = 0; r < 4; r++)
+            if (r < left) o[r] = h[r];
+}
+// four values fit one store at every row
+inline bool rows_wide(const void *p, int64_t stride, int32_t dtype) {
+    const int64_t size = 4 * (int64_t)row_size(dtype);
+    return ((uintptr_t)p | (uintptr_t)(stride * (int64_t)row_size(dtype))) % size == 0;
+}
+
+// out[n][m] as the caller's rows.
+struct EpiRows {
+    void *out;
+    int64_t stride;
+    int64_t n, m;
+    int32_t dtype, wide;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int64_t row = (int64_t)(nb + j) * 16 + (lane & 15);
+            if (row >= n) continue;
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                const int64_t c = (int64_t)(mb + i) * 16 + 4 * (lane >> 4);
+                if (c >= m) continue;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                put_row4(out, dtype, row * stride + c, m - c, wide, v);
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// launches
+
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, typename Epi>
+void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
+    const int64_t tm = ceil_div(mblocks, WGM * MI), tn = ceil_div(nblocks, WGN * NJ);
+    DITCH_CHECK(tm * tn < (int64_t)1 << 31 && g.parts < 65536, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
+    g.tiles_m = (int32_t)tm;
+    g.tiles_n = (int32_t)tn;
+    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
+                       dim3(WGM * WGN * 64), 0, s, g, epi);
+    DITCH_TRY_HIP(hipGetLastError());
+}
+
+// Tiles of 256 x 256, or of 256 x 64 where n holds few blocks.
+inline bool rows_tall(int64_t nblocks) { return nblocks <= 8; }
+template <bool AO, bool BO, typename Epi>
+void launch_rows_gemm(const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
+    if (rows_tall(nblocks)) launch_rows_gemm_tile<4, 2, 4, 2, AO, BO>(g, mblocks, nblocks, epi, s);
+    else launch_rows_gemm_tile<2, 4, 8, 4, AO, BO>(g, mblocks, nblocks, epi, s);
+}
+
+// Parts of a product's stages so that its tiles fill the chip's 256 CUs, each
+// of at least 8 stages.
+inline int rows_parts(int64_t mblocks, int64_t nblocks, int64_t stages) {
+    const int64_t tiles = ceil_div(mblocks, 16) * ceil_div(nblocks, rows_tall(nblocks) ? 4 : 16);
+    int64_t parts = tiles >= 256 ? 1 : ceil_div(512, tiles);
+    parts = parts < stages / 8 ? parts : stages / 8;
+    return (int)(parts < 1 ? 1 : parts);
+}
+
+}  // namespace ditch

@@ -338,8 +338,73 @@ class Tensor:
         self.dev.check(self.dev.lib.ditch_hip_glu_device(self.dev.h, d_out_frags, out_bytes, d_frags, frag_bytes, n,
                                                          self.handle, up.handle, act, stream))
 
+    # losses against this tensor as a head, the gated block over rows, their gradients; rows are Device.kv_rows
+    # descriptors of dtype "f32", "f16" or "bf16", the rest device pointers
+
+    def head_loss_workspace(self, n, dtype):
+        return self.dev.lib.ditch_hip_head_loss_workspace(self.handle, n, abi.ROW_DTYPE[dtype])
+
+    def head_loss(self, dtype, d_loss, d_lse, x, n, d_targets, ws, ws_bytes, stream=None):
+        """Cross entropy and log sums of n rows (ditch_hip_head_loss_device)."""
+        self.dev.check(self.dev.lib.ditch_hip_head_loss_device(self.dev.h, d_loss, d_lse, abi.ROW_DTYPE[dtype], _ref(x),
+                                                               n, self.handle, d_targets, ws, ws_bytes, stream))
+
+    def head_loss_grad_workspace(self, n, dtype, dw=True):
+        return self.dev.lib.ditch_hip_head_loss_grad_workspace(self.handle, n, abi.ROW_DTYPE[dtype], int(dw))
+
+    def head_loss_grad(self, dtype, dx, dw, x, n, d_targets, d_lse, d_dloss, ws, ws_bytes, stream=None):
+        """Its gradient (ditch_hip_head_loss_grad_device); dx or dw may be None."""
+        self.dev.check(self.dev.lib.ditch_hip_head_loss_grad_device(
+            self.dev.h, abi.ROW_DTYPE[dtype], _ref(dx), _ref(dw), _ref(x), n, self.handle, d_targets, d_lse, d_dloss, ws,
+            ws_bytes, stream))
+
+    def head_kl_workspace(self, n, dtype):
+        return self.dev.lib.ditch_hip_head_kl_workspace(self.handle, n, abi.ROW_DTYPE[dtype])
+
+    def head_kl(self, dtype, d_kl, d_lse_base, d_lse_trial, base, trial, n, ws, ws_bytes, stream=None):
+        """KL(base || trial) of two sets of rows over this head (ditch_hip_head_kl_device)."""
+        self.dev.check(self.dev.lib.ditch_hip_head_kl_device(self.dev.h, d_kl, d_lse_base, d_lse_trial,
+                                                             abi.ROW_DTYPE[dtype], _ref(base), _ref(trial), n,
+                                                             self.handle, ws, ws_bytes, stream))
+
+    def head_kl_grad_workspace(self, n, dtype):
+        return self.dev.lib.ditch_hip_head_kl_grad_workspace(self.handle, n, abi.ROW_DTYPE[dtype])
+
+    def head_kl_grad(self, dtype, dx, base, trial, n, d_lse_base, d_lse_trial, d_dkl, ws, ws_bytes, stream=None):
+        """Its gradient with respect to the trial rows (ditch_hip_head_kl_grad_device)."""
+        self.dev.check(self.dev.lib.ditch_hip_head_kl_grad_device(
+            self.dev.h, abi.ROW_DTYPE[dtype], _ref(dx), _ref(base), _ref(trial), n, self.handle, d_lse_base,
+            d_lse_trial, d_dkl, ws, ws_bytes, stream))
+
+    def glu_rows_workspace(self, up, n, dtype):
+        return self.dev.lib.ditch_hip_glu_rows_workspace(self.handle, up.handle, n, abi.ROW_DTYPE[dtype])
+
+    def glu_rows(self, up, dtype, out, x, n, ws, ws_bytes, act=0, stream=None):
+        """act(x self^T) * (x up^T) as rows (ditch_hip_glu_rows_device)."""
+        self.dev.check(self.dev.lib.ditch_hip_glu_rows_device(self.dev.h, abi.ROW_DTYPE[dtype], _ref(out), _ref(x), n,
+                                                              self.handle, up.handle, act, ws, ws_bytes, stream))
+
+    def glu_rows_grad_workspace(self, up, n, dtype, dw=True):
+        return self.dev.lib.ditch_hip_glu_rows_grad_workspace(self.handle, up.handle, n, abi.ROW_DTYPE[dtype], int(dw))
+
+    def glu_rows_grad(self, up, dtype, dx, dgate, dup, dout, x, n, ws, ws_bytes, act=0, stream=None):
+        """Its gradient (ditch_hip_glu_rows_grad_device); dx, dgate or dup may be None."""
+        self.dev.check(self.dev.lib.ditch_hip_glu_rows_grad_device(
+            self.dev.h, abi.ROW_DTYPE[dtype], _ref(dx), _ref(dgate), _ref(dup), _ref(dout), _ref(x), n, self.handle,
+            up.handle, act, ws, ws_bytes, stream))
+
     def dequant_device(self, d_out, out_bytes, row0, nrows):
         self.dev.check(self.dev.lib.ditch_hip_tensor_dequant(self.dev.h, d_out, out_bytes, self.handle, row0, nrows))
+
+
+class _ModelTensor(Tensor):
+    """A tensor that a model owns."""
+
+    def __init__(self, dev, handle, rows, cols):
+        self.dev, self.handle, self.rows, self.cols, self.dtype = dev, handle, rows, cols, None
+
+    def free(self):
+        self.handle = None
 
 
 class _LoadedSpec:
@@ -474,6 +539,20 @@ class Model:
         self.dev.check(self.dev.lib.ditch_hip_forward_device(self.h, d_tokens, d_rows, n, n_prompts, max_len,
                                                              d_capture, n_capture, d_res, rb, d_logit_rows, n_logit,
                                                              d_logits, lb))
+
+    def head(self):
+        """The model's head as a tensor (ditch_hip_model_head), as long as the model lives."""
+        t = self.dev.lib.ditch_hip_model_head(self.h)
+        if not t:
+            raise DeviceError(abi.UNSUPPORTED, self.dev.lib.ditch_hip_last_error(self.dev.h).decode())
+        return _ModelTensor(self.dev, t, self.spec.config["vocab"], self.spec.config["hidden"])
+
+    def forward_hidden_device(self, d_tokens, d_rows, n, n_prompts, max_len, d_hidden_rows, n_hidden, d_hidden,
+                              hidden_bytes=None):
+        """The rows' hidden states after the last norm (ditch_hip_forward_hidden_device)."""
+        hb = n_hidden * self.spec.config["hidden"] * 4 if hidden_bytes is None else hidden_bytes
+        self.dev.check(self.dev.lib.ditch_hip_forward_hidden_device(self.h, d_tokens, d_rows, n, n_prompts, max_len,
+                                                                    d_hidden_rows, n_hidden, d_hidden, hb))
 
     def kv_cache(self, n_prompts, max_len):
         """A persistent KV cache (ditch_hip_kv_cache_create); free it with

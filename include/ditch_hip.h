@@ -878,6 +878,94 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
                                 uint64_t vocab, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Losses of rows against a head and the gated block over rows, with their
+ * gradients, on device memory, enqueued on `stream` (NULL = the context
+ * stream) and not waited for. No reference counterpart: the reference scores
+ * kept logits.
+ *
+ * Rows are ditch_kv_rows of `dtype` (DITCH_F32, DITCH_F16 or DITCH_BF16), one
+ * dtype a call. The weights are registered tensors of any format, taken at the
+ * values they decode to. 16-bit rows are rounded once where they leave a call,
+ * and once to as many bits between the two products of a gradient; f32 ones
+ * are exact to about f32 rounding. `ws` is device scratch of the call's
+ * ..._workspace bytes (16-byte aligned; its contents do not matter, nothing is
+ * kept in it, calls that overlap need one each); the sizes are 0 for arguments
+ * that the call refuses. Outputs may not overlap inputs or each other. n = 0
+ * does nothing; most rows 2^24. Nothing is allocated: the calls can be
+ * captured.
+ *
+ * Cross entropy against the head w [vocab][hidden]: lse[i] = log sum_v
+ * e^(x_i . w_v), loss[i] = lse[i] - x_i . w_target. A negative target has no
+ * loss (0, and no gradient), one past the vocabulary gives NaN. The logits are
+ * never stored.                                                             */
+uint64_t ditch_hip_head_loss_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype);
+int32_t ditch_hip_head_loss_device(ditch_hip *h, float *d_loss, float *d_lse, int32_t dtype,
+                                   const ditch_kv_rows *x, uint64_t n,
+                                   const ditch_hip_tensor *w, const int32_t *d_targets,
+                                   void *ws, uint64_t ws_bytes, void *stream);
+/* Its gradient for d_dloss [n], with the lse that the call above gave: dx
+ * [n][hidden] and dw [vocab][hidden] (with respect to the decoded weights), of
+ * `dtype`; either may be NULL. `want_dw`: whether dw will be given.          */
+uint64_t ditch_hip_head_loss_grad_workspace(const ditch_hip_tensor *w, uint64_t n,
+                                            int32_t dtype, int32_t want_dw);
+int32_t ditch_hip_head_loss_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx,
+                                        const ditch_kv_rows *dw, const ditch_kv_rows *x,
+                                        uint64_t n, const ditch_hip_tensor *w,
+                                        const int32_t *d_targets, const float *d_lse,
+                                        const float *d_dloss, void *ws, uint64_t ws_bytes,
+                                        void *stream);
+/* KL(base || trial) of the distributions that two sets of rows have over the
+ * head (what ditch_hip_klRows_device gives from kept log-probabilities), and
+ * both log sums. Small divergences keep their relative accuracy.            */
+uint64_t ditch_hip_head_kl_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype);
+int32_t ditch_hip_head_kl_device(ditch_hip *h, float *d_kl, float *d_lse_base,
+                                 float *d_lse_trial, int32_t dtype, const ditch_kv_rows *base,
+                                 const ditch_kv_rows *trial, uint64_t n,
+                                 const ditch_hip_tensor *w, void *ws, uint64_t ws_bytes,
+                                 void *stream);
+/* Its gradient with respect to the trial rows.                              */
+uint64_t ditch_hip_head_kl_grad_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype);
+int32_t ditch_hip_head_kl_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx,
+                                      const ditch_kv_rows *base, const ditch_kv_rows *trial,
+                                      uint64_t n, const ditch_hip_tensor *w,
+                                      const float *d_lse_base, const float *d_lse_trial,
+                                      const float *d_dkl, void *ws, uint64_t ws_bytes,
+                                      void *stream);
+/* out [n][gate.rows] = act(x gate^T) * (x up^T), the block of
+ * ditch_hip_glu_device over plain rows and any number of them. gate and up
+ * have one format and shape (else Unsupported); `act` as in
+ * ditch_hip_gatedActivation.                                                */
+uint64_t ditch_hip_glu_rows_workspace(const ditch_hip_tensor *gate, const ditch_hip_tensor *up,
+                                      uint64_t n, int32_t dtype);
+int32_t ditch_hip_glu_rows_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *out,
+                                  const ditch_kv_rows *x, uint64_t n,
+                                  const ditch_hip_tensor *gate, const ditch_hip_tensor *up,
+                                  uint32_t act, void *ws, uint64_t ws_bytes, void *stream);
+/* Its gradient for dout [n][gate.rows]: dx [n][cols], dgate and dup
+ * [gate.rows][cols] (with respect to the decoded weights); each may be NULL.
+ * `want_dw`: whether dgate or dup will be given.                            */
+uint64_t ditch_hip_glu_rows_grad_workspace(const ditch_hip_tensor *gate,
+                                           const ditch_hip_tensor *up, uint64_t n,
+                                           int32_t dtype, int32_t want_dw);
+int32_t ditch_hip_glu_rows_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx,
+                                       const ditch_kv_rows *dgate, const ditch_kv_rows *dup,
+                                       const ditch_kv_rows *dout, const ditch_kv_rows *x,
+                                       uint64_t n, const ditch_hip_tensor *gate,
+                                       const ditch_hip_tensor *up, uint32_t act, void *ws,
+                                       uint64_t ws_bytes, void *stream);
+/* What joins them to a model: its head's tensor (the embedding where they are
+ * tied; NULL, with a message, where there is none or it carries a low-rank
+ * delta; it lives as long as the model), and ditch_hip_forward_device with the
+ * final hidden rows (after the last norm, d_hidden [n_hidden][hidden] f32)
+ * in place of their logits: what the losses above take.                     */
+const ditch_hip_tensor *ditch_hip_model_head(ditch_hip_model *m);
+int32_t ditch_hip_forward_hidden_device(ditch_hip_model *m, const uint32_t *d_tokens,
+                                        const ditch_row *d_rows, uint64_t n,
+                                        uint32_t n_prompts, uint32_t max_len,
+                                        const uint64_t *d_hidden_rows, uint64_t n_hidden,
+                                        float *d_hidden, uint64_t hidden_bytes);
+
+/* ------------------------------------------------------------------------ */
 /* The step after residual capture, on device memory (enqueued on `stream`,
  * NULL = the context stream, not waited for). These take no buffer
  * lengths: every device buffer must hold the elements its shape below
