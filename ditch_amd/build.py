@@ -44,8 +44,8 @@ EXTRA = {"gemm_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disab
          "gemm_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "gemm_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"],
          "gemm_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-         "head.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"],
-         "glu.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"],
+         **{f: ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"]
+            for f in ("head.hip", "head_grad.hip", "glu.hip", "rows_products.hip")},
          "pages_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "pages_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 

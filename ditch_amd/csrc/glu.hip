@@ -170,7 +170,7 @@ static RowsGemm glu_gemm(const GluPlan &p, const Planes &wg, const Planes &wu) {
     g.a.paired = 1;
     g.a.pair = wu.p - wg.p;
     g.b = rows_inner(p.x);
-    g.stages = (int32_t)(p.x.units / 2);
+    g.k32 = (int32_t)p.x.units;
     rows_pairs(g, wg, p.x, wg.terms > p.x.terms ? wg.terms : p.x.terms);
     return g;
 }
@@ -181,14 +181,16 @@ void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const Til
     launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
     const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
     const EpiGlu epi{out.p, out.stride, n, gate.rows, dtype, rows_wide(out.p, out.stride, dtype), act};
-    launch_rows_gemm<false, false>(glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
+    with_terms(p.x.terms, [&](auto terms) {
+        launch_rows_gemm<false, false, decltype(terms)::value>(glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
+    });
 }
 
 template <int T>
 static void fill_glu(const GluPlan &p, const RowsGemm &g, int32_t dtype, RowsArg dout, int64_t n, int64_t rows,
                      uint32_t act, hipStream_t s) {
     const EpiGluGrad<T> epi{p.dg, p.du, dout.p, dout.stride, n, rows, dtype, act};
-    launch_rows_gemm<false, false>(g, 4 * p.dg.units, p.x.groups, epi, s);
+    launch_rows_gemm<false, false, T>(g, 4 * p.dg.units, p.x.groups, epi, s);
 }
 
 void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
@@ -202,12 +204,11 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         RowsGemm g;
         g.a = rows_outer(wg);
         g.b = rows_inner(p.dg);
-        g.stages = (int32_t)(p.dg.units / 2);
+        g.k32 = (int32_t)p.dg.units;
         g.parts = p.parts;
         rows_pairs(g, wg, p.dg, p.order);
         rows_pairs(g, wu, p.du, p.order);
-        const EpiParts epi{p.part, n * p.ld, p.ld, n, p.ld, 0};
-        launch_rows_gemm<true, false>(g, ceil_div(gate.cols, 16), p.x.groups, epi, s);
+        launch_rows_parts(g, p.part, p.ld, n, gate.cols, false, s);
         launch_join_parts(dx.p, dtype, dx.stride, p.part, p.parts, n * p.ld, p.ld, n, gate.cols, s);
     }
     const RowsArg dw[2] = {dgate, dup};
@@ -217,10 +218,9 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         RowsGemm g;
         g.a = rows_outer(p.x);
         g.b = rows_outer(*d[i]);
-        g.stages = (int32_t)(p.x.groups / 4);
+        g.k32 = (int32_t)(p.x.groups / 2);
         rows_pairs(g, p.x, *d[i], p.x.terms);
-        const EpiRows epi{dw[i].p, dw[i].stride, gate.rows, gate.cols, dtype, rows_wide(dw[i].p, dw[i].stride, dtype)};
-        launch_rows_gemm<true, true>(g, ceil_div(gate.cols, 16), ceil_div(gate.rows, 16), epi, s);
+        launch_rows_out(g, dw[i].p, dtype, dw[i].stride, gate.rows, gate.cols, s);
     }
 }
 

@@ -1,0 +1,187 @@
+// head_grad.hip — the gradients of the head's losses (head.hip has the
+// formulas). The logits are formed again, a piece of the vocabulary at a time;
+// the epilogue leaves d = dloss/dlogits of the piece as bf16 terms, [row][word],
+// and two products over them give the piece's share of dx = d W and its rows of
+// dW = d^T x.
+#include "head.h"
+
+namespace ditch {
+
+// d of a piece as terms. Rows without a target give zeros, targets past the
+// vocabulary NaN.
+template <int T>
+struct EpiLossGrad {
+    Planes d;
+    const int32_t *targets;
+    const float *lse, *dloss;
+    int64_t n, rows, row0, vocab;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (nb + j >= d.groups) continue;
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+            float g = 0.f, l = 0.f;
+            int64_t t = -1;
+            bool live = false;
+            if (tok < n) {
+                const int32_t tt = targets[tok];
+                live = tt >= 0;
+                l = lse[tok];
+                g = tt >= vocab ? __builtin_nanf("") : dloss[tok];
+                t = (int64_t)tt - row0 - v0;
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                if (((mb + i) >> 1) >= d.units) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = fast_exp(acc[i][j][r] - l) - (t == i * 16 + r ? 1.f : 0.f);
+                    v[r] = live && v0 + i * 16 + r < rows ? __fmul_rn(g, p) : 0.f;
+                }
+                put_grad_terms<T>(d, mb + i, nb + j, lane, v);
+            }
+        }
+    }
+};
+
+template <int T>
+struct EpiKlGrad {
+    Planes d;
+    const float *lse_base, *lse_trial, *dkl;
+    int64_t n, rows;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+            const int tb = (nb + j) / 2;
+            if (tb >= d.groups) continue;
+            const int64_t tok = (int64_t)tb * 16 + (lane & 15);
+            float g = 0.f, lb = 0.f, lt = 0.f;
+            if (tok < n) {
+                g = dkl[tok];
+                lb = lse_base[tok];
+                lt = lse_trial[tok];
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                if (((mb + i) >> 1) >= d.units) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float q = fast_exp(acc[i][j + 1][r] - lt) - fast_exp(acc[i][j][r] - lb);
+                    v[r] = tok < n && v0 + i * 16 + r < rows ? __fmul_rn(g, q) : 0.f;
+                }
+                put_grad_terms<T>(d, mb + i, tb, lane, v);
+            }
+        }
+    }
+};
+
+struct HeadGradPlan {
+    Planes x[2], d;
+    int64_t piece = 0, nblocks = 0, ld = 0;
+    int parts = 1;
+    int order = 1;  // of the products with d
+    char *room = nullptr;
+    float *part = nullptr;
+    size_t bytes = 0;
+};
+static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, void *ws) {
+    HeadGradPlan p;
+    Carver c(ws);
+    const int terms = row_terms(dtype);
+    for (int i = 0; i < (kl ? 2 : 1); i++) {
+        p.x[i] = row_planes(n, w.cols, terms);
+        p.x[i].p = c.take(p.x[i].bytes());
+    }
+    p.nblocks = p.x[0].groups;
+    p.piece = piece_rows(w.rows, p.nblocks * 32 * terms + weight_row_bytes(w));
+    if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;
+    p.d = Planes{nullptr, p.nblocks, p.piece / 32, terms};
+    p.d.p = c.take(p.d.bytes());
+    p.ld = ceil_div(w.cols, 4) * 4;
+    p.parts = rows_parts(ceil_div(w.cols, 16), p.nblocks, p.piece / 64);
+    p.part = c.take<float>((size_t)p.parts * n * p.ld);
+    p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
+    if (weight_row_bytes(w)) p.room = c.take(weight_planes_shape(w, p.piece).bytes());
+    p.bytes = c.at;
+    return p;
+}
+
+size_t head_loss_grad_workspace(const TileView &w, int64_t n, int32_t dtype, bool dw) {
+    return head_grad_plan(w, n, dtype, false, nullptr).bytes;
+}
+size_t head_kl_grad_workspace(const TileView &w, int64_t n, int32_t dtype) {
+    return head_grad_plan(w, n, dtype, true, nullptr).bytes;
+}
+
+// `fill` launches the product that leaves a piece's d.
+template <typename Fill>
+static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg dw, int64_t n, const TileView &w,
+                      hipStream_t s, Fill &&fill) {
+    for (int64_t r = 0; r < w.rows; r += p.piece) {
+        const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
+        const Planes wp = weight_planes(w, r, rows, p.room, s);
+        Planes d = p.d;
+        d.units = ceil_div(rows, 64) * 2;
+        fill(wp, d, r, rows);
+        if (dx.p) {
+            RowsGemm g;
+            g.a = rows_outer(wp);
+            g.b = rows_inner(d);
+            g.k32 = (int32_t)d.units;
+            g.parts = p.parts;
+            rows_pairs(g, wp, d, p.order);
+            launch_rows_parts(g, p.part, p.ld, n, w.cols, r > 0, s);
+        }
+        if (dw.p) {
+            RowsGemm g;
+            g.a = rows_outer(p.x[0]);
+            g.b = rows_outer(d);
+            g.k32 = (int32_t)(d.groups / 2);
+            rows_pairs(g, p.x[0], d, d.terms);
+            launch_rows_out(g, (char *)dw.p + r * dw.stride * (int64_t)row_size(dtype), dtype, dw.stride, rows, w.cols, s);
+        }
+    }
+    if (dx.p) launch_join_parts(dx.p, dtype, dx.stride, p.part, p.parts, n * p.ld, p.ld, n, w.cols, s);
+}
+
+template <int T>
+static void fill_loss(const HeadGradPlan &p, const Planes &wp, const Planes &d, int64_t row0, int64_t rows, int64_t n,
+                      int64_t vocab, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
+    const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, vocab};
+    launch_rows_gemm<false, false, T>(logits_gemm(wp, p.x[0], nullptr), d.units * 2, p.nblocks, epi, s);
+}
+template <int T>
+static void fill_kl(const HeadGradPlan &p, const Planes &wp, const Planes &d, int64_t rows, int64_t n,
+                    const float *lse_base, const float *lse_trial, const float *dkl, hipStream_t s) {
+    const EpiKlGrad<T> epi{d, lse_base, lse_trial, dkl, n, rows};
+    launch_rows_gemm<false, false, T>(logits_gemm(wp, p.x[0], &p.x[1]), d.units * 2, 2 * p.nblocks, epi, s);
+}
+
+void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int64_t n, const TileView &w,
+                           const int32_t *targets, const float *lse, const float *dloss, void *ws, hipStream_t s) {
+    const HeadGradPlan p = head_grad_plan(w, n, dtype, false, ws);
+    launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);
+    head_grad(p, dtype, dx, dw, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
+        auto f = p.d.terms == 1 ? fill_loss<1> : p.d.terms == 2 ? fill_loss<2> : fill_loss<3>;
+        f(p, wp, d, row0, rows, n, w.rows, targets, lse, dloss, s);
+    });
+}
+
+void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial, int64_t n, const TileView &w,
+                         const float *lse_base, const float *lse_trial, const float *dkl, void *ws, hipStream_t s) {
+    const HeadGradPlan p = head_grad_plan(w, n, dtype, true, ws);
+    launch_pack_rows(p.x[0], base.p, dtype, n, w.cols, base.stride, s);
+    launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
+    head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t, int64_t rows) {
+        auto f = p.d.terms == 1 ? fill_kl<1> : p.d.terms == 2 ? fill_kl<2> : fill_kl<3>;
+        f(p, wp, d, rows, n, lse_base, lse_trial, dkl, s);
+    });
+}
+
+}  // namespace ditch

@@ -16,7 +16,7 @@
 
 namespace ditch {
 
-constexpr int ROWS_MAX_SEG = 6;
+constexpr int ROWS_MAX_TERMS = 3;
 
 // Planes of terms: plane e at p + e * plane_bytes().
 struct Planes {
@@ -64,7 +64,13 @@ struct Carver {
 void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
                        int64_t ld, int64_t n, int64_t cols, hipStream_t s);
 
-// head.hip
+// rows_products.hip: c as parts of sums [part][n][ld] (added where `add`), a outer
+// and b inner; and as rows of `dtype`, both outer
+struct RowsGemm;
+void launch_rows_parts(const RowsGemm &g, float *part, int64_t ld, int64_t n, int64_t m, bool add, hipStream_t s);
+void launch_rows_out(const RowsGemm &g, void *out, int32_t dtype, int64_t stride, int64_t n, int64_t m, hipStream_t s);
+
+// head.hip, head_grad.hip
 struct RowsArg {
     void *p = nullptr;
     int64_t stride = 0;

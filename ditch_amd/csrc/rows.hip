@@ -2,6 +2,7 @@
 // as planes of bf16 terms, and the joining of partial sums.
 #include "rows.h"
 
+#include "tile_decode.h"
 #include "tiled.h"
 
 namespace ditch {
@@ -104,27 +105,79 @@ Planes weight_planes_shape(const TileView &w, int64_t rows) {
     return Planes{nullptr, ceil_div(rows, 16), ceil_div(w.cols, 32), weight_terms(w)};
 }
 
-// A wave a unit, each lane 8 columns of a row.
-template <int T>
-__global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView w, int64_t row0) {
+// The tiles' own words: a wave a unit of the weight (32 to 128 columns), each
+// lane the 8 columns that it holds of each 32 as one word a term. FP8, MXFP4 and
+// INT4 by the conversions of the tiled products (tensors that these decode
+// exactly), f16, f32 and Q8_0 value by value. (An element at a time through
+// decode_any_kernel took 199 us for 14336 x 4096 in FP8.)
+template <int TF>
+__global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView w, int64_t group0) {
+    constexpr int T = TF == TF_F16 ? 2 : TF == TF_F32 || TF == TF_Q8 ? 3 : 1;
+    constexpr int TILES = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= out.groups * w.units_k) return;
+    const int64_t g = unit / w.units_k, u = unit % w.units_k, src = (group0 + g) * w.units_k + u;
+    u32x4 words[TF == TF_F32 ? 2 : 1];
+    if constexpr (TF == TF_F32) {
+        words[0] = *(const u32x4 *)(w.codes + src * 2048 + lane * 16);
+        words[1] = *(const u32x4 *)(w.codes + src * 2048 + 1024 + lane * 16);
+    } else words[0] = *(const u32x4 *)(w.codes + src * 1024 + lane * 16);
+    uint32_t sd[2] = {0, 0};
+    if constexpr (T == 1) {
+        const SideStep st = side_step<TF>(w);
+        const uint32_t *side = w.side + side_row(w, group0 + g, lane);
+        for (int j = 0; j < TileCfg<TF>::NS; j++) sd[j] = *side_word<TF>(st, side, u, j);
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+        const int64_t ou = u * TILES + t;
+        if (ou >= out.units) return;
+        char *at = out.p + (g * out.units + ou) * 1024 + lane * 16;
+        if constexpr (T == 1) {
+            *(u32x4 *)at = decode_tile_lds<TF>(w, words, sd, t, true);
+        } else {
+            float v[8];
+            if constexpr (TF == TF_F32) {
+                for (int j = 0; j < 8; j++) v[j] = u2f(words[j / 4][j % 4]);
+            } else if constexpr (TF == TF_F16) {
+                for (int j = 0; j < 8; j++) v[j] = f16_to_f32_hw((uint16_t)(words[0][j / 2] >> (16 * (j & 1))));
+            } else {
+                int64_t row = (group0 + g) * 16 + (lane & 15);
+                row = row < w.rows ? row : w.rows - 1;
+                const float d = f16_to_f32(((const uint16_t *)w.scale)[row * w.scale_cols + (ou < w.scale_cols ? ou : 0)]);
+                for (int j = 0; j < 8; j++)
+                    v[j] = __fmul_rn((float)(int8_t)(words[0][2 * t + j / 4] >> (8 * (j % 4))), d);
+            }
+            uint16_t e[8][T];
+#pragma unroll
+            for (int j = 0; j < 8; j++) to_terms<T>(v[j], e[j]);
+#pragma unroll
+            for (int k = 0; k < T; k++) {
+                u32x4 o;
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = (uint32_t)e[2 * j][k] | (uint32_t)e[2 * j + 1][k] << 16;
+                *(u32x4 *)(at + k * out.plane_bytes()) = o;
+            }
+        }
+    }
+}
+
+// Tensors that the conversions do not decode exactly (codes or scales that are
+// not finite, odd blocks): a wave a unit, each lane 8 columns of a row.
+__global__ __launch_bounds__(256) void decode_any_kernel(Planes out, TileView w, int64_t row0) {
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= out.groups * out.units) return;
     const int64_t g = unit / out.units, u = unit % out.units;
     const int64_t row = row0 + g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
-    uint16_t t[8][T];
-    for (int j = 0; j < 8; j++) {
-        uint16_t bits = 0;
-        const float v = row < w.rows && k + j < w.cols ? tiled_element_f32(w, row, k + j, &bits) : 0.f;
-        to_terms<T>(v, t[j]);
-    }
+    uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int j = 0; j < 8; j++)
+        if (row < w.rows && k + j < w.cols) (void)tiled_element_f32(w, row, k + j, &t[j]);
+    u32x4 o;
 #pragma unroll
-    for (int e = 0; e < T; e++) {
-        u32x4 o;
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = (uint32_t)t[2 * j][e] | (uint32_t)t[2 * j + 1][e] << 16;
-        *(u32x4 *)(out.p + e * out.plane_bytes() + unit * 1024 + lane * 16) = o;
-    }
+    for (int j = 0; j < 4; j++) o[j] = (uint32_t)t[2 * j] | (uint32_t)t[2 * j + 1] << 16;
+    *(u32x4 *)(out.p + unit * 1024 + lane * 16) = o;
 }
 
 Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, hipStream_t s) {
@@ -134,10 +187,14 @@ Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, 
         return out;
     }
     out.p = room;
-    const dim3 grid((unsigned)ceil_div(out.groups * out.units, 4));
-    if (out.terms == 1) hipLaunchKernelGGL(decode_planes_kernel<1>, grid, dim3(256), 0, s, out, w, row0);
-    else if (out.terms == 2) hipLaunchKernelGGL(decode_planes_kernel<2>, grid, dim3(256), 0, s, out, w, row0);
-    else hipLaunchKernelGGL(decode_planes_kernel<3>, grid, dim3(256), 0, s, out, w, row0);
+    const dim3 grid((unsigned)ceil_div(out.groups * w.units_k, 4)), each((unsigned)ceil_div(out.groups * out.units, 4));
+    if (w.tf == TF_F16) hipLaunchKernelGGL(decode_planes_kernel<TF_F16>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else if (w.tf == TF_F32) hipLaunchKernelGGL(decode_planes_kernel<TF_F32>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else if (w.tf == TF_Q8) hipLaunchKernelGGL(decode_planes_kernel<TF_Q8>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else if (!w.fast) hipLaunchKernelGGL(decode_any_kernel, each, dim3(256), 0, s, out, w, row0);
+    else if (w.tf == TF_FP8) hipLaunchKernelGGL(decode_planes_kernel<TF_FP8>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else if (w.tf == TF_MX4) hipLaunchKernelGGL(decode_planes_kernel<TF_MX4>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else hipLaunchKernelGGL(decode_planes_kernel<TF_INT4>, grid, dim3(256), 0, s, out, w, row0 / 16);
     DITCH_TRY_HIP(hipGetLastError());
     return out;
 }

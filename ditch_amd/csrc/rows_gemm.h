@@ -3,10 +3,12 @@
 //
 // c[m][n] = sum over the pairs of terms and k of a[m][k] b[n][k]. Each operand
 // is inner (its columns are k) or outer (its rows are k). A workgroup computes
-// BM x BN; a stage is 64 k of one pair: whole units are copied global -> LDS, two
-// stage buffers, the next stage on its way while this one is multiplied. Fragments
-// of inner operands are one 16-byte LDS read a lane, those of outer ones two
-// transposing reads (ds_read_b64_tr_b16: lane t of 16 gets column t of four
+// BM x BN; a stage is one term of a and all TB terms of b over 32 KS k: whole units
+// are copied global -> LDS, two stage buffers, the next stage on its way while this
+// one is multiplied. (A fragment of a then serves every term of b: with a stage a
+// pair, f32 rows read a three times and the LDS was what they waited for.)
+// Fragments of inner operands are one 16-byte LDS read a lane, those of outer ones
+// two transposing reads (ds_read_b64_tr_b16: lane t of 16 gets column t of four
 // 16-column rows whose quarters the 16 lanes address).
 // v_mfma_f32_16x16x32_bf16 leaves lane l with c[4 (l / 16) + r][l % 16], r =
 // 0..3: four neighbours along m, one n. Every use has what must be contiguous
@@ -16,6 +18,8 @@
 // planes hold zeros there. Tiles past an operand's end repeat its last rows and
 // are not stored.
 #pragma once
+#include <type_traits>
+
 #include "rows.h"
 
 namespace ditch {
@@ -34,22 +38,26 @@ struct RowsOperand {
 
 struct RowsGemm {
     RowsOperand a, b;
-    const char *sa[2 * ROWS_MAX_SEG], *sb[2 * ROWS_MAX_SEG];  // the planes of each pair of terms
+    // a term of a and the first count of b's that it meets
+    const char *sa[2 * ROWS_MAX_TERMS], *sb[2 * ROWS_MAX_TERMS];
+    int32_t count[2 * ROWS_MAX_TERMS];
+    int64_t b_plane = 0;  // bytes from one of b's planes to the next
+    int32_t terms = 1;    // of b
     int32_t nseg = 0;
-    int32_t stages = 0;   // of 64 k, of one pair
+    int32_t k32 = 0;      // 32 k each
     int32_t parts = 1;    // the stages are split over blockIdx.y
     int32_t tiles_m = 0, tiles_n = 0;
 };
 
 // The pairs of terms i + j < order of two operands' planes.
 inline void rows_pairs(RowsGemm &g, const Planes &a, const Planes &b, int order) {
-    for (int t = 0; t < order; t++)
-        for (int i = 0; i <= t; i++) {
-            const int j = t - i;
-            if (i >= a.terms || j >= b.terms) continue;
-            g.sa[g.nseg] = a.p + i * a.plane_bytes();
-            g.sb[g.nseg++] = b.p + j * b.plane_bytes();
-        }
+    for (int i = 0; i < a.terms && i < order; i++) {
+        g.sa[g.nseg] = a.p + i * a.plane_bytes();
+        g.sb[g.nseg] = b.p;
+        g.count[g.nseg++] = order - i < b.terms ? order - i : b.terms;
+    }
+    g.b_plane = b.plane_bytes();
+    g.terms = b.terms;
 }
 inline RowsOperand rows_inner(const Planes &p) {
     RowsOperand o;
@@ -78,16 +86,16 @@ __device__ __forceinline__ void rows_map_tile(int g, int total, int tm, int tn, 
     nt = r / gs;
 }
 
-template <bool OUTER>
+template <bool OUTER, int KS>
 __device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int kk, int lane) {
     if constexpr (!OUTER) {
-        return S[(block * 2 + kk) * 64 + lane];
+        return S[(block * KS + kk) * 64 + lane];
     } else {
         // k 8 g .. +8 of the step for lane group g: unit g / 2, rows 8 (g % 2) .. +8, four a read
         const int t = lane & 15, g = lane >> 4;
         const char *p = (const char *)S + (g >> 1) * 1024 + (8 * (g & 1) + (t >> 2) + 16 * ((t & 3) >> 1)) * 16 +
                         (t & 1) * 8;
-        p += ((block >> 1) * 4 + 2 * kk) * 1024 + (block & 1) * 512;
+        p += ((block >> 1) * 2 * KS + 2 * kk) * 1024 + (block & 1) * 512;
         const rows_short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)p);
         const rows_short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)(p + 64));
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -97,14 +105,14 @@ __device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int kk
 }
 
 // WGM x WGN waves of MI x NJ blocks of 16 x 16.
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, typename Epi>
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, int KS, typename Epi>
 __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, Epi epi) {
     constexpr int WAVES = WGM * WGN, BM = WGM * MI, BN = WGN * NJ;  // tile in 16-row blocks
     static_assert(BM % 2 == 0 && BN % 2 == 0, "whole 32-column units");
-    constexpr int UA = BM * 2, UB = BN * 2, PER = (UA + UB) / WAVES;
-    static_assert((UA + UB) % WAVES == 0, "copies split evenly");
+    constexpr int UA = BM * KS, UB = BN * KS, PER = (UA + TB * UB) / WAVES;
+    static_assert((UA + TB * UB) % WAVES == 0, "copies split evenly");
     // distinct objects: the compiler sees that the copies into one do not touch what is read from the other
-    __shared__ u32x4 S0[(UA + UB) * 64], S1[(UA + UB) * 64];
+    __shared__ u32x4 S0[(UA + TB * UB) * 64], S1[(UA + TB * UB) * 64];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -113,21 +121,19 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
     rows_map_tile(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, mt, nt);
 
     // this wave's copies: where in the planes each begins (the k part is added a stage)
-    const char *unused = nullptr;
-    (void)unused;
     int64_t off[PER];
 #pragma unroll
     for (int j = 0; j < PER; j++) {
         const int q = wave * PER + j;
         const bool is_a = q < UA;
         const RowsOperand &o = is_a ? p.a : p.b;
-        const int l = is_a ? q : q - UA, first = is_a ? mt * BM : nt * BN;
+        const int l = is_a ? q : (q - UA) % UB, first = is_a ? mt * BM : nt * BN;
         if (is_a ? AO : BO) {
-            int u = first / 2 + (l >> 2);
+            int u = first / 2 + l / (2 * KS);
             u = u < o.blocks ? u : o.blocks - 1;
             off[j] = (int64_t)u * 1024;
         } else {
-            int g = first + (l >> 1), second = 0;
+            int g = first + l / KS, second = 0;
             if (o.paired) {
                 second = g & 1;
                 g >>= 1;
@@ -135,14 +141,14 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
             g = g < o.blocks ? g : o.blocks - 1;
             off[j] = (int64_t)g * o.ldu * 1024 + (second ? o.pair : 0);
         }
+        if (!is_a) off[j] += (q - UA) / UB * p.b_plane;
     }
-    // a linear stage is (stage of 64 k, pair of terms): the pairs of a stage
-    // follow each other, so that what they share is read from near
-    const int total = p.stages * p.nseg;
-    const int first_t = (int)((int64_t)p.stages * blockIdx.y / p.parts) * p.nseg;
-    const int last_t = (int)((int64_t)p.stages * (blockIdx.y + 1) / p.parts) * p.nseg;
-    (void)total;
-    int cs = first_t / p.nseg, seg = 0;  // of the next copy
+    // a linear stage is (32 KS k, term of a): the terms of a stage follow each
+    // other, so that what they share is read from near
+    const int steps = (p.k32 + KS - 1) / KS;
+    const int first_t = (int)((int64_t)steps * blockIdx.y / p.parts) * p.nseg;
+    const int last_t = (int)((int64_t)steps * (blockIdx.y + 1) / p.parts) * p.nseg;
+    int cs = first_t / p.nseg, seg = 0, cur = 0;  // of the next copy; of the product
     auto copy = [&](u32x4 *S) {
         const char *ba = p.sa[seg], *bb = p.sb[seg];
 #pragma unroll
@@ -152,7 +158,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
             const RowsOperand &o = is_a ? p.a : p.b;
             const int l = is_a ? q : q - UA;
             const bool outer = is_a ? AO : BO;
-            int k = outer ? 4 * cs + (l & 3) : 2 * cs + (l & 1);
+            int k = outer ? 2 * KS * cs + l % (2 * KS) : KS * cs + l % KS;
             k = k < o.ks ? k : o.ks - 1;
             const char *src = (is_a ? ba : bb) + off[j] + (outer ? k * o.ldu : (int64_t)k) * 1024;
             __builtin_amdgcn_global_load_lds((const void *)(src + lane * 16), (rows_lds_void *)&S[q * 64], 16, 0, 0);
@@ -172,18 +178,25 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
         if (more) copy(N);
         __builtin_amdgcn_sched_barrier(0);
         const u32x4 *A = S, *B = S + UA * 64;
+        const int count = TB == 1 ? 1 : p.count[cur];
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            u32x4 a[MI], b[NJ];
+        for (int kk = 0; kk < KS; kk++) {
+            u32x4 a[MI];
 #pragma unroll
-            for (int j = 0; j < NJ; j++) b[j] = rows_fragment<BO>(B, wn * NJ + j, kk, lane);
+            for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO, KS>(A, wm * MI + i, kk, lane);
 #pragma unroll
-            for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO>(A, wm * MI + i, kk, lane);
+            for (int e = 0; e < TB; e++) {
+                if (e > 0 && e >= count) continue;
+                u32x4 b[NJ];
 #pragma unroll
-            for (int i = 0; i < MI; i++)
+                for (int j = 0; j < NJ; j++) b[j] = rows_fragment<BO, KS>(B + e * UB * 64, wn * NJ + j, kk, lane);
 #pragma unroll
-                for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
+                for (int i = 0; i < MI; i++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
+            }
         }
+        if (TB > 1) cur = cur + 1 == p.nseg ? 0 : cur + 1;
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies have landed
         __builtin_amdgcn_s_barrier();
@@ -324,23 +337,31 @@ struct EpiRows {
 // ---------------------------------------------------------------------------
 // launches
 
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, typename Epi>
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, int KS, typename Epi>
 void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     const int64_t tm = ceil_div(mblocks, WGM * MI), tn = ceil_div(nblocks, WGN * NJ);
     DITCH_CHECK(tm * tn < (int64_t)1 << 31 && g.parts < 65536, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
+    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, TB, KS, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
                        dim3(WGM * WGN * 64), 0, s, g, epi);
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Tiles of 256 x 256, or of 256 x 64 where n holds few blocks.
+// Tiles of 256 x 256, or of 256 x 64 where n holds few blocks. Stages of as many
+// k as two buffers of the LDS hold.
 inline bool rows_tall(int64_t nblocks) { return nblocks <= 8; }
-template <bool AO, bool BO, typename Epi>
+template <bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm(const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
-    if (rows_tall(nblocks)) launch_rows_gemm_tile<4, 2, 4, 2, AO, BO>(g, mblocks, nblocks, epi, s);
-    else launch_rows_gemm_tile<2, 4, 8, 4, AO, BO>(g, mblocks, nblocks, epi, s);
+    if (rows_tall(nblocks)) launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s);
+    else launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s);
+}
+
+template <typename F>
+void with_terms(int terms, F &&f) {
+    if (terms == 1) f(std::integral_constant<int, 1>{});
+    else if (terms == 2) f(std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 3>{});
 }
 
 // Parts of a product's stages so that its tiles fill the chip's 256 CUs, each
