@@ -131,7 +131,8 @@ struct GluPlan {
     Planes x, dg, du;
     char *room[2] = {nullptr, nullptr};
     int64_t ld = 0;
-    int parts = 1, order = 1;
+    int order = 1, tile = 0;
+    RowsTiling back;
     float *part = nullptr;
     size_t bytes = 0;
 };
@@ -149,10 +150,13 @@ static GluPlan glu_plan(const TileView &w, int64_t n, int32_t dtype, bool grad, 
             d->p = c.take(d->bytes());
         }
         p.ld = ceil_div(w.cols, 4) * 4;
-        p.parts = rows_parts(ceil_div(w.cols, 16), p.x.groups, p.dg.units / 2);
-        p.part = c.take<float>((size_t)p.parts * n * p.ld);
         p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
+        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units,
+                             2 * rows_pair_count(weight_terms(w), terms, p.order), true);
+        p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
+    const int a = weight_terms(w), order = a > terms ? a : terms;
+    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, p.x.units, rows_pair_count(a, terms, order), false).tile;
     p.bytes = c.at;
     return p;
 }
@@ -182,7 +186,7 @@ void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const Til
     const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
     const EpiGlu epi{out.p, out.stride, n, gate.rows, dtype, rows_wide(out.p, out.stride, dtype), act};
     with_terms(p.x.terms, [&](auto terms) {
-        launch_rows_gemm<false, false, decltype(terms)::value>(glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
+        launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
     });
 }
 
@@ -190,7 +194,7 @@ template <int T>
 static void fill_glu(const GluPlan &p, const RowsGemm &g, int32_t dtype, RowsArg dout, int64_t n, int64_t rows,
                      uint32_t act, hipStream_t s) {
     const EpiGluGrad<T> epi{p.dg, p.du, dout.p, dout.stride, n, rows, dtype, act};
-    launch_rows_gemm<false, false, T>(g, 4 * p.dg.units, p.x.groups, epi, s);
+    launch_rows_gemm<false, false, T>(p.tile, g, 4 * p.dg.units, p.x.groups, epi, s);
 }
 
 void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
@@ -205,11 +209,11 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         g.a = rows_outer(wg);
         g.b = rows_inner(p.dg);
         g.k32 = (int32_t)p.dg.units;
-        g.parts = p.parts;
+        g.parts = p.back.parts;
         rows_pairs(g, wg, p.dg, p.order);
         rows_pairs(g, wu, p.du, p.order);
-        launch_rows_parts(g, p.part, p.ld, n, gate.cols, false, s);
-        launch_join_parts(dx.p, dtype, dx.stride, p.part, p.parts, n * p.ld, p.ld, n, gate.cols, s);
+        launch_rows_parts(p.back.tile, g, p.part, p.ld, n, gate.cols, false, s);
+        launch_join_parts(dx.p, dtype, dx.stride, p.part, p.back.parts, n * p.ld, p.ld, n, gate.cols, s);
     }
     const RowsArg dw[2] = {dgate, dup};
     const Planes *d[2] = {&p.dg, &p.du};

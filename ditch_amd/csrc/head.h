@@ -34,4 +34,9 @@ inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *sec
     return g;
 }
 
+inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
+    const int a = weight_terms(w);
+    return rows_tiling(ceil_div(rows, 16), nblocks, x.units, rows_pair_count(a, x.terms, order_of(a, x.terms)), false).tile;
+}
+
 }  // namespace ditch

@@ -118,23 +118,21 @@ static void with_join_rows(int64_t n, F &&f) {
 // ---------------------------------------------------------------------------
 // divergence
 
-// phi(u) = u + e^-u - 1 for |u| <= 1: its series to u^12 / 12!, 2^-30 of it
+// phi(u) = u + e^-u - 1 for |u| <= 1/4: its series to u^7, off by 2^-27 of it
 __device__ __forceinline__ float phi_near(float u) {
-    float s = 1.f / 479001600.f;
-    s = __builtin_fmaf(s, -u, 1.f / 39916800.f);
-    s = __builtin_fmaf(s, -u, 1.f / 3628800.f);
-    s = __builtin_fmaf(s, -u, 1.f / 362880.f);
-    s = __builtin_fmaf(s, -u, 1.f / 40320.f);
-    s = __builtin_fmaf(s, -u, 1.f / 5040.f);
-    s = __builtin_fmaf(s, -u, 1.f / 720.f);
-    s = __builtin_fmaf(s, -u, 1.f / 120.f);
-    s = __builtin_fmaf(s, -u, 1.f / 24.f);
-    s = __builtin_fmaf(s, -u, 1.f / 6.f);
-    s = __builtin_fmaf(s, -u, 0.5f);
+    float s = -1.f / 5040.f;
+    s = __builtin_fmaf(s, u, 1.f / 720.f);
+    s = __builtin_fmaf(s, u, -1.f / 120.f);
+    s = __builtin_fmaf(s, u, 1.f / 24.f);
+    s = __builtin_fmaf(s, u, -1.f / 6.f);
+    s = __builtin_fmaf(s, u, 0.5f);
     return s * u * u;
 }
 
-constexpr int KL_STATS = 6;  // of a strip: base maximum, sum; trial maximum, sum; sums of w phi(D) and of w D
+// Of a strip: the base's maximum and sum, the trial's maximum and sum, the sum of
+// e^(l_base - m) phi(D) relative to m = the larger of the maxima (so that neither
+// e^l_base nor e^l_trial in it overflows), the sum of e^(l_base - its maximum) D.
+constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
     float *part;  // [strip][KL_STATS][npad]
@@ -144,6 +142,7 @@ struct EpiKlStats {
     __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
         const int64_t strip = strip0 + mb / MI;
         const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+        const bool whole = (int64_t)(mb + MI) * 16 <= rows;
 #pragma unroll
         for (int j = 0; j < NJ; j += 2) {
             const int64_t tok = (int64_t)(nb + j) / 2 * 16 + (lane & 15);
@@ -154,23 +153,25 @@ struct EpiKlStats {
                 for (int i = 0; i < MI; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        if (v0 + i * 16 + r >= rows) acc[i][j + h][r] = LOWEST;
+                        // (both at LOWEST: no weight and no difference)
+                        if (!whole && v0 + i * 16 + r >= rows) acc[i][j + h][r] = LOWEST;
                         mx[h] = fmaxf(mx[h], acc[i][j + h][r]);
                     }
                 mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 16));
                 mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 32));
             }
+            const float m = fmaxf(mx[0], mx[1]), sb = fast_exp(mx[0] - m), st = fast_exp(mx[1] - m);
 #pragma unroll
             for (int i = 0; i < MI; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    if (v0 + i * 16 + r >= rows) continue;
                     const float b = acc[i][j][r], t = acc[i][j + 1][r], u = b - t;
-                    const float w = fast_exp(b - mx[0]);
+                    const float w = fast_exp(b - mx[0]), x = fast_exp(t - mx[1]);
                     sum[0] += w;
-                    sum[1] += fast_exp(t - mx[1]);
+                    sum[1] += x;
                     far = __builtin_fmaf(w, u, far);
-                    near += fabsf(u) <= 1.f ? w * phi_near(u) : w * (u - 1.f) + fast_exp(t - mx[0]);
+                    const float wm = w * sb;
+                    near += fabsf(u) <= 0.25f ? wm * phi_near(u) : __builtin_fmaf(wm, u - 1.f, x * st);
                 }
             float v[KL_STATS] = {mx[0], sum[0], mx[1], sum[1], near, far};
 #pragma unroll
@@ -189,49 +190,50 @@ template <int TOK>
 __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base, float *lse_trial, const float *part,
                                                       int64_t n, int64_t npad, int64_t strips) {
     constexpr int SL = 512 / TOK;
-    __shared__ float ms[SL][2][TOK];
-    __shared__ double ss[SL][4][TOK];  // base sum, trial sum, near, far
+    // base sum, trial sum, near, far, and what they are relative to: the maxima of base and trial, the larger, base's
+    constexpr int OF[4] = {0, 1, 2, 0};
+    __shared__ float ms[SL][3][TOK];
+    __shared__ double ss[SL][4][TOK];
     const int c = threadIdx.x % TOK, sl = threadIdx.x / TOK;
     const int64_t tok = (int64_t)blockIdx.x * TOK + c;
-    float m[2] = {LOWEST, LOWEST};
+    float m[3] = {LOWEST, LOWEST, LOWEST};
     double s[4] = {0, 0, 0, 0};
     if (tok < n) {
 #pragma unroll 2
         for (int64_t k = sl; k < strips; k += SL) {
             const float *p = part + k * KL_STATS * npad + tok;
-            const float v[KL_STATS] = {p[0], p[npad], p[2 * npad], p[3 * npad], p[4 * npad], p[5 * npad]};
-            const float to = fmaxf(m[0], v[0]), tt = fmaxf(m[1], v[2]);
-            const double a = expf(m[0] - to), b = expf(v[0] - to);
-            s[0] = s[0] * a + b * v[1];
-            s[1] = s[1] * (double)expf(m[1] - tt) + (double)expf(v[2] - tt) * v[3];
-            s[2] = s[2] * a + b * v[4];
-            s[3] = s[3] * a + b * v[5];
-            m[0] = to;
-            m[1] = tt;
+            const float v[4] = {p[npad], p[3 * npad], p[4 * npad], p[5 * npad]}, b = p[0], t = p[2 * npad];
+            const float at[3] = {b, t, fmaxf(b, t)};
+            double mine[3], theirs[3];
+            for (int h = 0; h < 3; h++) {
+                const float to = fmaxf(m[h], at[h]);
+                mine[h] = expf(m[h] - to);
+                theirs[h] = expf(at[h] - to);
+                m[h] = to;
+            }
+            for (int q = 0; q < 4; q++) s[q] = s[q] * mine[OF[q]] + theirs[OF[q]] * v[q];
         }
     }
-    for (int h = 0; h < 2; h++) ms[sl][h][c] = m[h];
-    for (int k = 0; k < 4; k++) ss[sl][k][c] = s[k];
+    for (int h = 0; h < 3; h++) ms[sl][h][c] = m[h];
+    for (int q = 0; q < 4; q++) ss[sl][q][c] = s[q];
     __syncthreads();
     for (int half = SL / 2; half > 0; half /= 2) {
         if (sl < half) {
-            double e[2][2];
-            for (int h = 0; h < 2; h++) {
+            double mine[3], theirs[3];
+            for (int h = 0; h < 3; h++) {
                 const float a = ms[sl][h][c], b = ms[sl + half][h][c], to = fmaxf(a, b);
-                e[h][0] = exp((double)a - (double)to);
-                e[h][1] = exp((double)b - (double)to);
+                mine[h] = exp((double)a - (double)to);
+                theirs[h] = exp((double)b - (double)to);
                 ms[sl][h][c] = to;
             }
-            for (int k = 0; k < 4; k++) {
-                const int h = k == 1;
-                ss[sl][k][c] = ss[sl][k][c] * e[h][0] + ss[sl + half][k][c] * e[h][1];
-            }
+            for (int q = 0; q < 4; q++) ss[sl][q][c] = ss[sl][q][c] * mine[OF[q]] + ss[sl + half][q][c] * theirs[OF[q]];
         }
         __syncthreads();
     }
     if (sl != 0 || tok >= n) return;
-    for (int k = 0; k < 4; k++) s[k] = ss[0][k][c];
-    const double lb = (double)ms[0][0][c] + log(s[0]), lt = (double)ms[0][1][c] + log(s[1]), d = lt - lb;
+    for (int q = 0; q < 4; q++) s[q] = ss[0][q][c];
+    const double mb = ms[0][0][c], lb = mb + log(s[0]), lt = (double)ms[0][1][c] + log(s[1]), d = lt - lb;
+    s[2] *= exp((double)ms[0][2][c] - mb);
     lse_base[tok] = (float)lb;
     lse_trial[tok] = (float)lt;
     kl[tok] = (float)(fabs(d) <= 1 ? s[2] / s[0] - (expm1(d) - d) : s[3] / s[0] + d);
@@ -241,14 +243,15 @@ __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base
 // pieces of the vocabulary
 
 // strips of the vocabulary in a piece: one for each wave's rows of a tile
-static int64_t strips_of(int64_t rows, int64_t nblocks) {
-    return ceil_div(rows, 256) * (rows_tall(nblocks) ? 4 : 2);
+static int64_t strips_of(int64_t rows, int tile) {
+    return ceil_div(ceil_div(rows, 16), rows_tile_blocks(tile)) * rows_tile_blocks(tile) / rows_strip_blocks(tile);
 }
 
 // The forward of either loss: stats(g, piece's epilogue arguments).
 struct HeadPlan {
     Planes x[2];
     int64_t piece = 0, strips = 0, npad = 0, nblocks = 0;
+    int tile = 0;
     char *room = nullptr;
     char *part = nullptr;
     float *picked = nullptr;
@@ -265,8 +268,9 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
     p.nblocks = p.x[0].groups * (kl ? 2 : 1);
     const int64_t per = weight_row_bytes(w);
     p.piece = per ? piece_rows(w.rows, per) : w.rows;
+    p.tile = logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks);
     for (int64_t r = 0; r < w.rows; r += p.piece)
-        p.strips += strips_of(w.rows - r < p.piece ? w.rows - r : p.piece, p.nblocks);
+        p.strips += strips_of(w.rows - r < p.piece ? w.rows - r : p.piece, p.tile);
     p.part = c.take((size_t)p.strips * p.npad * (kl ? KL_STATS * sizeof(float) : sizeof(float2)));
     p.picked = c.take<float>(p.npad);
     if (per) p.room = c.take(weight_planes_shape(w, p.piece).bytes());
@@ -291,10 +295,10 @@ void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t
         const Planes wp = weight_planes(w, r, rows, p.room, s);
         const EpiLossStats epi{(float2 *)p.part, p.picked, targets, p.npad, n, rows, r, strip};
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(logits_gemm(wp, p.x[0], nullptr), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], nullptr), wp.groups,
                                                                    p.nblocks, epi, s);
         });
-        strip += strips_of(rows, p.nblocks);
+        strip += strips_of(rows, p.tile);
     }
     with_join_rows(n, [&](auto rows) {
         constexpr int TOK = decltype(rows)::value;
@@ -315,10 +319,10 @@ void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype,
         const Planes wp = weight_planes(w, r, rows, p.room, s);
         const EpiKlStats epi{(float *)p.part, p.npad, n, rows, strip};
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(logits_gemm(wp, p.x[0], &p.x[1]), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], &p.x[1]), wp.groups,
                                                                    p.nblocks, epi, s);
         });
-        strip += strips_of(rows, p.nblocks);
+        strip += strips_of(rows, p.tile);
     }
     with_join_rows(n, [&](auto rows) {
         constexpr int TOK = decltype(rows)::value;

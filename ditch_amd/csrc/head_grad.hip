@@ -84,7 +84,7 @@ struct EpiKlGrad {
 struct HeadGradPlan {
     Planes x[2], d;
     int64_t piece = 0, nblocks = 0, ld = 0;
-    int parts = 1;
+    RowsTiling tiling;
     int order = 1;  // of the products with d
     char *room = nullptr;
     float *part = nullptr;
@@ -104,9 +104,10 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     p.d = Planes{nullptr, p.nblocks, p.piece / 32, terms};
     p.d.p = c.take(p.d.bytes());
     p.ld = ceil_div(w.cols, 4) * 4;
-    p.parts = rows_parts(ceil_div(w.cols, 16), p.nblocks, p.piece / 64);
-    p.part = c.take<float>((size_t)p.parts * n * p.ld);
     p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
+    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32,
+                           rows_pair_count(weight_terms(w), terms, p.order), true);
+    p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
     if (weight_row_bytes(w)) p.room = c.take(weight_planes_shape(w, p.piece).bytes());
     p.bytes = c.at;
     return p;
@@ -134,9 +135,9 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
             g.a = rows_outer(wp);
             g.b = rows_inner(d);
             g.k32 = (int32_t)d.units;
-            g.parts = p.parts;
+            g.parts = p.tiling.parts;
             rows_pairs(g, wp, d, p.order);
-            launch_rows_parts(g, p.part, p.ld, n, w.cols, r > 0, s);
+            launch_rows_parts(p.tiling.tile, g, p.part, p.ld, n, w.cols, r > 0, s);
         }
         if (dw.p) {
             RowsGemm g;
@@ -147,20 +148,22 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
             launch_rows_out(g, (char *)dw.p + r * dw.stride * (int64_t)row_size(dtype), dtype, dw.stride, rows, w.cols, s);
         }
     }
-    if (dx.p) launch_join_parts(dx.p, dtype, dx.stride, p.part, p.parts, n * p.ld, p.ld, n, w.cols, s);
+    if (dx.p) launch_join_parts(dx.p, dtype, dx.stride, p.part, p.tiling.parts, n * p.ld, p.ld, n, w.cols, s);
 }
 
 template <int T>
-static void fill_loss(const HeadGradPlan &p, const Planes &wp, const Planes &d, int64_t row0, int64_t rows, int64_t n,
-                      int64_t vocab, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
-    const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, vocab};
-    launch_rows_gemm<false, false, T>(logits_gemm(wp, p.x[0], nullptr), d.units * 2, p.nblocks, epi, s);
+static void fill_loss(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
+                      int64_t rows, int64_t n, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
+    const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, w.rows};
+    launch_rows_gemm<false, false, T>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, p.x[0], nullptr),
+                                      d.units * 2, p.nblocks, epi, s);
 }
 template <int T>
-static void fill_kl(const HeadGradPlan &p, const Planes &wp, const Planes &d, int64_t rows, int64_t n,
+static void fill_kl(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t rows, int64_t n,
                     const float *lse_base, const float *lse_trial, const float *dkl, hipStream_t s) {
     const EpiKlGrad<T> epi{d, lse_base, lse_trial, dkl, n, rows};
-    launch_rows_gemm<false, false, T>(logits_gemm(wp, p.x[0], &p.x[1]), d.units * 2, 2 * p.nblocks, epi, s);
+    launch_rows_gemm<false, false, T>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, p.x[0], &p.x[1]),
+                                      d.units * 2, 2 * p.nblocks, epi, s);
 }
 
 void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int64_t n, const TileView &w,
@@ -169,7 +172,7 @@ void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int
     launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);
     head_grad(p, dtype, dx, dw, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
         auto f = p.d.terms == 1 ? fill_loss<1> : p.d.terms == 2 ? fill_loss<2> : fill_loss<3>;
-        f(p, wp, d, row0, rows, n, w.rows, targets, lse, dloss, s);
+        f(p, w, wp, d, row0, rows, n, targets, lse, dloss, s);
     });
 }
 
@@ -180,7 +183,7 @@ void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial,
     launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
     head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t, int64_t rows) {
         auto f = p.d.terms == 1 ? fill_kl<1> : p.d.terms == 2 ? fill_kl<2> : fill_kl<3>;
-        f(p, wp, d, rows, n, lse_base, lse_trial, dkl, s);
+        f(p, w, wp, d, rows, n, lse_base, lse_trial, dkl, s);
     });
 }
 

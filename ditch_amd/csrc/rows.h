@@ -64,10 +64,26 @@ struct Carver {
 void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
                        int64_t ld, int64_t n, int64_t cols, hipStream_t s);
 
+// The tile and the parts (of k) of a product of mblocks x nblocks 16-row blocks
+// over k32 steps of 32 k and `pairs` pairs of terms (rows.hip). Parts are
+// tried only where `split`.
+struct RowsTiling {
+    int tile = 0, parts = 1;
+};
+RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int pairs, bool split);
+// 16-row blocks of a wave's strip and of a tile along m
+inline int rows_strip_blocks(int tile) { return tile == 0 ? 8 : tile == 3 ? 2 : 4; }
+inline int rows_tile_blocks(int tile) { return tile == 0 || tile == 2 ? 16 : tile == 1 ? 8 : 4; }
+inline int rows_pair_count(int a, int b, int order) {
+    int n = 0;
+    for (int i = 0; i < a; i++) n += order - i < 0 ? 0 : order - i < b ? order - i : b;
+    return n;
+}
+
 // rows_products.hip: c as parts of sums [part][n][ld] (added where `add`), a outer
 // and b inner; and as rows of `dtype`, both outer
 struct RowsGemm;
-void launch_rows_parts(const RowsGemm &g, float *part, int64_t ld, int64_t n, int64_t m, bool add, hipStream_t s);
+void launch_rows_parts(int tile, const RowsGemm &g, float *part, int64_t ld, int64_t n, int64_t m, bool add, hipStream_t s);
 void launch_rows_out(const RowsGemm &g, void *out, int32_t dtype, int64_t stride, int64_t n, int64_t m, hipStream_t s);
 
 // head.hip, head_grad.hip

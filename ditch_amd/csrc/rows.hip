@@ -98,6 +98,37 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
     DITCH_TRY_HIP(hipGetLastError());
 }
 
+// Tiles of 256 x 256 (one workgroup a CU), 128 x 128 (two), 256 x 64 (one) and 64 x
+// 64 (four), with what a stage of 64 k takes one workgroup alone on its CU and each of
+// as many as fit (us; fitted to products of 4096 to 128256 rows, 64 to 8192 columns).
+// The cheapest by rounds over the chip's 256 CUs: large products take the largest
+// tiles, where the LDS feeds the matrix cores best, few rows the narrow ones, small
+// ones whichever spreads over the chip.
+RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int pairs, bool split) {
+    static const struct {
+        int bm, bn, fit;
+        double one, all;
+    } tiles[4] = {{16, 16, 1, 0.93, 0.93}, {8, 8, 2, 0.42, 0.55}, {16, 4, 1, 0.36, 0.36}, {4, 4, 4, 0.25, 0.32}};
+    RowsTiling best;
+    double least = 1e30;
+    for (int t = 0; t < 4; t++) {
+        const int64_t tiles_mn = ceil_div(mblocks, tiles[t].bm) * ceil_div(nblocks, tiles[t].bn);
+        for (int64_t parts = 1; parts <= (split ? 64 : 1) && (parts == 1 || k32 / parts >= 8); parts++) {
+            const int64_t wgs = tiles_mn * parts, full = 256 * tiles[t].fit, rest = wgs % full;
+            const double stages = (double)ceil_div(k32, parts) * pairs / 2;
+            double us = stages * (wgs / full * tiles[t].all + (rest == 0 ? 0 : rest <= 256 ? tiles[t].one : tiles[t].all));
+            // parts are written, read and added: 4 bytes twice at 4 TB/s
+            us += parts * (double)mblocks * nblocks * 256 * 8 / 4e6;
+            if (us < least) {
+                least = us;
+                best.tile = t;
+                best.parts = (int)parts;
+            }
+        }
+    }
+    return best;
+}
+
 bool weight_is_planes(const TileView &w) { return w.tf == TF_BF16; }
 
 Planes weight_planes_shape(const TileView &w, int64_t rows) {

@@ -348,13 +348,15 @@ void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const E
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Tiles of 256 x 256, or of 256 x 64 where n holds few blocks. Stages of as many
-// k as two buffers of the LDS hold.
-inline bool rows_tall(int64_t nblocks) { return nblocks <= 8; }
+// Stages of as many k as two buffers of the LDS hold. `tile`: rows_tile()'s choice.
 template <bool AO, bool BO, int TB, typename Epi>
-void launch_rows_gemm(const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
-    if (rows_tall(nblocks)) launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s);
-    else launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s);
+void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
+    switch (tile) {
+    case 0: launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s); break;
+    case 1: launch_rows_gemm_tile<2, 2, 4, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s); break;
+    case 2: launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s); break;
+    default: launch_rows_gemm_tile<2, 2, 2, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s); break;
+    }
 }
 
 template <typename F>
@@ -362,15 +364,6 @@ void with_terms(int terms, F &&f) {
     if (terms == 1) f(std::integral_constant<int, 1>{});
     else if (terms == 2) f(std::integral_constant<int, 2>{});
     else f(std::integral_constant<int, 3>{});
-}
-
-// Parts of a product's stages so that its tiles fill the chip's 256 CUs, each
-// of at least 8 stages.
-inline int rows_parts(int64_t mblocks, int64_t nblocks, int64_t stages) {
-    const int64_t tiles = ceil_div(mblocks, 16) * ceil_div(nblocks, rows_tall(nblocks) ? 4 : 16);
-    int64_t parts = tiles >= 256 ? 1 : ceil_div(512, tiles);
-    parts = parts < stages / 8 ? parts : stages / 8;
-    return (int)(parts < 1 ? 1 : parts);
 }
 
 }  // namespace ditch
