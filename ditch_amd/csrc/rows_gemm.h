@@ -3,10 +3,11 @@
 //
 // c[m][n] = sum over the pairs of terms and k of a[m][k] b[n][k]. Each operand
 // is inner (its columns are k) or outer (its rows are k). A workgroup computes
-// BM x BN; a stage is one term of a and all TB terms of b over 32 KS k: whole units
-// are copied global -> LDS, two stage buffers, the next stage on its way while this
-// one is multiplied. (A fragment of a then serves every term of b: with a stage a
-// pair, f32 rows read a three times and the LDS was what they waited for.)
+// BM x BN; a stage is one term of a and all TB terms of b over 32 k: whole units are
+// copied global -> LDS into a ring of buffers, some stages ahead. (A fragment of a
+// then serves every term of b: with a stage a pair, f32 rows read a three times
+// and the LDS was what they waited for.) With one term the next stage's fragments
+// are read while this one's are multiplied.
 // Fragments of inner operands are one 16-byte LDS read a lane, those of outer ones
 // two transposing reads (ds_read_b64_tr_b16: lane t of 16 gets column t of four
 // 16-column rows whose quarters the 16 lanes address).
@@ -86,16 +87,16 @@ __device__ __forceinline__ void rows_map_tile(int g, int total, int tm, int tn, 
     nt = r / gs;
 }
 
-template <bool OUTER, int KS>
-__device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int kk, int lane) {
+template <bool OUTER>
+__device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int lane) {
     if constexpr (!OUTER) {
-        return S[(block * KS + kk) * 64 + lane];
+        return S[block * 64 + lane];
     } else {
         // k 8 g .. +8 of the step for lane group g: unit g / 2, rows 8 (g % 2) .. +8, four a read
         const int t = lane & 15, g = lane >> 4;
         const char *p = (const char *)S + (g >> 1) * 1024 + (8 * (g & 1) + (t >> 2) + 16 * ((t & 3) >> 1)) * 16 +
                         (t & 1) * 8;
-        p += ((block >> 1) * 2 * KS + 2 * kk) * 1024 + (block & 1) * 512;
+        p += (block >> 1) * 2048 + (block & 1) * 512;
         const rows_short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)p);
         const rows_short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rows_lds_short4 *)(p + 64));
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -104,68 +105,116 @@ __device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int kk
     }
 }
 
+// 1 KiB of `src` (16 bytes a lane at lane16) to the LDS at `to`. As an instruction
+// of its own text: the compiler makes the transposing LDS reads wait for every
+// copy in flight, whichever buffer it fills. It writes no register; the kernel
+// below waits for it (rows_vmcnt). M0 needs a wait state before its use; nothing
+// else in these kernels uses it.
+__device__ __forceinline__ void rows_copy_unit(const char *src, uint32_t lane16, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane16), "s"(src)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t rows_lds_at(const u32x4 *p) { return (uint32_t)(uintptr_t)(rows_lds_void *)p; }
+
+// A wave's copies of one operand's planes: PER units of each of TERMS planes. Of
+// an inner operand a stage is a unit of each 16-row block, of an outer one two
+// 16-row groups of each 32-column unit.
+template <bool OUTER, int PER, int TERMS>
+struct RowsCopies {
+    int64_t off[PER];      // where each begins
+    int64_t step, plane;   // bytes from a unit along k to the next, from a plane to the next
+    int32_t ks;
+    int odd;               // outer, one unit a wave: which of the two groups
+    __device__ __forceinline__ RowsCopies(const RowsOperand &o, int wave, int first, int64_t plane_bytes) {
+        step = (OUTER ? o.ldu : 1) * 1024;
+        plane = plane_bytes;
+        ks = o.ks;
+        odd = OUTER && PER == 1 ? wave & 1 : 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int l = wave * PER + j;
+            if (OUTER) {
+                int u = first / 2 + l / 2;
+                u = u < o.blocks ? u : o.blocks - 1;
+                off[j] = (int64_t)u * 1024;
+            } else {
+                int g = first + l, second = 0;
+                if (o.paired) {
+                    second = g & 1;
+                    g >>= 1;
+                }
+                g = g < o.blocks ? g : o.blocks - 1;
+                off[j] = (int64_t)g * o.ldu * 1024 + (second ? o.pair : 0);
+            }
+        }
+    }
+    // stage cs of the planes at `base` to S, this wave's first unit at unit wave * PER of every plane of `units`
+    __device__ __forceinline__ void copy(const char *base, int cs, uint32_t S, int wave, int units, uint32_t lane16) const {
+        static_assert(!OUTER || PER == 1 || PER % 2 == 0, "whole pairs of groups, or one unit");
+        const int k0 = OUTER ? 2 * cs + odd : cs;
+        const int64_t at0 = (k0 < ks ? k0 : ks - 1) * step;
+        const int64_t at1 = OUTER ? (k0 + 1 < ks ? k0 + 1 : ks - 1) * step : 0;
+#pragma unroll
+        for (int e = 0; e < TERMS; e++)
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const char *src = base + (off[j] + (OUTER && (j & 1) ? at1 : at0) + e * plane);
+                rows_copy_unit(src, lane16, S + (e * units + wave * PER + j) * 1024);
+            }
+    }
+};
+
+// s_waitcnt's operand for at most n vector memory operations in flight
+constexpr int rows_vmcnt(int n) { return (n & 15) | (n >> 4) << 14 | 0x0f70; }
+
 // WGM x WGN waves of MI x NJ blocks of 16 x 16.
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, int KS, typename Epi>
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, typename Epi>
 __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, Epi epi) {
-    constexpr int WAVES = WGM * WGN, BM = WGM * MI, BN = WGN * NJ;  // tile in 16-row blocks
-    static_assert(BM % 2 == 0 && BN % 2 == 0, "whole 32-column units");
-    constexpr int UA = BM * KS, UB = BN * KS, PER = (UA + TB * UB) / WAVES;
-    static_assert((UA + TB * UB) % WAVES == 0, "copies split evenly");
-    // distinct objects: the compiler sees that the copies into one do not touch what is read from the other
-    __shared__ u32x4 S0[(UA + TB * UB) * 64], S1[(UA + TB * UB) * 64];
+    constexpr int WAVES = WGM * WGN, UA = WGM * MI, UB = WGN * NJ;  // tile in 16-row blocks: units of a stage
+    static_assert(UA % 2 == 0 && UB % 2 == 0, "whole 32-column units");
+    static_assert(UA % WAVES == 0 && (UB % WAVES == 0 || UB * 2 == WAVES), "copies split evenly");
+    constexpr bool HALF = UB * 2 == WAVES;  // every other wave copies of b
+    constexpr int PA = UA / WAVES, PB = HALF ? 1 : UB / WAVES;
+    constexpr int STAGE = UA + TB * UB;  // units
+    // a ring within half of the 160 KB of LDS (two workgroups a CU), within all of it for the largest tile
+    constexpr int ROOM = WAVES * MI * NJ >= 256 ? 156 : 80, FIT = ROOM / STAGE;
+    constexpr int NB = FIT > 4 ? 4 : FIT < 2 ? 2 : FIT;
+    constexpr bool AHEAD = TB == 1;  // the next stage's fragments in registers
+    // distinct objects: the compiler sees that the copies into one do not touch what is read from the others
+    __shared__ u32x4 S0[STAGE * 64], S1[STAGE * 64], S2[NB > 2 ? STAGE * 64 : 1], S3[NB > 3 ? STAGE * 64 : 1];
 
     const int lane = threadIdx.x & 63;
+    const uint32_t lane16 = lane * 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
     int mt, nt;
     rows_map_tile(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, mt, nt);
+    const bool copies_b = !HALF || wave < UB;
+    const RowsCopies<AO, PA, 1> ca(p.a, wave, mt * UA, 0);
+    const RowsCopies<BO, PB, TB> cb(p.b, copies_b ? wave : 0, nt * UB, p.b_plane);
 
-    // this wave's copies: where in the planes each begins (the k part is added a stage)
-    int64_t off[PER];
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int q = wave * PER + j;
-        const bool is_a = q < UA;
-        const RowsOperand &o = is_a ? p.a : p.b;
-        const int l = is_a ? q : (q - UA) % UB, first = is_a ? mt * BM : nt * BN;
-        if (is_a ? AO : BO) {
-            int u = first / 2 + l / (2 * KS);
-            u = u < o.blocks ? u : o.blocks - 1;
-            off[j] = (int64_t)u * 1024;
-        } else {
-            int g = first + l / KS, second = 0;
-            if (o.paired) {
-                second = g & 1;
-                g >>= 1;
-            }
-            g = g < o.blocks ? g : o.blocks - 1;
-            off[j] = (int64_t)g * o.ldu * 1024 + (second ? o.pair : 0);
-        }
-        if (!is_a) off[j] += (q - UA) / UB * p.b_plane;
-    }
-    // a linear stage is (32 KS k, term of a): the terms of a stage follow each
+    // a linear stage is (32 k, term of a): the terms of a step follow each
     // other, so that what they share is read from near
-    const int steps = (p.k32 + KS - 1) / KS;
-    const int first_t = (int)((int64_t)steps * blockIdx.y / p.parts) * p.nseg;
-    const int last_t = (int)((int64_t)steps * (blockIdx.y + 1) / p.parts) * p.nseg;
-    int cs = first_t / p.nseg, seg = 0, cur = 0;  // of the next copy; of the product
+    const int nseg = p.nseg;
+    const int first_t = (int)((int64_t)p.k32 * blockIdx.y / p.parts) * nseg;
+    const int last_t = (int)((int64_t)p.k32 * (blockIdx.y + 1) / p.parts) * nseg;
+    int cs = first_t / nseg, seg = 0, cur = 0;  // of the next copy; of the product
+    const char *ba = p.sa[0], *bb = p.sb[0];
+    int copied = first_t;
     auto copy = [&](u32x4 *S) {
-        const char *ba = p.sa[seg], *bb = p.sb[seg];
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int q = wave * PER + j;
-            const bool is_a = q < UA;
-            const RowsOperand &o = is_a ? p.a : p.b;
-            const int l = is_a ? q : q - UA;
-            const bool outer = is_a ? AO : BO;
-            int k = outer ? 2 * KS * cs + l % (2 * KS) : KS * cs + l % KS;
-            k = k < o.ks ? k : o.ks - 1;
-            const char *src = (is_a ? ba : bb) + off[j] + (outer ? k * o.ldu : (int64_t)k) * 1024;
-            __builtin_amdgcn_global_load_lds((const void *)(src + lane * 16), (rows_lds_void *)&S[q * 64], 16, 0, 0);
-        }
-        if (++seg == p.nseg) {
-            seg = 0;
-            cs++;
+        if (copied >= last_t) return;
+        copied++;
+        const uint32_t to = rows_lds_at(S);
+        ca.copy(ba, cs, to, wave, UA, lane16);
+        if (copies_b) cb.copy(bb, cs, to + UA * 1024, wave, UB, lane16);
+        if (nseg == 1) cs++;
+        else {
+            if (++seg == nseg) {
+                seg = 0;
+                cs++;
+            }
+            ba = p.sa[seg];
+            bb = p.sb[seg];
         }
     };
     floatx4 acc[MI][NJ];
@@ -174,48 +223,106 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-    auto step = [&](const u32x4 *S, u32x4 *N, bool more) {
-        if (more) copy(N);
+    constexpr int FLIGHT = PA + (HALF ? 0 : TB * PB);  // copies of a stage that every wave makes at least
+    u32x4 fa[AHEAD ? 2 : 1][MI], fb[AHEAD ? 2 : 1][NJ];
+    auto read_a = [&](const u32x4 *S, u32x4 (&a)[MI]) {
+#pragma unroll
+        for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO>(S, wm * MI + i, lane);
+    };
+    auto read_b = [&](const u32x4 *S, int e, u32x4 (&b)[NJ]) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) b[j] = rows_fragment<BO>(S + (UA + e * UB) * 64, wn * NJ + j, lane);
+    };
+    auto products = [&](const u32x4 (&a)[MI], const u32x4 (&b)[NJ]) {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
+    };
+    // every wave's copies but those of the last `later` stages have landed, and
+    // every wave is done with what it read before
+    auto meet = [&](bool all) {
         __builtin_amdgcn_sched_barrier(0);
-        const u32x4 *A = S, *B = S + UA * 64;
-        const int count = TB == 1 ? 1 : p.count[cur];
-#pragma unroll
-        for (int kk = 0; kk < KS; kk++) {
-            u32x4 a[MI];
-#pragma unroll
-            for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO, KS>(A, wm * MI + i, kk, lane);
-#pragma unroll
-            for (int e = 0; e < TB; e++) {
-                if (e > 0 && e >= count) continue;
-                u32x4 b[NJ];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) b[j] = rows_fragment<BO, KS>(B + e * UB * 64, wn * NJ + j, kk, lane);
-#pragma unroll
-                for (int i = 0; i < MI; i++)
-#pragma unroll
-                    for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
-            }
-        }
-        if (TB > 1) cur = cur + 1 == p.nseg ? 0 : cur + 1;
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies have landed
+        constexpr int later = NB - 2;
+        if (all || later == 0) __builtin_amdgcn_s_waitcnt(rows_vmcnt(0) & ~0x0f00);  // and lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(rows_vmcnt(later * FLIGHT) & ~0x0f00);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (first_t < last_t) {
-        copy(S0);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        int t = first_t;
-        for (; t + 1 < last_t; t += 2) {
-            step(S0, S1, true);
-            step(S1, S0, t + 2 < last_t);
+    if constexpr (AHEAD) {
+        // stage t: multiply the fragments in set t % 2; read t + 1's from its buffer; copy t + NB to t's
+        auto step = [&](int t, u32x4 *S, const u32x4 *N, auto set) {
+            constexpr int c = decltype(set)::value;
+            meet(t + NB > last_t);
+            copy(S);
+            __builtin_amdgcn_sched_barrier(0);
+            read_a(N, fa[c ^ 1]);  // (behind the last stage: whatever lies there, not used)
+            read_b(N, 0, fb[c ^ 1]);
+            products(fa[c], fb[c]);
+            // a read of the next stage after each product, while there are any
+            constexpr int READS = (AO ? 2 : 1) * MI + (BO ? 2 : 1) * NJ;
+#pragma unroll
+            for (int i = 0; i < MI * NJ; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, READS > MI * NJ ? 2 : 1, 0);
+            }
+        };
+        if (first_t < last_t) {
+            copy(S0);
+            copy(S1);
+            if (NB > 2) copy(S2);
+            if (NB > 3) copy(S3);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(rows_vmcnt(0));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            read_a(S0, fa[0]);
+            read_b(S0, 0, fb[0]);
+            using Zero = std::integral_constant<int, 0>;
+            using One = std::integral_constant<int, 1>;
+            static_assert(NB == 4, "a ring of four");
+            for (int t = first_t; t < last_t; t += 4) {
+                step(t, S0, S1, Zero{});
+                if (t + 1 < last_t) step(t + 1, S1, S2, One{});
+                if (t + 2 < last_t) step(t + 2, S2, S3, Zero{});
+                if (t + 3 < last_t) step(t + 3, S3, S0, One{});
+            }
         }
-        if (t < last_t) step(S0, S1, false);
+    } else {
+        // stage t: multiply from its buffer; copy t + NB - 1 to the one before
+        auto step = [&](int t, const u32x4 *S, u32x4 *before) {
+            meet(t + NB - 1 > last_t);
+            copy(before);
+            const int count = p.count[cur];
+            cur = cur + 1 == nseg ? 0 : cur + 1;
+            read_a(S, fa[0]);
+#pragma unroll
+            for (int e = 0; e < TB; e++) {
+                if (e > 0 && e >= count) continue;
+                read_b(S, e, fb[0]);
+                products(fa[0], fb[0]);
+            }
+        };
+        copy(S0);
+        if (NB > 2) copy(S1);
+        if (NB > 3) copy(S2);
+        for (int t = first_t; t < last_t; t += NB) {
+            if constexpr (NB == 2) {
+                step(t, S0, S1);
+                if (t + 1 < last_t) step(t + 1, S1, S0);
+            } else if constexpr (NB == 3) {
+                step(t, S0, S2);
+                if (t + 1 < last_t) step(t + 1, S1, S0);
+                if (t + 2 < last_t) step(t + 2, S2, S1);
+            } else {
+                step(t, S0, S3);
+                if (t + 1 < last_t) step(t + 1, S1, S0);
+                if (t + 2 < last_t) step(t + 2, S2, S1);
+                if (t + 3 < last_t) step(t + 3, S3, S2);
+            }
+        }
     }
-    epi(acc, mt * BM + wm * MI, nt * BN + wn * NJ, lane);
+    epi(acc, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -337,25 +444,25 @@ struct EpiRows {
 // ---------------------------------------------------------------------------
 // launches
 
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, int KS, typename Epi>
+template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     const int64_t tm = ceil_div(mblocks, WGM * MI), tn = ceil_div(nblocks, WGN * NJ);
     DITCH_CHECK(tm * tn < (int64_t)1 << 31 && g.parts < 65536, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, TB, KS, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
+    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, TB, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
                        dim3(WGM * WGN * 64), 0, s, g, epi);
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Stages of as many k as two buffers of the LDS hold. `tile`: rows_tile()'s choice.
+// `tile`: rows_tiling's choice.
 template <bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     switch (tile) {
-    case 0: launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s); break;
-    case 1: launch_rows_gemm_tile<2, 2, 4, 4, AO, BO, TB, TB == 1 ? 2 : 1>(g, mblocks, nblocks, epi, s); break;
-    case 2: launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s); break;
-    default: launch_rows_gemm_tile<2, 2, 2, 2, AO, BO, TB, 2>(g, mblocks, nblocks, epi, s); break;
+    case 0: launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
+    case 1: launch_rows_gemm_tile<2, 2, 4, 4, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
+    case 2: launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
+    default: launch_rows_gemm_tile<2, 2, 2, 2, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
     }
 }
 
