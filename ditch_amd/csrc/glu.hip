@@ -151,12 +151,11 @@ static GluPlan glu_plan(const TileView &w, int64_t n, int32_t dtype, bool grad, 
         }
         p.ld = ceil_div(w.cols, 4) * 4;
         p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
-        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units,
-                             2 * rows_pair_count(weight_terms(w), terms, p.order), true);
+        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, weight_terms(w), terms, p.order, 2, true);
         p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
     const int a = weight_terms(w), order = a > terms ? a : terms;
-    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, p.x.units, rows_pair_count(a, terms, order), false).tile;
+    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, p.x.units, a, terms, order, 1, false).tile;
     p.bytes = c.at;
     return p;
 }

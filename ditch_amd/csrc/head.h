@@ -36,7 +36,7 @@ inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *sec
 
 inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
     const int a = weight_terms(w);
-    return rows_tiling(ceil_div(rows, 16), nblocks, x.units, rows_pair_count(a, x.terms, order_of(a, x.terms)), false).tile;
+    return rows_tiling(ceil_div(rows, 16), nblocks, x.units, a, x.terms, order_of(a, x.terms), 1, false).tile;
 }
 
 }  // namespace ditch

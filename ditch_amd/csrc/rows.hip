@@ -98,25 +98,39 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Tiles of 256 x 256 (one workgroup a CU), 128 x 128 (two), 256 x 64 (one) and 64 x
-// 64 (four), with what a stage of 64 k takes one workgroup alone on its CU and each of
-// as many as fit (us; fitted to products of 4096 to 128256 rows, 64 to 8192 columns).
-// The cheapest by rounds over the chip's 256 CUs: large products take the largest
-// tiles, where the LDS feeds the matrix cores best, few rows the narrow ones, small
-// ones whichever spreads over the chip.
-RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int pairs, bool split) {
+// Tiles of 256 x 256, 128 x 128, 256 x 64 and 64 x 64: how many workgroups fit a CU
+// (by their LDS), and what 32 k of one, two or three terms of b take (us) where a
+// workgroup is alone on its CU and where as many as fit share it; measured over
+// products of 4864 to 151936 rows, 1 to 1000 columns, 896 and 4096 k, and within a
+// fifth of them. A round of workgroups begins and ends in about 4 us. The cheapest
+// by rounds over the chip's 256 CUs: large products take the largest tiles, where
+// the LDS feeds the matrix cores best (872 us for 128256 x 1000 x 4096, against 996,
+// 1143 and 1624), few columns the narrow ones (64 f32 columns: 179 us for 256 x 64,
+// 546 for 256 x 256), small ones whichever spreads over the chip.
+RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_terms, int b_terms, int order, int sets,
+                       bool split) {
     static const struct {
-        int bm, bn, fit;
-        double one, all;
-    } tiles[4] = {{16, 16, 1, 0.93, 0.93}, {8, 8, 2, 0.42, 0.55}, {16, 4, 1, 0.36, 0.36}, {4, 4, 4, 0.25, 0.32}};
+        int bm, bn, fit[3];
+        double one[3], all[3];
+    } tiles[4] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.80, 1.52, 2.17}},
+                  {8, 8, {2, 2, 2}, {0.29, 0.51, 0.67}, {0.46, 0.75, 1.18}},
+                  {16, 4, {2, 2, 2}, {0.28, 0.47, 0.58}, {0.54, 0.80, 1.11}},
+                  {4, 4, {4, 3, 2}, {0.19, 0.27, 0.32}, {0.40, 0.45, 0.48}}};
+    const int b = b_terms - 1;
+    const double terms = (double)rows_pair_count(a_terms, b_terms, order) / b_terms * sets;  // stages a step
+    // a is read once at least, 5.5 TB/s
+    const double memory = (double)mblocks * k32 * a_terms * sets * 1024 / 5.5e6;
     RowsTiling best;
     double least = 1e30;
     for (int t = 0; t < 4; t++) {
         const int64_t tiles_mn = ceil_div(mblocks, tiles[t].bm) * ceil_div(nblocks, tiles[t].bn);
+        const int fit = tiles[t].fit[b];
         for (int64_t parts = 1; parts <= (split ? 64 : 1) && (parts == 1 || k32 / parts >= 8); parts++) {
-            const int64_t wgs = tiles_mn * parts, full = 256 * tiles[t].fit, rest = wgs % full;
-            const double stages = (double)ceil_div(k32, parts) * pairs / 2;
-            double us = stages * (wgs / full * tiles[t].all + (rest == 0 ? 0 : rest <= 256 ? tiles[t].one : tiles[t].all));
+            const int64_t wgs = tiles_mn * parts, full = 256 * fit, rest = wgs % full;
+            const double stages = (double)ceil_div(k32, parts) * terms, share = tiles[t].all[b] / fit * ceil_div(rest, 256);
+            double us = (wgs / full) * (stages * tiles[t].all[b] + 4);
+            if (rest) us += stages * (share > tiles[t].one[b] ? share : tiles[t].one[b]) + 4;
+            if (us < memory) us = memory + us / 100;
             // parts are written, read and added: 4 bytes twice at 4 TB/s
             us += parts * (double)mblocks * nblocks * 256 * 8 / 4e6;
             if (us < least) {

@@ -13,9 +13,7 @@ void launch_rows_parts(int tile, const RowsGemm &g, float *part, int64_t ld, int
 
 void launch_rows_out(const RowsGemm &g, void *out, int32_t dtype, int64_t stride, int64_t n, int64_t m, hipStream_t s) {
     const int64_t mb = ceil_div(m, 16), nb = ceil_div(n, 16);
-    int pairs = 0;
-    for (int i = 0; i < g.nseg; i++) pairs += g.count[i];
-    const int tile = rows_tiling(mb, nb, g.k32, pairs, false).tile;
+    const int tile = rows_tiling(mb, nb, g.k32, g.nseg, g.terms, g.count[0], 1, false).tile;
     const EpiRows epi{out, stride, n, m, dtype, rows_wide(out, stride, dtype)};
     with_terms(g.terms, [&](auto terms) {
         launch_rows_gemm<true, true, decltype(terms)::value>(tile, g, mb, nb, epi, s);
