@@ -66,16 +66,45 @@ struct EpiLossStats {
     }
 };
 
-// The strips of TOK rows, 512 / TOK slices of them at a time; few rows a block
-// where there are few, so that their strips are read side by side (1 row x 2376
-// strips: 8 slices took 220 us).
+// Sums of strips, each relative to its own reference (a maximum), over a block of
+// 512: TOK rows, 512 / TOK slices of the strips each; row tid % TOK. The largest
+// reference first, then every thread's sums once rescaled to it.
+template <int TOK>
+__device__ __forceinline__ float block_max(float m, float *lds) {  // lds[8][TOK]
+#pragma unroll
+    for (int o = TOK; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane < TOK) lds[wave * TOK + lane] = m;
+    __syncthreads();
+    m = lds[threadIdx.x % TOK];
+#pragma unroll
+    for (int w = 1; w < 8; w++) m = fmaxf(m, lds[w * TOK + threadIdx.x % TOK]);
+    __syncthreads();
+    return m;
+}
+template <int TOK>
+__device__ __forceinline__ double block_sum(double s, double *lds) {
+#pragma unroll
+    for (int o = TOK; o < 64; o *= 2) s += __shfl_xor(s, o);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane < TOK) lds[wave * TOK + lane] = s;
+    __syncthreads();
+    s = lds[threadIdx.x % TOK];
+#pragma unroll
+    for (int w = 1; w < 8; w++) s += lds[w * TOK + threadIdx.x % TOK];
+    __syncthreads();
+    return s;
+}
+
+// Few rows a block where there are few, so that their strips are read side by
+// side (1 row x 2376 strips by 8 threads took 220 us).
 template <int TOK>
 __global__ __launch_bounds__(512) void loss_join_kernel(float *loss, float *lse, const float2 *part,
                                                         const float *picked, const int32_t *targets, int64_t n,
                                                         int64_t npad, int64_t strips, int64_t vocab) {
     constexpr int SL = 512 / TOK;
-    __shared__ float mx[SL][TOK];
-    __shared__ double sx[SL][TOK];
+    __shared__ float fl[8 * TOK];
+    __shared__ double dl[8 * TOK];
     const int c = threadIdx.x % TOK, sl = threadIdx.x / TOK;
     const int64_t tok = (int64_t)blockIdx.x * TOK + c;
     float m = LOWEST;
@@ -89,19 +118,10 @@ __global__ __launch_bounds__(512) void loss_join_kernel(float *loss, float *lse,
             m = to;
         }
     }
-    mx[sl][c] = m;
-    sx[sl][c] = sum;
-    __syncthreads();
-    for (int half = SL / 2; half > 0; half /= 2) {
-        if (sl < half) {
-            const float a = mx[sl][c], b = mx[sl + half][c], to = fmaxf(a, b);
-            sx[sl][c] = sx[sl][c] * exp((double)a - (double)to) + sx[sl + half][c] * exp((double)b - (double)to);
-            mx[sl][c] = to;
-        }
-        __syncthreads();
-    }
+    const float top = block_max<TOK>(m, fl);
+    sum = block_sum<TOK>(sum * exp((double)m - (double)top), dl);
     if (sl != 0 || tok >= n) return;
-    const double l = (double)mx[0][c] + log(sx[0][c]);
+    const double l = (double)top + log(sum);
     lse[tok] = (float)l;
     const int32_t t = targets[tok];
     loss[tok] = t < 0 ? 0.f : t >= vocab ? __builtin_nanf("") : (float)(l - (double)picked[tok]);
@@ -135,7 +155,7 @@ __device__ __forceinline__ float phi_near(float u) {
 constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
-    float *part;  // [strip][KL_STATS][npad]
+    float *part;  // [strip][npad][KL_STATS]
     int64_t npad, n;
     int64_t rows, strip0;
     template <int MI, int NJ>
@@ -180,7 +200,12 @@ struct EpiKlStats {
                     v[k] += __shfl_xor(v[k], 16);
                     v[k] += __shfl_xor(v[k], 32);
                 }
-                if (tok < n && lane < 16) part[(strip * KL_STATS + k) * npad + tok] = v[k];
+            }
+            if (tok < n && lane < 16) {
+                float2 *o = (float2 *)(part + (strip * npad + tok) * KL_STATS);
+                o[0] = make_float2(v[0], v[1]);
+                o[1] = make_float2(v[2], v[3]);
+                o[2] = make_float2(v[4], v[5]);
             }
         }
     }
@@ -192,8 +217,8 @@ __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base
     constexpr int SL = 512 / TOK;
     // base sum, trial sum, near, far, and what they are relative to: the maxima of base and trial, the larger, base's
     constexpr int OF[4] = {0, 1, 2, 0};
-    __shared__ float ms[SL][3][TOK];
-    __shared__ double ss[SL][4][TOK];
+    __shared__ float fl[8 * TOK];
+    __shared__ double dl[8 * TOK];
     const int c = threadIdx.x % TOK, sl = threadIdx.x / TOK;
     const int64_t tok = (int64_t)blockIdx.x * TOK + c;
     float m[3] = {LOWEST, LOWEST, LOWEST};
@@ -201,8 +226,9 @@ __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base
     if (tok < n) {
 #pragma unroll 2
         for (int64_t k = sl; k < strips; k += SL) {
-            const float *p = part + k * KL_STATS * npad + tok;
-            const float v[4] = {p[npad], p[3 * npad], p[4 * npad], p[5 * npad]}, b = p[0], t = p[2 * npad];
+            const float2 *p = (const float2 *)(part + (k * npad + tok) * KL_STATS);
+            const float2 base = p[0], trial = p[1], sums = p[2];
+            const float v[4] = {base.y, trial.y, sums.x, sums.y}, b = base.x, t = trial.x;
             const float at[3] = {b, t, fmaxf(b, t)};
             double mine[3], theirs[3];
             for (int h = 0; h < 3; h++) {
@@ -214,26 +240,16 @@ __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base
             for (int q = 0; q < 4; q++) s[q] = s[q] * mine[OF[q]] + theirs[OF[q]] * v[q];
         }
     }
-    for (int h = 0; h < 3; h++) ms[sl][h][c] = m[h];
-    for (int q = 0; q < 4; q++) ss[sl][q][c] = s[q];
-    __syncthreads();
-    for (int half = SL / 2; half > 0; half /= 2) {
-        if (sl < half) {
-            double mine[3], theirs[3];
-            for (int h = 0; h < 3; h++) {
-                const float a = ms[sl][h][c], b = ms[sl + half][h][c], to = fmaxf(a, b);
-                mine[h] = exp((double)a - (double)to);
-                theirs[h] = exp((double)b - (double)to);
-                ms[sl][h][c] = to;
-            }
-            for (int q = 0; q < 4; q++) ss[sl][q][c] = ss[sl][q][c] * mine[OF[q]] + ss[sl + half][q][c] * theirs[OF[q]];
-        }
-        __syncthreads();
+    float top[3];
+    double scale[3];
+    for (int h = 0; h < 3; h++) {
+        top[h] = block_max<TOK>(m[h], fl);
+        scale[h] = exp((double)m[h] - (double)top[h]);
     }
+    for (int q = 0; q < 4; q++) s[q] = block_sum<TOK>(s[q] * scale[OF[q]], dl);
     if (sl != 0 || tok >= n) return;
-    for (int q = 0; q < 4; q++) s[q] = ss[0][q][c];
-    const double mb = ms[0][0][c], lb = mb + log(s[0]), lt = (double)ms[0][1][c] + log(s[1]), d = lt - lb;
-    s[2] *= exp((double)ms[0][2][c] - mb);
+    const double mb = top[0], lb = mb + log(s[0]), lt = (double)top[1] + log(s[1]), d = lt - lb;
+    s[2] *= exp((double)top[2] - mb);
     lse_base[tok] = (float)lb;
     lse_trial[tok] = (float)lt;
     kl[tok] = (float)(fabs(d) <= 1 ? s[2] / s[0] - (expm1(d) - d) : s[3] / s[0] + d);

@@ -74,7 +74,7 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
                        bool split);
 // 16-row blocks of a wave's strip and of a tile along m
 inline int rows_strip_blocks(int tile) { return tile == 0 ? 8 : tile == 3 ? 2 : 4; }
-inline int rows_tile_blocks(int tile) { return tile == 0 || tile == 2 ? 16 : tile == 1 ? 8 : 4; }
+inline int rows_tile_blocks(int tile) { return tile == 1 ? 8 : tile == 3 ? 4 : 16; }
 inline int rows_pair_count(int a, int b, int order) {
     int n = 0;
     for (int i = 0; i < a; i++) n += order - i < 0 ? 0 : order - i < b ? order - i : b;

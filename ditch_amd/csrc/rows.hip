@@ -98,7 +98,10 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Tiles of 256 x 256, 128 x 128, 256 x 64 and 64 x 64: how many workgroups fit a CU
+// Tiles of 256 x 256, 128 x 128, 256 x 64, 64 x 64, and 256 x 64 with the whole LDS
+// as its ring (three terms only: two stages of them fill half of it, and 224
+// workgroups on as many CUs then wait for memory, 147 us against 109; where there
+// are more than CUs two on each are better, 184 against 207): how many workgroups fit a CU
 // (by their LDS), and what 32 k of one, two or three terms of b take (us) where a
 // workgroup is alone on its CU and where as many as fit share it; measured over
 // products of 4864 to 151936 rows, 1 to 1000 columns, 896 and 4096 k, and within a
@@ -112,17 +115,18 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
     static const struct {
         int bm, bn, fit[3];
         double one[3], all[3];
-    } tiles[4] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.80, 1.52, 2.17}},
-                  {8, 8, {2, 2, 2}, {0.29, 0.51, 0.67}, {0.46, 0.75, 1.18}},
-                  {16, 4, {2, 2, 2}, {0.28, 0.47, 0.58}, {0.54, 0.80, 1.11}},
-                  {4, 4, {4, 3, 2}, {0.19, 0.27, 0.32}, {0.40, 0.45, 0.48}}};
+    } tiles[5] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.78, 1.50, 2.13}},
+                  {8, 8, {2, 2, 2}, {0.30, 0.49, 0.63}, {0.46, 0.77, 1.13}},
+                  {16, 4, {2, 2, 2}, {0.29, 0.47, 0.90}, {0.54, 0.79, 1.08}},
+                  {4, 4, {4, 3, 2}, {0.19, 0.27, 0.31}, {0.40, 0.45, 0.47}},
+                  {16, 4, {1, 1, 1}, {9, 9, 0.60}, {9, 9, 0.72}}};
     const int b = b_terms - 1;
     const double terms = (double)rows_pair_count(a_terms, b_terms, order) / b_terms * sets;  // stages a step
     // a is read once at least, 5.5 TB/s
     const double memory = (double)mblocks * k32 * a_terms * sets * 1024 / 5.5e6;
     RowsTiling best;
     double least = 1e30;
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < 5; t++) {
         const int64_t tiles_mn = ceil_div(mblocks, tiles[t].bm) * ceil_div(nblocks, tiles[t].bn);
         const int fit = tiles[t].fit[b];
         for (int64_t parts = 1; parts <= (split ? 64 : 1) && (parts == 1 || k32 / parts >= 8); parts++) {
@@ -130,7 +134,9 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
             const double stages = (double)ceil_div(k32, parts) * terms, share = tiles[t].all[b] / fit * ceil_div(rest, 256);
             double us = (wgs / full) * (stages * tiles[t].all[b] + 4);
             if (rest) us += stages * (share > tiles[t].one[b] ? share : tiles[t].one[b]) + 4;
-            if (us < memory) us = memory + us / 100;
+            // (256 workgroups, each with a stage or two on its way, reach three quarters of that, 512 nine tenths)
+            const double read = memory * (1 + 90.0 / (wgs < 90 ? 90 : wgs));
+            if (us < read) us = read + us / 100;
             // parts are written, read and added: 4 bytes twice at 4 TB/s
             us += parts * (double)mblocks * nblocks * 256 * 8 / 4e6;
             if (us < least) {
@@ -257,6 +263,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtyp
     if (i >= n * per) return;
     const int64_t row = i / per, c = i % per * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int p = 0; p < parts; p++) {
         const float4 v = *(const float4 *)(part + p * part_stride + row * ld + c);
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;

@@ -6,8 +6,8 @@
 // BM x BN; a stage is one term of a and all TB terms of b over 32 k: whole units are
 // copied global -> LDS into a ring of buffers, some stages ahead. (A fragment of a
 // then serves every term of b: with a stage a pair, f32 rows read a three times
-// and the LDS was what they waited for.) With one term the next stage's fragments
-// are read while this one's are multiplied.
+// and the LDS was what they waited for.) Fragments are read while the ones
+// before them are multiplied, across stages too.
 // Fragments of inner operands are one 16-byte LDS read a lane, those of outer ones
 // two transposing reads (ds_read_b64_tr_b16: lane t of 16 gets column t of four
 // 16-column rows whose quarters the 16 lanes address).
@@ -167,8 +167,19 @@ struct RowsCopies {
 // s_waitcnt's operand for at most n vector memory operations in flight
 constexpr int rows_vmcnt(int n) { return (n & 15) | (n >> 4) << 14 | 0x0f70; }
 
-// WGM x WGN waves of MI x NJ blocks of 16 x 16.
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, typename Epi>
+// The order of a region's instructions: after each product a read, or two, while there are any.
+template <int PRODUCTS, int READS>
+__device__ __forceinline__ void rows_order() {
+    constexpr int EACH = (READS + PRODUCTS - 1) / PRODUCTS;
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i * EACH < READS) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+}
+
+// WGM x WGN waves of MI x NJ blocks of 16 x 16; WHOLE: one workgroup a CU.
+template <int WGM, int WGN, int MI, int NJ, bool WHOLE, bool AO, bool BO, int TB, typename Epi>
 __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, Epi epi) {
     constexpr int WAVES = WGM * WGN, UA = WGM * MI, UB = WGN * NJ;  // tile in 16-row blocks: units of a stage
     static_assert(UA % 2 == 0 && UB % 2 == 0, "whole 32-column units");
@@ -176,10 +187,9 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
     constexpr bool HALF = UB * 2 == WAVES;  // every other wave copies of b
     constexpr int PA = UA / WAVES, PB = HALF ? 1 : UB / WAVES;
     constexpr int STAGE = UA + TB * UB;  // units
-    // a ring within half of the 160 KB of LDS (two workgroups a CU), within all of it for the largest tile
-    constexpr int ROOM = WAVES * MI * NJ >= 256 ? 156 : 80, FIT = ROOM / STAGE;
+    // a ring within half of the 160 KB of LDS (two workgroups a CU), or within all of it
+    constexpr int ROOM = WHOLE ? 156 : 80, FIT = ROOM / STAGE;
     constexpr int NB = FIT > 4 ? 4 : FIT < 2 ? 2 : FIT;
-    constexpr bool AHEAD = TB == 1;  // the next stage's fragments in registers
     // distinct objects: the compiler sees that the copies into one do not touch what is read from the others
     __shared__ u32x4 S0[STAGE * 64], S1[STAGE * 64], S2[NB > 2 ? STAGE * 64 : 1], S3[NB > 3 ? STAGE * 64 : 1];
 
@@ -223,8 +233,11 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
+    // the next stage's fragments in registers, where they fit beside the sums (the
+    // largest tile holds 128 of these, and with several terms more fragments)
+    constexpr bool AHEAD = TB == 1 || MI * NJ < 32;
     constexpr int FLIGHT = PA + (HALF ? 0 : TB * PB);  // copies of a stage that every wave makes at least
-    u32x4 fa[AHEAD ? 2 : 1][MI], fb[AHEAD ? 2 : 1][NJ];
+    u32x4 fa[AHEAD ? 2 : 1][MI], fb[2][NJ];
     auto read_a = [&](const u32x4 *S, u32x4 (&a)[MI]) {
 #pragma unroll
         for (int i = 0; i < MI; i++) a[i] = rows_fragment<AO>(S, wm * MI + i, lane);
@@ -240,7 +253,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
             for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(a[i], b[j], acc[i][j]);
     };
     // every wave's copies but those of the last `later` stages have landed, and
-    // every wave is done with what it read before
+    // every wave has the fragments that it asked for
     auto meet = [&](bool all) {
         __builtin_amdgcn_sched_barrier(0);
         constexpr int later = NB - 2;
@@ -249,22 +262,47 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
+    constexpr int READS_A = (AO ? 2 : 1) * MI, READS_B = (BO ? 2 : 1) * NJ;
     if constexpr (AHEAD) {
-        // stage t: multiply the fragments in set t % 2; read t + 1's from its buffer; copy t + NB to t's
-        auto step = [&](int t, u32x4 *S, const u32x4 *N, auto set) {
-            constexpr int c = decltype(set)::value;
+        // stage t, its fragments of a and of b's first term in set t % 2: each
+        // further term of b is read while the one before is multiplied, and with the
+        // last product the next stage's first fragments, from its buffer, while the
+        // stage NB ahead is copied to this one's.
+        auto last = [&](int t, u32x4 *S, const u32x4 *N, const u32x4 (&a)[MI], const u32x4 (&b)[NJ], u32x4 (&an)[MI],
+                        u32x4 (&bn)[NJ]) {
             meet(t + NB > last_t);
             copy(S);
             __builtin_amdgcn_sched_barrier(0);
-            read_a(N, fa[c ^ 1]);  // (behind the last stage: whatever lies there, not used)
-            read_b(N, 0, fb[c ^ 1]);
-            products(fa[c], fb[c]);
-            // a read of the next stage after each product, while there are any
-            constexpr int READS = (AO ? 2 : 1) * MI + (BO ? 2 : 1) * NJ;
+            read_a(N, an);  // (behind the last stage: whatever lies there, not used)
+            read_b(N, 0, bn);
+            products(a, b);
+            rows_order<MI * NJ, READS_A + READS_B>();
+        };
+        auto step = [&](int t, u32x4 *S, const u32x4 *N, auto set) {
+            constexpr int c = decltype(set)::value;
+            if constexpr (TB == 1) {
+                last(t, S, N, fa[c], fb[c], fa[c ^ 1], fb[c ^ 1]);
+            } else {
+                const int count = p.count[cur];
+                cur = cur + 1 == nseg ? 0 : cur + 1;
+                if (count > 1) {
+                    u32x4 more[NJ];
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_b(S, 1, more);
+                    products(fa[c], fb[c]);
+                    rows_order<MI * NJ, READS_B>();
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (TB == 3 && count == 3) {
+                        read_b(S, TB - 1, fb[c]);
+                        products(fa[c], more);
+                        rows_order<MI * NJ, READS_B>();
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else {
 #pragma unroll
-            for (int i = 0; i < MI * NJ; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, READS > MI * NJ ? 2 : 1, 0);
+                        for (int j = 0; j < NJ; j++) fb[c][j] = more[j];
+                    }
+                }
+                last(t, S, N, fa[c], fb[c], fa[c ^ 1], fb[c ^ 1]);
             }
         };
         if (first_t < last_t) {
@@ -280,45 +318,58 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
             read_b(S0, 0, fb[0]);
             using Zero = std::integral_constant<int, 0>;
             using One = std::integral_constant<int, 1>;
-            static_assert(NB == 4, "a ring of four");
-            for (int t = first_t; t < last_t; t += 4) {
-                step(t, S0, S1, Zero{});
-                if (t + 1 < last_t) step(t + 1, S1, S2, One{});
-                if (t + 2 < last_t) step(t + 2, S2, S3, Zero{});
-                if (t + 3 < last_t) step(t + 3, S3, S0, One{});
+            for (int t = first_t; t < last_t; t += NB == 3 ? 6 : NB) {
+                if constexpr (NB == 2) {
+                    step(t, S0, S1, Zero{});
+                    if (t + 1 < last_t) step(t + 1, S1, S0, One{});
+                } else if constexpr (NB == 3) {
+                    step(t, S0, S1, Zero{});
+                    if (t + 1 < last_t) step(t + 1, S1, S2, One{});
+                    if (t + 2 < last_t) step(t + 2, S2, S0, Zero{});
+                    if (t + 3 < last_t) step(t + 3, S0, S1, One{});
+                    if (t + 4 < last_t) step(t + 4, S1, S2, Zero{});
+                    if (t + 5 < last_t) step(t + 5, S2, S0, One{});
+                } else {
+                    step(t, S0, S1, Zero{});
+                    if (t + 1 < last_t) step(t + 1, S1, S2, One{});
+                    if (t + 2 < last_t) step(t + 2, S2, S3, Zero{});
+                    if (t + 3 < last_t) step(t + 3, S3, S0, One{});
+                }
             }
         }
     } else {
-        // stage t: multiply from its buffer; copy t + NB - 1 to the one before
+        // stage t from its buffer, a further term of b read while the one before
+        // is multiplied; the stage NB - 1 ahead copied to the buffer of the one before
         auto step = [&](int t, const u32x4 *S, u32x4 *before) {
             meet(t + NB - 1 > last_t);
             copy(before);
             const int count = p.count[cur];
             cur = cur + 1 == nseg ? 0 : cur + 1;
+            __builtin_amdgcn_sched_barrier(0);
+            read_b(S, 0, fb[0]);
             read_a(S, fa[0]);
-#pragma unroll
-            for (int e = 0; e < TB; e++) {
-                if (e > 0 && e >= count) continue;
-                read_b(S, e, fb[0]);
-                products(fa[0], fb[0]);
+            read_b(S, 1, fb[1]);
+            products(fa[0], fb[0]);
+            if (count > 1) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (TB == 3) read_b(S, TB - 1, fb[0]);
+                products(fa[0], fb[1]);
+                rows_order<MI * NJ, TB == 3 ? READS_B : 0>();
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (TB == 3 && count == 3) products(fa[0], fb[0]);
         };
         copy(S0);
         if (NB > 2) copy(S1);
-        if (NB > 3) copy(S2);
         for (int t = first_t; t < last_t; t += NB) {
             if constexpr (NB == 2) {
                 step(t, S0, S1);
                 if (t + 1 < last_t) step(t + 1, S1, S0);
-            } else if constexpr (NB == 3) {
+            } else {
+                static_assert(NB <= 3, "no ring of four here");
                 step(t, S0, S2);
                 if (t + 1 < last_t) step(t + 1, S1, S0);
                 if (t + 2 < last_t) step(t + 2, S2, S1);
-            } else {
-                step(t, S0, S3);
-                if (t + 1 < last_t) step(t + 1, S1, S0);
-                if (t + 2 < last_t) step(t + 2, S2, S1);
-                if (t + 3 < last_t) step(t + 3, S3, S2);
             }
         }
     }
@@ -444,13 +495,13 @@ struct EpiRows {
 // ---------------------------------------------------------------------------
 // launches
 
-template <int WGM, int WGN, int MI, int NJ, bool AO, bool BO, int TB, typename Epi>
+template <int WGM, int WGN, int MI, int NJ, bool WHOLE, bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     const int64_t tm = ceil_div(mblocks, WGM * MI), tn = ceil_div(nblocks, WGN * NJ);
     DITCH_CHECK(tm * tn < (int64_t)1 << 31 && g.parts < 65536, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, AO, BO, TB, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
+    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, WHOLE, AO, BO, TB, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
                        dim3(WGM * WGN * 64), 0, s, g, epi);
     DITCH_TRY_HIP(hipGetLastError());
 }
@@ -459,11 +510,12 @@ void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const E
 template <bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     switch (tile) {
-    case 0: launch_rows_gemm_tile<2, 4, 8, 4, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
-    case 1: launch_rows_gemm_tile<2, 2, 4, 4, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
-    case 2: launch_rows_gemm_tile<4, 2, 4, 2, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
-    default: launch_rows_gemm_tile<2, 2, 2, 2, AO, BO, TB>(g, mblocks, nblocks, epi, s); break;
+    case 0: launch_rows_gemm_tile<2, 4, 8, 4, true, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
+    case 1: launch_rows_gemm_tile<2, 2, 4, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
+    case 2: launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
+    case 3: launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
     }
+    if constexpr (TB == 3) launch_rows_gemm_tile<4, 2, 4, 2, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
 }
 
 template <typename F>
