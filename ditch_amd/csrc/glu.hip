@@ -6,74 +6,9 @@
 // all that is written. Gradient: the same product again, its epilogue reads dy and
 // leaves dg = dy u act'(g) and du = dy act(g) as bf16 terms; then dx = dg Wg +
 // du Wu is one product over both pairs, and dWg = dg^T x, dWu = du^T x.
-#include "rows_gemm.h"
+#include "glu.h"
 
 namespace ditch {
-
-// act(g) and its derivative; the activations of ditch_hip_gatedActivation.
-template <int A>
-__device__ __forceinline__ void act_both(float g, float &y, float &dy) {
-    if constexpr (A == 0 || A == 5) {
-        constexpr float c = A == 0 ? 1.f : 1.702f;
-        const float s = __fdiv_rn(1.f, 1.f + expf(-c * g));
-        y = g * s;
-        dy = s * __builtin_fmaf(c * g, 1.f - s, 1.f);
-    } else if constexpr (A == 1) {
-        const float k = 0.7978845608028654f, g2 = g * g;
-        const float t = tanhf(k * __builtin_fmaf(0.044715f * g2, g, g));
-        y = 0.5f * g * (1.f + t);
-        dy = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * k * __builtin_fmaf(3.f * 0.044715f, g2, 1.f);
-    } else if constexpr (A == 2) {
-        const float c = 0.5f * (1.f + erff(g * 0.7071067811865476f));
-        y = g * c;
-        dy = __builtin_fmaf(g * 0.3989422804014327f, expf(-0.5f * g * g), c);
-    } else {
-        const float r = fmaxf(g, 0.f);
-        y = A == 3 ? r : r * r;
-        dy = A == 3 ? (g > 0.f ? 1.f : 0.f) : 2.f * r;
-        if (g != g) y = dy = g;
-    }
-}
-
-// Blocks 2i of m are gate rows, 2i + 1 the same up rows.
-struct EpiGlu {
-    void *out;
-    int64_t stride, n, rows;
-    int32_t dtype, wide;
-    uint32_t act;
-    template <int A, int MI, int NJ>
-    __device__ __forceinline__ void store(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
-            if (tok >= n) continue;
-#pragma unroll
-            for (int i = 0; i < MI; i += 2) {
-                const int64_t c = (int64_t)(mb + i) / 2 * 16 + 4 * (lane >> 4);
-                if (c >= rows) continue;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float y, dy;
-                    act_both<A>(acc[i][j][r], y, dy);
-                    v[r] = y * acc[i + 1][j][r];
-                }
-                put_row4(out, dtype, tok * stride + c, rows - c, wide, v);
-            }
-        }
-    }
-    template <int MI, int NJ>
-    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-        switch (act) {
-        case 0: store<0>(acc, mb, nb, lane); break;
-        case 1: store<1>(acc, mb, nb, lane); break;
-        case 2: store<2>(acc, mb, nb, lane); break;
-        case 3: store<3>(acc, mb, nb, lane); break;
-        case 4: store<4>(acc, mb, nb, lane); break;
-        default: store<5>(acc, mb, nb, lane); break;
-        }
-    }
-};
 
 template <int T>
 struct EpiGluGrad {
@@ -131,18 +66,19 @@ struct GluPlan {
     Planes x, dg, du;
     char *room[2] = {nullptr, nullptr};
     int64_t ld = 0;
-    int order = 1, tile = 0;
+    int order = 1, tile = 0, coded = 0;  // coded: the tile of rows_coded.h's product, 0: planes
     RowsTiling back;
     float *part = nullptr;
     size_t bytes = 0;
 };
-static GluPlan glu_plan(const TileView &w, int64_t n, int32_t dtype, bool grad, void *ws) {
+static GluPlan glu_plan(const TileView &w, const TileView &up, int64_t n, int32_t dtype, bool grad, void *ws) {
     GluPlan p;
     Carver c(ws);
     const int terms = row_terms(dtype);
     p.x = row_planes(n, w.cols, terms);
     p.x.p = c.take(p.x.bytes());
-    if (!weight_is_planes(w))
+    p.coded = grad || !rows_coded_pair(w, up) ? 0 : rows_coded_tile(w, 2 * ceil_div(w.rows, 16), p.x.groups, terms);
+    if (!weight_is_planes(w) && !p.coded)
         for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows).bytes());
     if (grad) {
         for (Planes *d : {&p.dg, &p.du}) {
@@ -155,16 +91,16 @@ static GluPlan glu_plan(const TileView &w, int64_t n, int32_t dtype, bool grad, 
         p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
     const int a = weight_terms(w), order = a > terms ? a : terms;
-    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, p.x.units, a, terms, order, 1, false).tile;
+    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, a, terms, order, 1, false).tile;
     p.bytes = c.at;
     return p;
 }
 
 size_t glu_rows_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype) {
-    return glu_plan(gate, n, dtype, false, nullptr).bytes;
+    return glu_plan(gate, up, n, dtype, false, nullptr).bytes;
 }
 size_t glu_rows_grad_workspace(const TileView &gate, const TileView &up, int64_t n, int32_t dtype, bool dw) {
-    return glu_plan(gate, n, dtype, true, nullptr).bytes;
+    return glu_plan(gate, up, n, dtype, true, nullptr).bytes;
 }
 
 static RowsGemm glu_gemm(const GluPlan &p, const Planes &wg, const Planes &wu) {
@@ -173,17 +109,30 @@ static RowsGemm glu_gemm(const GluPlan &p, const Planes &wg, const Planes &wu) {
     g.a.paired = 1;
     g.a.pair = wu.p - wg.p;
     g.b = rows_inner(p.x);
-    g.k32 = (int32_t)p.x.units;
+    g.k32 = (int32_t)ceil_div(wg.units, 2) * 2;
     rows_pairs(g, wg, p.x, wg.terms > p.x.terms ? wg.terms : p.x.terms);
     return g;
 }
 
 void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const TileView &gate, const TileView &up,
                      uint32_t act, void *ws, hipStream_t s) {
-    const GluPlan p = glu_plan(gate, n, dtype, false, ws);
+    const GluPlan p = glu_plan(gate, up, n, dtype, false, ws);
     launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
-    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
     const EpiGlu epi{out.p, out.stride, n, gate.rows, dtype, rows_wide(out.p, out.stride, dtype), act};
+    if (p.coded) {
+        RowsCoded c;
+        c.w[0] = gate;
+        c.w[1] = up;
+        c.paired = 1;
+        c.b = rows_inner(p.x);
+        c.x = p.x.p;
+        c.x_plane = p.x.plane_bytes();
+        c.blocks = (int32_t)ceil_div(gate.rows, 16);
+        c.stages = (int32_t)gate.units_k;
+        launch_glu_coded(p.coded, c, p.x.terms, 2 * c.blocks, p.x.groups, epi, s);
+        return;
+    }
+    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
     with_terms(p.x.terms, [&](auto terms) {
         launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
     });
@@ -198,7 +147,7 @@ static void fill_glu(const GluPlan &p, const RowsGemm &g, int32_t dtype, RowsArg
 
 void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
                           const TileView &gate, const TileView &up, uint32_t act, void *ws, hipStream_t s) {
-    const GluPlan p = glu_plan(gate, n, dtype, true, ws);
+    const GluPlan p = glu_plan(gate, up, n, dtype, true, ws);
     launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
     const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
     auto fill = p.x.terms == 1 ? fill_glu<1> : p.x.terms == 2 ? fill_glu<2> : fill_glu<3>;
@@ -214,17 +163,18 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         launch_rows_parts(p.back.tile, g, p.part, p.ld, n, gate.cols, false, s);
         launch_join_parts(dx.p, dtype, dx.stride, p.part, p.back.parts, n * p.ld, p.ld, n, gate.cols, s);
     }
-    const RowsArg dw[2] = {dgate, dup};
-    const Planes *d[2] = {&p.dg, &p.du};
-    for (int i = 0; i < 2; i++) {
-        if (!dw[i].p) continue;
-        RowsGemm g;
-        g.a = rows_outer(p.x);
-        g.b = rows_outer(*d[i]);
-        g.k32 = (int32_t)(p.x.groups / 2);
-        rows_pairs(g, p.x, *d[i], p.x.terms);
-        launch_rows_out(g, dw[i].p, dtype, dw[i].stride, gate.rows, gate.cols, s);
+    if (!dgate.p && !dup.p) return;
+    const Planes &d = dgate.p ? p.dg : p.du;
+    RowsGemm g;
+    g.a = rows_outer(p.x);
+    g.b = rows_outer(d);
+    if (dgate.p && dup.p) {
+        g.b.paired = 1;
+        g.b.pair = p.du.p - p.dg.p;
     }
+    g.k32 = (int32_t)(p.x.groups / 2);
+    rows_pairs(g, p.x, d, p.x.terms);
+    launch_rows_out(g, dgate.p ? dgate : dup, dgate.p ? dup : RowsArg{}, dtype, gate.rows, gate.cols, s);
 }
 
 }  // namespace ditch

@@ -1,12 +1,141 @@
 // head.h — what the head's losses (head.hip) and their gradients
 // (head_grad.hip) share: pieces of the vocabulary, the logits' product.
 #pragma once
-#include "rows_gemm.h"
+#include "rows_coded.h"
 
 namespace ditch {
 
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(__fmul_rn(x, 1.4426950408889634f)); }
 
+
+constexpr float LOWEST = -3.0e38f;  // in place of words that are not there
+
+// ---------------------------------------------------------------------------
+// what the forward products keep of their tiles (head.hip joins it)
+
+struct EpiLossStats {
+    float2 *part;  // [strip][npad]: maximum, sum
+    float *picked;  // [n]
+    const int32_t *targets;
+    int64_t npad, n;
+    int64_t rows, row0, strip0;  // rows of this piece, its first word, its first strip
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t strip = strip0 + mb / MI;
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+            float m = LOWEST;
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (v0 + i * 16 + r >= rows) acc[i][j][r] = -__builtin_inff();
+                    m = fmaxf(m, acc[i][j][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) sum += fast_exp(acc[i][j][r] - m);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (tok >= n) continue;
+            if (lane < 16) part[strip * npad + tok] = make_float2(m, sum);
+            const int64_t t = (int64_t)targets[tok] - row0 - v0;  // in this lane's words?
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (t == i * 16 + r && v0 + t < rows) picked[tok] = acc[i][j][r];
+        }
+    }
+};
+
+// phi(u) = u + e^-u - 1 for |u| <= 1/4: its series to u^7, off by 2^-27 of it
+__device__ __forceinline__ float phi_near(float u) {
+    float s = -1.f / 5040.f;
+    s = __builtin_fmaf(s, u, 1.f / 720.f);
+    s = __builtin_fmaf(s, u, -1.f / 120.f);
+    s = __builtin_fmaf(s, u, 1.f / 24.f);
+    s = __builtin_fmaf(s, u, -1.f / 6.f);
+    s = __builtin_fmaf(s, u, 0.5f);
+    return s * u * u;
+}
+
+// Of a strip: the base's maximum and sum, the trial's maximum and sum, the sum of
+// e^(l_base - m) phi(D) relative to m = the larger of the maxima (so that neither
+// e^l_base nor e^l_trial in it overflows), the sum of e^(l_base - its maximum) D.
+constexpr int KL_STATS = 6;
+// The blocks 2i of n are base rows, 2i + 1 the same trial rows.
+struct EpiKlStats {
+    float *part;  // [strip][npad][KL_STATS]
+    int64_t npad, n;
+    int64_t rows, strip0;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t strip = strip0 + mb / MI;
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+        const bool whole = (int64_t)(mb + MI) * 16 <= rows;
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+            const int64_t tok = (int64_t)(nb + j) / 2 * 16 + (lane & 15);
+            float mx[2] = {LOWEST, LOWEST}, sum[2] = {0.f, 0.f}, far = 0.f, near = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < MI; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        // (both at LOWEST: no weight and no difference)
+                        if (!whole && v0 + i * 16 + r >= rows) acc[i][j + h][r] = LOWEST;
+                        mx[h] = fmaxf(mx[h], acc[i][j + h][r]);
+                    }
+                mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 16));
+                mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 32));
+            }
+            const float m = fmaxf(mx[0], mx[1]), sb = fast_exp(mx[0] - m), st = fast_exp(mx[1] - m);
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float b = acc[i][j][r], t = acc[i][j + 1][r], u = b - t;
+                    const float w = fast_exp(b - mx[0]), x = fast_exp(t - mx[1]);
+                    sum[0] += w;
+                    sum[1] += x;
+                    far = __builtin_fmaf(w, u, far);
+                    const float wm = w * sb;
+                    near += fabsf(u) <= 0.25f ? wm * phi_near(u) : __builtin_fmaf(wm, u - 1.f, x * st);
+                }
+            float v[KL_STATS] = {mx[0], sum[0], mx[1], sum[1], near, far};
+#pragma unroll
+            for (int k = 0; k < KL_STATS; k++) {
+                if (k != 0 && k != 2) {
+                    v[k] += __shfl_xor(v[k], 16);
+                    v[k] += __shfl_xor(v[k], 32);
+                }
+            }
+            if (tok < n && lane < 16) {
+                float2 *o = (float2 *)(part + (strip * npad + tok) * KL_STATS);
+                o[0] = make_float2(v[0], v[1]);
+                o[1] = make_float2(v[2], v[3]);
+                o[2] = make_float2(v[4], v[5]);
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// products
+
+// head_coded.hip: the same on weights that are not planes (rows_coded.h)
+void launch_loss_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks, const EpiLossStats &epi,
+                       hipStream_t s);
+void launch_kl_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks, const EpiKlStats &epi,
+                     hipStream_t s);
 
 // Words of a piece: what is held for one (d, and the weight's planes where they
 // are decoded) stays within about 256 MB, the size of the last cache; pieces of
@@ -29,14 +158,29 @@ inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *sec
         g.b.paired = 1;
         g.b.pair = second->p - x.p;
     }
-    g.k32 = (int32_t)x.units;
+    g.k32 = (int32_t)ceil_div(wp.units, 2) * 2;
     rows_pairs(g, wp, x, order_of(wp.terms, x.terms));
     return g;
 }
 
 inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
     const int a = weight_terms(w);
-    return rows_tiling(ceil_div(rows, 16), nblocks, x.units, a, x.terms, order_of(a, x.terms), 1, false).tile;
+    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order_of(a, x.terms), 1, false).tile;
+}
+
+inline RowsCoded coded_product(const TileView &w, const Planes &x, const Planes *second) {
+    RowsCoded p;
+    p.w[0] = p.w[1] = w;
+    p.b = rows_inner(x);
+    if (second) {
+        p.b.paired = 1;
+        p.b.pair = second->p - x.p;
+    }
+    p.x = x.p;
+    p.x_plane = x.plane_bytes();
+    p.blocks = (int32_t)ceil_div(w.rows, 16);
+    p.stages = (int32_t)w.units_k;
+    return p;
 }
 
 }  // namespace ditch

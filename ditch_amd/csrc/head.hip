@@ -19,52 +19,8 @@
 
 namespace ditch {
 
-constexpr float LOWEST = -3.0e38f;  // in place of words that are not there
-
 // ---------------------------------------------------------------------------
 // cross entropy
-
-struct EpiLossStats {
-    float2 *part;  // [strip][npad]: maximum, sum
-    float *picked;  // [n]
-    const int32_t *targets;
-    int64_t npad, n;
-    int64_t rows, row0, strip0;  // rows of this piece, its first word, its first strip
-    template <int MI, int NJ>
-    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-        const int64_t strip = strip0 + mb / MI;
-        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
-            float m = LOWEST;
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if (v0 + i * 16 + r >= rows) acc[i][j][r] = -__builtin_inff();
-                    m = fmaxf(m, acc[i][j][r]);
-                }
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) sum += fast_exp(acc[i][j][r] - m);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (tok >= n) continue;
-            if (lane < 16) part[strip * npad + tok] = make_float2(m, sum);
-            const int64_t t = (int64_t)targets[tok] - row0 - v0;  // in this lane's words?
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (t == i * 16 + r && v0 + t < rows) picked[tok] = acc[i][j][r];
-        }
-    }
-};
 
 // Sums of strips, each relative to its own reference (a maximum), over a block of
 // 512: TOK rows, 512 / TOK slices of the strips each; row tid % TOK. The largest
@@ -138,79 +94,6 @@ static void with_join_rows(int64_t n, F &&f) {
 // ---------------------------------------------------------------------------
 // divergence
 
-// phi(u) = u + e^-u - 1 for |u| <= 1/4: its series to u^7, off by 2^-27 of it
-__device__ __forceinline__ float phi_near(float u) {
-    float s = -1.f / 5040.f;
-    s = __builtin_fmaf(s, u, 1.f / 720.f);
-    s = __builtin_fmaf(s, u, -1.f / 120.f);
-    s = __builtin_fmaf(s, u, 1.f / 24.f);
-    s = __builtin_fmaf(s, u, -1.f / 6.f);
-    s = __builtin_fmaf(s, u, 0.5f);
-    return s * u * u;
-}
-
-// Of a strip: the base's maximum and sum, the trial's maximum and sum, the sum of
-// e^(l_base - m) phi(D) relative to m = the larger of the maxima (so that neither
-// e^l_base nor e^l_trial in it overflows), the sum of e^(l_base - its maximum) D.
-constexpr int KL_STATS = 6;
-// The blocks 2i of n are base rows, 2i + 1 the same trial rows.
-struct EpiKlStats {
-    float *part;  // [strip][npad][KL_STATS]
-    int64_t npad, n;
-    int64_t rows, strip0;
-    template <int MI, int NJ>
-    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-        const int64_t strip = strip0 + mb / MI;
-        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
-        const bool whole = (int64_t)(mb + MI) * 16 <= rows;
-#pragma unroll
-        for (int j = 0; j < NJ; j += 2) {
-            const int64_t tok = (int64_t)(nb + j) / 2 * 16 + (lane & 15);
-            float mx[2] = {LOWEST, LOWEST}, sum[2] = {0.f, 0.f}, far = 0.f, near = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                for (int i = 0; i < MI; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        // (both at LOWEST: no weight and no difference)
-                        if (!whole && v0 + i * 16 + r >= rows) acc[i][j + h][r] = LOWEST;
-                        mx[h] = fmaxf(mx[h], acc[i][j + h][r]);
-                    }
-                mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 16));
-                mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 32));
-            }
-            const float m = fmaxf(mx[0], mx[1]), sb = fast_exp(mx[0] - m), st = fast_exp(mx[1] - m);
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float b = acc[i][j][r], t = acc[i][j + 1][r], u = b - t;
-                    const float w = fast_exp(b - mx[0]), x = fast_exp(t - mx[1]);
-                    sum[0] += w;
-                    sum[1] += x;
-                    far = __builtin_fmaf(w, u, far);
-                    const float wm = w * sb;
-                    near += fabsf(u) <= 0.25f ? wm * phi_near(u) : __builtin_fmaf(wm, u - 1.f, x * st);
-                }
-            float v[KL_STATS] = {mx[0], sum[0], mx[1], sum[1], near, far};
-#pragma unroll
-            for (int k = 0; k < KL_STATS; k++) {
-                if (k != 0 && k != 2) {
-                    v[k] += __shfl_xor(v[k], 16);
-                    v[k] += __shfl_xor(v[k], 32);
-                }
-            }
-            if (tok < n && lane < 16) {
-                float2 *o = (float2 *)(part + (strip * npad + tok) * KL_STATS);
-                o[0] = make_float2(v[0], v[1]);
-                o[1] = make_float2(v[2], v[3]);
-                o[2] = make_float2(v[4], v[5]);
-            }
-        }
-    }
-};
-
 template <int TOK>
 __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base, float *lse_trial, const float *part,
                                                       int64_t n, int64_t npad, int64_t strips) {
@@ -267,7 +150,7 @@ static int64_t strips_of(int64_t rows, int tile) {
 struct HeadPlan {
     Planes x[2];
     int64_t piece = 0, strips = 0, npad = 0, nblocks = 0;
-    int tile = 0;
+    int tile = 0, coded = 0;  // coded: the tile of rows_coded.h's product, 0: planes
     char *room = nullptr;
     char *part = nullptr;
     float *picked = nullptr;
@@ -282,9 +165,10 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
     }
     p.npad = ceil_div(n, 32) * 32;
     p.nblocks = p.x[0].groups * (kl ? 2 : 1);
-    const int64_t per = weight_row_bytes(w);
+    p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), p.nblocks, p.x[0].terms);
+    const int64_t per = p.coded ? 0 : weight_row_bytes(w);
     p.piece = per ? piece_rows(w.rows, per) : w.rows;
-    p.tile = logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks);
+    p.tile = p.coded ? p.coded : logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks);
     for (int64_t r = 0; r < w.rows; r += p.piece)
         p.strips += strips_of(w.rows - r < p.piece ? w.rows - r : p.piece, p.tile);
     p.part = c.take((size_t)p.strips * p.npad * (kl ? KL_STATS * sizeof(float) : sizeof(float2)));
@@ -308,8 +192,12 @@ void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t
     int64_t strip = 0;
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
-        const Planes wp = weight_planes(w, r, rows, p.room, s);
         const EpiLossStats epi{(float2 *)p.part, p.picked, targets, p.npad, n, rows, r, strip};
+        if (p.coded) {
+            launch_loss_coded(p.tile, coded_product(w, p.x[0], nullptr), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
+            break;
+        }
+        const Planes wp = weight_planes(w, r, rows, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
             launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], nullptr), wp.groups,
                                                                    p.nblocks, epi, s);
@@ -332,8 +220,12 @@ void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype,
     int64_t strip = 0;
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
-        const Planes wp = weight_planes(w, r, rows, p.room, s);
         const EpiKlStats epi{(float *)p.part, p.npad, n, rows, strip};
+        if (p.coded) {
+            launch_kl_coded(p.tile, coded_product(w, p.x[0], &p.x[1]), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
+            break;
+        }
+        const Planes wp = weight_planes(w, r, rows, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
             launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], &p.x[1]), wp.groups,
                                                                    p.nblocks, epi, s);

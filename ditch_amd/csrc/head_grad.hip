@@ -144,7 +144,8 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
             g.b = rows_outer(d);
             g.k32 = (int32_t)(d.groups / 2);
             rows_pairs(g, p.x[0], d, d.terms);
-            launch_rows_out(g, (char *)dw.p + r * dw.stride * (int64_t)row_size(dtype), dtype, dw.stride, rows, w.cols, s);
+            const RowsArg out{(char *)dw.p + r * dw.stride * (int64_t)row_size(dtype), dw.stride};
+            launch_rows_out(g, out, RowsArg{}, dtype, rows, w.cols, s);
         }
     }
     if (dx.p) launch_join_parts(dx.p, dtype, dx.stride, p.part, p.tiling.parts, n * p.ld, p.ld, n, w.cols, s);

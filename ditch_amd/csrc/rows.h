@@ -33,10 +33,10 @@ inline int row_terms(int32_t dtype) { return dtype == DITCH_BF16 ? 1 : dtype == 
 inline size_t row_size(int32_t dtype) { return dtype == DITCH_F32 ? 4 : 2; }
 int weight_terms(const TileView &w);
 
-// Rows of activations: whole stages of 64 in both directions, zeros behind the
-// last row and column.
+// Rows of activations: 64 rows and 128 columns (a unit of 4-bit codes), zeros
+// behind the last row and column.
 inline Planes row_planes(int64_t n, int64_t cols, int terms) {
-    return Planes{nullptr, ceil_div(n, 64) * 4, ceil_div(cols, 64) * 2, terms};
+    return Planes{nullptr, ceil_div(n, 64) * 4, ceil_div(cols, 128) * 4, terms};
 }
 void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
                       hipStream_t s);
@@ -82,16 +82,16 @@ inline int rows_pair_count(int a, int b, int order) {
 }
 
 // rows_products.hip: c as parts of sums [part][n][ld] (added where `add`), a outer
-// and b inner; and as rows of `dtype`, both outer
-struct RowsGemm;
-void launch_rows_parts(int tile, const RowsGemm &g, float *part, int64_t ld, int64_t n, int64_t m, bool add, hipStream_t s);
-void launch_rows_out(const RowsGemm &g, void *out, int32_t dtype, int64_t stride, int64_t n, int64_t m, hipStream_t s);
-
-// head.hip, head_grad.hip
+// and b inner; and as rows of `dtype`, both outer (b paired: of two outputs)
 struct RowsArg {
     void *p = nullptr;
     int64_t stride = 0;
 };
+struct RowsGemm;
+void launch_rows_parts(int tile, const RowsGemm &g, float *part, int64_t ld, int64_t n, int64_t m, bool add, hipStream_t s);
+void launch_rows_out(const RowsGemm &g, RowsArg out, RowsArg second, int32_t dtype, int64_t n, int64_t m, hipStream_t s);
+
+// head.hip, head_grad.hip
 size_t head_loss_workspace(const TileView &w, int64_t n, int32_t dtype);
 void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t n, const TileView &w,
                       const int32_t *targets, void *ws, hipStream_t s);

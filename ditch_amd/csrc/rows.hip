@@ -116,10 +116,10 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
         int bm, bn, fit[3];
         double one[3], all[3];
     } tiles[5] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.78, 1.50, 2.13}},
-                  {8, 8, {2, 2, 2}, {0.30, 0.49, 0.63}, {0.46, 0.77, 1.13}},
-                  {16, 4, {2, 2, 2}, {0.29, 0.47, 0.90}, {0.54, 0.79, 1.08}},
+                  {8, 8, {2, 2, 2}, {0.34, 0.59, 0.85}, {0.46, 0.77, 1.13}},
+                  {16, 4, {2, 2, 2}, {0.35, 0.55, 0.85}, {0.54, 0.79, 1.08}},
                   {4, 4, {4, 3, 2}, {0.19, 0.27, 0.31}, {0.40, 0.45, 0.47}},
-                  {16, 4, {1, 1, 1}, {9, 9, 0.60}, {9, 9, 0.72}}};
+                  {16, 4, {1, 1, 1}, {9, 9, 0.70}, {9, 9, 0.72}}};
     const int b = b_terms - 1;
     const double terms = (double)rows_pair_count(a_terms, b_terms, order) / b_terms * sets;  // stages a step
     // a is read once at least, 5.5 TB/s

@@ -34,7 +34,7 @@ struct RowsOperand {
     int64_t pair = 0;     // interleaved: bytes from the first planes to the second's
     int32_t blocks = 0;   // along the output: 16-row groups (inner), 32-column units (outer); of one of a pair
     int32_t ks = 0;       // along k: units (inner), groups (outer)
-    int32_t paired = 0;   // blocks 2i and 2i + 1 are block i of the first and of the second planes
+    int32_t paired = 0;   // blocks (units) 2i and 2i + 1 are block i of the first and of the second planes
 };
 
 struct RowsGemm {
@@ -134,9 +134,13 @@ struct RowsCopies {
         for (int j = 0; j < PER; j++) {
             const int l = wave * PER + j;
             if (OUTER) {
-                int u = first / 2 + l / 2;
+                int u = first / 2 + l / 2, second = 0;
+                if (o.paired) {
+                    second = u & 1;
+                    u >>= 1;
+                }
                 u = u < o.blocks ? u : o.blocks - 1;
-                off[j] = (int64_t)u * 1024;
+                off[j] = (int64_t)u * 1024 + (second ? o.pair : 0);
             } else {
                 int g = first + l, second = 0;
                 if (o.paired) {
@@ -469,24 +473,29 @@ inline bool rows_wide(const void *p, int64_t stride, int32_t dtype) {
     return ((uintptr_t)p | (uintptr_t)(stride * (int64_t)row_size(dtype))) % size == 0;
 }
 
-// out[n][m] as the caller's rows.
+// out[n][m] as the caller's rows; with a second output, the 32-row units 2i of n
+// are the first's unit i and 2i + 1 the second's.
 struct EpiRows {
-    void *out;
-    int64_t stride;
+    void *out, *second;
+    int64_t stride, second_stride;
     int64_t n, m;
     int32_t dtype, wide;
     template <int MI, int NJ>
     __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int64_t row = (int64_t)(nb + j) * 16 + (lane & 15);
+            const int block = nb + j;
+            const bool other = second && (block & 2);
+            const int64_t row = (int64_t)(second ? block >> 2 << 1 | (block & 1) : block) * 16 + (lane & 15);
             if (row >= n) continue;
+            void *to = other ? second : out;
+            const int64_t at = row * (other ? second_stride : stride);
 #pragma unroll
             for (int i = 0; i < MI; i++) {
                 const int64_t c = (int64_t)(mb + i) * 16 + 4 * (lane >> 4);
                 if (c >= m) continue;
                 const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                put_row4(out, dtype, row * stride + c, m - c, wide, v);
+                put_row4(to, dtype, at + c, m - c, wide, v);
             }
         }
     }

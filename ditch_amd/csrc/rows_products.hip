@@ -11,10 +11,11 @@ void launch_rows_parts(int tile, const RowsGemm &g, float *part, int64_t ld, int
     });
 }
 
-void launch_rows_out(const RowsGemm &g, void *out, int32_t dtype, int64_t stride, int64_t n, int64_t m, hipStream_t s) {
-    const int64_t mb = ceil_div(m, 16), nb = ceil_div(n, 16);
+void launch_rows_out(const RowsGemm &g, RowsArg out, RowsArg second, int32_t dtype, int64_t n, int64_t m, hipStream_t s) {
+    const int64_t mb = ceil_div(m, 16), nb = second.p ? 2 * ceil_div(ceil_div(n, 16), 2) * 2 : ceil_div(n, 16);
     const int tile = rows_tiling(mb, nb, g.k32, g.nseg, g.terms, g.count[0], 1, false).tile;
-    const EpiRows epi{out, stride, n, m, dtype, rows_wide(out, stride, dtype)};
+    const bool wide = rows_wide(out.p, out.stride, dtype) && (!second.p || rows_wide(second.p, second.stride, dtype));
+    const EpiRows epi{out.p, second.p, out.stride, second.stride, n, m, dtype, wide};
     with_terms(g.terms, [&](auto terms) {
         launch_rows_gemm<true, true, decltype(terms)::value>(tile, g, mb, nb, epi, s);
     });
