@@ -98,28 +98,27 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// Tiles of 256 x 256, 128 x 128, 256 x 64, 64 x 64, and 256 x 64 with the whole LDS
-// as its ring (three terms only: two stages of them fill half of it, and 224
+// Tiles of 256 x 256, 128 x 128, 256 x 64, 64 x 64, and 256 x 64 with the whole LDS as
+// its ring (three terms only: two stages of them fill half of it, and 224
 // workgroups on as many CUs then wait for memory, 147 us against 109; where there
-// are more than CUs two on each are better, 184 against 207): how many workgroups fit a CU
-// (by their LDS), and what 32 k of one, two or three terms of b take (us) where a
-// workgroup is alone on its CU and where as many as fit share it; measured over
-// products of 4864 to 151936 rows, 1 to 1000 columns, 896 and 4096 k, and within a
-// fifth of them. A round of workgroups begins and ends in about 4 us. The cheapest
-// by rounds over the chip's 256 CUs: large products take the largest tiles, where
-// the LDS feeds the matrix cores best (872 us for 128256 x 1000 x 4096, against 996,
-// 1143 and 1624), few columns the narrow ones (64 f32 columns: 179 us for 256 x 64,
-// 546 for 256 x 256), small ones whichever spreads over the chip.
+// are more than CUs two on each are better, 184 against 207). For each: how many workgroups fit a CU (by their LDS), and what 32 k of one, two or three terms of
+// b take (us) where a workgroup is alone on its CU and where as many as fit share it,
+// and what a round of workgroups takes to begin and end; measured over products of
+// 4864 to 151936 rows, 1 to 3000 columns, 896 to 4096 k, and within a fifth of them.
+// The cheapest by rounds over the chip's 256 CUs: large products take large tiles,
+// where the LDS feeds the matrix cores best (872 us for 128256 x 1000 x 4096 in 256 x
+// 256, 996 in 128 x 128, 1624 in 64 x 64), few columns the narrow ones (64 f32 columns:
+// 179 us for 256 x 64, 546 for 256 x 256), small ones whichever spreads over the chip.
 RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_terms, int b_terms, int order, int sets,
                        bool split) {
     static const struct {
         int bm, bn, fit[3];
-        double one[3], all[3];
-    } tiles[5] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.78, 1.50, 2.13}},
-                  {8, 8, {2, 2, 2}, {0.34, 0.59, 0.85}, {0.46, 0.77, 1.13}},
-                  {16, 4, {2, 2, 2}, {0.35, 0.55, 0.85}, {0.54, 0.79, 1.08}},
-                  {4, 4, {4, 3, 2}, {0.19, 0.27, 0.31}, {0.40, 0.45, 0.47}},
-                  {16, 4, {1, 1, 1}, {9, 9, 0.70}, {9, 9, 0.72}}};
+        double one[3], all[3], ends;
+    } tiles[5] = {{16, 16, {1, 1, 1}, {0.67, 1.25, 1.72}, {0.78, 1.50, 2.13}, 8},
+                  {8, 8, {2, 2, 2}, {0.34, 0.59, 0.85}, {0.46, 0.77, 1.13}, 4},
+                  {16, 4, {2, 2, 2}, {0.35, 0.55, 0.85}, {0.54, 0.79, 1.08}, 4},
+                  {4, 4, {4, 3, 2}, {0.19, 0.27, 0.31}, {0.40, 0.45, 0.47}, 4},
+                  {16, 4, {1, 1, 1}, {9, 9, 0.70}, {9, 9, 0.72}, 4}};
     const int b = b_terms - 1;
     const double terms = (double)rows_pair_count(a_terms, b_terms, order) / b_terms * sets;  // stages a step
     // a is read once at least, 5.5 TB/s
@@ -132,8 +131,8 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
         for (int64_t parts = 1; parts <= (split ? 64 : 1) && (parts == 1 || k32 / parts >= 8); parts++) {
             const int64_t wgs = tiles_mn * parts, full = 256 * fit, rest = wgs % full;
             const double stages = (double)ceil_div(k32, parts) * terms, share = tiles[t].all[b] / fit * ceil_div(rest, 256);
-            double us = (wgs / full) * (stages * tiles[t].all[b] + 4);
-            if (rest) us += stages * (share > tiles[t].one[b] ? share : tiles[t].one[b]) + 4;
+            double us = (wgs / full) * (stages * tiles[t].all[b] + tiles[t].ends);
+            if (rest) us += stages * (share > tiles[t].one[b] ? share : tiles[t].one[b]) + tiles[t].ends;
             // (256 workgroups, each with a stage or two on its way, reach three quarters of that, 512 nine tenths)
             const double read = memory * (1 + 90.0 / (wgs < 90 ? 90 : wgs));
             if (us < read) us = read + us / 100;

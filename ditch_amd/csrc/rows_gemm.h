@@ -524,6 +524,7 @@ void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblo
     case 2: launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
     case 3: launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
     }
+    if constexpr (TB == 1 && AO && BO) launch_rows_gemm_tile<2, 2, 8, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
     if constexpr (TB == 3) launch_rows_gemm_tile<4, 2, 4, 2, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
 }
 
