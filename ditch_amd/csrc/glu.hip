@@ -87,11 +87,11 @@ static GluPlan glu_plan(const TileView &w, const TileView &up, int64_t n, int32_
         }
         p.ld = ceil_div(w.cols, 4) * 4;
         p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
-        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, weight_terms(w), terms, p.order, 2, true);
+        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, weight_terms(w), terms, p.order, 2, true, false);
         p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
     const int a = weight_terms(w), order = a > terms ? a : terms;
-    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, a, terms, order, 1, false).tile;
+    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, a, terms, order, 1, false, true).tile;
     p.bytes = c.at;
     return p;
 }

@@ -165,7 +165,7 @@ inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *sec
 
 inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
     const int a = weight_terms(w);
-    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order_of(a, x.terms), 1, false).tile;
+    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order_of(a, x.terms), 1, false, true).tile;
 }
 
 inline RowsCoded coded_product(const TileView &w, const Planes &x, const Planes *second) {

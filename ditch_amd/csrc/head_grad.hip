@@ -105,7 +105,7 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     p.d.p = c.take(p.d.bytes());
     p.ld = ceil_div(w.cols, 4) * 4;
     p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
-    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, weight_terms(w), terms, p.order, 1, true);
+    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, weight_terms(w), terms, p.order, 1, true, false);
     p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
     if (weight_row_bytes(w)) p.room = c.take(weight_planes_shape(w, p.piece).bytes());
     p.bytes = c.at;

@@ -110,7 +110,7 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
 // 256, 996 in 128 x 128, 1624 in 64 x 64), few columns the narrow ones (64 f32 columns:
 // 179 us for 256 x 64, 546 for 256 x 256), small ones whichever spreads over the chip.
 RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_terms, int b_terms, int order, int sets,
-                       bool split) {
+                       bool split, bool inner) {
     static const struct {
         int bm, bn, fit[3];
         double one[3], all[3], ends;
@@ -125,7 +125,7 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
     const double memory = (double)mblocks * k32 * a_terms * sets * 1024 / 5.5e6;
     RowsTiling best;
     double least = 1e30;
-    for (int t = 0; t < 5; t++) {
+    for (int t = inner && b_terms == 3 ? 1 : 0; t < 5; t++) {  // (three terms: sums in two levels)
         const int64_t tiles_mn = ceil_div(mblocks, tiles[t].bm) * ceil_div(nblocks, tiles[t].bn);
         const int fit = tiles[t].fit[b];
         for (int64_t parts = 1; parts <= (split ? 64 : 1) && (parts == 1 || k32 / parts >= 8); parts++) {

@@ -236,6 +236,31 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
     for (int i = 0; i < MI; i++)
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // f32 rows' logits in two levels: a sum of some stages from zero, then one
+    // rounding of the whole. A logit of 10 over 896 k, 84 roundings of which each is
+    // of the size of the sum, is off by 3e-6 in one level (over 4096 k by 6e-6): more
+    // than the gradient of a divergence between near rows can have.
+    constexpr bool LEVELS = TB == 3 && !AO && !BO;
+    static_assert(!LEVELS || MI * NJ < 32, "no room for two sums in the largest tile");
+    floatx4 whole[LEVELS ? MI : 1][LEVELS ? NJ : 1];
+    auto lift = [&] {
+        if constexpr (LEVELS) {
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    whole[i][j] += acc[i][j];
+                    acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+    };
+    if constexpr (LEVELS) {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) whole[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    int rounds = 0;
 
     // the next stage's fragments in registers, where they fit beside the sums (the
     // largest tile holds 128 of these, and with several terms more fragments)
@@ -339,6 +364,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
                     if (t + 2 < last_t) step(t + 2, S2, S3, Zero{});
                     if (t + 3 < last_t) step(t + 3, S3, S0, One{});
                 }
+                if (LEVELS && (++rounds & (NB == 2 ? 3 : 1)) == 0) lift();
             }
         }
     } else {
@@ -377,7 +403,9 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
             }
         }
     }
-    epi(acc, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
+    lift();
+    if constexpr (LEVELS) epi(whole, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
+    else epi(acc, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -519,7 +547,11 @@ void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const E
 template <bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     switch (tile) {
-    case 0: launch_rows_gemm_tile<2, 4, 8, 4, true, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
+    case 0:
+        // (sums in two levels do not fit it)
+        if constexpr (TB == 3 && !AO && !BO) break;
+        else launch_rows_gemm_tile<2, 4, 8, 4, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+        return;
     case 1: launch_rows_gemm_tile<2, 2, 4, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
     case 2: launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
     case 3: launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
