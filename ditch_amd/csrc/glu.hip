@@ -74,24 +74,23 @@ struct GluPlan {
 static GluPlan glu_plan(const TileView &w, const TileView &up, int64_t n, int32_t dtype, bool grad, void *ws) {
     GluPlan p;
     Carver c(ws);
-    const int terms = row_terms(dtype);
+    const int terms = row_terms(dtype), wt = rows_weight_terms(w, terms);
+    p.order = rows_order_of(wt, terms);
     p.x = row_planes(n, w.cols, terms);
     p.x.p = c.take(p.x.bytes());
     p.coded = grad || !rows_coded_pair(w, up) ? 0 : rows_coded_tile(w, 2 * ceil_div(w.rows, 16), p.x.groups, terms);
     if (!weight_is_planes(w) && !p.coded)
-        for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows).bytes());
+        for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows, terms).bytes());
     if (grad) {
         for (Planes *d : {&p.dg, &p.du}) {
             *d = Planes{nullptr, p.x.groups, ceil_div(w.rows, 64) * 2, terms};
             d->p = c.take(d->bytes());
         }
         p.ld = ceil_div(w.cols, 4) * 4;
-        p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
-        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, weight_terms(w), terms, p.order, 2, true, false);
+        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, wt, terms, p.order, 2, true, false);
         p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
-    const int a = weight_terms(w), order = a > terms ? a : terms;
-    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, a, terms, order, 1, false, true).tile;
+    p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, wt, terms, p.order, 1, false, true).tile;
     p.bytes = c.at;
     return p;
 }
@@ -110,7 +109,7 @@ static RowsGemm glu_gemm(const GluPlan &p, const Planes &wg, const Planes &wu) {
     g.a.pair = wu.p - wg.p;
     g.b = rows_inner(p.x);
     g.k32 = (int32_t)ceil_div(wg.units, 2) * 2;
-    rows_pairs(g, wg, p.x, wg.terms > p.x.terms ? wg.terms : p.x.terms);
+    rows_pairs(g, wg, p.x, p.order);
     return g;
 }
 
@@ -132,7 +131,8 @@ void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const Til
         launch_glu_coded(p.coded, c, p.x.terms, 2 * c.blocks, p.x.groups, epi, s);
         return;
     }
-    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
+    const Planes wg = weight_planes(gate, 0, gate.rows, p.x.terms, p.room[0], s),
+                 wu = weight_planes(up, 0, up.rows, p.x.terms, p.room[1], s);
     with_terms(p.x.terms, [&](auto terms) {
         launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, glu_gemm(p, wg, wu), 2 * wg.groups, p.x.groups, epi, s);
     });
@@ -149,7 +149,8 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
                           const TileView &gate, const TileView &up, uint32_t act, void *ws, hipStream_t s) {
     const GluPlan p = glu_plan(gate, up, n, dtype, true, ws);
     launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
-    const Planes wg = weight_planes(gate, 0, gate.rows, p.room[0], s), wu = weight_planes(up, 0, up.rows, p.room[1], s);
+    const Planes wg = weight_planes(gate, 0, gate.rows, p.x.terms, p.room[0], s),
+                 wu = weight_planes(up, 0, up.rows, p.x.terms, p.room[1], s);
     auto fill = p.x.terms == 1 ? fill_glu<1> : p.x.terms == 2 ? fill_glu<2> : fill_glu<3>;
     fill(p, glu_gemm(p, wg, wu), dtype, dout, n, gate.rows, act, s);
     if (dx.p) {

@@ -146,10 +146,9 @@ inline int64_t piece_rows(int64_t vocab, int64_t per_row) {
     return ceil_div(ceil_div(vocab, pieces), 256) * 256;
 }
 
-inline int64_t weight_row_bytes(const TileView &w) {
-    return weight_is_planes(w) ? 0 : weight_planes_shape(w, 16).plane_bytes() * weight_terms(w) / 16;
+inline int64_t weight_row_bytes(const TileView &w, int x_terms) {
+    return weight_is_planes(w) ? 0 : (int64_t)weight_planes_shape(w, 16, x_terms).bytes() / 16;
 }
-inline int order_of(int a, int b) { return a > b ? a : b; }
 inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *second) {
     RowsGemm g;
     g.a = rows_inner(wp);
@@ -159,13 +158,13 @@ inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *sec
         g.b.pair = second->p - x.p;
     }
     g.k32 = (int32_t)ceil_div(wp.units, 2) * 2;
-    rows_pairs(g, wp, x, order_of(wp.terms, x.terms));
+    rows_pairs(g, wp, x, rows_order_of(wp.terms, x.terms));
     return g;
 }
 
 inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
-    const int a = weight_terms(w);
-    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order_of(a, x.terms), 1, false, true).tile;
+    const int a = rows_weight_terms(w, x.terms);
+    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, rows_order_of(a, x.terms), 1, false, true).tile;
 }
 
 inline RowsCoded coded_product(const TileView &w, const Planes &x, const Planes *second) {

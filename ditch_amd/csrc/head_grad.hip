@@ -99,15 +99,15 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
         p.x[i].p = c.take(p.x[i].bytes());
     }
     p.nblocks = p.x[0].groups;
-    p.piece = piece_rows(w.rows, p.nblocks * 32 * terms + weight_row_bytes(w));
+    p.piece = piece_rows(w.rows, p.nblocks * 32 * terms + weight_row_bytes(w, terms));
     if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;
     p.d = Planes{nullptr, p.nblocks, p.piece / 32, terms};
     p.d.p = c.take(p.d.bytes());
     p.ld = ceil_div(w.cols, 4) * 4;
-    p.order = terms > 1 || weight_terms(w) == 1 ? terms : 2;
-    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, weight_terms(w), terms, p.order, 1, true, false);
+    p.order = rows_order_of(rows_weight_terms(w, terms), terms);
+    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, rows_weight_terms(w, terms), terms, p.order, 1, true, false);
     p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
-    if (weight_row_bytes(w)) p.room = c.take(weight_planes_shape(w, p.piece).bytes());
+    if (weight_row_bytes(w, terms)) p.room = c.take(weight_planes_shape(w, p.piece, terms).bytes());
     p.bytes = c.at;
     return p;
 }
@@ -125,7 +125,7 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
                       hipStream_t s, Fill &&fill) {
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
-        const Planes wp = weight_planes(w, r, rows, p.room, s);
+        const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
         Planes d = p.d;
         d.units = ceil_div(rows, 64) * 2;
         fill(wp, d, r, rows);

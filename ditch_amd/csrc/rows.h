@@ -9,7 +9,7 @@
 // so the same planes serve x W^T, d W and d^T x. bf16 values are one term, f16
 // values exactly two, f32 values exactly three (each term the next 8 bits), FP8,
 // MXFP4 and INT4 weights one (what they decode to), f16 weights two, Q8_0 and
-// f32 weights three. A product of several terms adds the pairs i + j < order.
+// f32 weights three, or two beside 16-bit rows. A product of several terms adds the pairs i + j < order.
 #pragma once
 #include "gemm_common.h"
 #include "internal.h"
@@ -31,7 +31,12 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline int row_terms(int32_t dtype) { return dtype == DITCH_BF16 ? 1 : dtype == DITCH_F16 ? 2 : 3; }
 inline size_t row_size(int32_t dtype) { return dtype == DITCH_F32 ? 4 : 2; }
-int weight_terms(const TileView &w);
+// The terms of a weight that rows of x_terms take: all of them f32 rows, at most
+// two (16 bits, rounded) 16-bit ones, whose own rounding is far above what is left
+// out.
+int rows_weight_terms(const TileView &w, int x_terms);
+// and the pairs of terms that are multiplied: i + j < order
+inline int rows_order_of(int w_terms, int x_terms) { return w_terms > x_terms ? w_terms : x_terms; }
 
 // Rows of activations: 64 rows and 128 columns (a unit of 4-bit codes), zeros
 // behind the last row and column.
@@ -43,8 +48,8 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
 // The weight's rows [row0, row0 + rows) as planes: its own tiles where they are
 // that already (nothing launched), else decoded to `room` (row0 a multiple of 16).
 bool weight_is_planes(const TileView &w);
-Planes weight_planes_shape(const TileView &w, int64_t rows);
-Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, hipStream_t s);
+Planes weight_planes_shape(const TileView &w, int64_t rows, int x_terms);
+Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, int x_terms, char *room, hipStream_t s);
 
 // Scratch as one run of the caller's workspace.
 struct Carver {

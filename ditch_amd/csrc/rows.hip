@@ -7,12 +7,10 @@
 
 namespace ditch {
 
-int weight_terms(const TileView &w) {
-    switch (w.tf) {
-    case TF_F16: return 2;
-    case TF_F32: case TF_Q8: return 3;
-    default: return 1;
-    }
+int rows_weight_terms(const TileView &w, int x_terms) {
+    const int most = x_terms == 3 ? 3 : 2;
+    const int own = w.tf == TF_F16 ? 2 : w.tf == TF_F32 || w.tf == TF_Q8 ? 3 : 1;
+    return own < most ? own : most;
 }
 
 // v as terms: each but the last the next 8 bits of the remainder (cut, so that
@@ -150,9 +148,9 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
 
 bool weight_is_planes(const TileView &w) { return w.tf == TF_BF16; }
 
-Planes weight_planes_shape(const TileView &w, int64_t rows) {
+Planes weight_planes_shape(const TileView &w, int64_t rows, int x_terms) {
     if (weight_is_planes(w)) return Planes{nullptr, ceil_div(rows, 16), w.units_k, 1};
-    return Planes{nullptr, ceil_div(rows, 16), ceil_div(w.cols, 32), weight_terms(w)};
+    return Planes{nullptr, ceil_div(rows, 16), ceil_div(w.cols, 32), rows_weight_terms(w, x_terms)};
 }
 
 // The tiles' own words: a wave a unit of the weight (32 to 128 columns), each
@@ -160,9 +158,8 @@ Planes weight_planes_shape(const TileView &w, int64_t rows) {
 // INT4 by the conversions of the tiled products (tensors that these decode
 // exactly), f16, f32 and Q8_0 value by value. (An element at a time through
 // decode_any_kernel took 199 us for 14336 x 4096 in FP8.)
-template <int TF>
+template <int TF, int T>
 __global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView w, int64_t group0) {
-    constexpr int T = TF == TF_F16 ? 2 : TF == TF_F32 || TF == TF_Q8 ? 3 : 1;
     constexpr int TILES = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -230,21 +227,30 @@ __global__ __launch_bounds__(256) void decode_any_kernel(Planes out, TileView w,
     *(u32x4 *)(out.p + unit * 1024 + lane * 16) = o;
 }
 
-Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, char *room, hipStream_t s) {
-    Planes out = weight_planes_shape(w, rows);
+Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, int x_terms, char *room, hipStream_t s) {
+    Planes out = weight_planes_shape(w, rows, x_terms);
     if (weight_is_planes(w)) {
         out.p = (char *)w.codes + row0 / 16 * w.units_k * 1024;
         return out;
     }
     out.p = room;
     const dim3 grid((unsigned)ceil_div(out.groups * w.units_k, 4)), each((unsigned)ceil_div(out.groups * out.units, 4));
-    if (w.tf == TF_F16) hipLaunchKernelGGL(decode_planes_kernel<TF_F16>, grid, dim3(256), 0, s, out, w, row0 / 16);
-    else if (w.tf == TF_F32) hipLaunchKernelGGL(decode_planes_kernel<TF_F32>, grid, dim3(256), 0, s, out, w, row0 / 16);
-    else if (w.tf == TF_Q8) hipLaunchKernelGGL(decode_planes_kernel<TF_Q8>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    auto go = [&](auto tf, auto terms) {
+        hipLaunchKernelGGL((decode_planes_kernel<decltype(tf)::value, decltype(terms)::value>), grid, dim3(256), 0, s, out,
+                           w, row0 / 16);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Three = std::integral_constant<int, 3>;
+    if (w.tf == TF_F16) go(std::integral_constant<int, TF_F16>{}, Two{});
+    else if (w.tf == TF_F32 && out.terms == 2) go(std::integral_constant<int, TF_F32>{}, Two{});
+    else if (w.tf == TF_F32) go(std::integral_constant<int, TF_F32>{}, Three{});
+    else if (w.tf == TF_Q8 && out.terms == 2) go(std::integral_constant<int, TF_Q8>{}, Two{});
+    else if (w.tf == TF_Q8) go(std::integral_constant<int, TF_Q8>{}, Three{});
     else if (!w.fast) hipLaunchKernelGGL(decode_any_kernel, each, dim3(256), 0, s, out, w, row0);
-    else if (w.tf == TF_FP8) hipLaunchKernelGGL(decode_planes_kernel<TF_FP8>, grid, dim3(256), 0, s, out, w, row0 / 16);
-    else if (w.tf == TF_MX4) hipLaunchKernelGGL(decode_planes_kernel<TF_MX4>, grid, dim3(256), 0, s, out, w, row0 / 16);
-    else hipLaunchKernelGGL(decode_planes_kernel<TF_INT4>, grid, dim3(256), 0, s, out, w, row0 / 16);
+    else if (w.tf == TF_FP8) go(std::integral_constant<int, TF_FP8>{}, One{});
+    else if (w.tf == TF_MX4) go(std::integral_constant<int, TF_MX4>{}, One{});
+    else go(std::integral_constant<int, TF_INT4>{}, One{});
     DITCH_TRY_HIP(hipGetLastError());
     return out;
 }

@@ -50,10 +50,17 @@ __device__ __forceinline__ void rows_copy_words(const uint32_t *src, uint32_t to
 }
 
 // The next term of eight values as a fragment's words, and what it leaves: their
-// high halves, cut, which is exact (f32 values have three terms' bits, f16 and Q8_0
-// ones fewer). An infinite or NaN value leaves NaN.
+// high halves, cut (three of them hold all bits of f32 values, two of f16 ones), or
+// rounded to nearest where it is the last and more is left. An infinite or NaN
+// value leaves NaN.
+template <bool ROUND>
 __device__ __forceinline__ u32x4 coded_term(float (&v)[8]) {
     u32x4 w;
+    if constexpr (ROUND) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = cvt_pk_bf16(v[2 * j], v[2 * j + 1]);
+        return w;
+    }
 #pragma unroll
     for (int j = 0; j < 4; j++) w[j] = pack_hi(v[2 * j], v[2 * j + 1]);
 #pragma unroll
@@ -63,7 +70,8 @@ __device__ __forceinline__ u32x4 coded_term(float (&v)[8]) {
 
 template <int WGM, int WGN, int MI, int NJ, int TF, int TB, typename Epi>
 __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p, Epi epi) {
-    constexpr int TA = TF == TF_F16 ? 2 : TF == TF_F32 || TF == TF_Q8 ? 3 : 1;
+    constexpr int OWN = TF == TF_F16 ? 2 : TF == TF_F32 || TF == TF_Q8 ? 3 : 1;
+    constexpr int TA = TB == 3 || OWN < 2 ? OWN : 2;  // rows_weight_terms
     constexpr int KT = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
     constexpr int HALVES = TF == TF_F32 ? 2 : 1;
     constexpr int NS = TF == TF_INT4 ? 2 : TF == TF_F16 || TF == TF_F32 ? 0 : 1;
@@ -163,6 +171,26 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
+    // f32 rows' sums in two levels, as in rows_gemm.h
+    constexpr bool LEVELS = TB == 3;
+    floatx4 whole[LEVELS ? MI : 1][LEVELS ? NJ : 1];
+#pragma unroll
+    for (int i = 0; i < (LEVELS ? MI : 1); i++)
+#pragma unroll
+        for (int j = 0; j < (LEVELS ? NJ : 1); j++) whole[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto lift = [&] {
+        if constexpr (LEVELS) {
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    whole[i][j] += acc[i][j];
+                    acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+    };
+    int rounds = 0;
+
     constexpr int FLIGHT = PA + (HALF ? 0 : TB * PB);  // copies of a stage that every wave makes at least
     // stage t from its buffer; the stage NB - 1 ahead copied to the buffer of the one before
     auto step = [&](int t, const u32x4 *S, u32x4 *before) {
@@ -204,8 +232,10 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
                 u32x4 a[MI];
 #pragma unroll
                 for (int i = 0; i < MI; i++) {
-                    if constexpr (TA > 1) a[i] = coded_term(v[TA > 1 ? i : 0]);
-                    else a[i] = decode_tile_lds<TF>(p.w[0], c[i], sd[i], kt, true);
+                    if constexpr (TA > 1) {
+                        if (ta + 1 == TA && TA < OWN) a[i] = coded_term<true>(v[TA > 1 ? i : 0]);
+                        else a[i] = coded_term<false>(v[TA > 1 ? i : 0]);
+                    } else a[i] = decode_tile_lds<TF>(p.w[0], c[i], sd[i], kt, true);
                 }
 #pragma unroll
                 for (int e = 0; e < TB; e++) {
@@ -238,8 +268,11 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
             if (t + 2 < stages) step(t + 2, S2, S1);
             if (t + 3 < stages) step(t + 3, S3, S2);
         }
+        if (LEVELS && (KT > 1 || (++rounds & 1) == 0)) lift();
     }
-    epi(acc, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
+    lift();
+    if constexpr (LEVELS) epi(whole, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
+    else epi(acc, mt * UA + wm * MI, nt * UB + wn * NJ, lane);
 }
 
 template <int WGM, int WGN, int MI, int NJ, int TF, int TB, typename Epi>

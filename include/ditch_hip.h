@@ -886,8 +886,8 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
  * Rows are ditch_kv_rows of `dtype` (DITCH_F32, DITCH_F16 or DITCH_BF16), one
  * dtype a call. The weights are registered tensors of any format, taken at the
  * values they decode to. 16-bit rows are rounded once where they leave a call,
- * and once to as many bits between the two products of a gradient; f32 ones
- * are exact to about f32 rounding. `ws` is device scratch of the call's
+ * and once to as many bits between the two products of a gradient, and take f32
+ * and Q8_0 weights at 16 bits; f32 ones are exact to about f32 rounding. `ws` is device scratch of the call's
  * ..._workspace bytes (16-byte aligned; its contents do not matter, nothing is
  * kept in it, calls that overlap need one each); the sizes are 0 for arguments
  * that the call refuses. Outputs may not overlap inputs or each other. n = 0

@@ -4,8 +4,9 @@ what the kernels may be off by.
 Products: operands are sums of bf16 terms. Terms that are left out weigh at
 most 2^-13 of a product for 16-bit rows (the second of two times the second,
 each below 2^-7 of its value), 2^-19 for f32 ones (the second times the third
-and the third times the second, 2^-21 each). One of the two operands exact in a
-single term leaves out nothing. Sums are f32: a matrix instruction adds 32
+and the third times the second, 2^-21 each); beside 16-bit rows a weight has two
+terms at most, cut at 2^-7 and rounded at 2^-8, so that Q8_0 and f32 ones are off by
+2^-15 more. Where every pair is multiplied and the weight whole nothing is left out. Sums are f32: a matrix instruction adds 32
 products to a running sum and rounds once, by 2^-23 of what it has at most.
 Exponentials are the hardware's, 2^-22, of an argument rounded by 2^-24 twice.
 A value held as T terms between two products is off by 2^-8 (one), 2^-15 (two:
@@ -115,9 +116,10 @@ def _pairs(order, a, b):
 
 def product_off(size, k, dtype, fmt, order=None):
     """How far a product whose absolute terms sum to `size` may be off."""
-    a, b = TERMS[dtype], W_TERMS[fmt] if fmt in W_TERMS else int(fmt)
+    a, full = TERMS[dtype], W_TERMS[fmt] if fmt in W_TERMS else int(fmt)
+    b = full if a == 3 else min(full, 2)
     order = max(a, b) if order is None else order
-    left = 0 if _pairs(order, a, b) == a * b else LEFT_OUT[TERMS[dtype] if order < 3 else 3]
+    left = 0 if _pairs(order, a, b) == a * b and b == full else LEFT_OUT[a]
     return size * (left + (_pairs(order, a, b) * (k // 32 + 2) + 1) * 2.0 ** -23)
 
 
@@ -162,7 +164,7 @@ def _back(d, d_off, other, k, dtype, fmt, order):
 
 
 def _order(dtype, fmt):
-    return TERMS[dtype] if TERMS[dtype] > 1 or W_TERMS[fmt] == 1 else 2
+    return max(TERMS[dtype], W_TERMS[fmt] if dtype == "f32" else min(W_TERMS[fmt], 2))
 
 
 def loss_grad(x, w, targets, g, dtype, fmt):
