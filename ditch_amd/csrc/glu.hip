@@ -68,6 +68,7 @@ struct GluPlan {
     int64_t ld = 0;
     int order = 1, tile = 0, coded = 0;  // coded: the tile of rows_coded.h's product, 0: planes
     RowsTiling back;
+    int back_order = 1;  // of the product with d
     float *part = nullptr;
     size_t bytes = 0;
 };
@@ -82,12 +83,14 @@ static GluPlan glu_plan(const TileView &w, const TileView &up, int64_t n, int32_
     if (!weight_is_planes(w) && !p.coded)
         for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows, terms).bytes());
     if (grad) {
+        const int td = grad_term_count(terms, n);
+        p.back_order = rows_order_of(wt, td);
         for (Planes *d : {&p.dg, &p.du}) {
-            *d = Planes{nullptr, p.x.groups, ceil_div(w.rows, 64) * 2, terms};
+            *d = Planes{nullptr, p.x.groups, ceil_div(w.rows, 64) * 2, td};
             d->p = c.take(d->bytes());
         }
         p.ld = ceil_div(w.cols, 4) * 4;
-        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, wt, terms, p.order, 2, true, false);
+        p.back = rows_tiling(ceil_div(w.cols, 16), p.x.groups, p.dg.units, wt, td, p.back_order, 2, true, false);
         p.part = c.take<float>((size_t)p.back.parts * n * p.ld);
     }
     p.tile = rows_tiling(2 * ceil_div(w.rows, 16), p.x.groups, ceil_div(w.cols, 64) * 2, wt, terms, p.order, 1, false, true).tile;
@@ -138,11 +141,11 @@ void launch_glu_rows(int32_t dtype, RowsArg out, RowsArg x, int64_t n, const Til
     });
 }
 
-template <int T>
+template <int TB, int T>
 static void fill_glu(const GluPlan &p, const RowsGemm &g, int32_t dtype, RowsArg dout, int64_t n, int64_t rows,
                      uint32_t act, hipStream_t s) {
     const EpiGluGrad<T> epi{p.dg, p.du, dout.p, dout.stride, n, rows, dtype, act};
-    launch_rows_gemm<false, false, T>(p.tile, g, 4 * p.dg.units, p.x.groups, epi, s);
+    launch_rows_gemm<false, false, TB>(p.tile, g, 4 * p.dg.units, p.x.groups, epi, s);
 }
 
 void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup, RowsArg dout, RowsArg x, int64_t n,
@@ -151,7 +154,7 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
     launch_pack_rows(p.x, x.p, dtype, n, gate.cols, x.stride, s);
     const Planes wg = weight_planes(gate, 0, gate.rows, p.x.terms, p.room[0], s),
                  wu = weight_planes(up, 0, up.rows, p.x.terms, p.room[1], s);
-    auto fill = p.x.terms == 1 ? fill_glu<1> : p.x.terms == 2 ? fill_glu<2> : fill_glu<3>;
+    auto fill = p.x.terms == 3 ? fill_glu<3, 3> : p.x.terms == 2 ? fill_glu<2, 2> : p.dg.terms == 2 ? fill_glu<1, 2> : fill_glu<1, 1>;
     fill(p, glu_gemm(p, wg, wu), dtype, dout, n, gate.rows, act, s);
     if (dx.p) {
         RowsGemm g;
@@ -159,8 +162,8 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         g.b = rows_inner(p.dg);
         g.k32 = (int32_t)p.dg.units;
         g.parts = p.back.parts;
-        rows_pairs(g, wg, p.dg, p.order);
-        rows_pairs(g, wu, p.du, p.order);
+        rows_pairs(g, wg, p.dg, p.back_order);
+        rows_pairs(g, wu, p.du, p.back_order);
         launch_rows_parts(p.back.tile, g, p.part, p.ld, n, gate.cols, false, s);
         launch_join_parts(dx.p, dtype, dx.stride, p.part, p.back.parts, n * p.ld, p.ld, n, gate.cols, s);
     }
@@ -174,7 +177,7 @@ void launch_glu_rows_grad(int32_t dtype, RowsArg dx, RowsArg dgate, RowsArg dup,
         g.b.pair = p.du.p - p.dg.p;
     }
     g.k32 = (int32_t)(p.x.groups / 2);
-    rows_pairs(g, p.x, d, p.x.terms);
+    rows_pairs(g, p.x, d, d.terms);
     launch_rows_out(g, dgate.p ? dgate : dup, dgate.p ? dup : RowsArg{}, dtype, gate.rows, gate.cols, s);
 }
 

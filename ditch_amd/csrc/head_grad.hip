@@ -99,13 +99,14 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
         p.x[i].p = c.take(p.x[i].bytes());
     }
     p.nblocks = p.x[0].groups;
-    p.piece = piece_rows(w.rows, p.nblocks * 32 * terms + weight_row_bytes(w, terms));
+    const int td = grad_term_count(terms, n), wt = rows_weight_terms(w, terms);
+    p.piece = piece_rows(w.rows, p.nblocks * 32 * td + weight_row_bytes(w, terms));
     if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;
-    p.d = Planes{nullptr, p.nblocks, p.piece / 32, terms};
+    p.d = Planes{nullptr, p.nblocks, p.piece / 32, td};
     p.d.p = c.take(p.d.bytes());
     p.ld = ceil_div(w.cols, 4) * 4;
-    p.order = rows_order_of(rows_weight_terms(w, terms), terms);
-    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, rows_weight_terms(w, terms), terms, p.order, 1, true, false);
+    p.order = rows_order_of(wt, td);
+    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, wt, td, p.order, 1, true, false);
     p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
     if (weight_row_bytes(w, terms)) p.room = c.take(weight_planes_shape(w, p.piece, terms).bytes());
     p.bytes = c.at;
@@ -151,18 +152,18 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
     if (dx.p) launch_join_parts(dx.p, dtype, dx.stride, p.part, p.tiling.parts, n * p.ld, p.ld, n, w.cols, s);
 }
 
-template <int T>
+template <int TB, int T>
 static void fill_loss(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
                       int64_t rows, int64_t n, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
     const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, w.rows};
-    launch_rows_gemm<false, false, T>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, p.x[0], nullptr),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, p.x[0], nullptr),
                                       d.units * 2, p.nblocks, epi, s);
 }
-template <int T>
+template <int TB, int T>
 static void fill_kl(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t rows, int64_t n,
                     const float *lse_base, const float *lse_trial, const float *dkl, hipStream_t s) {
     const EpiKlGrad<T> epi{d, lse_base, lse_trial, dkl, n, rows};
-    launch_rows_gemm<false, false, T>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, p.x[0], &p.x[1]),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, p.x[0], &p.x[1]),
                                       d.units * 2, 2 * p.nblocks, epi, s);
 }
 
@@ -171,7 +172,7 @@ void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int
     const HeadGradPlan p = head_grad_plan(w, n, dtype, false, ws);
     launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);
     head_grad(p, dtype, dx, dw, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
-        auto f = p.d.terms == 1 ? fill_loss<1> : p.d.terms == 2 ? fill_loss<2> : fill_loss<3>;
+        auto f = p.x[0].terms == 3 ? fill_loss<3, 3> : p.x[0].terms == 2 ? fill_loss<2, 2> : p.d.terms == 2 ? fill_loss<1, 2> : fill_loss<1, 1>;
         f(p, w, wp, d, row0, rows, n, targets, lse, dloss, s);
     });
 }
@@ -182,7 +183,7 @@ void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial,
     launch_pack_rows(p.x[0], base.p, dtype, n, w.cols, base.stride, s);
     launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
     head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t, int64_t rows) {
-        auto f = p.d.terms == 1 ? fill_kl<1> : p.d.terms == 2 ? fill_kl<2> : fill_kl<3>;
+        auto f = p.x[0].terms == 3 ? fill_kl<3, 3> : p.x[0].terms == 2 ? fill_kl<2, 2> : p.d.terms == 2 ? fill_kl<1, 2> : fill_kl<1, 1>;
         f(p, w, wp, d, rows, n, lse_base, lse_trial, dkl, s);
     });
 }

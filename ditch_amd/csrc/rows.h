@@ -35,6 +35,11 @@ inline size_t row_size(int32_t dtype) { return dtype == DITCH_F32 ? 4 : 2; }
 // two (16 bits, rounded) 16-bit ones, whose own rounding is far above what is left
 // out.
 int rows_weight_terms(const TileView &w, int x_terms);
+// The terms that d, what a gradient's two products hand over, is held in: those of
+// the rows' type; bf16 rows up to 64 get a second one, which costs nothing while
+// the products wait for the weight (one value of d makes most of such a gradient,
+// and its rounding would be the gradient's).
+inline int grad_term_count(int x_terms, int64_t n) { return x_terms == 1 && n <= 64 ? 2 : x_terms; }
 // and the pairs of terms that are multiplied: i + j < order
 inline int rows_order_of(int w_terms, int x_terms) { return w_terms > x_terms ? w_terms : x_terms; }
 
