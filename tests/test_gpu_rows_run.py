@@ -1,0 +1,298 @@
+"""The head's losses, the gated block and their gradients as a program runs
+them: on a model's own hidden rows, on other streams, in graphs, with offsets
+past 32 bits."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import model_gen as mg
+import rows_ref as rr
+from ditch_amd import abi, hipmem
+from ditch_amd.hip import DeviceError, Model
+from ditch_amd.weights import HostWeight
+from test_gpu_head import _kl, _kl_grad, _loss, _loss_grad, _weight
+
+pytestmark = pytest.mark.gpu
+
+
+def _hidden(model, tokens, rows, want, prompts, max_len, width):
+    """The final hidden rows `want` of a batch, in device memory."""
+    bt, br = hipmem.Buffer.from_array(np.asarray(tokens, np.uint32)), hipmem.Buffer.from_array(np.asarray(rows, np.uint32))
+    bw, out = hipmem.Buffer.from_array(np.asarray(want, np.uint64)), hipmem.Buffer(len(want) * width * 4)
+    model.forward_hidden_device(bt.ptr, br.ptr, len(tokens), prompts, max_len, bw.ptr, len(want), out.ptr)
+    model.dev.sync()
+    return out
+
+
+@pytest.mark.parametrize("tie", [True, False])
+def test_a_trial_scored_and_its_gradient(dev, tie):
+    """A search's trial: the unedited model's final rows, an edit, the edited
+    model's; their divergence over the head against the one from kept logits,
+    the loss of the next tokens against their log-softmax, and gradients.
+
+    The forward's own logits come from two-term products, off by 2^-18 of their
+    absolute terms (four times that allowed); through a row's divergence that
+    goes by p |u - kl| and |q - p|, and by its square."""
+    spec = mg.dense(tie=tie, seed=5)
+    c = spec.config
+    model = Model(dev, spec)
+    try:
+        rng = np.random.default_rng(2)
+        lens = [9, 1, 14]
+        tokens = rng.integers(0, c["vocab"], sum(lens)).astype(np.uint32)
+        rows = [(b, p) for b, n in enumerate(lens) for p in range(n)]
+        n = len(rows)
+        head = model.head()
+        assert (head.rows, head.cols) == (c["vocab"], c["hidden"])
+        w = rr.from_rows(dev.dequant(spec.tensors[(-1, abi.SLOT["EMBED" if tie else "LM_HEAD"], -1)]), "f32")
+
+        def run():
+            out = _hidden(model, tokens, rows, range(n), len(lens), max(lens), c["hidden"])
+            x = rr.Rows(dev, n, c["hidden"], "f32", out.download(np.float32, (n, c["hidden"])))
+            return x, model.forward(tokens, rows, logit_rows=range(n))[1]
+
+        base, base_logits = run()
+        v = rng.standard_normal((1, c["hidden"]))
+        for layer in range(c["layers"]):
+            for slot in ("O", "DOWN"):
+                model.edit(layer, abi.SLOT[slot], -1, (v / np.linalg.norm(v)).astype(np.float32), 1.0)
+        trial, trial_logits = run()
+        got = _kl(dev, head, base, trial)
+        for k, (value, off) in rr.kl(base.values, trial.values, w, "f32", "bf16").items():
+            rr.check(got[k], value, off, k)
+        assert (got["kl"] > 1e-6).all()
+        kept = dev.klRows(dev.logSoftmaxRows(base_logits), trial_logits)
+        lb, lt = base.values @ w.T, trial.values @ w.T
+        p, q = (np.exp(l - rr._lse(l)[:, None]) for l in (lb, lt))
+        u = np.log(p) - np.log(q)
+        ob, ot = (2.0 ** -16 * np.abs(r.values) @ np.abs(w).T for r in (base, trial))
+        off = (p * np.abs(u - got["kl"][:, None]) * ob + np.abs(q - p) * ot + (p + q) * (ob + ot) ** 2).sum(1)
+        # (the f32 log-probabilities of the kept form: 2^-24 of each, p times)
+        off += (p * np.abs(np.log(p))).sum(1) * 2.0 ** -23 + rr.kl(base.values, trial.values, w, "f32", "bf16")["kl"][1]
+        assert (np.abs(kept - got["kl"]) <= off).all()
+        # the loss of each prompt's next token; the last rows have none
+        targets = np.array([tokens[i + 1] if i + 1 < n and rows[i + 1][0] == rows[i][0] else -100 for i in range(n)], np.int32)
+        loss = _loss(dev, head, trial, targets)
+        for k, (value, off) in rr.loss(trial.values, w, targets, "f32", "bf16").items():
+            rr.check(loss[k], value, off, k)
+        live = targets >= 0
+        kept = -dev.logSoftmaxRows(trial_logits)[np.arange(n)[live], targets[live]]
+        assert (np.abs(kept - loss["loss"][live]) <= 2 * ot.max(1)[live] + 2.0 ** -20 * np.abs(kept)).all()
+        g = np.full(n, 1 / live.sum(), np.float32)
+        grads = _loss_grad(dev, head, trial, targets, loss["lse"], g, c["vocab"], c["hidden"])
+        for k, (value, off) in rr.loss_grad(trial.values, w, targets, g.astype(np.float64), "f32", "bf16").items():
+            rr.check(grads[k], value, off, k)
+        value, off = rr.kl_grad(base.values, trial.values, w, g.astype(np.float64), "f32", "bf16")["dx"]
+        rr.check(_kl_grad(dev, head, base, trial, got, g), value, off, "dx")
+    finally:
+        model.free()
+
+
+def test_an_edited_head_is_refused(dev):
+    spec = mg.dense(tie=False, layers=1, seed=1)
+    c = spec.config
+    model = Model(dev, spec)
+    try:
+        model.head()
+        model.set_delta(-1, abi.SLOT["LM_HEAD"], -1, np.ones((1, c["hidden"])), np.ones((c["vocab"], 1)))
+        with pytest.raises(DeviceError, match="delta"):
+            model.head()
+        buf = hipmem.Buffer(4096)
+        with pytest.raises(DeviceError):
+            model.forward_hidden_device(buf.ptr, buf.ptr, 4, 1, 4, buf.ptr, 2, buf.ptr, hidden_bytes=2 * c["hidden"] * 4 - 1)
+        with pytest.raises(DeviceError):
+            model.forward_hidden_device(buf.ptr, buf.ptr, 4, 1, 4, None, 2, buf.ptr)
+    finally:
+        model.free()
+
+
+class Step:
+    """Everything of a training step of a head and a block on fixed buffers: loss and gradient, divergence and
+    gradient, block and gradient, on one stream."""
+
+    def __init__(self, dev, head, gate, up, dtype, n, hidden, seed, share=None):
+        rng = np.random.default_rng(seed)
+        self.dev, self.head, self.gate, self.up, self.dtype, self.n = dev, head, gate, up, dtype, n
+        inter, vocab = gate.rows, head.rows
+        self.x, self.y, self.dout = (rr.Rows(dev, n, k, dtype, rng.standard_normal((n, k))) for k in (hidden, hidden, inter))
+        self.targets = hipmem.Buffer.from_array(rng.integers(-1, vocab, n).astype(np.int32))
+        self.g = rr.Floats(n, rng.standard_normal(n).astype(np.float32))
+        self.f = {k: rr.Floats(n) for k in ("loss", "lse", "kl", "lse_base", "lse_trial")}
+        self.r = {"dx": rr.Rows(dev, n, hidden, dtype), "dw": rr.Rows(dev, vocab, hidden, dtype),
+                  "dt": rr.Rows(dev, n, hidden, dtype), "out": rr.Rows(dev, n, inter, dtype),
+                  "dh": rr.Rows(dev, n, hidden, dtype), "dgate": rr.Rows(dev, inter, hidden, dtype),
+                  "dup": rr.Rows(dev, inter, hidden, dtype)}
+        # one scratch for all of them: they follow each other
+        self.ws = share or rr.Workspace(max(
+            head.head_loss_workspace(n, dtype), head.head_loss_grad_workspace(n, dtype), head.head_kl_workspace(n, dtype),
+            head.head_kl_grad_workspace(n, dtype), gate.glu_rows_workspace(up, n, dtype),
+            gate.glu_rows_grad_workspace(up, n, dtype)))
+
+    def renew(self, rng):
+        for r in (self.x, self.y, self.dout):
+            raw = r.buf.download(rr.STORE[self.dtype], (r.size,))
+            raw[:r.n * r.stride] = rr.to_rows(rng.standard_normal((r.n, r.stride)), self.dtype)[0].reshape(-1)
+            r.buf.upload(raw)
+        self.targets.upload(rng.integers(-1, self.head.rows, self.n).astype(np.int32))
+
+    def run(self, stream=None):
+        h, f, r, n, ws, t = self.head, self.f, self.r, self.n, self.ws.args, self.dtype
+        h.head_loss(t, f["loss"].ptr, f["lse"].ptr, self.x.desc, n, self.targets.ptr, *ws, stream=stream)
+        h.head_loss_grad(t, r["dx"].desc, r["dw"].desc, self.x.desc, n, self.targets.ptr, f["lse"].ptr, self.g.ptr, *ws,
+                         stream=stream)
+        h.head_kl(t, f["kl"].ptr, f["lse_base"].ptr, f["lse_trial"].ptr, self.x.desc, self.y.desc, n, *ws, stream=stream)
+        h.head_kl_grad(t, r["dt"].desc, self.x.desc, self.y.desc, n, f["lse_base"].ptr, f["lse_trial"].ptr, self.g.ptr,
+                       *ws, stream=stream)
+        self.gate.glu_rows(self.up, t, r["out"].desc, self.x.desc, n, *ws, stream=stream)
+        self.gate.glu_rows_grad(self.up, t, r["dh"].desc, r["dgate"].desc, r["dup"].desc, self.dout.desc, self.x.desc, n,
+                                *ws, stream=stream)
+
+    def get(self):
+        return {k: v.get() for k, v in {**self.f, **self.r}.items()}
+
+
+def _same(a, b):
+    for k in a:
+        np.testing.assert_array_equal(a[k], b[k], err_msg=k)
+
+
+@pytest.mark.parametrize("dtype,fmt,n", [("bf16", "bf16", 70), ("f32", "fp8", 20), ("f16", "f32", 300)])
+def test_steps_on_two_streams_at_once(dev, dtype, fmt, n):
+    """Two steps queued on two streams, each with its own scratch, give what they give one after the other."""
+    lib = hipmem.hip()
+    (head, _), (gate, _), (up, _) = (_weight(dev, fmt, r, 256, i) for i, r in enumerate((1100, 300, 300)))
+    streams = [ctypes.c_void_p() for _ in range(2)]
+    for s in streams:
+        assert lib.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+    try:
+        steps = [Step(dev, head, gate, up, dtype, n + i, 256, i) for i in range(2)]
+        want = []
+        for s in steps:
+            s.run()
+            dev.sync()
+            want.append(s.get())
+        for _ in range(3):
+            for s, st in zip(steps, streams):
+                s.run(st.value)
+            for st in streams:
+                assert lib.hipStreamSynchronize(st) == 0
+            for s, w in zip(steps, want):
+                _same(s.get(), w)
+                s.ws.check()
+    finally:
+        for st in streams:
+            lib.hipStreamDestroy(st)
+        for t in (head, gate, up):
+            t.free()
+
+
+@pytest.mark.parametrize("dtype,fmt,n", [("bf16", "bf16", 5), ("f32", "bf16", 150), ("f16", "fp8", 40)])
+def test_steps_replayed_from_graphs(dev, dtype, fmt, n):
+    """Two steps captured into two graphs that share one scratch, replayed in turn on one stream with new rows and
+    eager calls between the replays: every replay is the eager step on the same rows."""
+    lib = hipmem.hip()
+    P = ctypes.c_void_p
+    for name, args in {"hipStreamBeginCapture": [P, ctypes.c_int], "hipStreamEndCapture": [P, ctypes.POINTER(P)],
+                       "hipGraphInstantiate": [ctypes.POINTER(P), P, P, P, ctypes.c_size_t],
+                       "hipGraphLaunch": [P, P], "hipGraphExecDestroy": [P], "hipGraphDestroy": [P]}.items():
+        getattr(lib, name).argtypes = args
+        getattr(lib, name).restype = ctypes.c_int
+    (head, _), (gate, _), (up, _) = (_weight(dev, fmt, r, 192, i) for i, r in enumerate((900, 260, 260)))
+    stream, graphs, exes = P(), [P(), P()], [P(), P()]
+    assert lib.hipStreamCreateWithFlags(ctypes.byref(stream), 1) == 0
+    try:
+        first = Step(dev, head, gate, up, dtype, n + 3, 192, 1)
+        steps = [first, Step(dev, head, gate, up, dtype, n, 192, 2, share=first.ws)]
+        hipmem.synchronize()
+        for s, g, e in zip(steps, graphs, exes):
+            assert lib.hipStreamBeginCapture(stream, 0) == 0
+            s.run(stream.value)
+            assert lib.hipStreamEndCapture(stream, ctypes.byref(g)) == 0
+            assert lib.hipGraphInstantiate(ctypes.byref(e), g, None, None, 0) == 0
+        rng = np.random.default_rng(3)
+        for _ in range(4):
+            for s in steps:
+                s.renew(rng)
+            hipmem.synchronize()
+            for e in exes:
+                assert lib.hipGraphLaunch(e, stream) == 0
+            assert lib.hipStreamSynchronize(stream) == 0
+            got = [s.get() for s in steps]
+            for s, g in zip(steps, got):
+                s.run()
+                dev.sync()
+                _same(g, s.get())
+    finally:
+        for e in exes:
+            if e.value:
+                lib.hipGraphExecDestroy(e)
+        for g in graphs:
+            if g.value:
+                lib.hipGraphDestroy(g)
+        lib.hipStreamDestroy(stream)
+        for t in (head, gate, up):
+            t.free()
+
+
+def test_rows_far_apart(dev):
+    """Two bf16 rows 2^31 + 64 elements apart."""
+    hidden, vocab, stride = 48, 300, 2 ** 31 + 64
+    t, w = _weight(dev, "bf16", vocab, hidden, 3)
+    lib = hipmem.hip()
+    try:
+        rng = np.random.default_rng(1)
+        stored, values = rr.to_rows(rng.standard_normal((2, hidden)), "bf16")
+        buf = hipmem.Buffer((stride + hidden) * 2)
+        for i in range(2):
+            hipmem.check(lib.hipMemcpy(ctypes.c_void_p(buf.ptr.value + i * stride * 2), stored[i].ctypes.data_as(ctypes.c_void_p),
+                                       hidden * 2, hipmem.H2D), "hipMemcpy")
+        x = rr.Rows(dev, 2, hidden, "bf16")
+        x.desc = dev.kv_rows(buf.ptr, (stride + hidden) * 2, stride)
+        targets = np.array([7, 299], np.int32)
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(values, w, targets, "bf16", "bf16").items():
+            rr.check(got[k], v, off, k)
+    finally:
+        t.free()
+
+
+def test_a_weight_gradient_past_32_bits(dev):
+    """dW of 262400 x 4096 f32: 4.3 GB, its last rows past 2^32 bytes (MXFP4 weights, in many pieces). lse is an input
+    here: any number."""
+    vocab, hidden, n, lse = 262400, 4096, 3, 9.0
+    rng = np.random.default_rng(7)
+    host = HostWeight.mxfp4(rng.integers(0, 256, (vocab, hidden // 2), dtype=np.uint8),
+                            rng.integers(118, 121, (vocab, hidden // 32), dtype=np.uint8))
+    t = dev.upload(host)
+    try:
+        x = rr.Rows(dev, n, hidden, "f32", rng.standard_normal((n, hidden)) * 0.3)
+        targets = hipmem.Buffer.from_array(np.array([vocab - 1, 5, -1], np.int32))
+        g = np.array([1.0, -2.0, 1.0], np.float32)
+        dw = hipmem.Buffer(vocab * hidden * 4)
+        ws = rr.Workspace(t.head_loss_grad_workspace(n, "f32"))
+        d_lse, d_g = rr.Floats(n, np.full(n, lse, np.float32)), rr.Floats(n, g)
+        t.head_loss_grad("f32", None, dev.kv_rows(dw.ptr, vocab * hidden * 4, hidden), x.desc, n, targets.ptr, d_lse.ptr,
+                         d_g.ptr, *ws.args)
+        hipmem.synchronize()
+        ws.check()
+        for first in (0, 131072, 262144 - 8, vocab - 16):
+            w = rr.from_rows(dev.dequant(host, first, 16), "bf16")
+            l, off = rr.logits(x.values, w, "f32", "mxfp4")
+            p = np.exp(l - lse)
+            one = np.zeros_like(p)
+            for i, v in enumerate((vocab - 1, 5)):
+                if first <= v < first + 16:
+                    one[i, v - first] = 1
+            weight = np.array([1.0, -2.0, 0.0])
+            d = (p - one) * weight[:, None]
+            d_off = p * (off + 2.0 ** -21 + np.abs(l - lse) * 2.0 ** -22) * np.abs(weight)[:, None] + np.abs(d) * 2.0 ** -21
+            got = np.empty((16, hidden), np.float32)
+            hipmem.check(hipmem.hip().hipMemcpy(got.ctypes.data_as(ctypes.c_void_p),
+                                                ctypes.c_void_p(dw.ptr.value + first * hidden * 4), got.nbytes,
+                                                hipmem.D2H), "hipMemcpy")
+            want = d.T @ x.values
+            size = np.abs(d).T @ np.abs(x.values)
+            rr.check(got, want, d_off.T @ np.abs(x.values) + size * 2.0 ** -18, f"rows from {first}")
+    finally:
+        t.free()
