@@ -45,7 +45,8 @@ EXTRA = {"gemm_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disab
          "gemm_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"],
          "gemm_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          **{f: ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disable-machine-sink"]
-            for f in ("head.hip", "head_coded.hip", "head_grad.hip", "glu.hip", "glu_coded.hip", "rows_products.hip")},
+            for f in ("head.hip", "head_coded.hip", "head_grad.hip", "glu.hip", "glu_coded.hip", "rows_products.hip",
+                      "rows_coded_parts.hip")},
          "pages_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "pages_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
@@ -55,7 +56,9 @@ EXTRA = {"gemm_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-disab
 # with those kernels, plus one with the dispatch; they compile in parallel)
 VARIANTS = {"gemv.hip": [("gemv", [])] + [(f"gemv_tf{tf}_x{xt}", [f"-DGEMV_TF={tf}", f"-DGEMV_XT={xt}"])
                                            for tf in range(7) for xt in (2, 3) if xt == 2 or tf not in (1, 2)],
-            "head_coded.hip": [("head_coded", []), ("head_coded_kl", ["-DCODED_KL"])]}
+            "head_coded.hip": [(f"head_coded_{name}", [f"-DCODED={i}"])
+                               for i, name in enumerate(("loss", "kl", "loss_grad", "kl_grad"))],
+            "glu_coded.hip": [("glu_coded", []), ("glu_coded_grad", ["-DCODED_GRAD"])]}
 
 
 def sources():

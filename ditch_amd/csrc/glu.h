@@ -70,7 +70,62 @@ struct EpiGlu {
     }
 };
 
+// dg and du of the block as terms.
+template <int T>
+struct EpiGluGrad {
+    Planes dg, du;
+    const void *dout;
+    int64_t stride, n, rows;
+    int32_t dtype;
+    uint32_t act;
+    __device__ __forceinline__ float dout_at(int64_t i) const {
+        if (dtype == DITCH_F32) return ((const float *)dout)[i];
+        const uint16_t b = ((const uint16_t *)dout)[i];
+        return dtype == DITCH_F16 ? f16_to_f32_hw(b) : bf16_to_f32(b);
+    }
+    template <int A, int MI, int NJ>
+    __device__ __forceinline__ void store(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (nb + j >= dg.groups) continue;
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < MI; i += 2) {
+                const int wb = (mb + i) / 2;
+                if ((wb >> 1) >= dg.units) continue;
+                const int64_t c = (int64_t)wb * 16 + 4 * (lane >> 4);
+                float a[4], b[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float y, dy;
+                    act_both<A>(acc[i][j][r], y, dy);
+                    const bool in = tok < n && c + r < rows;
+                    const float d = in ? dout_at(tok * stride + c + r) : 0.f;
+                    a[r] = in ? d * acc[i + 1][j][r] * dy : 0.f;
+                    b[r] = in ? d * y : 0.f;
+                }
+                put_grad_terms<T>(dg, wb, nb + j, lane, a);
+                put_grad_terms<T>(du, wb, nb + j, lane, b);
+            }
+        }
+    }
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        switch (act) {
+        case 0: store<0>(acc, mb, nb, lane); break;
+        case 1: store<1>(acc, mb, nb, lane); break;
+        case 2: store<2>(acc, mb, nb, lane); break;
+        case 3: store<3>(acc, mb, nb, lane); break;
+        case 4: store<4>(acc, mb, nb, lane); break;
+        default: store<5>(acc, mb, nb, lane); break;
+        }
+    }
+};
+
 void launch_glu_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks, const EpiGlu &epi,
                       hipStream_t s);
+template <int T>
+void launch_glu_grad_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks,
+                           const EpiGluGrad<T> &epi, hipStream_t s);
 
 }  // namespace ditch

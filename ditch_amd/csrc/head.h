@@ -129,6 +129,83 @@ struct EpiKlStats {
 };
 
 // ---------------------------------------------------------------------------
+// what the gradients' products leave of theirs (head_grad.hip)
+
+// d of a piece as terms. Rows without a target give zeros, targets past the
+// vocabulary NaN.
+template <int T>
+struct EpiLossGrad {
+    Planes d;
+    const int32_t *targets;
+    const float *lse, *dloss;
+    int64_t n, rows, row0, vocab;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (nb + j >= d.groups) continue;
+            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
+            float g = 0.f, l = 0.f;
+            int64_t t = -1;
+            bool live = false;
+            if (tok < n) {
+                const int32_t tt = targets[tok];
+                live = tt >= 0;
+                l = lse[tok];
+                g = tt >= vocab ? __builtin_nanf("") : dloss[tok];
+                t = (int64_t)tt - row0 - v0;
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                if (((mb + i) >> 1) >= d.units) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = fast_exp(acc[i][j][r] - l) - (t == i * 16 + r ? 1.f : 0.f);
+                    v[r] = live && v0 + i * 16 + r < rows ? __fmul_rn(g, p) : 0.f;
+                }
+                put_grad_terms<T>(d, mb + i, nb + j, lane, v);
+            }
+        }
+    }
+};
+
+template <int T>
+struct EpiKlGrad {
+    Planes d;
+    const float *lse_base, *lse_trial, *dkl;
+    int64_t n, rows;
+    template <int MI, int NJ>
+    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
+        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+            const int tb = (nb + j) / 2;
+            if (tb >= d.groups) continue;
+            const int64_t tok = (int64_t)tb * 16 + (lane & 15);
+            float g = 0.f, lb = 0.f, lt = 0.f;
+            if (tok < n) {
+                g = dkl[tok];
+                lb = lse_base[tok];
+                lt = lse_trial[tok];
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                if (((mb + i) >> 1) >= d.units) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float q = fast_exp(acc[i][j + 1][r] - lt) - fast_exp(acc[i][j][r] - lb);
+                    v[r] = tok < n && v0 + i * 16 + r < rows ? __fmul_rn(g, q) : 0.f;
+                }
+                put_grad_terms<T>(d, mb + i, tb, lane, v);
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
 // products
 
 // head_coded.hip: the same on weights that are not planes (rows_coded.h)
@@ -136,6 +213,12 @@ void launch_loss_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks,
                        hipStream_t s);
 void launch_kl_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks, const EpiKlStats &epi,
                      hipStream_t s);
+template <int T>
+void launch_loss_grad_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks,
+                            const EpiLossGrad<T> &epi, hipStream_t s);
+template <int T>
+void launch_kl_grad_coded(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks,
+                          const EpiKlGrad<T> &epi, hipStream_t s);
 
 // Words of a piece: what is held for one (d, and the weight's planes where they
 // are decoded) stays within about 256 MB, the size of the last cache; pieces of

@@ -7,85 +7,12 @@
 
 namespace ditch {
 
-// d of a piece as terms. Rows without a target give zeros, targets past the
-// vocabulary NaN.
-template <int T>
-struct EpiLossGrad {
-    Planes d;
-    const int32_t *targets;
-    const float *lse, *dloss;
-    int64_t n, rows, row0, vocab;
-    template <int MI, int NJ>
-    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            if (nb + j >= d.groups) continue;
-            const int64_t tok = (int64_t)(nb + j) * 16 + (lane & 15);
-            float g = 0.f, l = 0.f;
-            int64_t t = -1;
-            bool live = false;
-            if (tok < n) {
-                const int32_t tt = targets[tok];
-                live = tt >= 0;
-                l = lse[tok];
-                g = tt >= vocab ? __builtin_nanf("") : dloss[tok];
-                t = (int64_t)tt - row0 - v0;
-            }
-#pragma unroll
-            for (int i = 0; i < MI; i++) {
-                if (((mb + i) >> 1) >= d.units) continue;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float p = fast_exp(acc[i][j][r] - l) - (t == i * 16 + r ? 1.f : 0.f);
-                    v[r] = live && v0 + i * 16 + r < rows ? __fmul_rn(g, p) : 0.f;
-                }
-                put_grad_terms<T>(d, mb + i, nb + j, lane, v);
-            }
-        }
-    }
-};
-
-template <int T>
-struct EpiKlGrad {
-    Planes d;
-    const float *lse_base, *lse_trial, *dkl;
-    int64_t n, rows;
-    template <int MI, int NJ>
-    __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
-        const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
-#pragma unroll
-        for (int j = 0; j < NJ; j += 2) {
-            const int tb = (nb + j) / 2;
-            if (tb >= d.groups) continue;
-            const int64_t tok = (int64_t)tb * 16 + (lane & 15);
-            float g = 0.f, lb = 0.f, lt = 0.f;
-            if (tok < n) {
-                g = dkl[tok];
-                lb = lse_base[tok];
-                lt = lse_trial[tok];
-            }
-#pragma unroll
-            for (int i = 0; i < MI; i++) {
-                if (((mb + i) >> 1) >= d.units) continue;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float q = fast_exp(acc[i][j + 1][r] - lt) - fast_exp(acc[i][j][r] - lb);
-                    v[r] = tok < n && v0 + i * 16 + r < rows ? __fmul_rn(g, q) : 0.f;
-                }
-                put_grad_terms<T>(d, mb + i, tb, lane, v);
-            }
-        }
-    }
-};
-
 struct HeadGradPlan {
     Planes x[2], d;
     int64_t piece = 0, nblocks = 0, ld = 0;
     RowsTiling tiling;
     int order = 1;  // of the products with d
+    int coded = 0;  // the tile of rows_coded.h's product, 0: planes
     char *room = nullptr;
     float *part = nullptr;
     size_t bytes = 0;
@@ -100,15 +27,18 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     }
     p.nblocks = p.x[0].groups;
     const int td = grad_term_count(terms, n), wt = rows_weight_terms(w, terms);
-    p.piece = piece_rows(w.rows, p.nblocks * 32 * td + weight_row_bytes(w, terms));
+    p.coded = rows_coded_grad_tile(w, ceil_div(w.rows, 16), (kl ? 2 : 1) * p.nblocks, terms);
+    const int64_t held = p.coded ? 0 : weight_row_bytes(w, terms);
+    p.piece = piece_rows(w.rows, p.nblocks * 32 * td + held);
     if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;
     p.d = Planes{nullptr, p.nblocks, p.piece / 32, td};
     p.d.p = c.take(p.d.bytes());
     p.ld = ceil_div(w.cols, 4) * 4;
     p.order = rows_order_of(wt, td);
-    p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, wt, td, p.order, 1, true, false);
+    if (p.coded) p.tiling.parts = coded_parts_count(w, p.piece, n, 1);
+    else p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, wt, td, p.order, 1, true, false);
     p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
-    if (weight_row_bytes(w, terms)) p.room = c.take(weight_planes_shape(w, p.piece, terms).bytes());
+    if (held) p.room = c.take(weight_planes_shape(w, p.piece, terms).bytes());
     p.bytes = c.at;
     return p;
 }
@@ -126,11 +56,22 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
                       hipStream_t s, Fill &&fill) {
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
-        const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
+        const Planes wp = p.coded ? Planes{} : weight_planes(w, r, rows, p.x[0].terms, p.room, s);
         Planes d = p.d;
         d.units = ceil_div(rows, 64) * 2;
         fill(wp, d, r, rows);
-        if (dx.p) {
+        if (dx.p && p.coded) {
+            CodedParts g;
+            g.w[0] = w;
+            g.d[0] = d.p;
+            g.d_units = d.units;
+            g.d_plane = d.plane_bytes();
+            g.first = (int32_t)(r / 16);
+            g.blocks = (int32_t)ceil_div(rows, 16);
+            g.steps = (int32_t)ceil_div(rows, 32);
+            g.parts = p.tiling.parts;
+            launch_coded_parts(g, d.terms, p.part, p.ld, n, r > 0, s);
+        } else if (dx.p) {
             RowsGemm g;
             g.a = rows_outer(wp);
             g.b = rows_inner(d);
@@ -156,13 +97,28 @@ template <int TB, int T>
 static void fill_loss(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
                       int64_t rows, int64_t n, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
     const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, w.rows};
+    if (p.coded) {
+        RowsCoded c = coded_product(w, p.x[0], nullptr);
+        c.first = (int32_t)(row0 / 16);
+        c.blocks = (int32_t)ceil_div(rows, 16);
+        launch_loss_grad_coded<T>(p.coded, c, TB, d.units * 2, p.nblocks, epi, s);
+        return;
+    }
     launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, p.x[0], nullptr),
                                       d.units * 2, p.nblocks, epi, s);
 }
 template <int TB, int T>
-static void fill_kl(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t rows, int64_t n,
-                    const float *lse_base, const float *lse_trial, const float *dkl, hipStream_t s) {
+static void fill_kl(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
+                    int64_t rows, int64_t n, const float *lse_base, const float *lse_trial,
+                    const float *dkl, hipStream_t s) {
     const EpiKlGrad<T> epi{d, lse_base, lse_trial, dkl, n, rows};
+    if (p.coded) {
+        RowsCoded c = coded_product(w, p.x[0], &p.x[1]);
+        c.first = (int32_t)(row0 / 16);
+        c.blocks = (int32_t)ceil_div(rows, 16);
+        launch_kl_grad_coded<T>(p.coded, c, TB, d.units * 2, 2 * p.nblocks, epi, s);
+        return;
+    }
     launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, p.x[0], &p.x[1]),
                                       d.units * 2, 2 * p.nblocks, epi, s);
 }
@@ -182,9 +138,9 @@ void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial,
     const HeadGradPlan p = head_grad_plan(w, n, dtype, true, ws);
     launch_pack_rows(p.x[0], base.p, dtype, n, w.cols, base.stride, s);
     launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
-    head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t, int64_t rows) {
+    head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
         auto f = p.x[0].terms == 3 ? fill_kl<3, 3> : p.x[0].terms == 2 ? fill_kl<2, 2> : p.d.terms == 2 ? fill_kl<1, 2> : fill_kl<1, 1>;
-        f(p, w, wp, d, rows, n, lse_base, lse_trial, dkl, s);
+        f(p, w, wp, d, row0, rows, n, lse_base, lse_trial, dkl, s);
     });
 }
 

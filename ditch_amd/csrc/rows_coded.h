@@ -33,13 +33,23 @@ inline int rows_coded_tile(const TileView &w, int64_t mblocks, int64_t nblocks, 
     return ceil_div(mblocks, 16) * ceil_div(nblocks, 4) < 160 ? 3 : 2;
 }
 
+// A gradient reads the weight twice: as it stands for as many blocks, weights of one
+// term for half as many (loss gradients of 14336 x 4096: f16 and 256 rows 180 us, by planes
+// 255; FP8 and 128 rows 85 and 94, 200 rows 150 and 123; one row 49 and 82 of FP8, 112
+// and 405 of f32).
+inline int rows_coded_grad_tile(const TileView &w, int64_t mblocks, int64_t nblocks, int terms) {
+    if (rows_weight_terms(w, 3) == 1 && nblocks > ROWS_CODED_BLOCKS / 2) return 0;
+    return rows_coded_tile(w, mblocks, nblocks, terms);
+}
+
 struct RowsCoded {
     TileView w[2];   // paired: row blocks 2i and 2i + 1 of a are block i of the first and of the second
     int32_t paired = 0;
     RowsOperand b;
     const char *x = nullptr;
     int64_t x_plane = 0;
-    int32_t blocks = 0;  // 16-row blocks of one weight
+    int32_t blocks = 0;  // 16-row blocks of one weight, from `first` on
+    int32_t first = 0;
     int32_t stages = 0;
     int32_t tiles_m = 0, tiles_n = 0;
 };
@@ -105,7 +115,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
             which = g & 1;
             g >>= 1;
         }
-        return g < p.blocks ? g : p.blocks - 1;
+        return p.first + (g < p.blocks ? g : p.blocks - 1);
     };
     // this wave's copies: of the weight's units, of its side words, of x
     const char *pa[PA];
@@ -303,5 +313,32 @@ void launch_rows_coded(int tile, const RowsCoded &p, int64_t mblocks, int64_t nb
     default: go(std::integral_constant<int, TF_INT4>{}); break;
     }
 }
+
+// A gradient's epilogue, which leaves T terms: those of x, or two of one (grad_term_count).
+template <int T, typename Epi>
+void launch_rows_coded_grad(int tile, const RowsCoded &p, int terms, int64_t mblocks, int64_t nblocks, const Epi &epi,
+                            hipStream_t s) {
+    if constexpr (T == 2) {
+        if (terms == 1) {
+            launch_rows_coded<1>(tile, p, mblocks, nblocks, epi, s);
+            return;
+        }
+    }
+    launch_rows_coded<T>(tile, p, mblocks, nblocks, epi, s);
+}
+
+// rows_coded_parts.hip: d W of weights that are not planes, as parts of sums
+// [part][n][ld]; d inner planes, of each weight.
+struct CodedParts {
+    TileView w[2];
+    const char *d[2] = {nullptr, nullptr};
+    int64_t d_units = 0, d_plane = 0;
+    int32_t first = 0, blocks = 0;  // the weights' 16-row groups
+    int32_t steps = 0, sets = 1;    // of 32 rows; weights
+    int32_t parts = 1;
+    int32_t tiles_m = 0, tiles_n = 0;
+};
+int coded_parts_count(const TileView &w, int64_t rows, int64_t n, int sets);
+void launch_coded_parts(CodedParts p, int terms, float *part, int64_t ld, int64_t n, bool add, hipStream_t s);
 
 }  // namespace ditch
