@@ -11,6 +11,7 @@ import rows_ref as rr
 from ditch_amd import abi, hipmem
 from ditch_amd.hip import DeviceError, Model
 from ditch_amd.weights import HostWeight
+from test_gpu_glu import _glu_grad
 from test_gpu_head import _kl, _kl_grad, _loss, _loss_grad, _weight
 
 pytestmark = pytest.mark.gpu
@@ -294,5 +295,92 @@ def test_a_weight_gradient_past_32_bits(dev):
             want = d.T @ x.values
             size = np.abs(d).T @ np.abs(x.values)
             rr.check(got, want, d_off.T @ np.abs(x.values) + size * 2.0 ** -18, f"rows from {first}")
+    finally:
+        t.free()
+
+
+# a gradient's few rows on weights that are not planes, around the blocks of rows and of words that it counts in:
+# (weights' format, rows' type, rows, vocabulary or block's width, hidden)
+CODED = [("f16", "bf16", 16, 16, 32), ("f16", "f32", 17, 47, 64), ("f16", "f16", 256, 2100, 96), ("f32", "bf16", 65, 1045, 40),
+         ("f32", "f32", 128, 3333, 72), ("f32", "f16", 129, 600, 320), ("q8_0", "bf16", 64, 335, 96), ("q8_0", "f32", 100, 31, 64),
+         ("fp8", "bf16", 128, 4111, 200), ("fp8", "f16", 129, 300, 128), ("mxfp4", "bf16", 65, 2333, 160),
+         ("mxfp4", "f32", 16, 1040, 288), ("int4", "f32", 100, 777, 256), ("int4", "bf16", 1, 1500, 128)]
+
+
+@pytest.mark.parametrize("fmt,dtype,n,rows,hidden", CODED, ids=["-".join(map(str, c)) for c in CODED])
+def test_gradients_of_few_rows_on_coded_weights(dev, fmt, dtype, n, rows, hidden):
+    rng = np.random.default_rng(rows + n)
+    (t, w), (up, wu) = (_weight(dev, fmt, rows, hidden, i) for i in range(2))
+    try:
+        x = rr.Rows(dev, n, hidden, dtype, rng.standard_normal((n, hidden)))
+        y = rr.Rows(dev, n, hidden, dtype, x.values + rng.standard_normal((n, hidden)))
+        targets = rng.integers(-1, rows, n).astype(np.int32)
+        g = rng.standard_normal(n).astype(np.float32)
+        lse = rr.loss(x.values, w, targets, dtype, fmt)["lse"][0].astype(np.float32)
+        got = _loss_grad(dev, t, x, targets, lse, g, rows, hidden)
+        for k, (v, off) in rr.loss_grad(x.values, w, targets, g.astype(np.float64), dtype, fmt).items():
+            rr.check(got[k], v, off, k)
+        v, off = rr.kl_grad(x.values, y.values, w, g.astype(np.float64), dtype, fmt)["dx"]
+        rr.check(_kl_grad(dev, t, x, y, _kl(dev, t, x, y), g), v, off, "dx")
+        dout = rr.Rows(dev, n, rows, dtype, rng.standard_normal((n, rows)))
+        got = _glu_grad(dev, t, up, x, dout, rows, 1)
+        for k, (v, off) in rr.glu_grad(x.values, w, wu, dout.values, 1, dtype, fmt).items():
+            rr.check(got[k], v, off, k)
+    finally:
+        t.free()
+        up.free()
+
+
+def test_a_coded_gradient_in_several_pieces(dev):
+    """200 x 240000 values of d as three terms: 288 MB, two pieces of a weight that is read as it stands."""
+    n, vocab, hidden = 200, 240000, 32
+    rng = np.random.default_rng(9)
+    t, w = _weight(dev, "f16", vocab, hidden, 1)
+    try:
+        x = rr.Rows(dev, n, hidden, "f32", rng.standard_normal((n, hidden)))
+        targets = rng.integers(0, vocab, n).astype(np.int32)
+        few = np.array([0, 77, 199])
+        targets[few] = [vocab - 1, vocab // 2, 3]
+        lse = np.full(n, 14.0, np.float32)
+        want = rr.loss(x.values[few], w, targets[few], "f32", "f16")
+        lse[few] = want["lse"][0]
+        g = np.zeros(n, np.float32)
+        g[few] = [1.0, -0.5, 2.0]
+        got = _loss_grad(dev, t, x, targets, lse, g, vocab, hidden)
+        want = rr.loss_grad(x.values[few], w, targets[few], g[few].astype(np.float64), "f32", "f16")
+        rr.check(got["dx"][few], *want["dx"], "dx")
+        # the others weigh nothing, but lengthen the sums
+        rr.check(got["dw"], want["dw"][0], want["dw"][1] * (1 + n / 32), "dw")
+    finally:
+        t.free()
+
+
+@pytest.mark.parametrize("dtype,n", [("bf16", 20), ("f32", 150)])
+@pytest.mark.parametrize("kind", ["e5m2", "odd blocks", "special"])
+def test_fp8_that_the_conversions_do_not_decode(dev, kind, dtype, n):
+    """E5M2 codes, scale blocks of 32 columns, and a NaN code (whose word has no logit)."""
+    rows, hidden = 203, 160
+    rng = np.random.default_rng(n)
+    codes = rng.integers(0, 256, (rows, hidden), dtype=np.uint8) & 0xbb  # finite in either form
+    if kind == "special":
+        codes[0, 0] = 0x7f
+    block = 32 if kind == "odd blocks" else 64
+    scale = (rng.random((-(-rows // 64), -(-hidden // block))) * 0.01 + 0.001).astype(np.float32)
+    host = HostWeight.fp8(codes, scale, 64, block, e5m2=kind == "e5m2")
+    t, w = dev.upload(host), rr.from_rows(dev.dequant(host), "bf16")
+    try:
+        x = rr.Rows(dev, n, hidden, dtype, rng.standard_normal((n, hidden)) * 0.1)
+        targets = rng.integers(0, rows, n).astype(np.int32)
+        if kind == "special":
+            got = _loss(dev, t, x, targets)
+            assert np.isnan(got["lse"]).all() and np.isnan(got["loss"]).all()
+            return
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(x.values, w, targets, dtype, "fp8").items():
+            rr.check(got[k], v, off, k)
+        g = rng.standard_normal(n).astype(np.float32)
+        grads = _loss_grad(dev, t, x, targets, got["lse"], g, rows, hidden)
+        for k, (v, off) in rr.loss_grad(x.values, w, targets, g.astype(np.float64), dtype, "fp8").items():
+            rr.check(grads[k], v, off, k)
     finally:
         t.free()
