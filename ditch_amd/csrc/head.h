@@ -232,16 +232,12 @@ inline int64_t piece_rows(int64_t vocab, int64_t per_row) {
 inline int64_t weight_row_bytes(const TileView &w, int x_terms) {
     return weight_is_planes(w) ? 0 : (int64_t)weight_planes_shape(w, 16, x_terms).bytes() / 16;
 }
-inline RowsGemm logits_gemm(const Planes &wp, const Planes &x, const Planes *second) {
+inline RowsGemm logits_gemm(const Planes &wp, const RowsIn &in) {
     RowsGemm g;
     g.a = rows_inner(wp);
-    g.b = rows_inner(x);
-    if (second) {
-        g.b.paired = 1;
-        g.b.pair = second->p - x.p;
-    }
+    g.b = in.op;
     g.k32 = (int32_t)ceil_div(wp.units, 2) * 2;
-    rows_pairs(g, wp, x, rows_order_of(wp.terms, x.terms));
+    rows_pairs(g, wp, in.x, rows_order_of(wp.terms, in.x.terms));
     return g;
 }
 
@@ -250,16 +246,12 @@ inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t
     return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, rows_order_of(a, x.terms), 1, false, true).tile;
 }
 
-inline RowsCoded coded_product(const TileView &w, const Planes &x, const Planes *second) {
+inline RowsCoded coded_product(const TileView &w, const RowsIn &in) {
     RowsCoded p;
     p.w[0] = p.w[1] = w;
-    p.b = rows_inner(x);
-    if (second) {
-        p.b.paired = 1;
-        p.b.pair = second->p - x.p;
-    }
-    p.x = x.p;
-    p.x_plane = x.plane_bytes();
+    p.b = in.op;
+    p.x = in.x.p;
+    p.x_plane = in.x.plane_bytes();
     p.blocks = (int32_t)ceil_div(w.rows, 16);
     p.stages = (int32_t)w.units_k;
     return p;

@@ -63,9 +63,12 @@ __global__ __launch_bounds__(512) void loss_join_kernel(float *loss, float *lse,
     __shared__ double dl[8 * TOK];
     const int c = threadIdx.x % TOK, sl = threadIdx.x / TOK;
     const int64_t tok = (int64_t)blockIdx.x * TOK + c;
-    float m = LOWEST;
+    float m = LOWEST, pick = 0.f;
     double sum = 0;
+    int32_t t = -1;
     if (tok < n) {
+        t = targets[tok];
+        pick = picked[tok];  // (read ahead: whatever is there for rows without a target)
 #pragma unroll 4
         for (int64_t k = sl; k < strips; k += SL) {
             const float2 v = part[k * npad + tok];
@@ -79,8 +82,7 @@ __global__ __launch_bounds__(512) void loss_join_kernel(float *loss, float *lse,
     if (sl != 0 || tok >= n) return;
     const double l = (double)top + log(sum);
     lse[tok] = (float)l;
-    const int32_t t = targets[tok];
-    loss[tok] = t < 0 ? 0.f : t >= vocab ? __builtin_nanf("") : (float)(l - (double)picked[tok]);
+    loss[tok] = t < 0 ? 0.f : t >= vocab ? __builtin_nanf("") : (float)(l - (double)pick);
 }
 
 // Rows of a join's block.
@@ -163,8 +165,8 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
         p.x[i] = row_planes(n, w.cols, row_terms(dtype));
         p.x[i].p = c.take(p.x[i].bytes());
     }
-    p.npad = ceil_div(n, 32) * 32;
-    p.nblocks = p.x[0].groups * (kl ? 2 : 1);
+    p.npad = n < 32 ? n : ceil_div(n, 32) * 32;  // (one row's strips follow each other)
+    p.nblocks = row_blocks(n) * (kl ? 2 : 1);
     p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), p.nblocks, p.x[0].terms);
     const int64_t per = p.coded ? 0 : weight_row_bytes(w, p.x[0].terms);
     p.piece = per ? piece_rows(w.rows, per) : w.rows;
@@ -172,7 +174,7 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
     for (int64_t r = 0; r < w.rows; r += p.piece)
         p.strips += strips_of(w.rows - r < p.piece ? w.rows - r : p.piece, p.tile);
     p.part = c.take((size_t)p.strips * p.npad * (kl ? KL_STATS * sizeof(float) : sizeof(float2)));
-    p.picked = c.take<float>(p.npad);
+    p.picked = c.take<float>(n);
     if (per) p.room = c.take(weight_planes_shape(w, p.piece, p.x[0].terms).bytes());
     p.bytes = c.at;
     return p;
@@ -188,18 +190,18 @@ size_t head_kl_workspace(const TileView &w, int64_t n, int32_t dtype) {
 void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t n, const TileView &w,
                       const int32_t *targets, void *ws, hipStream_t s) {
     const HeadPlan p = head_plan(w, n, dtype, false, ws);
-    launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);
+    const RowsIn in = rows_in(dtype, n, w.cols, x, nullptr, p.x, s);
     int64_t strip = 0;
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
         const EpiLossStats epi{(float2 *)p.part, p.picked, targets, p.npad, n, rows, r, strip};
         if (p.coded) {
-            launch_loss_coded(p.tile, coded_product(w, p.x[0], nullptr), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
+            launch_loss_coded(p.tile, coded_product(w, in), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
             break;
         }
         const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], nullptr), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);
@@ -215,19 +217,18 @@ void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t
 void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype, RowsArg base, RowsArg trial,
                     int64_t n, const TileView &w, void *ws, hipStream_t s) {
     const HeadPlan p = head_plan(w, n, dtype, true, ws);
-    launch_pack_rows(p.x[0], base.p, dtype, n, w.cols, base.stride, s);
-    launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
+    const RowsIn in = rows_in(dtype, n, w.cols, base, &trial, p.x, s);
     int64_t strip = 0;
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
         const EpiKlStats epi{(float *)p.part, p.npad, n, rows, strip};
         if (p.coded) {
-            launch_kl_coded(p.tile, coded_product(w, p.x[0], &p.x[1]), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
+            launch_kl_coded(p.tile, coded_product(w, in), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
             break;
         }
         const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, p.x[0], &p.x[1]), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);

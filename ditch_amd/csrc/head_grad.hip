@@ -25,7 +25,7 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
         p.x[i] = row_planes(n, w.cols, terms);
         p.x[i].p = c.take(p.x[i].bytes());
     }
-    p.nblocks = p.x[0].groups;
+    p.nblocks = grad_blocks(n);
     const int td = grad_term_count(terms, n), wt = rows_weight_terms(w, terms);
     p.coded = rows_coded_grad_tile(w, ceil_div(w.rows, 16), (kl ? 2 : 1) * p.nblocks, terms);
     const int64_t held = p.coded ? 0 : weight_row_bytes(w, terms);
@@ -64,6 +64,7 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
             CodedParts g;
             g.w[0] = w;
             g.d[0] = d.p;
+            g.d_groups = (int32_t)d.groups;
             g.d_units = d.units;
             g.d_plane = d.plane_bytes();
             g.first = (int32_t)(r / 16);
@@ -94,53 +95,53 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
 }
 
 template <int TB, int T>
-static void fill_loss(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
+static void fill_loss(const HeadGradPlan &p, const RowsIn &in, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
                       int64_t rows, int64_t n, const int32_t *targets, const float *lse, const float *dloss, hipStream_t s) {
     const EpiLossGrad<T> epi{d, targets, lse, dloss, n, rows, row0, w.rows};
     if (p.coded) {
-        RowsCoded c = coded_product(w, p.x[0], nullptr);
+        RowsCoded c = coded_product(w, in);
         c.first = (int32_t)(row0 / 16);
         c.blocks = (int32_t)ceil_div(rows, 16);
         launch_loss_grad_coded<T>(p.coded, c, TB, d.units * 2, p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, p.x[0], nullptr),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, in),
                                       d.units * 2, p.nblocks, epi, s);
 }
 template <int TB, int T>
-static void fill_kl(const HeadGradPlan &p, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
+static void fill_kl(const HeadGradPlan &p, const RowsIn &in, const TileView &w, const Planes &wp, const Planes &d, int64_t row0,
                     int64_t rows, int64_t n, const float *lse_base, const float *lse_trial,
                     const float *dkl, hipStream_t s) {
     const EpiKlGrad<T> epi{d, lse_base, lse_trial, dkl, n, rows};
     if (p.coded) {
-        RowsCoded c = coded_product(w, p.x[0], &p.x[1]);
+        RowsCoded c = coded_product(w, in);
         c.first = (int32_t)(row0 / 16);
         c.blocks = (int32_t)ceil_div(rows, 16);
         launch_kl_grad_coded<T>(p.coded, c, TB, d.units * 2, 2 * p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, p.x[0], &p.x[1]),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, in),
                                       d.units * 2, 2 * p.nblocks, epi, s);
 }
 
 void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int64_t n, const TileView &w,
                            const int32_t *targets, const float *lse, const float *dloss, void *ws, hipStream_t s) {
     const HeadGradPlan p = head_grad_plan(w, n, dtype, false, ws);
-    launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);
+    const RowsIn in = rows_in(dtype, n, w.cols, x, nullptr, p.x, s);
+    if (dw.p && in.x.p != p.x[0].p) launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);  // (read transposed)
     head_grad(p, dtype, dx, dw, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
         auto f = p.x[0].terms == 3 ? fill_loss<3, 3> : p.x[0].terms == 2 ? fill_loss<2, 2> : p.d.terms == 2 ? fill_loss<1, 2> : fill_loss<1, 1>;
-        f(p, w, wp, d, row0, rows, n, targets, lse, dloss, s);
+        f(p, in, w, wp, d, row0, rows, n, targets, lse, dloss, s);
     });
 }
 
 void launch_head_kl_grad(int32_t dtype, RowsArg dx, RowsArg base, RowsArg trial, int64_t n, const TileView &w,
                          const float *lse_base, const float *lse_trial, const float *dkl, void *ws, hipStream_t s) {
     const HeadGradPlan p = head_grad_plan(w, n, dtype, true, ws);
-    launch_pack_rows(p.x[0], base.p, dtype, n, w.cols, base.stride, s);
-    launch_pack_rows(p.x[1], trial.p, dtype, n, w.cols, trial.stride, s);
+    const RowsIn in = rows_in(dtype, n, w.cols, base, &trial, p.x, s);
     head_grad(p, dtype, dx, RowsArg{}, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
         auto f = p.x[0].terms == 3 ? fill_kl<3, 3> : p.x[0].terms == 2 ? fill_kl<2, 2> : p.d.terms == 2 ? fill_kl<1, 2> : fill_kl<1, 1>;
-        f(p, w, wp, d, row0, rows, n, lse_base, lse_trial, dkl, s);
+        f(p, in, w, wp, d, row0, rows, n, lse_base, lse_trial, dkl, s);
     });
 }
 

@@ -48,6 +48,9 @@ inline int rows_order_of(int w_terms, int x_terms) { return w_terms > x_terms ? 
 inline Planes row_planes(int64_t n, int64_t cols, int terms) {
     return Planes{nullptr, ceil_div(n, 64) * 4, ceil_div(cols, 128) * 4, terms};
 }
+// Of which a product needs those with rows in them; d, read transposed too, 32 rows at a time.
+inline int64_t row_blocks(int64_t n) { return ceil_div(n, 16); }
+inline int64_t grad_blocks(int64_t n) { return ceil_div(n, 32) * 2; }
 void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
                       hipStream_t s);
 // The weight's rows [row0, row0 + rows) as planes: its own tiles where they are

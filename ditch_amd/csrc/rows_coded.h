@@ -152,6 +152,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
         ob[j] = (int64_t)g * p.b.ldu * 1024 + (second ? p.b.pair : 0);
         kb[j] = q % KT;
     }
+    const uint32_t lane_b = TB == 1 ? p.b.lane_at(lane) : lane16;
     int next = 0;
     const int stages = p.stages;
     auto copy = [&](u32x4 *S) {
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
 #pragma unroll
                 for (int j = 0; j < PB; j++) {
                     const int k = next * KT + kb[j] < p.b.ks ? next * KT + kb[j] : p.b.ks - 1;
-                    rows_copy_unit(p.x + ob[j] + e * p.x_plane + (int64_t)k * 1024, lane16,
+                    rows_copy_unit(p.x + ob[j] + e * p.x_plane + (int64_t)k * p.b.unit, lane_b,
                                    to + (NA + e * NBP + wave * PB + j) * 1024);
                 }
         }
@@ -333,6 +334,7 @@ struct CodedParts {
     TileView w[2];
     const char *d[2] = {nullptr, nullptr};
     int64_t d_units = 0, d_plane = 0;
+    int32_t d_groups = 0;
     int32_t first = 0, blocks = 0;  // the weights' 16-row groups
     int32_t steps = 0, sets = 1;    // of 32 rows; weights
     int32_t parts = 1;

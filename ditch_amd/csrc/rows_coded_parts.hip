@@ -71,11 +71,12 @@ __global__ __launch_bounds__(256) void rows_coded_parts_kernel(CodedParts p, Epi
             }
         }
 #pragma unroll
-        for (int e = 0; e < TB; e++)
+        for (int j = 0; j < NJ; j++) {
+            const int g = nt * NJ + j < p.d_groups ? nt * NJ + j : p.d_groups - 1;  // (those behind are not stored)
 #pragma unroll
-            for (int j = 0; j < NJ; j++)
-                q.b[e][j] = *(const u32x4 *)(p.d[set] + e * p.d_plane + ((int64_t)(nt * NJ + j) * p.d_units + s) * 1024 +
-                                             lane * 16);
+            for (int e = 0; e < TB; e++)
+                q.b[e][j] = *(const u32x4 *)(p.d[set] + e * p.d_plane + ((int64_t)g * p.d_units + s) * 1024 + lane * 16);
+        }
     };
     floatx4 acc[MB][NJ];
 #pragma unroll

@@ -11,7 +11,7 @@ import rows_ref as rr
 from ditch_amd import abi, hipmem
 from ditch_amd.hip import DeviceError, Model
 from ditch_amd.weights import HostWeight
-from test_gpu_glu import _glu_grad
+from test_gpu_glu import _glu, _glu_grad
 from test_gpu_head import _kl, _kl_grad, _loss, _loss_grad, _weight
 
 pytestmark = pytest.mark.gpu
@@ -384,3 +384,44 @@ def test_fp8_that_the_conversions_do_not_decode(dev, kind, dtype, n):
             rr.check(grads[k], v, off, k)
     finally:
         t.free()
+
+
+# up to 16 bf16 rows, read where they are if aligned; around the blocks of 16 and 32 rows:
+# (weights' format, rows, vocabulary or block's width, hidden, elements between rows)
+FEW = [("bf16", 1, 300, 128, 0), ("bf16", 16, 515, 256, 8), ("bf16", 7, 700, 384, 3), ("bf16", 15, 70, 128, 64),
+       ("bf16", 32, 300, 64, 0), ("bf16", 33, 300, 128, 8), ("bf16", 96, 333, 40, 1), ("fp8", 16, 400, 256, 8),
+       ("mxfp4", 5, 333, 128, 0), ("int4", 2, 90, 384, 24), ("q8_0", 3, 129, 128, 16), ("f16", 9, 100, 640, 0),
+       ("f32", 16, 65, 256, 8), ("f16", 80, 100, 128, 0)]
+
+
+@pytest.mark.parametrize("fmt,n,rows,hidden,gap", FEW, ids=["-".join(map(str, c)) for c in FEW])
+def test_few_bf16_rows(dev, fmt, n, rows, hidden, gap):
+    rng = np.random.default_rng(rows * 7 + n)
+    (t, w), (up, wu) = (_weight(dev, fmt, rows, hidden, i) for i in range(2))
+    try:
+        a = rng.standard_normal((n, hidden))
+        x, y, far = (rr.Rows(dev, n, hidden, "bf16", v, g) for v, g in
+                     ((a, gap), (a + rng.standard_normal((n, hidden)), gap), (a * 0.5, gap + 8)))
+        targets = rng.integers(-1, rows, n).astype(np.int32)
+        g = rng.standard_normal(n).astype(np.float32)
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(x.values, w, targets, "bf16", fmt).items():
+            rr.check(got[k], v, off, k)
+        got = _loss_grad(dev, t, x, targets, got["lse"], g, rows, hidden)
+        for k, (v, off) in rr.loss_grad(x.values, w, targets, g.astype(np.float64), "bf16", fmt).items():
+            rr.check(got[k], v, off, k)
+        for trial in (y, far):  # (of the base's stride, and of another)
+            got = _kl(dev, t, x, trial)
+            for k, (v, off) in rr.kl(x.values, trial.values, w, "bf16", fmt).items():
+                rr.check(got[k], v, off, k)
+            v, off = rr.kl_grad(x.values, trial.values, w, g.astype(np.float64), "bf16", fmt)["dx"]
+            rr.check(_kl_grad(dev, t, x, trial, got, g), v, off, "dx")
+        v, off = rr.glu(x.values, w, wu, 2, "bf16", fmt)
+        rr.check(_glu(dev, t, up, x, rows, 2), v, off, "out")
+        dout = rr.Rows(dev, n, rows, "bf16", rng.standard_normal((n, rows)))
+        got = _glu_grad(dev, t, up, x, dout, rows, 2)
+        for k, (v, off) in rr.glu_grad(x.values, w, wu, dout.values, 2, "bf16", fmt).items():
+            rr.check(got[k], v, off, k)
+    finally:
+        t.free()
+        up.free()
