@@ -29,8 +29,7 @@ static GluPlan glu_plan(const TileView &w, const TileView &up, int64_t n, int32_
     p.order = rows_order_of(wt, terms);
     p.x = row_planes(n, w.cols, terms);
     p.x.p = c.take(p.x.bytes());
-    if (rows_coded_pair(w, up))
-        p.coded = (grad ? rows_coded_grad_tile : rows_coded_tile)(w, 2 * ceil_div(w.rows, 16), nblocks, terms);
+    if (rows_coded_pair(w, up)) p.coded = rows_coded_tile(w, 2 * ceil_div(w.rows, 16), nblocks, grad);
     if (!weight_is_planes(w) && !p.coded)
         for (int i = 0; i < 2; i++) p.room[i] = c.take(weight_planes_shape(w, w.rows, terms).bytes());
     if (grad) {

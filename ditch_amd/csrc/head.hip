@@ -167,7 +167,7 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
     }
     p.npad = n < 32 ? n : ceil_div(n, 32) * 32;  // (one row's strips follow each other)
     p.nblocks = row_blocks(n) * (kl ? 2 : 1);
-    p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), p.nblocks, p.x[0].terms);
+    p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), p.nblocks, false);
     const int64_t per = p.coded ? 0 : weight_row_bytes(w, p.x[0].terms);
     p.piece = per ? piece_rows(w.rows, per) : w.rows;
     p.tile = p.coded ? p.coded : logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks);

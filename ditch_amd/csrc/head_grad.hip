@@ -27,7 +27,7 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     }
     p.nblocks = grad_blocks(n);
     const int td = grad_term_count(terms, n), wt = rows_weight_terms(w, terms);
-    p.coded = rows_coded_grad_tile(w, ceil_div(w.rows, 16), (kl ? 2 : 1) * p.nblocks, terms);
+    p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), (kl ? 2 : 1) * p.nblocks, true);
     const int64_t held = p.coded ? 0 : weight_row_bytes(w, terms);
     p.piece = piece_rows(w.rows, p.nblocks * 32 * td + held);
     if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;

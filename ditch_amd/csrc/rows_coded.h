@@ -26,20 +26,21 @@ inline bool rows_coded_pair(const TileView &a, const TileView &b) {
 }
 
 // The tile of such a product, 0 where the weight's planes serve better: where x
-// has more than ROWS_CODED_BLOCKS 16-row blocks.
-constexpr int ROWS_CODED_BLOCKS = 16;
-inline int rows_coded_tile(const TileView &w, int64_t mblocks, int64_t nblocks, int terms) {
-    if (!rows_coded_takes(w) || nblocks > ROWS_CODED_BLOCKS) return 0;
+// has many 16-row blocks, each of which has the weight decoded again. The planes
+// cost the more the wider their words are to the weight's own. Measured over 4864 x
+// 896, 14336 x 4096 and 64000 x 2048: f32 weights and 800 f32 rows 52, 543 and 1230 us,
+// by planes 65, 692 and 1545, from 1000 rows on alike; f16 and 640 bf16 rows 34, 250 and
+// 407, and 43, 232 and 523; MXFP4 and 800 bf16 rows 19, 101 and 208, and 27, 122 and
+// 268; FP8 and 300 bf16 rows 18, 99 and 130, and 26, 85 and 196, more rows worse.
+// A gradient reads the weight once more, transposed: f32 weights and 512 f32 rows
+// 89, 675 and 1535 (107, 868 and 1889); f16 and 300 bf16 rows 37, 263 and 426 (50, 283
+// and 635), 400 up to a fifth worse; MXFP4 and 200 bf16 rows 30, 111 and 211 (34, 123
+// and 244); FP8 and 128 31, 86 and 156 (31, 94 and 219), 200 worse.
+inline int rows_coded_tile(const TileView &w, int64_t mblocks, int64_t nblocks, bool grad) {
+    const int most = w.tf == TF_F16 ? (grad ? 24 : 40) : w.tf == TF_FP8 ? (grad ? 8 : 16)
+                     : w.tf == TF_F32 || w.tf == TF_Q8 ? (grad ? 32 : 56) : grad ? 16 : 56;
+    if (!rows_coded_takes(w) || nblocks > most) return 0;
     return ceil_div(mblocks, 16) * ceil_div(nblocks, 4) < 160 ? 3 : 2;
-}
-
-// A gradient reads the weight twice: as it stands for as many blocks, weights of one
-// term for half as many (loss gradients of 14336 x 4096: f16 and 256 rows 180 us, by planes
-// 255; FP8 and 128 rows 85 and 94, 200 rows 150 and 123; one row 49 and 82 of FP8, 112
-// and 405 of f32).
-inline int rows_coded_grad_tile(const TileView &w, int64_t mblocks, int64_t nblocks, int terms) {
-    if (rows_weight_terms(w, 3) == 1 && nblocks > ROWS_CODED_BLOCKS / 2) return 0;
-    return rows_coded_tile(w, mblocks, nblocks, terms);
 }
 
 struct RowsCoded {

@@ -304,7 +304,8 @@ def test_a_weight_gradient_past_32_bits(dev):
 CODED = [("f16", "bf16", 16, 16, 32), ("f16", "f32", 17, 47, 64), ("f16", "f16", 256, 2100, 96), ("f32", "bf16", 65, 1045, 40),
          ("f32", "f32", 128, 3333, 72), ("f32", "f16", 129, 600, 320), ("q8_0", "bf16", 64, 335, 96), ("q8_0", "f32", 100, 31, 64),
          ("fp8", "bf16", 128, 4111, 200), ("fp8", "f16", 129, 300, 128), ("mxfp4", "bf16", 65, 2333, 160),
-         ("mxfp4", "f32", 16, 1040, 288), ("int4", "f32", 100, 777, 256), ("int4", "bf16", 1, 1500, 128)]
+         ("mxfp4", "f32", 16, 1040, 288), ("int4", "f32", 100, 777, 256), ("int4", "bf16", 1, 1500, 128),
+         ("f32", "f32", 500, 333, 64), ("f16", "bf16", 380, 700, 96), ("int4", "f16", 250, 130, 128)]
 
 
 @pytest.mark.parametrize("fmt,dtype,n,rows,hidden", CODED, ids=["-".join(map(str, c)) for c in CODED])
@@ -422,6 +423,30 @@ def test_few_bf16_rows(dev, fmt, n, rows, hidden, gap):
         got = _glu_grad(dev, t, up, x, dout, rows, 2)
         for k, (v, off) in rr.glu_grad(x.values, w, wu, dout.values, 2, "bf16", fmt).items():
             rr.check(got[k], v, off, k)
+    finally:
+        t.free()
+        up.free()
+
+
+@pytest.mark.parametrize("fmt,dtype,n,rows,hidden", [("f32", "f32", 890, 200, 72), ("f16", "bf16", 600, 450, 96),
+                                                     ("mxfp4", "f32", 450, 333, 160), ("q8_0", "f16", 700, 129, 64),
+                                                     ("int4", "bf16", 800, 90, 128), ("fp8", "f16", 250, 515, 200)])
+def test_losses_of_many_rows_on_coded_weights(dev, fmt, dtype, n, rows, hidden):
+    rng = np.random.default_rng(n)
+    (t, w), (up, wu) = (_weight(dev, fmt, rows, hidden, i) for i in range(2))
+    try:
+        x = rr.Rows(dev, n, hidden, dtype, rng.standard_normal((n, hidden)))
+        targets = rng.integers(-1, rows, n).astype(np.int32)
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(x.values, w, targets, dtype, fmt).items():
+            rr.check(got[k], v, off, k)
+        half = rr.Rows(dev, n // 2, hidden, dtype, x.values[: n // 2])
+        other = rr.Rows(dev, n // 2, hidden, dtype, x.values[n // 2: n // 2 * 2])
+        got = _kl(dev, t, half, other)
+        for k, (v, off) in rr.kl(half.values, other.values, w, dtype, fmt).items():
+            rr.check(got[k], v, off, k)
+        v, off = rr.glu(x.values, w, wu, 0, dtype, fmt)
+        rr.check(_glu(dev, t, up, x, rows, 0), v, off, "out")
     finally:
         t.free()
         up.free()
