@@ -14,6 +14,7 @@ constexpr float LOWEST = -3.0e38f;  // in place of words that are not there
 // what the forward products keep of their tiles (head.hip joins it)
 
 struct EpiLossStats {
+    static constexpr bool F32_RESULT = true;
     float2 *part;  // [strip][npad]: maximum, sum
     float *picked;  // [n]
     const int32_t *targets;
@@ -72,6 +73,7 @@ __device__ __forceinline__ float phi_near(float u) {
 constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
+    static constexpr bool F32_RESULT = true;
     float *part;  // [strip][npad][KL_STATS]
     int64_t npad, n;
     int64_t rows, strip0;
@@ -135,6 +137,7 @@ struct EpiKlStats {
 // vocabulary NaN.
 template <int T>
 struct EpiLossGrad {
+    static constexpr bool F32_RESULT = false;
     Planes d;
     const int32_t *targets;
     const float *lse, *dloss;
@@ -173,6 +176,7 @@ struct EpiLossGrad {
 
 template <int T>
 struct EpiKlGrad {
+    static constexpr bool F32_RESULT = true;  // (of near rows' logits a difference is left)
     Planes d;
     const float *lse_base, *lse_trial, *dkl;
     int64_t n, rows;
@@ -232,18 +236,18 @@ inline int64_t piece_rows(int64_t vocab, int64_t per_row) {
 inline int64_t weight_row_bytes(const TileView &w, int x_terms) {
     return weight_is_planes(w) ? 0 : (int64_t)weight_planes_shape(w, 16, x_terms).bytes() / 16;
 }
-inline RowsGemm logits_gemm(const Planes &wp, const RowsIn &in) {
+inline RowsGemm logits_gemm(const Planes &wp, const RowsIn &in, bool f32_result) {
     RowsGemm g;
     g.a = rows_inner(wp);
     g.b = in.op;
     g.k32 = (int32_t)ceil_div(wp.units, 2) * 2;
-    rows_pairs(g, wp, in.x, rows_order_of(wp.terms, in.x.terms));
+    rows_pairs(g, wp, in.x, rows_order_of(wp.terms, in.x.terms, f32_result));
     return g;
 }
 
-inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks) {
-    const int a = rows_weight_terms(w, x.terms);
-    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, rows_order_of(a, x.terms), 1, false, true).tile;
+inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks, bool f32_result) {
+    const int a = rows_weight_terms(w, f32_result ? ROWS_MAX_TERMS : x.terms), order = rows_order_of(a, x.terms, f32_result);
+    return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order, 1, false, true).tile;
 }
 
 inline RowsCoded coded_product(const TileView &w, const RowsIn &in) {

@@ -168,14 +168,14 @@ static HeadPlan head_plan(const TileView &w, int64_t n, int32_t dtype, bool kl, 
     p.npad = n < 32 ? n : ceil_div(n, 32) * 32;  // (one row's strips follow each other)
     p.nblocks = row_blocks(n) * (kl ? 2 : 1);
     p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), p.nblocks, false);
-    const int64_t per = p.coded ? 0 : weight_row_bytes(w, p.x[0].terms);
+    const int64_t per = p.coded ? 0 : weight_row_bytes(w, ROWS_MAX_TERMS);
     p.piece = per ? piece_rows(w.rows, per) : w.rows;
-    p.tile = p.coded ? p.coded : logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks);
+    p.tile = p.coded ? p.coded : logits_tile(w, p.piece < w.rows ? p.piece : w.rows, p.x[0], p.nblocks, true);
     for (int64_t r = 0; r < w.rows; r += p.piece)
         p.strips += strips_of(w.rows - r < p.piece ? w.rows - r : p.piece, p.tile);
     p.part = c.take((size_t)p.strips * p.npad * (kl ? KL_STATS * sizeof(float) : sizeof(float2)));
     p.picked = c.take<float>(n);
-    if (per) p.room = c.take(weight_planes_shape(w, p.piece, p.x[0].terms).bytes());
+    if (per) p.room = c.take(weight_planes_shape(w, p.piece, ROWS_MAX_TERMS).bytes());
     p.bytes = c.at;
     return p;
 }
@@ -199,9 +199,9 @@ void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t
             launch_loss_coded(p.tile, coded_product(w, in), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
             break;
         }
-        const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
+        const Planes wp = weight_planes(w, r, rows, ROWS_MAX_TERMS, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in, true), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);
@@ -226,9 +226,9 @@ void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype,
             launch_kl_coded(p.tile, coded_product(w, in), p.x[0].terms, ceil_div(w.rows, 16), p.nblocks, epi, s);
             break;
         }
-        const Planes wp = weight_planes(w, r, rows, p.x[0].terms, p.room, s);
+        const Planes wp = weight_planes(w, r, rows, ROWS_MAX_TERMS, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in, true), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);

@@ -12,6 +12,7 @@ struct HeadGradPlan {
     int64_t piece = 0, nblocks = 0, ld = 0;
     RowsTiling tiling;
     int order = 1;  // of the products with d
+    int w_terms = 1;  // rows_weight_terms: what the planes are for
     int coded = 0;  // the tile of rows_coded.h's product, 0: planes
     char *room = nullptr;
     float *part = nullptr;
@@ -28,7 +29,8 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     p.nblocks = grad_blocks(n);
     const int td = grad_term_count(terms, n), wt = rows_weight_terms(w, terms);
     p.coded = rows_coded_tile(w, ceil_div(w.rows, 16), (kl ? 2 : 1) * p.nblocks, true);
-    const int64_t held = p.coded ? 0 : weight_row_bytes(w, terms);
+    p.w_terms = kl ? ROWS_MAX_TERMS : terms;
+    const int64_t held = p.coded ? 0 : weight_row_bytes(w, p.w_terms);
     p.piece = piece_rows(w.rows, p.nblocks * 32 * td + held);
     if (p.piece > ceil_div(w.rows, 64) * 64) p.piece = ceil_div(w.rows, 64) * 64;
     p.d = Planes{nullptr, p.nblocks, p.piece / 32, td};
@@ -38,7 +40,7 @@ static HeadGradPlan head_grad_plan(const TileView &w, int64_t n, int32_t dtype, 
     if (p.coded) p.tiling.parts = coded_parts_count(w, p.piece, n, 1);
     else p.tiling = rows_tiling(ceil_div(w.cols, 16), p.nblocks, p.piece / 32, wt, td, p.order, 1, true, false);
     p.part = c.take<float>((size_t)p.tiling.parts * n * p.ld);
-    if (held) p.room = c.take(weight_planes_shape(w, p.piece, terms).bytes());
+    if (held) p.room = c.take(weight_planes_shape(w, p.piece, p.w_terms).bytes());
     p.bytes = c.at;
     return p;
 }
@@ -56,7 +58,7 @@ static void head_grad(const HeadGradPlan &p, int32_t dtype, RowsArg dx, RowsArg 
                       hipStream_t s, Fill &&fill) {
     for (int64_t r = 0; r < w.rows; r += p.piece) {
         const int64_t rows = w.rows - r < p.piece ? w.rows - r : p.piece;
-        const Planes wp = p.coded ? Planes{} : weight_planes(w, r, rows, p.x[0].terms, p.room, s);
+        const Planes wp = p.coded ? Planes{} : weight_planes(w, r, rows, p.w_terms, p.room, s);
         Planes d = p.d;
         d.units = ceil_div(rows, 64) * 2;
         fill(wp, d, r, rows);
@@ -105,7 +107,7 @@ static void fill_loss(const HeadGradPlan &p, const RowsIn &in, const TileView &w
         launch_loss_grad_coded<T>(p.coded, c, TB, d.units * 2, p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks), logits_gemm(wp, in),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks, false), logits_gemm(wp, in, false),
                                       d.units * 2, p.nblocks, epi, s);
 }
 template <int TB, int T>
@@ -120,7 +122,7 @@ static void fill_kl(const HeadGradPlan &p, const RowsIn &in, const TileView &w, 
         launch_kl_grad_coded<T>(p.coded, c, TB, d.units * 2, 2 * p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks), logits_gemm(wp, in),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks, true), logits_gemm(wp, in, true),
                                       d.units * 2, 2 * p.nblocks, epi, s);
 }
 

@@ -31,17 +31,22 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline int row_terms(int32_t dtype) { return dtype == DITCH_BF16 ? 1 : dtype == DITCH_F16 ? 2 : 3; }
 inline size_t row_size(int32_t dtype) { return dtype == DITCH_F32 ? 4 : 2; }
-// The terms of a weight that rows of x_terms take: all of them f32 rows, at most
-// two (16 bits, rounded) 16-bit ones, whose own rounding is far above what is left
-// out.
+// The terms of a weight that results of x_terms take: all of them f32 ones, at
+// most two (16 bits, rounded) 16-bit ones, whose own rounding is far above what is
+// left out.
 int rows_weight_terms(const TileView &w, int x_terms);
 // The terms that d, what a gradient's two products hand over, is held in: those of
 // the rows' type; bf16 rows up to 64 get a second one, which costs nothing while
 // the products wait for the weight (one value of d makes most of such a gradient,
 // and its rounding would be the gradient's).
 inline int grad_term_count(int x_terms, int64_t n) { return x_terms == 1 && n <= 64 ? 2 : x_terms; }
-// and the pairs of terms that are multiplied: i + j < order
-inline int rows_order_of(int w_terms, int x_terms) { return w_terms > x_terms ? w_terms : x_terms; }
+// and the pairs of terms that are multiplied: i + j < order; f32 results of 16-bit
+// rows, and differences of two rows' logits, take all that count in 24 bits (logits
+// off by 2^-17 of their terms left divergences of f16 rows 2^-6 apart off by 3e-4).
+constexpr int rows_order_of(int w_terms, int x_terms, bool f32_result = false) {
+    const int all = w_terms + x_terms - 1, most = w_terms > x_terms ? w_terms : x_terms;
+    return f32_result ? (all < ROWS_MAX_TERMS ? all : ROWS_MAX_TERMS) : most;
+}
 
 // Rows of activations: 64 rows and 128 columns (a unit of 4-bit codes), zeros
 // behind the last row and column.

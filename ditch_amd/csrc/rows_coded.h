@@ -82,11 +82,11 @@ __device__ __forceinline__ u32x4 coded_term(float (&v)[8]) {
 template <int WGM, int WGN, int MI, int NJ, int TF, int TB, typename Epi>
 __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p, Epi epi) {
     constexpr int OWN = TF == TF_F16 ? 2 : TF == TF_F32 || TF == TF_Q8 ? 3 : 1;
-    constexpr int TA = TB == 3 || OWN < 2 ? OWN : 2;  // rows_weight_terms
+    constexpr int TA = TB == 3 || OWN < 2 || Epi::F32_RESULT ? OWN : 2;  // rows_weight_terms
     constexpr int KT = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
     constexpr int HALVES = TF == TF_F32 ? 2 : 1;
     constexpr int NS = TF == TF_INT4 ? 2 : TF == TF_F16 || TF == TF_F32 ? 0 : 1;
-    constexpr int ORDER = TA > TB ? TA : TB;
+    constexpr int ORDER = rows_order_of(TA, TB, Epi::F32_RESULT);
     constexpr int WAVES = WGM * WGN, UA = WGM * MI, UB = WGN * NJ;
     constexpr int NA = UA * HALVES, PA = NA / WAVES, NBP = UB * KT;
     constexpr bool HALF = NBP * 2 == WAVES;

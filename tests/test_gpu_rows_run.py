@@ -450,3 +450,36 @@ def test_losses_of_many_rows_on_coded_weights(dev, fmt, dtype, n, rows, hidden):
     finally:
         t.free()
         up.free()
+
+
+@pytest.mark.parametrize("dtype,fmt,n,vocab,hidden", [("f16", "f16", 4, 40000, 40), ("bf16", "f32", 3, 30000, 64),
+                                                      ("f16", "f32", 70, 2000, 96), ("bf16", "q8_0", 40, 3000, 128),
+                                                      ("f16", "q8_0", 1000, 300, 64), ("f16", "f16", 700, 515, 72)])
+def test_losses_of_16_bit_rows_are_as_exact_as_f32_ones(dev, dtype, fmt, n, vocab, hidden):
+    """Losses, log sums and divergences are f32, so 16-bit rows' products with any weights are held to the bounds of
+    f32 rows (near ones: a divergence of 2^-8 of the logits would show what a 16-bit product leaves out)."""
+    rng = np.random.default_rng(vocab)
+    t, w = _weight(dev, fmt, vocab, hidden, 4)
+    try:
+        a = rng.standard_normal((n, hidden))
+        x, y = (rr.Rows(dev, n, hidden, dtype, v) for v in (a, a + 0.02 * rng.standard_normal((n, hidden))))
+        targets = rng.integers(0, vocab, n).astype(np.int32)
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(x.values, w, targets, "f32", fmt).items():
+            rr.check(got[k], v, off, k)
+        got = _kl(dev, t, x, y)
+        for k, (v, off) in rr.kl(x.values, y.values, w, "f32", fmt).items():
+            rr.check(got[k], v, off, k)
+        # and, those bounds being far wider than what f32 sums lose: no worse than the same values as f32 rows, whose
+        # terms are all multiplied (16 times, for sums in another order)
+        full = _kl(dev, t, *(rr.Rows(dev, n, hidden, "f32", v.values) for v in (x, y)))["kl"]
+        want = rr.kl(x.values, y.values, w, "f32", fmt)["kl"][0]
+        worst = lambda v: (np.abs(v - want) / want).max()
+        assert worst(got["kl"]) <= 16 * max(worst(full), 2.0 ** -23)
+        if dtype == "f16":  # its gradient: d is held in 16 bits and the result rounded to 11
+            g = rng.standard_normal(n).astype(np.float32)
+            want = rr.kl_grad(x.values, y.values, w, g.astype(np.float64), "f32", fmt)["dx"][0]
+            off = np.linalg.norm(_kl_grad(dev, t, x, y, got, g) - want, axis=1)
+            assert (off <= 2.0 ** -11 * np.linalg.norm(want, axis=1) + 2.0 ** -24 * hidden ** 0.5).all()
+    finally:
+        t.free()
