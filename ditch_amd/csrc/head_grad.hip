@@ -129,8 +129,9 @@ static void fill_kl(const HeadGradPlan &p, const RowsIn &in, const TileView &w, 
 void launch_head_loss_grad(int32_t dtype, RowsArg dx, RowsArg dw, RowsArg x, int64_t n, const TileView &w,
                            const int32_t *targets, const float *lse, const float *dloss, void *ws, hipStream_t s) {
     const HeadGradPlan p = head_grad_plan(w, n, dtype, false, ws);
-    const RowsIn in = rows_in(dtype, n, w.cols, x, nullptr, p.x, s);
-    if (dw.p && in.x.p != p.x[0].p) launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s);  // (read transposed)
+    // (rows without a target are zeros in d^T x, where an infinity or NaN times their zero d would stay)
+    const RowsIn in = rows_in(dtype, n, w.cols, x, nullptr, p.x, s, targets);
+    if (dw.p && in.x.p != p.x[0].p) launch_pack_rows(p.x[0], x.p, dtype, n, w.cols, x.stride, s, targets);  // (read transposed)
     head_grad(p, dtype, dx, dw, n, w, s, [&](const Planes &wp, const Planes &d, int64_t row0, int64_t rows) {
         auto f = p.x[0].terms == 3 ? fill_loss<3, 3> : p.x[0].terms == 2 ? fill_loss<2, 2> : p.d.terms == 2 ? fill_loss<1, 2> : fill_loss<1, 1>;
         f(p, in, w, wp, d, row0, rows, n, targets, lse, dloss, s);

@@ -56,8 +56,9 @@ inline Planes row_planes(int64_t n, int64_t cols, int terms) {
 // Of which a product needs those with rows in them; d, read transposed too, 32 rows at a time.
 inline int64_t row_blocks(int64_t n) { return ceil_div(n, 16); }
 inline int64_t grad_blocks(int64_t n) { return ceil_div(n, 32) * 2; }
+// (live: rows where it is negative are zeros, whatever they hold)
 void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
-                      hipStream_t s);
+                      hipStream_t s, const int32_t *live = nullptr);
 // The weight's rows [row0, row0 + rows) as planes: its own tiles where they are
 // that already (nothing launched), else decoded to `room` (row0 a multiple of 16).
 bool weight_is_planes(const TileView &w);

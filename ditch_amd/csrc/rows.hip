@@ -44,15 +44,16 @@ __device__ __forceinline__ float row_value(const void *x, int64_t i) {
 // rows are aligned to them.
 template <int DT, int T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(Planes out, const void *x, int64_t n, int64_t cols,
-                                                        int64_t stride, int wide) {
+                                                        int64_t stride, int wide, const int32_t *live) {
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= out.groups * out.units) return;
     const int64_t g = unit / out.units, u = unit % out.units;
     const int64_t row = g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
+    const bool there = row < n && (!live || live[row] >= 0);
     float v[8];
     uint16_t t[8][T];
-    if (row < n && k + 8 <= cols && wide) {
+    if (there && k + 8 <= cols && wide) {
         const int64_t at = row * stride + k;
         if constexpr (DT == DITCH_F32) {
             const float4 a = *(const float4 *)((const float *)x + at), b = *(const float4 *)((const float *)x + at + 4);
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(Planes out, const void *
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = row < n && k + j < cols ? row_value<DT>(x, row * stride + k + j) : 0.f;
+        for (int j = 0; j < 8; j++) v[j] = there && k + j < cols ? row_value<DT>(x, row * stride + k + j) : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) to_terms<T>(v[j], t[j]);
@@ -82,17 +83,17 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(Planes out, const void *
 }
 
 void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n, int64_t cols, int64_t stride,
-                      hipStream_t s) {
+                      hipStream_t s, const int32_t *live) {
     const int64_t units = out.groups * out.units;
     if (units == 0) return;
     const int wide = ((uintptr_t)x | (uintptr_t)(stride * (int64_t)row_size(dtype))) % 16 == 0;
     const dim3 grid((unsigned)ceil_div(units, 4));
     if (dtype == DITCH_F32)
-        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F32, 3>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F32, 3>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide, live);
     else if (dtype == DITCH_F16)
-        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F16, 2>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_F16, 2>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide, live);
     else
-        hipLaunchKernelGGL((pack_rows_kernel<DITCH_BF16, 1>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide);
+        hipLaunchKernelGGL((pack_rows_kernel<DITCH_BF16, 1>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide, live);
     DITCH_TRY_HIP(hipGetLastError());
 }
 

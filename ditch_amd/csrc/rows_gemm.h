@@ -96,14 +96,14 @@ struct RowsIn {
 // whole units of any weight (128 columns). A pass and a launch less: the block of 4864
 // x 896 and 1 row 8.0 us, packed 10.7.
 inline RowsIn rows_in(int32_t dtype, int64_t n, int64_t cols, RowsArg x, const RowsArg *second, const Planes *planes,
-                      hipStream_t s) {
+                      hipStream_t s, const int32_t *live = nullptr) {
     RowsIn in{planes[0], rows_inner(planes[0])};
     in.op.paired = second ? 1 : 0;
     const bool direct = dtype == DITCH_BF16 && n <= 16 && cols % 128 == 0 && (uintptr_t)x.p % 16 == 0 &&
                         x.stride % 8 == 0 && x.stride < (int64_t)1 << 26 &&
                         (!second || ((uintptr_t)second->p % 16 == 0 && second->stride == x.stride));
     if (!direct) {
-        launch_pack_rows(planes[0], x.p, dtype, n, cols, x.stride, s);
+        launch_pack_rows(planes[0], x.p, dtype, n, cols, x.stride, s, live);
         if (second) {
             launch_pack_rows(planes[1], second->p, dtype, n, cols, second->stride, s);
             in.op.pair = planes[1].p - planes[0].p;

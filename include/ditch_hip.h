@@ -885,9 +885,12 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
  *
  * Rows are ditch_kv_rows of `dtype` (DITCH_F32, DITCH_F16 or DITCH_BF16), one
  * dtype a call. The weights are registered tensors of any format, taken at the
- * values they decode to. 16-bit rows are rounded once where they leave a call,
- * and once to as many bits between the two products of a gradient, and take f32
- * and Q8_0 weights at 16 bits; f32 ones are exact to about f32 rounding. `ws` is device scratch of the call's
+ * values they decode to. Losses, log sums and divergences are exact to about
+ * f32 rounding for rows of any type, and so are f32 rows' other results; 16-bit
+ * results are rounded once where they leave a call, and once to at least as many
+ * bits between the two products of a gradient, and take f32 and Q8_0 weights at
+ * 16 bits. A row that is not finite has no finite result, nor has the weights'
+ * gradient then; a weight that is not may give NaN wherever it enters. `ws` is device scratch of the call's
  * ..._workspace bytes (16-byte aligned; its contents do not matter, nothing is
  * kept in it, calls that overlap need one each); the sizes are 0 for arguments
  * that the call refuses. Outputs may not overlap inputs or each other. n = 0
@@ -896,8 +899,8 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
  *
  * Cross entropy against the head w [vocab][hidden]: lse[i] = log sum_v
  * e^(x_i . w_v), loss[i] = lse[i] - x_i . w_target. A negative target has no
- * loss (0, and no gradient), one past the vocabulary gives NaN. The logits are
- * never stored.                                                             */
+ * loss and no gradient (0, whatever its row holds), one past the vocabulary
+ * gives NaN. The logits are never stored.                                   */
 uint64_t ditch_hip_head_loss_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype);
 int32_t ditch_hip_head_loss_device(ditch_hip *h, float *d_loss, float *d_lse, int32_t dtype,
                                    const ditch_kv_rows *x, uint64_t n,

@@ -483,3 +483,33 @@ def test_losses_of_16_bit_rows_are_as_exact_as_f32_ones(dev, dtype, fmt, n, voca
             assert (off <= 2.0 ** -11 * np.linalg.norm(want, axis=1) + 2.0 ** -24 * hidden ** 0.5).all()
     finally:
         t.free()
+
+
+@pytest.mark.parametrize("dtype,fmt,n,hidden", [("bf16", "bf16", 12, 128), ("bf16", "bf16", 90, 200), ("f32", "bf16", 40, 72),
+                                                ("f16", "fp8", 20, 128), ("bf16", "f16", 9, 256)])
+def test_padding_holds_anything(dev, dtype, fmt, n, hidden):
+    """A padded batch: rows without a target hold infinities, NaN and what their memory held, and change nothing."""
+    vocab = 300
+    rng = np.random.default_rng(n)
+    t, w = _weight(dev, fmt, vocab, hidden, 2)
+    try:
+        a = rng.standard_normal((n, hidden))
+        targets = rng.integers(0, vocab, n).astype(np.int32)
+        pad = np.arange(n) % 3 == 1
+        targets[pad] = np.where(np.arange(pad.sum()) % 2, -100, -1)
+        a[pad] = 0
+        x = rr.Rows(dev, n, hidden, dtype, a)
+        a[pad] = rng.choice([np.nan, np.inf, -np.inf, 3.0], (pad.sum(), hidden))
+        dirty = rr.Rows(dev, n, hidden, dtype, a)
+        g = rng.standard_normal(n).astype(np.float32)
+        g[pad] = np.nan
+        want, got = _loss(dev, t, x, targets), _loss(dev, t, dirty, targets)
+        np.testing.assert_array_equal(got["loss"], want["loss"])
+        assert not got["loss"][pad].any()
+        grads = _loss_grad(dev, t, dirty, targets, got["lse"], g, vocab, hidden)
+        g[pad] = 0
+        for k, (v, off) in rr.loss_grad(x.values, w, targets, g.astype(np.float64), dtype, fmt).items():
+            rr.check(grads[k], v, off, k)
+        assert not grads["dx"][pad].any()
+    finally:
+        t.free()
