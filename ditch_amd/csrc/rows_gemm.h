@@ -589,21 +589,20 @@ void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const E
     DITCH_TRY_HIP(hipGetLastError());
 }
 
-// `tile`: rows_tiling's choice.
+// `tile`: rows_tiling's choice, or rows_out_tile's.
 template <bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
-    switch (tile) {
-    case 0:
-        // (sums in two levels do not fit it)
-        if constexpr (TB == 3 && !AO && !BO) break;
-        else launch_rows_gemm_tile<2, 4, 8, 4, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
-        return;
-    case 1: launch_rows_gemm_tile<2, 2, 4, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
-    case 2: launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
-    case 3: launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s); return;
+    // (sums in two levels do not fit the largest tile)
+    if constexpr (TB != 3 || AO || BO)
+        if (tile == 0) return launch_rows_gemm_tile<2, 4, 8, 4, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+    if (tile == 1) return launch_rows_gemm_tile<2, 2, 4, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+    if constexpr (AO && BO) {  // rows_out_tile
+        if constexpr (TB == 1) launch_rows_gemm_tile<2, 2, 8, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+    } else {
+        if (tile == 2) return launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+        if (tile == 3) return launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+        if constexpr (TB == 3) launch_rows_gemm_tile<4, 2, 4, 2, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
     }
-    if constexpr (TB == 1 && AO && BO) launch_rows_gemm_tile<2, 2, 8, 4, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
-    if constexpr (TB == 3) launch_rows_gemm_tile<4, 2, 4, 2, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
 }
 
 template <typename F>

@@ -258,6 +258,31 @@ def test_rows_far_apart(dev):
         t.free()
 
 
+def test_direct_rows_far_apart(dev):
+    """Sixteen bf16 rows as far apart as rows are read where they are: the last begins 1.9 GiB on."""
+    n, hidden, vocab, stride = 16, 128, 300, 2 ** 26 - 8
+    (t, w), (up, wu) = (_weight(dev, "bf16", vocab, hidden, i) for i in range(2))
+    lib = hipmem.hip()
+    try:
+        stored, values = rr.to_rows(np.random.default_rng(1).standard_normal((n, hidden)), "bf16")
+        size = ((n - 1) * stride + hidden) * 2
+        buf = hipmem.Buffer(size)
+        for i in range(n):
+            hipmem.check(lib.hipMemcpy(ctypes.c_void_p(buf.ptr.value + i * stride * 2), stored[i].ctypes.data_as(ctypes.c_void_p),
+                                       hidden * 2, hipmem.H2D), "hipMemcpy")
+        x = rr.Rows(dev, n, hidden, "bf16")
+        x.desc = dev.kv_rows(buf.ptr, size, stride)
+        targets = np.arange(n, dtype=np.int32) * 9
+        got = _loss(dev, t, x, targets)
+        for k, (v, off) in rr.loss(values, w, targets, "bf16", "bf16").items():
+            rr.check(got[k], v, off, k)
+        v, off = rr.glu(values, w, wu, 0, "bf16", "bf16")
+        rr.check(_glu(dev, t, up, x, vocab, 0), v, off, "out")
+    finally:
+        t.free()
+        up.free()
+
+
 def test_a_weight_gradient_past_32_bits(dev):
     """dW of 262400 x 4096 f32: 4.3 GB, its last rows past 2^32 bytes (MXFP4 weights, in many pieces). lse is an input
     here: any number."""
