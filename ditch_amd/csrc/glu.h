@@ -32,6 +32,7 @@ __device__ __forceinline__ void act_both(float g, float &y, float &dy) {
 
 // Blocks 2i of m are gate rows, 2i + 1 the same up rows.
 struct EpiGlu {
+    static constexpr bool PAIRS = false;
     static constexpr bool F32_RESULT = false;
     void *out;
     int64_t stride, n, rows;
@@ -74,6 +75,7 @@ struct EpiGlu {
 // dg and du of the block as terms.
 template <int T>
 struct EpiGluGrad {
+    static constexpr bool PAIRS = false;
     static constexpr bool F32_RESULT = false;
     Planes dg, du;
     const void *dout;

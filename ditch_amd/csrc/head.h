@@ -14,6 +14,7 @@ constexpr float LOWEST = -3.0e38f;  // in place of words that are not there
 // what the forward products keep of their tiles (head.hip joins it)
 
 struct EpiLossStats {
+    static constexpr bool PAIRS = false;
     static constexpr bool F32_RESULT = true;
     float2 *part;  // [strip][npad]: maximum, sum
     float *picked;  // [n]
@@ -73,6 +74,7 @@ __device__ __forceinline__ float phi_near(float u) {
 constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
+    static constexpr bool PAIRS = true;  // of n's blocks
     static constexpr bool F32_RESULT = true;
     float *part;  // [strip][npad][KL_STATS]
     int64_t npad, n;
@@ -137,6 +139,7 @@ struct EpiKlStats {
 // vocabulary NaN.
 template <int T>
 struct EpiLossGrad {
+    static constexpr bool PAIRS = false;
     static constexpr bool F32_RESULT = false;
     Planes d;
     const int32_t *targets;
@@ -176,6 +179,7 @@ struct EpiLossGrad {
 
 template <int T>
 struct EpiKlGrad {
+    static constexpr bool PAIRS = true;  // of n's blocks
     static constexpr bool F32_RESULT = true;  // (of near rows' logits a difference is left)
     Planes d;
     const float *lse_base, *lse_trial, *dkl;

@@ -87,14 +87,15 @@ void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *pa
 // over k32 steps of 32 k of the pairs of terms i + j < order, `sets` times
 // (rows.hip). Parts are tried only where `split`; inner: neither operand is read
 // transposed.
+constexpr int ROWS_FEW = 6;  // rows_gemm.h: no tile, k shared by the waves
 struct RowsTiling {
     int tile = 0, parts = 1;
 };
 RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_terms, int b_terms, int order, int sets,
                        bool split, bool inner);
 // 16-row blocks of a wave's strip and of a tile along m
-inline int rows_strip_blocks(int tile) { return tile == 0 ? 8 : tile == 3 ? 2 : 4; }
-inline int rows_tile_blocks(int tile) { return tile == 1 ? 8 : tile == 3 ? 4 : 16; }
+inline int rows_strip_blocks(int tile) { return tile == 0 ? 8 : tile == 3 || tile == ROWS_FEW ? 2 : 4; }
+inline int rows_tile_blocks(int tile) { return tile == 1 ? 8 : tile == 3 ? 4 : tile == ROWS_FEW ? 2 : 16; }
 inline int rows_pair_count(int a, int b, int order) {
     int n = 0;
     for (int i = 0; i < a; i++) n += order - i < 0 ? 0 : order - i < b ? order - i : b;

@@ -144,6 +144,10 @@ RowsTiling rows_tiling(int64_t mblocks, int64_t nblocks, int64_t k32, int a_term
             }
         }
     }
+    // up to 64 16-bit rows on up to 1024 blocks (rows_gemm.h; the block of 2048 x 2048 and
+    // one bf16 row 5.1 us, by tiles 13.6, of 4864 x 896 4.9 and 8.0; the loss of 16000 x 896 9.0
+    // and 11.6; of 30000 x 2048 and 30 rows 36 and 29)
+    if (inner && a_terms == 1 && b_terms < 3 && nblocks <= 4 && mblocks <= 1024) best.tile = ROWS_FEW;
     return best;
 }
 

@@ -94,7 +94,7 @@ struct RowsIn {
 // Packed to `planes`, unless they need no planes: up to 16 bf16 rows, of whose
 // units each lane copies 16 bytes of its row, where the rows are aligned and
 // whole units of any weight (128 columns). A pass and a launch less: the block of 4864
-// x 896 and 1 row 8.0 us, packed 10.7.
+// x 896 and 1 row 8.0 us by tiles, packed 10.7.
 inline RowsIn rows_in(int32_t dtype, int64_t n, int64_t cols, RowsArg x, const RowsArg *second, const Planes *planes,
                       hipStream_t s, const int32_t *live = nullptr) {
     RowsIn in{planes[0], rows_inner(planes[0])};
@@ -576,7 +576,115 @@ struct EpiRows {
 };
 
 // ---------------------------------------------------------------------------
+// x W^T for few 16-bit rows on weights of one term, where the grid of 64 x 64 tiles
+// does not fill the chip (rows_tiling). What those tiles take is then not memory but steps, each a
+// barrier and the LDS' latency (350 cycles, eight stages ahead as with four): here a
+// workgroup computes 32 words and its four waves share k, each with loads straight
+// to registers, which hold fragments as they lie in memory, and no barrier until
+// the sums are added.
+template <int NJ, int TB, typename Epi>
+__global__ __launch_bounds__(256) void rows_few_kernel(RowsGemm p, Epi epi) {
+    constexpr int MI = 2, AHEAD = NJ * TB <= 2 ? 8 : 4, SUMS = MI * NJ * 64;
+    __shared__ floatx4 sums[2 * SUMS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mt = blockIdx.x;
+    const char *pa[MI], *pb[NJ];
+    auto at = [](const RowsOperand &o, int q) {
+        int second = 0;
+        if (o.paired) {
+            second = q & 1;
+            q >>= 1;
+        }
+        return (int64_t)(q < o.blocks ? q : o.blocks - 1) * o.ldu * 1024 + (second ? o.pair : 0);
+    };
+#pragma unroll
+    for (int i = 0; i < MI; i++) pa[i] = p.sa[0] + at(p.a, mt * MI + i) + lane * 16;
+    const uint32_t lane_b = p.b.lane_at(lane);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) pb[j] = p.sb[0] + at(p.b, j) + lane_b;
+    struct Chunk {
+        u32x4 a[AHEAD][MI], b[AHEAD][TB][NJ];
+    };
+    const int first = (int)((int64_t)p.k32 * wave / 4), last = (int)((int64_t)p.k32 * (wave + 1) / 4);
+    auto load = [&](int t, Chunk &c) {
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) {
+            if (t + s >= last) break;
+            const int64_t ka = t + s < p.a.ks ? t + s : p.a.ks - 1, kb = t + s < p.b.ks ? t + s : p.b.ks - 1;
+#pragma unroll
+            for (int i = 0; i < MI; i++) c.a[s][i] = *(const u32x4 *)(pa[i] + ka * 1024);
+#pragma unroll
+            for (int e = 0; e < TB; e++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) c.b[s][e][j] = *(const u32x4 *)(pb[j] + e * p.b_plane + kb * p.b.unit);
+        }
+    };
+    floatx4 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int t, const Chunk &c) {
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) {
+            if (t + s >= last) break;
+#pragma unroll
+            for (int e = 0; e < TB; e++)
+#pragma unroll
+                for (int i = 0; i < MI; i++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) acc[i][j] = mfma_bf16(c.a[s][i], c.b[s][e][j], acc[i][j]);
+        }
+    };
+    Chunk one, two;
+    load(first, one);
+    for (int t = first; t < last; t += 2 * AHEAD) {
+        load(t + AHEAD, two);
+        multiply(t, one);
+        load(t + 2 * AHEAD, one);
+        multiply(t + AHEAD, two);
+    }
+    // the waves' sums, in the same order always: 0 + 2, 1 + 3, both
+    auto give = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) sums[slot * SUMS + (i * NJ + j) * 64 + lane] = acc[i][j];
+    };
+    auto take = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) acc[i][j] += sums[slot * SUMS + (i * NJ + j) * 64 + lane];
+    };
+    if (wave >= 2) give(wave - 2);
+    __syncthreads();
+    if (wave < 2) take(wave);
+    __syncthreads();
+    if (wave == 1) give(0);
+    __syncthreads();
+    if (wave == 0) {
+        take(0);
+        epi(acc, mt * MI, 0, lane);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // launches
+
+template <int TB, typename Epi>
+void launch_rows_few(const RowsGemm &g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
+    auto go = [&](auto nj) {
+        hipLaunchKernelGGL((rows_few_kernel<decltype(nj)::value, TB, Epi>), dim3((unsigned)ceil_div(mblocks, 2)), dim3(256), 0, s,
+                           g, epi);
+        DITCH_TRY_HIP(hipGetLastError());
+    };
+    if constexpr (!Epi::PAIRS)
+        if (nblocks == 1) return go(std::integral_constant<int, 1>{});
+    if (nblocks <= 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+}
 
 template <int WGM, int WGN, int MI, int NJ, bool WHOLE, bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
@@ -601,6 +709,7 @@ void launch_rows_gemm(int tile, const RowsGemm &g, int64_t mblocks, int64_t nblo
     } else {
         if (tile == 2) return launch_rows_gemm_tile<4, 2, 4, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
         if (tile == 3) return launch_rows_gemm_tile<2, 2, 2, 2, false, AO, BO, TB>(g, mblocks, nblocks, epi, s);
+        if constexpr (TB < 3 && !AO) return launch_rows_few<TB>(g, mblocks, nblocks, epi, s);
         if constexpr (TB == 3) launch_rows_gemm_tile<4, 2, 4, 2, true, AO, BO, TB>(g, mblocks, nblocks, epi, s);
     }
 }

@@ -417,7 +417,8 @@ def test_fp8_that_the_conversions_do_not_decode(dev, kind, dtype, n):
 FEW = [("bf16", 1, 300, 128, 0), ("bf16", 16, 515, 256, 8), ("bf16", 7, 700, 384, 3), ("bf16", 15, 70, 128, 64),
        ("bf16", 32, 300, 64, 0), ("bf16", 33, 300, 128, 8), ("bf16", 96, 333, 40, 1), ("fp8", 16, 400, 256, 8),
        ("mxfp4", 5, 333, 128, 0), ("int4", 2, 90, 384, 24), ("q8_0", 3, 129, 128, 16), ("f16", 9, 100, 640, 0),
-       ("f32", 16, 65, 256, 8), ("f16", 80, 100, 128, 0)]
+       ("f32", 16, 65, 256, 8), ("f16", 80, 100, 128, 0), ("bf16", 64, 8190, 32, 0), ("bf16", 40, 8210, 160, 0),
+       ("bf16", 1, 16384, 64, 0), ("bf16", 3, 16385, 128, 0), ("bf16", 17, 31, 2049, 5)]
 
 
 @pytest.mark.parametrize("fmt,n,rows,hidden,gap", FEW, ids=["-".join(map(str, c)) for c in FEW])
