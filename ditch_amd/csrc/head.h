@@ -68,9 +68,9 @@ __device__ __forceinline__ float phi_near(float u) {
     return s * u * u;
 }
 
-// Of a strip: the base's maximum and sum, the trial's maximum and sum, the sum of
-// e^(l_base - m) phi(D) relative to m = the larger of the maxima (so that neither
-// e^l_base nor e^l_trial in it overflows), the sum of e^(l_base - its maximum) D.
+// Of a strip: the base's maximum and sum, the trial's maximum and sum, and with w =
+// e^(l_base - its maximum) and u = D less the maxima's difference (words that moved
+// alike have small u, whatever they moved by) the sums of w phi(u) and of w u.
 constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
@@ -94,25 +94,24 @@ struct EpiKlStats {
                 for (int i = 0; i < MI; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        // (both at LOWEST: no weight and no difference)
+                        // (both at LOWEST: no weight)
                         if (!whole && v0 + i * 16 + r >= rows) acc[i][j + h][r] = LOWEST;
                         mx[h] = fmaxf(mx[h], acc[i][j + h][r]);
                     }
                 mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 16));
                 mx[h] = fmaxf(mx[h], __shfl_xor(mx[h], 32));
             }
-            const float m = fmaxf(mx[0], mx[1]), sb = fast_exp(mx[0] - m), st = fast_exp(mx[1] - m);
+            const float moved = mx[0] - mx[1];
 #pragma unroll
             for (int i = 0; i < MI; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float b = acc[i][j][r], t = acc[i][j + 1][r], u = b - t;
-                    const float w = fast_exp(b - mx[0]), x = fast_exp(t - mx[1]);
+                    const float b = acc[i][j][r], t = acc[i][j + 1][r], u = (b - t) - moved;
+                    const float w = fast_exp(b - mx[0]), x = fast_exp(t - mx[1]);  // x = w e^-u
                     sum[0] += w;
                     sum[1] += x;
                     far = __builtin_fmaf(w, u, far);
-                    const float wm = w * sb;
-                    near += fabsf(u) <= 0.25f ? wm * phi_near(u) : __builtin_fmaf(wm, u - 1.f, x * st);
+                    near += fabsf(u) <= 0.25f ? w * phi_near(u) : __builtin_fmaf(w, u - 1.f, x);
                 }
             float v[KL_STATS] = {mx[0], sum[0], mx[1], sum[1], near, far};
 #pragma unroll

@@ -10,10 +10,15 @@
 //
 // Divergence of trial rows from base rows, KL = sum p (log p - log q): the two
 // rows' blocks are interleaved in one product, so that a lane holds both logits
-// of a word. With D = l_base - l_trial and phi(u) = u + e^-u - 1 >= 0,
-//   KL = sum p phi(D) - (e^c - 1 - c),  c = lse_trial - lse_base,
-// where nothing cancels for rows near each other (sum p D + c would lose what a
-// small divergence is made of); for far ones, |c| > 1, sum p D + c is used.
+// of a word. With D = l_base - l_trial, c = lse_trial - lse_base and phi(u) = u +
+// e^-u - 1 >= 0,
+//   KL = sum p phi(D + c),
+// term by term at least 0 (sum p D + c would lose what a small divergence is made
+// of). c is known when all words have been seen: a strip sums phi(D - a) of a
+// shift of its own, and the join moves it by delta = -c - a,
+//   sum p phi(u - delta) = sum p (e^delta phi(u) - (e^delta - 1) u + e^delta - 1 - delta),
+// in 64 bits. (sum p phi(D) - phi(-c), without shifts, lost divergences to rows whose logits
+// moved alike: by 4, a divergence of 3e-5 was off by 2e-4 of itself, one of 5e-7 by 1e-2.)
 // d = g (q - p).
 #include "head.h"
 
@@ -100,44 +105,48 @@ template <int TOK>
 __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base, float *lse_trial, const float *part,
                                                       int64_t n, int64_t npad, int64_t strips) {
     constexpr int SL = 512 / TOK;
-    // base sum, trial sum, near, far, and what they are relative to: the maxima of base and trial, the larger, base's
-    constexpr int OF[4] = {0, 1, 2, 0};
     __shared__ float fl[8 * TOK];
     __shared__ double dl[8 * TOK];
     const int c = threadIdx.x % TOK, sl = threadIdx.x / TOK;
     const int64_t tok = (int64_t)blockIdx.x * TOK + c;
-    float m[3] = {LOWEST, LOWEST, LOWEST};
-    double s[4] = {0, 0, 0, 0};
+    float m[2] = {LOWEST, LOWEST};
+    double s[2] = {0, 0};
     if (tok < n) {
 #pragma unroll 2
         for (int64_t k = sl; k < strips; k += SL) {
             const float2 *p = (const float2 *)(part + (k * npad + tok) * KL_STATS);
-            const float2 base = p[0], trial = p[1], sums = p[2];
-            const float v[4] = {base.y, trial.y, sums.x, sums.y}, b = base.x, t = trial.x;
-            const float at[3] = {b, t, fmaxf(b, t)};
-            double mine[3], theirs[3];
-            for (int h = 0; h < 3; h++) {
-                const float to = fmaxf(m[h], at[h]);
-                mine[h] = expf(m[h] - to);
-                theirs[h] = expf(at[h] - to);
+            const float2 v[2] = {p[0], p[1]};
+            for (int h = 0; h < 2; h++) {
+                const float to = fmaxf(m[h], v[h].x);
+                s[h] = s[h] * (double)expf(m[h] - to) + (double)v[h].y * (double)expf(v[h].x - to);
                 m[h] = to;
             }
-            for (int q = 0; q < 4; q++) s[q] = s[q] * mine[OF[q]] + theirs[OF[q]] * v[q];
         }
     }
-    float top[3];
-    double scale[3];
-    for (int h = 0; h < 3; h++) {
-        top[h] = block_max<TOK>(m[h], fl);
-        scale[h] = exp((double)m[h] - (double)top[h]);
+    double lse[2];
+    for (int h = 0; h < 2; h++) {
+        const float top = block_max<TOK>(m[h], fl);
+        lse[h] = (double)top + log(block_sum<TOK>(s[h] * exp((double)m[h] - (double)top), dl));
     }
-    for (int q = 0; q < 4; q++) s[q] = block_sum<TOK>(s[q] * scale[OF[q]], dl);
+    const double shift = lse[0] - lse[1];
+    double sum = 0;
+    if (tok < n) {
+#pragma unroll 2
+        for (int64_t k = sl; k < strips; k += SL) {
+            const float2 *v = (const float2 *)(part + (k * npad + tok) * KL_STATS);
+            const float2 base = v[0], trial = v[1], sums = v[2];
+            const double delta = shift - (double)(base.x - trial.x);
+            // what the strip's sums weigh in p, and that times e^delta: neither overflows
+            const double p = exp((double)base.x - lse[0]);
+            const double more = fabs(delta) < 1 ? p * expm1(delta) : exp((double)trial.x - lse[1]) - p;
+            sum += (p + more) * sums.x - more * sums.y + (more - p * delta) * base.y;
+        }
+    }
+    sum = block_sum<TOK>(sum, dl);
     if (sl != 0 || tok >= n) return;
-    const double mb = top[0], lb = mb + log(s[0]), lt = (double)top[1] + log(s[1]), d = lt - lb;
-    s[2] *= exp((double)top[2] - mb);
-    lse_base[tok] = (float)lb;
-    lse_trial[tok] = (float)lt;
-    kl[tok] = (float)(fabs(d) <= 1 ? s[2] / s[0] - (expm1(d) - d) : s[3] / s[0] + d);
+    lse_base[tok] = (float)lse[0];
+    lse_trial[tok] = (float)lse[1];
+    kl[tok] = (float)sum;
 }
 
 // ---------------------------------------------------------------------------
