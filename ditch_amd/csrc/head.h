@@ -11,6 +11,47 @@ __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp
 constexpr float LOWEST = -3.0e38f;  // in place of words that are not there
 
 // ---------------------------------------------------------------------------
+// joins of what the strips leave
+
+// Sums of strips, each relative to its own reference (a maximum), over a block of
+// 512: TOK rows, 512 / TOK slices of the strips each; row tid % TOK. The largest
+// reference first, then every thread's sums once rescaled to it.
+template <int TOK>
+__device__ __forceinline__ float block_max(float m, float *lds) {  // lds[8][TOK]
+#pragma unroll
+    for (int o = TOK; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane < TOK) lds[wave * TOK + lane] = m;
+    __syncthreads();
+    m = lds[threadIdx.x % TOK];
+#pragma unroll
+    for (int w = 1; w < 8; w++) m = fmaxf(m, lds[w * TOK + threadIdx.x % TOK]);
+    __syncthreads();
+    return m;
+}
+template <int TOK>
+__device__ __forceinline__ double block_sum(double s, double *lds) {
+#pragma unroll
+    for (int o = TOK; o < 64; o *= 2) s += __shfl_xor(s, o);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane < TOK) lds[wave * TOK + lane] = s;
+    __syncthreads();
+    s = lds[threadIdx.x % TOK];
+#pragma unroll
+    for (int w = 1; w < 8; w++) s += lds[w * TOK + threadIdx.x % TOK];
+    __syncthreads();
+    return s;
+}
+
+// Rows of a join's block.
+template <typename F>
+void with_join_rows(int64_t n, F &&f) {
+    if (n >= 4096) f(std::integral_constant<int, 32>{});
+    else if (n >= 256) f(std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 1>{});
+}
+
+// ---------------------------------------------------------------------------
 // what the forward products keep of their tiles (head.hip joins it)
 
 struct EpiLossStats {
@@ -176,13 +217,32 @@ struct EpiLossGrad {
     }
 };
 
+// e^z - 1 for |z| <= 1/4: its series to z^8, off by 2^-34 of it
+__device__ __forceinline__ float expm1_near(float z) {
+    float s = 1.f / 40320.f;
+    s = __builtin_fmaf(s, z, 1.f / 5040.f);
+    s = __builtin_fmaf(s, z, 1.f / 720.f);
+    s = __builtin_fmaf(s, z, 1.f / 120.f);
+    s = __builtin_fmaf(s, z, 1.f / 24.f);
+    s = __builtin_fmaf(s, z, 1.f / 6.f);
+    s = __builtin_fmaf(s, z, 0.5f);
+    return __builtin_fmaf(s * z, z, z);
+}
+
+// d = g (q - p) = g p (e^z - 1), z = (l_trial - l_base) - (lse_trial - lse_base), the
+// latter form where z is small: what is left is as exact as z (d of one term, 2^-8 of
+// itself, does not show it: 2 % of 1500 bf16 rows' time for nothing). And what mends
+// the log sums' rounding (head_grad.hip): p as one term, the strips' sums of q - p.
 template <int T>
 struct EpiKlGrad {
     static constexpr bool PAIRS = true;  // of n's blocks
     static constexpr bool F32_RESULT = true;  // (of near rows' logits a difference is left)
+    static constexpr bool NEAR = T > 1;
     Planes d;
+    Planes p;     // (none: p.p NULL)
+    float *sums;  // [strip][npad]
     const float *lse_base, *lse_trial, *dkl;
-    int64_t n, rows;
+    int64_t n, rows, npad, strip0;
     template <int MI, int NJ>
     __device__ __forceinline__ void operator()(floatx4 (&acc)[MI][NJ], int mb, int nb, int lane) const {
         const int64_t v0 = (int64_t)mb * 16 + 4 * (lane >> 4);
@@ -191,23 +251,38 @@ struct EpiKlGrad {
             const int tb = (nb + j) / 2;
             if (tb >= d.groups) continue;
             const int64_t tok = (int64_t)tb * 16 + (lane & 15);
-            float g = 0.f, lb = 0.f, lt = 0.f;
+            float g = 0.f, lb = 0.f, c = 0.f, lt = 0.f, sum = 0.f;
             if (tok < n) {
                 g = dkl[tok];
                 lb = lse_base[tok];
                 lt = lse_trial[tok];
+                c = lt - lb;
             }
 #pragma unroll
             for (int i = 0; i < MI; i++) {
                 if (((mb + i) >> 1) >= d.units) continue;
-                float v[4];
+                float v[4], w[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float q = fast_exp(acc[i][j + 1][r] - lt) - fast_exp(acc[i][j][r] - lb);
-                    v[r] = tok < n && v0 + i * 16 + r < rows ? __fmul_rn(g, q) : 0.f;
+                    const bool in = tok < n && v0 + i * 16 + r < rows;
+                    const float b = acc[i][j][r], t = acc[i][j + 1][r], e = fast_exp(b - lb);
+                    float q = fast_exp(t - lt) - e;
+                    if constexpr (NEAR) {
+                        const float z = (t - b) - c;
+                        if (fabsf(z) <= 0.25f) q = e * expm1_near(z);
+                    }
+                    v[r] = in ? __fmul_rn(g, q) : 0.f;
+                    w[r] = in ? e : 0.f;
+                    sum += in ? q : 0.f;
                 }
                 put_grad_terms<T>(d, mb + i, tb, lane, v);
+                if constexpr (NEAR)
+                    if (p.p) put_grad_terms<1>(p, mb + i, tb, lane, w);
             }
+            if (!NEAR || !p.p) continue;
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (tok < n && lane < 16) sums[(strip0 + mb / MI) * npad + tok] = sum;
         }
     }
 };
@@ -234,6 +309,11 @@ inline int64_t piece_rows(int64_t vocab, int64_t per_row) {
     const int64_t most = ((int64_t)256 << 20) / (per_row > 0 ? per_row : 1);
     int64_t pieces = most >= vocab ? 1 : ceil_div(vocab, most < 256 ? 256 : most);
     return ceil_div(ceil_div(vocab, pieces), 256) * 256;
+}
+
+// strips of the vocabulary in a piece: one for each wave's rows of a tile
+inline int64_t strips_of(int64_t rows, int tile) {
+    return ceil_div(ceil_div(rows, 16), rows_tile_blocks(tile)) * rows_tile_blocks(tile) / rows_strip_blocks(tile);
 }
 
 inline int64_t weight_row_bytes(const TileView &w, int x_terms) {

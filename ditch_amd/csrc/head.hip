@@ -27,36 +27,6 @@ namespace ditch {
 // ---------------------------------------------------------------------------
 // cross entropy
 
-// Sums of strips, each relative to its own reference (a maximum), over a block of
-// 512: TOK rows, 512 / TOK slices of the strips each; row tid % TOK. The largest
-// reference first, then every thread's sums once rescaled to it.
-template <int TOK>
-__device__ __forceinline__ float block_max(float m, float *lds) {  // lds[8][TOK]
-#pragma unroll
-    for (int o = TOK; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane < TOK) lds[wave * TOK + lane] = m;
-    __syncthreads();
-    m = lds[threadIdx.x % TOK];
-#pragma unroll
-    for (int w = 1; w < 8; w++) m = fmaxf(m, lds[w * TOK + threadIdx.x % TOK]);
-    __syncthreads();
-    return m;
-}
-template <int TOK>
-__device__ __forceinline__ double block_sum(double s, double *lds) {
-#pragma unroll
-    for (int o = TOK; o < 64; o *= 2) s += __shfl_xor(s, o);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane < TOK) lds[wave * TOK + lane] = s;
-    __syncthreads();
-    s = lds[threadIdx.x % TOK];
-#pragma unroll
-    for (int w = 1; w < 8; w++) s += lds[w * TOK + threadIdx.x % TOK];
-    __syncthreads();
-    return s;
-}
-
 // Few rows a block where there are few, so that their strips are read side by
 // side (1 row x 2376 strips by 8 threads took 220 us).
 template <int TOK>
@@ -88,14 +58,6 @@ __global__ __launch_bounds__(512) void loss_join_kernel(float *loss, float *lse,
     const double l = (double)top + log(sum);
     lse[tok] = (float)l;
     loss[tok] = t < 0 ? 0.f : t >= vocab ? __builtin_nanf("") : (float)(l - (double)pick);
-}
-
-// Rows of a join's block.
-template <typename F>
-static void with_join_rows(int64_t n, F &&f) {
-    if (n >= 4096) f(std::integral_constant<int, 32>{});
-    else if (n >= 256) f(std::integral_constant<int, 8>{});
-    else f(std::integral_constant<int, 1>{});
 }
 
 // ---------------------------------------------------------------------------
@@ -151,11 +113,6 @@ __global__ __launch_bounds__(512) void kl_join_kernel(float *kl, float *lse_base
 
 // ---------------------------------------------------------------------------
 // pieces of the vocabulary
-
-// strips of the vocabulary in a piece: one for each wave's rows of a tile
-static int64_t strips_of(int64_t rows, int tile) {
-    return ceil_div(ceil_div(rows, 16), rows_tile_blocks(tile)) * rows_tile_blocks(tile) / rows_strip_blocks(tile);
-}
 
 // The forward of either loss: stats(g, piece's epilogue arguments).
 struct HeadPlan {

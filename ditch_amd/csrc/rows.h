@@ -79,9 +79,14 @@ struct Carver {
     }
 };
 
-// out[i][c] = the sum over parts of part[p][i][c], in f32, rounded to dtype.
+// out[i][c] = the sum over parts of part[p][i][c], in f32, rounded to dtype; with
+// `times`, and times[i] of the same of `more`.
+struct MoreParts {
+    const float *part = nullptr, *times = nullptr;
+    int parts = 0;
+};
 void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
-                       int64_t ld, int64_t n, int64_t cols, hipStream_t s);
+                       int64_t ld, int64_t n, int64_t cols, hipStream_t s, MoreParts more = {});
 
 // The tile and the parts (of k) of a product of mblocks x nblocks 16-row blocks
 // over k32 steps of 32 k of the pairs of terms i + j < order, `sets` times

@@ -268,7 +268,7 @@ __device__ __forceinline__ void put_row_value(void *out, int32_t dtype, int64_t 
 
 __global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtype, int64_t stride, const float *part,
                                                          int parts, int64_t part_stride, int64_t ld, int64_t n,
-                                                         int64_t cols) {
+                                                         int64_t cols, MoreParts more) {
     const int64_t per = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n * per) return;
     const int64_t row = i / per, c = i % per * 4;
@@ -278,16 +278,26 @@ __global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtyp
         const float4 v = *(const float4 *)(part + p * part_stride + row * ld + c);
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
+    if (more.times) {
+        const float times = more.times[row];
+        float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int p = 0; p < more.parts; p++) {
+            const float4 v = *(const float4 *)(more.part + p * part_stride + row * ld + c);
+            m.x += v.x, m.y += v.y, m.z += v.z, m.w += v.w;
+        }
+        sum.x += times * m.x, sum.y += times * m.y, sum.z += times * m.z, sum.w += times * m.w;
+    }
     const float v[4] = {sum.x, sum.y, sum.z, sum.w};
     for (int j = 0; j < 4; j++)
         if (c + j < cols) put_row_value(out, dtype, row * stride + c + j, v[j]);
 }
 
 void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
-                       int64_t ld, int64_t n, int64_t cols, hipStream_t s) {
+                       int64_t ld, int64_t n, int64_t cols, hipStream_t s, MoreParts more) {
     const int64_t total = n * ceil_div(cols, 4);
     hipLaunchKernelGGL(join_parts_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, s, out, dtype, stride,
-                       part, parts, part_stride, ld, n, cols);
+                       part, parts, part_stride, ld, n, cols, more);
     DITCH_TRY_HIP(hipGetLastError());
 }
 

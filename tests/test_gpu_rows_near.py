@@ -1,9 +1,11 @@
-"""Divergences of rows near each other, held to a share of themselves.
+"""Divergences of rows near each other, and their gradients, held to a share of
+themselves.
 
 The heads here have a mean direction: every word's row is a common one plus its
-own. What moves along it moves all logits alike, while the roundings of the words' logits are independent of each other, so that
-their sum over the words is taken as the root of the sum of squares (six times
-that).
+own. What moves along it moves all logits alike, and what is lost there is lost
+for all words alike, while the roundings of the words' logits are independent of
+each other, so that their sum over the words is taken as the root of the sum of
+squares (six times that for one number, four times for the norm of a row's many).
 
 A logit's own error: a product of k columns adds `pairs` matrix instructions for
 each 32, each of which rounds the running sum by 2^-23 of it at most; as
@@ -16,7 +18,7 @@ import torch
 import rows_ref as rr
 from ditch_amd import synth
 from ditch_amd.weights import HostWeight
-from test_gpu_head import _kl
+from test_gpu_head import _kl, _kl_grad
 
 pytestmark = pytest.mark.gpu
 
@@ -77,5 +79,38 @@ def test_near_divergences_under_a_common_shift(dev, dtype, fmt, n, vocab, hidden
         got = _kl(dev, t, base, trial)["kl"]
         v, off = _kl_exact(base.values, trial.values, w, dtype, fmt)
         rr.check(got, v, off, "kl")
+    finally:
+        t.free()
+
+
+@pytest.mark.parametrize("far", [2.0 ** -1, 2.0 ** -4, 2.0 ** -7, 2.0 ** -10])
+@pytest.mark.parametrize("dtype,fmt,n,vocab,hidden", [("f32", "bf16", 12, 40000, 256), ("f32", "fp8", 30, 20000, 256),
+                                                      ("f32", "f32", 5, 30000, 200), ("f32", "mxfp4", 70, 9000, 128),
+                                                      ("f32", "bf16", 700, 130000, 64), ("f32", "q8_0", 600, 5000, 64),
+                                                      ("f16", "bf16", 20, 40000, 256), ("f16", "f16", 100, 20000, 128)])
+def test_gradients_of_near_divergences(dev, dtype, fmt, n, vocab, hidden, far):
+    """The gradient's error against its norm, where the log sums' own rounding (2^-21 of what they are taken from, along
+    the head's mean direction) would be many times what the logits' roundings leave.
+
+    d = p (e^(t - b - c) - 1): the logits' errors enter as p times theirs, independent for each word; p, its
+    exponentials, the terms of d and the sums of the product by 2^-18 of the whole; a 16-bit result by half a step."""
+    rng = np.random.default_rng(n)
+    t, w = _head(dev, fmt, vocab, hidden, 5, rng.standard_normal(hidden))
+    try:
+        a = rng.standard_normal((n, hidden)) * 0.5
+        base = rr.Rows(dev, n, hidden, dtype, a)
+        trial = rr.Rows(dev, n, hidden, dtype, a + far * rng.standard_normal((n, hidden)))
+        g = rng.standard_normal(n).astype(np.float32)
+        dx = _kl_grad(dev, t, base, trial, _kl(dev, t, base, trial), g)
+        few = np.unique(np.r_[:min(n, 12), n - 1])
+        _, _, _, _, p, q, off = _distributions(base.values[few], trial.values[few], w, dtype, fmt)
+        want = ((q - p) * g[few, None]) @ w
+        size = np.linalg.norm(want, axis=1)
+        each = np.abs(g[few]) * off * np.sqrt(((p ** 2 + q ** 2) @ (w ** 2)).sum(1))
+        bound = 4 * each + 2.0 ** -18 * size
+        if dtype == "f16":
+            bound += 2.0 ** -11 * size + 2.0 ** -25 * hidden ** 0.5
+        err = np.linalg.norm(dx[few] - want, axis=1)
+        assert (err <= bound).all(), f"{(err / size).max():.3g} of the gradient, allowed {(bound / size)[np.argmax(err / bound)]:.3g}"
     finally:
         t.free()
