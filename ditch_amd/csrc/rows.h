@@ -65,6 +65,16 @@ bool weight_is_planes(const TileView &w);
 Planes weight_planes_shape(const TileView &w, int64_t rows, int x_terms);
 Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, int x_terms, char *room, hipStream_t s);
 
+// The grid of `blocks` workgroups, in rows of less than 2^32 threads, which is what a
+// launch takes along x (2^24 rows on 40000 words are 2^32.3 in the largest tiles); a
+// multiple of 8, so that rows_block() and the hardware number the XCDs alike. The
+// last row may have blocks behind the last.
+inline dim3 rows_grid(int64_t blocks, int threads, int64_t parts = 1) {
+    const int64_t most = (((int64_t)1 << 32) - 1) / threads / 8 * 8, x = blocks < 1 ? 1 : blocks < most ? blocks : most;
+    return dim3((unsigned)x, (unsigned)parts, (unsigned)ceil_div(blocks, x));
+}
+__device__ __forceinline__ int64_t rows_block() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
+
 // Scratch as one run of the caller's workspace.
 struct Carver {
     char *base;

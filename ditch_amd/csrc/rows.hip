@@ -46,7 +46,7 @@ template <int DT, int T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(Planes out, const void *x, int64_t n, int64_t cols,
                                                         int64_t stride, int wide, const int32_t *live) {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t unit = rows_block() * 4 + (threadIdx.x >> 6);
     if (unit >= out.groups * out.units) return;
     const int64_t g = unit / out.units, u = unit % out.units;
     const int64_t row = g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
@@ -87,7 +87,7 @@ void launch_pack_rows(const Planes &out, const void *x, int32_t dtype, int64_t n
     const int64_t units = out.groups * out.units;
     if (units == 0) return;
     const int wide = ((uintptr_t)x | (uintptr_t)(stride * (int64_t)row_size(dtype))) % 16 == 0;
-    const dim3 grid((unsigned)ceil_div(units, 4));
+    const dim3 grid = rows_grid(ceil_div(units, 4), 256);
     if (dtype == DITCH_F32)
         hipLaunchKernelGGL((pack_rows_kernel<DITCH_F32, 3>), grid, dim3(256), 0, s, out, x, n, cols, stride, wide, live);
     else if (dtype == DITCH_F16)
@@ -167,7 +167,7 @@ template <int TF, int T>
 __global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView w, int64_t group0) {
     constexpr int TILES = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t unit = rows_block() * 4 + (threadIdx.x >> 6);
     if (unit >= out.groups * w.units_k) return;
     const int64_t g = unit / w.units_k, u = unit % w.units_k, src = (group0 + g) * w.units_k + u;
     u32x4 words[TF == TF_F32 ? 2 : 1];
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256) void decode_planes_kernel(Planes out, TileView
 // not finite, odd blocks): a wave a unit, each lane 8 columns of a row.
 __global__ __launch_bounds__(256) void decode_any_kernel(Planes out, TileView w, int64_t row0) {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t unit = rows_block() * 4 + (threadIdx.x >> 6);
     if (unit >= out.groups * out.units) return;
     const int64_t g = unit / out.units, u = unit % out.units;
     const int64_t row = row0 + g * 16 + (lane & 15), k = u * 32 + (lane >> 4) * 8;
@@ -239,7 +239,7 @@ Planes weight_planes(const TileView &w, int64_t row0, int64_t rows, int x_terms,
         return out;
     }
     out.p = room;
-    const dim3 grid((unsigned)ceil_div(out.groups * w.units_k, 4)), each((unsigned)ceil_div(out.groups * out.units, 4));
+    const dim3 grid = rows_grid(ceil_div(out.groups * w.units_k, 4), 256), each = rows_grid(ceil_div(out.groups * out.units, 4), 256);
     auto go = [&](auto tf, auto terms) {
         hipLaunchKernelGGL((decode_planes_kernel<decltype(tf)::value, decltype(terms)::value>), grid, dim3(256), 0, s, out,
                            w, row0 / 16);
@@ -269,7 +269,7 @@ __device__ __forceinline__ void put_row_value(void *out, int32_t dtype, int64_t 
 __global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtype, int64_t stride, const float *part,
                                                          int parts, int64_t part_stride, int64_t ld, int64_t n,
                                                          int64_t cols, MoreParts more) {
-    const int64_t per = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t per = (cols + 3) / 4, i = rows_block() * 256 + threadIdx.x;
     if (i >= n * per) return;
     const int64_t row = i / per, c = i % per * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(void *out, int32_t dtyp
 void launch_join_parts(void *out, int32_t dtype, int64_t stride, const float *part, int parts, int64_t part_stride,
                        int64_t ld, int64_t n, int64_t cols, hipStream_t s, MoreParts more) {
     const int64_t total = n * ceil_div(cols, 4);
-    hipLaunchKernelGGL(join_parts_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, s, out, dtype, stride,
+    hipLaunchKernelGGL(join_parts_kernel, rows_grid(ceil_div(total, 256), 256), dim3(256), 0, s, out, dtype, stride,
                        part, parts, part_stride, ld, n, cols, more);
     DITCH_TRY_HIP(hipGetLastError());
 }

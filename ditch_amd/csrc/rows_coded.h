@@ -106,7 +106,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
     int mt, nt;
-    rows_map_tile(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, mt, nt);
+    if (!rows_tile_of_block(p.tiles_m, p.tiles_n, mt, nt)) return;
 
     const int64_t units = p.w[0].units_k;
     auto group = [&](int block, int &which) {
@@ -293,7 +293,7 @@ void launch_rows_coded_tile(RowsCoded p, int64_t mblocks, int64_t nblocks, const
     DITCH_CHECK(tm * tn < (int64_t)1 << 31, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
     p.tiles_m = (int32_t)tm;
     p.tiles_n = (int32_t)tn;
-    hipLaunchKernelGGL((rows_coded_kernel<WGM, WGN, MI, NJ, TF, TB, Epi>), dim3((unsigned)(tm * tn)),
+    hipLaunchKernelGGL((rows_coded_kernel<WGM, WGN, MI, NJ, TF, TB, Epi>), rows_grid(tm * tn, WGM * WGN * 64),
                        dim3(WGM * WGN * 64), 0, s, p, epi);
     DITCH_TRY_HIP(hipGetLastError());
 }

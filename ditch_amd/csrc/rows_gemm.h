@@ -132,6 +132,14 @@ __device__ __forceinline__ void rows_map_tile(int g, int total, int tm, int tn, 
     nt = r / gs;
 }
 
+// This workgroup's tile, if it has one.
+__device__ __forceinline__ bool rows_tile_of_block(int tm, int tn, int &mt, int &nt) {
+    const int64_t block = rows_block();
+    if (block >= tm * tn) return false;
+    rows_map_tile((int)block, tm * tn, tm, tn, mt, nt);
+    return true;
+}
+
 template <bool OUTER>
 __device__ __forceinline__ u32x4 rows_fragment(const u32x4 *S, int block, int lane) {
     if constexpr (!OUTER) {
@@ -247,7 +255,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_gemm_kernel(RowsGemm p, E
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
     int mt, nt;
-    rows_map_tile(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, mt, nt);
+    if (!rows_tile_of_block(p.tiles_m, p.tiles_n, mt, nt)) return;
     const bool copies_b = !HALF || wave < UB;
     const RowsCopies<AO, PA, 1> ca(p.a, wave, mt * UA, 0);
     const RowsCopies<BO, PB, TB> cb(p.b, copies_b ? wave : 0, nt * UB, p.b_plane);
@@ -689,10 +697,11 @@ void launch_rows_few(const RowsGemm &g, int64_t mblocks, int64_t nblocks, const 
 template <int WGM, int WGN, int MI, int NJ, bool WHOLE, bool AO, bool BO, int TB, typename Epi>
 void launch_rows_gemm_tile(RowsGemm g, int64_t mblocks, int64_t nblocks, const Epi &epi, hipStream_t s) {
     const int64_t tm = ceil_div(mblocks, WGM * MI), tn = ceil_div(nblocks, WGN * NJ);
+    // (what such a product leaves is more than a TB)
     DITCH_CHECK(tm * tn < (int64_t)1 << 31 && g.parts < 65536, DITCH_INVALID_ARGUMENT, "rows product: more tiles than one launch holds");
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, WHOLE, AO, BO, TB, Epi>), dim3((unsigned)(tm * tn), (unsigned)g.parts),
+    hipLaunchKernelGGL((rows_gemm_kernel<WGM, WGN, MI, NJ, WHOLE, AO, BO, TB, Epi>), rows_grid(tm * tn, WGM * WGN * 64, g.parts),
                        dim3(WGM * WGN * 64), 0, s, g, epi);
     DITCH_TRY_HIP(hipGetLastError());
 }

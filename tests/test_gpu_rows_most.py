@@ -1,0 +1,38 @@
+"""Losses of as many rows as a call takes, where a product has more threads than a
+launch holds along one side."""
+import numpy as np
+import pytest
+
+import rows_ref as rr
+from ditch_amd import hipmem
+from test_gpu_head import _weight
+
+pytestmark = pytest.mark.gpu
+
+PERIOD = 4099  # rows that are different: a prime, so that none of a tile's rows repeats with the tiles
+
+
+def test_losses_of_the_most_rows(dev):
+    """2^24 rows on 40000 words: 10.3 million tiles of 256 x 256, 512 threads each. The rows repeat after 4099, and so
+    do the results, bit for bit; some of the 4099 are compared with their values."""
+    n, hidden, vocab = 1 << 24, 8, 40000
+    rng = np.random.default_rng(6)
+    t, w = _weight(dev, "bf16", vocab, hidden, 6)
+    try:
+        stored, values = rr.to_rows(rng.standard_normal((PERIOD, hidden)) * 2, "bf16")
+        targets = rng.integers(-1, vocab, PERIOD).astype(np.int32)
+        at = np.arange(n) % PERIOD
+        x, tg = hipmem.Buffer.from_array(stored[at]), hipmem.Buffer.from_array(targets[at])
+        need = t.head_loss_workspace(n, "bf16")
+        assert need
+        ws, out = hipmem.Buffer(need), [rr.Floats(n) for _ in range(2)]
+        t.head_loss("bf16", out[0].ptr, out[1].ptr, dev.kv_rows(x.ptr, n * hidden * 2, hidden), n, tg.ptr, ws.ptr, need)
+        hipmem.synchronize()
+        few = np.r_[:20, PERIOD - 20:PERIOD]
+        want = rr.loss(values[few], w, targets[few], "bf16", "bf16")
+        for k, f in zip(("loss", "lse"), out):
+            got = f.get()
+            rr.check(got[few], *want[k], k)
+            np.testing.assert_array_equal(got, got[:PERIOD][at], err_msg=k)
+    finally:
+        t.free()
