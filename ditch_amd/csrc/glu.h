@@ -5,16 +5,18 @@
 
 namespace ditch {
 
-// act(g) and its derivative; the activations of ditch_hip_gatedActivation.
+// act(g) and its derivative; the activations of ditch_hip_gatedActivation. Towards
+// the ends of f32, where they have long been flat, 1.702 g and g^2 are held finite:
+// infinity times the 0 that is left of the slope would be NaN.
 template <int A>
 __device__ __forceinline__ void act_both(float g, float &y, float &dy) {
     if constexpr (A == 0 || A == 5) {
         constexpr float c = A == 0 ? 1.f : 1.702f;
         const float s = __fdiv_rn(1.f, 1.f + expf(-c * g));
         y = g * s;
-        dy = s * __builtin_fmaf(c * g, 1.f - s, 1.f);
+        dy = s * __builtin_fmaf(__builtin_amdgcn_fmed3f(c * g, -1e30f, 1e30f), 1.f - s, 1.f);
     } else if constexpr (A == 1) {
-        const float k = 0.7978845608028654f, g2 = g * g;
+        const float k = 0.7978845608028654f, g2 = fminf(g * g, 1e30f);
         const float t = tanhf(k * __builtin_fmaf(0.044715f * g2, g, g));
         y = 0.5f * g * (1.f + t);
         dy = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * k * __builtin_fmaf(3.f * 0.044715f, g2, 1.f);
