@@ -35,7 +35,7 @@ __device__ __forceinline__ void act_both(float g, float &y, float &dy) {
 // Blocks 2i of m are gate rows, 2i + 1 the same up rows.
 struct EpiGlu {
     static constexpr bool PAIRS = false;
-    static constexpr bool F32_RESULT = false;
+    static constexpr bool F32_RESULT = false, ALL_PAIRS = false;
     void *out;
     int64_t stride, n, rows;
     int32_t dtype, wide;
@@ -78,7 +78,7 @@ struct EpiGlu {
 template <int T>
 struct EpiGluGrad {
     static constexpr bool PAIRS = false;
-    static constexpr bool F32_RESULT = false;
+    static constexpr bool F32_RESULT = false, ALL_PAIRS = false;
     Planes dg, du;
     const void *dout;
     int64_t stride, n, rows;

@@ -56,7 +56,7 @@ void with_join_rows(int64_t n, F &&f) {
 
 struct EpiLossStats {
     static constexpr bool PAIRS = false;
-    static constexpr bool F32_RESULT = true;
+    static constexpr bool F32_RESULT = true, ALL_PAIRS = true;
     float2 *part;  // [strip][npad]: maximum, sum
     float *picked;  // [n]
     const int32_t *targets;
@@ -116,7 +116,7 @@ constexpr int KL_STATS = 6;
 // The blocks 2i of n are base rows, 2i + 1 the same trial rows.
 struct EpiKlStats {
     static constexpr bool PAIRS = true;  // of n's blocks
-    static constexpr bool F32_RESULT = true;
+    static constexpr bool F32_RESULT = true, ALL_PAIRS = true;
     float *part;  // [strip][npad][KL_STATS]
     int64_t npad, n;
     int64_t rows, strip0;
@@ -180,7 +180,7 @@ struct EpiKlStats {
 template <int T>
 struct EpiLossGrad {
     static constexpr bool PAIRS = false;
-    static constexpr bool F32_RESULT = false;
+    static constexpr bool F32_RESULT = false, ALL_PAIRS = true;  // (lse is of all of them)
     Planes d;
     const int32_t *targets;
     const float *lse, *dloss;
@@ -236,7 +236,7 @@ __device__ __forceinline__ float expm1_near(float z) {
 template <int T>
 struct EpiKlGrad {
     static constexpr bool PAIRS = true;  // of n's blocks
-    static constexpr bool F32_RESULT = true;  // (of near rows' logits a difference is left)
+    static constexpr bool F32_RESULT = true, ALL_PAIRS = true;  // (of near rows' logits a difference is left)
     static constexpr bool NEAR = T > 1;
     Planes d;
     Planes p;     // (none: p.p NULL)
@@ -319,17 +319,17 @@ inline int64_t strips_of(int64_t rows, int tile) {
 inline int64_t weight_row_bytes(const TileView &w, int x_terms) {
     return weight_is_planes(w) ? 0 : (int64_t)weight_planes_shape(w, 16, x_terms).bytes() / 16;
 }
-inline RowsGemm logits_gemm(const Planes &wp, const RowsIn &in, bool f32_result) {
+inline RowsGemm logits_gemm(const Planes &wp, const RowsIn &in) {
     RowsGemm g;
     g.a = rows_inner(wp);
     g.b = in.op;
     g.k32 = (int32_t)ceil_div(wp.units, 2) * 2;
-    rows_pairs(g, wp, in.x, rows_order_of(wp.terms, in.x.terms, f32_result));
+    rows_pairs(g, wp, in.x, rows_order_of(wp.terms, in.x.terms, true));
     return g;
 }
 
 inline int logits_tile(const TileView &w, int64_t rows, const Planes &x, int64_t nblocks, bool f32_result) {
-    const int a = rows_weight_terms(w, f32_result ? ROWS_MAX_TERMS : x.terms), order = rows_order_of(a, x.terms, f32_result);
+    const int a = rows_weight_terms(w, f32_result ? ROWS_MAX_TERMS : x.terms), order = rows_order_of(a, x.terms, true);
     return rows_tiling(ceil_div(rows, 16), nblocks, ceil_div(w.cols, 64) * 2, a, x.terms, order, 1, false, true).tile;
 }
 

@@ -167,7 +167,7 @@ void launch_head_loss(float *loss, float *lse, int32_t dtype, RowsArg x, int64_t
         }
         const Planes wp = weight_planes(w, r, rows, ROWS_MAX_TERMS, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in, true), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);
@@ -194,7 +194,7 @@ void launch_head_kl(float *kl, float *lse_base, float *lse_trial, int32_t dtype,
         }
         const Planes wp = weight_planes(w, r, rows, ROWS_MAX_TERMS, p.room, s);
         with_terms(p.x[0].terms, [&](auto terms) {
-            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in, true), wp.groups,
+            launch_rows_gemm<false, false, decltype(terms)::value>(p.tile, logits_gemm(wp, in), wp.groups,
                                                                    p.nblocks, epi, s);
         });
         strip += strips_of(rows, p.tile);

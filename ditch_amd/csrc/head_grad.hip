@@ -172,7 +172,7 @@ static void fill_loss(const HeadGradPlan &p, const RowsIn &in, const TileView &w
         launch_loss_grad_coded<T>(p.coded, c, TB, d.units * 2, p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks, false), logits_gemm(wp, in, false),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], p.nblocks, false), logits_gemm(wp, in),
                                       d.units * 2, p.nblocks, epi, s);
 }
 template <int TB, int T>
@@ -187,7 +187,7 @@ static void fill_kl(const HeadGradPlan &p, const RowsIn &in, const TileView &w, 
         launch_kl_grad_coded<T>(p.coded, c, TB, d.units * 2, 2 * p.nblocks, epi, s);
         return;
     }
-    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks, true), logits_gemm(wp, in, true),
+    launch_rows_gemm<false, false, TB>(logits_tile(w, rows, p.x[0], 2 * p.nblocks, true), logits_gemm(wp, in),
                                       d.units * 2, 2 * p.nblocks, epi, s);
 }
 

@@ -40,12 +40,14 @@ int rows_weight_terms(const TileView &w, int x_terms);
 // the products wait for the weight (one value of d makes most of such a gradient,
 // and its rounding would be the gradient's).
 inline int grad_term_count(int x_terms, int64_t n) { return x_terms == 1 && n <= 64 ? 2 : x_terms; }
-// and the pairs of terms that are multiplied: i + j < order; f32 results of 16-bit
-// rows, and differences of two rows' logits, take all that count in 24 bits (logits
-// off by 2^-17 of their terms left divergences of f16 rows 2^-6 apart off by 3e-4).
-constexpr int rows_order_of(int w_terms, int x_terms, bool f32_result = false) {
+// and the pairs of terms that are multiplied: i + j < order; logits take all that count
+// in 24 bits (off by 2^-17 of their terms they left divergences of f16 rows 2^-6 apart
+// off by 3e-4; and terms are cut, of their value's sign, so that what a pair left out
+// takes away is 7e-6 of every logit alike: at logits of 40 the loss' gradient, whose
+// log sum has it all, was off by 2e-3).
+constexpr int rows_order_of(int w_terms, int x_terms, bool logits = false) {
     const int all = w_terms + x_terms - 1, most = w_terms > x_terms ? w_terms : x_terms;
-    return f32_result ? (all < ROWS_MAX_TERMS ? all : ROWS_MAX_TERMS) : most;
+    return logits ? (all < ROWS_MAX_TERMS ? all : ROWS_MAX_TERMS) : most;
 }
 
 // Rows of activations: 64 rows and 128 columns (a unit of 4-bit codes), zeros

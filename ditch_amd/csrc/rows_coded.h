@@ -86,7 +86,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void rows_coded_kernel(RowsCoded p,
     constexpr int KT = TF == TF_FP8 || TF == TF_Q8 ? 2 : TF == TF_MX4 || TF == TF_INT4 ? 4 : 1;
     constexpr int HALVES = TF == TF_F32 ? 2 : 1;
     constexpr int NS = TF == TF_INT4 ? 2 : TF == TF_F16 || TF == TF_F32 ? 0 : 1;
-    constexpr int ORDER = rows_order_of(TA, TB, Epi::F32_RESULT);
+    constexpr int ORDER = rows_order_of(TA, TB, Epi::ALL_PAIRS);
     constexpr int WAVES = WGM * WGN, UA = WGM * MI, UB = WGN * NJ;
     constexpr int NA = UA * HALVES, PA = NA / WAVES, NBP = UB * KT;
     constexpr bool HALF = NBP * 2 == WAVES;
