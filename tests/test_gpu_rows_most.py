@@ -36,3 +36,39 @@ def test_losses_of_the_most_rows(dev):
             np.testing.assert_array_equal(got, got[:PERIOD][at], err_msg=k)
     finally:
         t.free()
+
+
+def test_gradients_of_the_most_rows(dev):
+    """The same over 600 words in pieces of 256, whose d are 8.6 GB each: dx repeats bit for bit, dW is the period's
+    taken as often as its rows come (sums of 2^24 / 32 steps)."""
+    n, hidden, vocab = 1 << 24, 8, 600
+    rng = np.random.default_rng(7)
+    t, w = _weight(dev, "bf16", vocab, hidden, 7)
+    try:
+        stored, values = rr.to_rows(rng.standard_normal((PERIOD, hidden)) * 2, "bf16")
+        targets = rng.integers(-1, vocab, PERIOD).astype(np.int32)
+        g = rng.standard_normal(PERIOD).astype(np.float32)
+        at = np.arange(n) % PERIOD
+        lse = rr._lse(values @ w.T).astype(np.float32)
+        x, tg = hipmem.Buffer.from_array(stored[at]), hipmem.Buffer.from_array(targets[at])
+        d_lse, d_g = rr.Floats(n, lse[at]), rr.Floats(n, g[at])
+        dx, dw = rr.Rows(dev, n, hidden, "bf16"), rr.Rows(dev, vocab, hidden, "bf16")
+        need = t.head_loss_grad_workspace(n, "bf16")
+        ws = hipmem.Buffer(need)
+        t.head_loss_grad("bf16", dx.desc, dw.desc, dev.kv_rows(x.ptr, n * hidden * 2, hidden), n, tg.ptr, d_lse.ptr,
+                         d_g.ptr, ws.ptr, need)
+        hipmem.synchronize()
+        few = np.r_[:20, PERIOD - 20:PERIOD]
+        got = dx.get()
+        rr.check(got[few], *rr.loss_grad(values[few], w, targets[few], g[few].astype(np.float64), "bf16", "bf16")["dx"], "dx")
+        np.testing.assert_array_equal(got, got[:PERIOD][at])
+        l, off = rr.logits(values, w, "bf16", "bf16")
+        _, _, p, p_off = rr._softmax(l, off)
+        live = targets >= 0
+        one = np.zeros_like(p)
+        one[np.arange(PERIOD)[live], targets[live]] = 1
+        weight = np.where(live, g.astype(np.float64), 0)[:, None] * np.bincount(at)[:, None]
+        v, off = rr._back(((p - one) * weight).T, ((p_off + 2.0 ** -24) * np.abs(weight)).T, values, n, "bf16", 1, 1)
+        rr.check(dw.get(), v, off, "dw")
+    finally:
+        t.free()
