@@ -1726,8 +1726,10 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
     }
     if (n_logit > 0 && (d_logits || d_hidden)) {
         float *hl = d_hidden ? d_hidden : m->logit_h.get<float>(n_logit * hidden);
-        launch_rmsnorm(hl, x, m->final_norm.p, m->final_norm.len, n_logit, hidden, c.rms_eps, 0, s,
-                       (const int64_t *)d_logit_rows, n);
+        constexpr int64_t MOST = 1 << 21;  // rows of a launch, which holds less than 2^32 threads
+        for (int64_t i = 0; i < n_logit; i += MOST)
+            launch_rmsnorm(hl + i * hidden, x, m->final_norm.p, m->final_norm.len, std::min(MOST, n_logit - i), hidden,
+                           c.rms_eps, 0, s, (const int64_t *)d_logit_rows + i, n);
         if (!d_logits) return;
         const Mat &lm = m->lm_head.ok() ? m->lm_head : m->embed;
         mm(m, lm, d_logits, hl, n_logit, nullptr, 0, s);

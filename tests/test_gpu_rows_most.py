@@ -1,10 +1,12 @@
-"""Losses of as many rows as a call takes, where a product has more threads than a
-launch holds along one side."""
+"""Calls of as many rows as they take, where a product or a norm has more threads
+than a launch holds along one side."""
 import numpy as np
 import pytest
 
+import model_gen as mg
 import rows_ref as rr
 from ditch_amd import hipmem
+from ditch_amd.hip import Model
 from test_gpu_head import _weight
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +74,26 @@ def test_gradients_of_the_most_rows(dev):
         rr.check(dw.get(), v, off, "dw")
     finally:
         t.free()
+
+
+def test_hidden_rows_past_a_launch(dev):
+    """2^24 + 77 final hidden rows, a workgroup of 256 threads each: the same few rows over and over."""
+    spec = mg.dense(hidden=36, inter=64, layers=1, heads=2, kv_heads=1, head_dim=32, vocab=50, seed=3)
+    model = Model(dev, spec)
+    try:
+        hidden, n, many = 36, 11, (1 << 24) + 77
+        rng = np.random.default_rng(1)
+        tokens = hipmem.Buffer.from_array(rng.integers(0, 50, n).astype(np.uint32))
+        rows = hipmem.Buffer.from_array(np.array([(0, p) for p in range(n)], np.uint32))
+        want = []
+        for count in (n, many):
+            at = hipmem.Buffer.from_array((np.arange(count) % n).astype(np.uint64))
+            out = hipmem.Buffer.from_array(np.full(count * hidden, np.nan, np.float32))
+            model.forward_hidden_device(tokens.ptr, rows.ptr, n, 1, n, at.ptr, count, out.ptr)
+            dev.sync()
+            want.append(out.download(np.float32, (count, hidden)))
+        assert np.isfinite(want[0]).all()
+        whole = many // n * n
+        assert (want[1][:whole].reshape(-1, n, hidden) == want[0]).all() and (want[1][whole:] == want[0][:many - whole]).all()
+    finally:
+        model.free()
