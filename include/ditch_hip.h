@@ -886,7 +886,13 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
  * Rows are ditch_kv_rows of `dtype` (DITCH_F32, DITCH_F16 or DITCH_BF16), one
  * dtype a call. The weights are registered tensors of any format, taken at the
  * values they decode to. Losses, log sums and divergences are exact to about
- * f32 rounding for rows of any type, and so are f32 rows' other results; 16-bit
+ * f32 rounding of the logits for rows of any type, and so are f32 rows' other
+ * results, save that gradients take the log sums as the f32 they are handed:
+ * a loss' gradient is off by their rounding (2^-24 of a log sum) times the
+ * probabilities' mean of the weight's rows. A divergence's has that taken off
+ * again for f32 and f16 rows: those of near rows are off by what the logits'
+ * roundings leave of their differences. bf16 rows' keep it (as much as their own
+ * rounding below divergences of about 1e-5). 16-bit
  * results are rounded once where they leave a call, and once to at least as many
  * bits between the two products of a gradient, and take f32 and Q8_0 weights at
  * 16 bits. A row that is not finite has no finite result, nor has the weights'
@@ -908,7 +914,8 @@ int32_t ditch_hip_head_loss_device(ditch_hip *h, float *d_loss, float *d_lse, in
                                    void *ws, uint64_t ws_bytes, void *stream);
 /* Its gradient for d_dloss [n], with the lse that the call above gave: dx
  * [n][hidden] and dw [vocab][hidden] (with respect to the decoded weights), of
- * `dtype`; either may be NULL. `want_dw`: whether dw will be given.          */
+ * `dtype`; either may be NULL. `want_dw`: whether dw will be given (one size
+ * serves either way).                                                        */
 uint64_t ditch_hip_head_loss_grad_workspace(const ditch_hip_tensor *w, uint64_t n,
                                             int32_t dtype, int32_t want_dw);
 int32_t ditch_hip_head_loss_grad_device(ditch_hip *h, int32_t dtype, const ditch_kv_rows *dx,
@@ -919,7 +926,8 @@ int32_t ditch_hip_head_loss_grad_device(ditch_hip *h, int32_t dtype, const ditch
                                         void *stream);
 /* KL(base || trial) of the distributions that two sets of rows have over the
  * head (what ditch_hip_klRows_device gives from kept log-probabilities), and
- * both log sums. Small divergences keep their relative accuracy.            */
+ * both log sums. Small divergences keep their relative accuracy, also of rows whose
+ * logits all moved alike.                                                    */
 uint64_t ditch_hip_head_kl_workspace(const ditch_hip_tensor *w, uint64_t n, int32_t dtype);
 int32_t ditch_hip_head_kl_device(ditch_hip *h, float *d_kl, float *d_lse_base,
                                  float *d_lse_trial, int32_t dtype, const ditch_kv_rows *base,
@@ -946,7 +954,7 @@ int32_t ditch_hip_glu_rows_device(ditch_hip *h, int32_t dtype, const ditch_kv_ro
                                   uint32_t act, void *ws, uint64_t ws_bytes, void *stream);
 /* Its gradient for dout [n][gate.rows]: dx [n][cols], dgate and dup
  * [gate.rows][cols] (with respect to the decoded weights); each may be NULL.
- * `want_dw`: whether dgate or dup will be given.                            */
+ * `want_dw`: whether dgate or dup will be given (one size serves either way). */
 uint64_t ditch_hip_glu_rows_grad_workspace(const ditch_hip_tensor *gate,
                                            const ditch_hip_tensor *up, uint64_t n,
                                            int32_t dtype, int32_t want_dw);
