@@ -737,6 +737,8 @@ const ditch_hip_tensor *ditch_hip_model_head(ditch_hip_model *m) {
     const int32_t rc = guarded(m->h, [&] {
         const Mat &lm = m->lm_head.ok() ? m->lm_head : m->embed;
         DITCH_CHECK(lm.ok(), DITCH_INVALID_ARGUMENT, "model head: not registered");
+        DITCH_CHECK(lm.t->v.rows == (int64_t)m->c.vocab, DITCH_INVALID_ARGUMENT,
+                    "model head: the embedding has other rows than the vocabulary");
         DITCH_CHECK(lm.rank == 0, DITCH_UNSUPPORTED, "model head: it carries a low-rank delta");
         t = lm.t;
     });

@@ -1428,6 +1428,9 @@ void model_forward(ditch_hip_model *m, const uint32_t *d_tokens, const ditch_row
     hipStream_t s = m->h->stream;
     if (n <= 0) return;
     DITCH_CHECK(m->embed.ok(), DITCH_INVALID_ARGUMENT, "forward: no embedding");
+    // (a row of logits is as long as its matrix has rows; an embedding may have others than the vocabulary's)
+    DITCH_CHECK(n_logit <= 0 || !d_logits || (m->lm_head.ok() ? m->lm_head : m->embed).t->v.rows == (int64_t)c.vocab,
+                DITCH_INVALID_ARGUMENT, "forward: no head, and the embedding has other rows than the vocabulary");
     int64_t hidden = (int64_t)c.hidden;
     DITCH_CHECK(B > 0 && T > 0 && B <= (int64_t)INT32_MAX, DITCH_INVALID_ARGUMENT, "forward: KV cache shape");
     const bool paged = pc && pc->paged();
