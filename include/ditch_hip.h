@@ -892,7 +892,7 @@ int32_t ditch_hip_klRows_device(ditch_hip *h, double *d_kl,
  * probabilities' mean of the weight's rows. A divergence's has that taken off
  * again for f32 and f16 rows: those of near rows are off by what the logits'
  * roundings leave of their differences. bf16 rows' keep it (as much as their own
- * rounding below divergences of about 1e-5). 16-bit
+ * rounding below divergences of 1e-5 to 1e-4, by how strong that mean is). 16-bit
  * results are rounded once where they leave a call, and once to at least as many
  * bits between the two products of a gradient, and take f32 and Q8_0 weights at
  * 16 bits. A row that is not finite has no finite result, nor has the weights'
